@@ -39,6 +39,7 @@ extern "C" {
 /* element types */
 #define NPL_F32 0
 #define NPL_F16 1
+#define NPL_BF16 2 /* the npl_fp8_* entries only */
 
 /* fused epilogues of npl_w8a8_linear / npl_w8a8_linear_ex */
 #define NPL_EPI_NONE 0     /* out = dequant(acc)                                  */
@@ -389,6 +390,70 @@ int npl_tp_absmax_quant(const npl_tp_peers* peers, const void* x, int M, int K, 
 int npl_tp_allreduce_dequant(const npl_tp_peers* peers, const int32_t* acc, int M, int N, const float* sa,
                              const float* sw, const float* bias_or_null, const void* residual_or_null, int ld_res,
                              void* out, int ld_out, void* stream);
+
+/*
+ * Block-scaled 8-bit floating point (e4m3) beside the int8 contract: one fp32
+ * scale for each block of 128 -- 128 consecutive columns of a token, or a
+ * 128 x 128 tile of a weight, the last ones possibly partial. No counterpart
+ * in the reference, whose only 8-bit form is int8. Quantisation of a block of
+ * fp32 values v:
+ *   scale = max(max |v| / 448, 2^-126),  q = e4m3(v * (1 / scale))
+ * each step one fp32 rounding; codes round to nearest even. A block that
+ * holds a NaN or an infinity gets a non-finite scale, so that all its values
+ * q * scale are NaN; no other block is affected.
+ *
+ * Sizes and strides are 64-bit, strides in elements between rows (>= the row's
+ * length; the columns of a row are contiguous). Any sizes: no row or column
+ * count has to be a multiple of anything, inputs need the alignment of their
+ * elements only (16-byte aligned rows are faster). Nothing beyond the given
+ * rows and columns is read or written. rows == 0 launches nothing.
+ * q: e4m3 codes [rows, cols], stride ldq. scale: fp32 [rows, ceil(cols /
+ * 128)], stride ld_scale. dtype: NPL_F16 or NPL_BF16, and NPL_F32 where said.
+ * No workspace: calls on different streams share nothing.
+ */
+
+/* Activations, per token and 128 columns. x_dtype may be NPL_F32. */
+int npl_fp8_quant_rows(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q, int64_t ldq,
+                       float* scale, int64_t ld_scale, void* stream);
+
+/* A weight per 128 x 128 block: scale fp32 [ceil(rows / 128), ceil(cols /
+ * 128)]. w_dtype may be NPL_F32; cols <= 65535 * 128. */
+int npl_fp8_quant_weight(const void* w, int w_dtype, int64_t rows, int64_t cols, int64_t ldw, uint8_t* q, int64_t ldq,
+                         float* scale, int64_t ld_scale, void* stream);
+
+/*
+ * Residual addition, RMSNorm and quantisation of 16-bit rows:
+ *   s = residual ? T(x + residual) : x               (sum_out <- s, with residual)
+ *   v = s * (1 / sqrt(mean(s^2) + eps)) * weight     (fp32, not rounded to T)
+ *   q, scale = npl_fp8_quant_rows of v
+ * residual and sum_out are given together or not at all; sum_out may be x or
+ * residual itself (same row stride). The mean is an fp32 sum.
+ */
+int npl_fp8_rmsnorm_quant(const void* x, int64_t ldx, const void* residual_or_null, int64_t ld_res, const void* weight,
+                          int dtype, float eps, int64_t rows, int64_t cols, void* sum_out_or_null, int64_t ld_sum,
+                          uint8_t* q, int64_t ldq, float* scale, int64_t ld_scale, void* stream);
+
+/* v = gate / (1 + exp(-gate)) * up (fp32), then npl_fp8_quant_rows of v. gate
+ * and up may be the two halves of one packed projection's rows. */
+int npl_fp8_silu_mul_quant(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int dtype, int64_t rows,
+                           int64_t cols, uint8_t* q, int64_t ldq, float* scale, int64_t ld_scale, void* stream);
+
+/*
+ * Linear of block-scaled codes:
+ *   v[m, n] = sum_b sa[m, b] * sw[n / 128, b] * (sum_{k in block b} qa[m, k] * qw[n, k])
+ *   out[m, n] = T(v + bias[n] + residual[m, n])
+ * with fp32 sums (the inner one on the tensor cores, the outer one in
+ * registers, block after block) and one rounding to T = out_dtype, NPL_F16 or
+ * NPL_BF16, which is residual's type too. qa e4m3 [M, K], qw e4m3 [N, K]: rows
+ * on 16-byte boundaries (lda, ldw multiples of 16); K itself is arbitrary.
+ * sa fp32 [M, ceil(K / 128)], sw fp32 [ceil(N / 128), ceil(K / 128)]; bias
+ * fp32 [N]. out may be residual itself (same row stride). Equal inputs give
+ * equal bits. The kernel runs on any stream, in any number at once.
+ */
+int npl_fp8_linear(const uint8_t* qa, int64_t lda, const float* sa, int64_t ld_sa, const uint8_t* qw, int64_t ldw,
+                   const float* sw, int64_t ld_sw, const float* bias_or_null, int64_t M, int64_t N, int64_t K,
+                   const void* residual_or_null, int64_t ld_res, void* out, int64_t ld_out, int out_dtype,
+                   void* stream);
 
 #ifdef __cplusplus
 }

@@ -11,6 +11,9 @@ Public surface, mirroring the reference ``nanopointllm`` API for this path:
   static_activation_qdq, dynamic_per_token_activation_qdq,
   integer_linear_per_output_reference), plus the decode-path forms
   (per_output_weight_quant, dynamic_per_token_quant, linear_q, W8A8Linear)
+* ``nanopointllm_b200.fp8``             - block-scaled e4m3 linears beside the
+  int8 ones (quantize_token_blocks, quantize_weight_blocks,
+  rmsnorm_quant_blocks, silu_mul_quant_blocks, linear_blocks, Fp8BlockLinear)
 * ``nanopointllm_b200.paged_attention`` - store_kvcache, paged_decode_attention,
   rope_store_kvcache
 * ``nanopointllm_b200.runner``          - W8A8 Llama decode runner
@@ -30,4 +33,4 @@ from ``csrc/``; there is no CPU or library fallback.
 """
 from __future__ import annotations
 
-__all__ = ["w8a8", "paged_attention", "runner", "synthetic", "tp", "package", "serving"]
+__all__ = ["w8a8", "fp8", "paged_attention", "runner", "synthetic", "tp", "package", "serving"]

@@ -23,6 +23,7 @@ NPL_ERR_UNSUPPORTED = 5
 
 NPL_F32 = 0
 NPL_F16 = 1
+NPL_BF16 = 2
 
 EPI_NONE = 0
 EPI_RESIDUAL = 1
@@ -37,6 +38,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _Z = ctypes.c_size_t
+_Q = ctypes.c_int64
 
 class NplRopeKV(ctypes.Structure):
     """npl_rope_kv (include/npl_w8a8.h)."""
@@ -92,6 +94,11 @@ SIGNATURES = {
     "npl_ipc_close": (_I, [_P]),
     "npl_tp_absmax_quant": (_I, [ctypes.POINTER(NplTpPeers), _P, _I, _I, _I, _P, _I, _P, _P]),
     "npl_tp_allreduce_dequant": (_I, [ctypes.POINTER(NplTpPeers), _P, _I, _I, _P, _P, _P, _P, _I, _P, _I, _P]),
+    "npl_fp8_quant_rows": (_I, [_P, _I, _Q, _Q, _Q, _P, _Q, _P, _Q, _P]),
+    "npl_fp8_quant_weight": (_I, [_P, _I, _Q, _Q, _Q, _P, _Q, _P, _Q, _P]),
+    "npl_fp8_rmsnorm_quant": (_I, [_P, _Q, _P, _Q, _P, _I, _F, _Q, _Q, _P, _Q, _P, _Q, _P, _Q, _P]),
+    "npl_fp8_silu_mul_quant": (_I, [_P, _Q, _P, _Q, _I, _Q, _Q, _P, _Q, _P, _Q, _P]),
+    "npl_fp8_linear": (_I, [_P, _Q, _P, _Q, _P, _Q, _P, _Q, _P, _Q, _Q, _Q, _P, _Q, _P, _Q, _I, _P]),
     "npl_paged_prefill_attention": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _I, _I, _F,
                                          _P, _I, _P]),
 }

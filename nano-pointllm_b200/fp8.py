@@ -1,0 +1,294 @@
+"""Block-scaled 8-bit floating point (e4m3) linears and their activation
+quantisers, beside the int8 contract of ``w8a8``.
+
+One fp32 scale for each block of 128: 128 consecutive columns of a token, or a
+128 x 128 tile of a weight (the last ones may be partial). For a block of
+values v
+
+    scale = max(max |v| / 448, 2^-126),  q = e4m3(v * (1 / scale)),  v ~ q * scale
+
+in fp32 (448 is the largest e4m3 value), and a linear is
+
+    out[m, n] = sum_b sa[m, b] * sw[n // 128, b] * sum_{k in block b} qa[m, k] * qw[n, k]
+
+with fp32 sums and one rounding to fp16 or bf16. A block that holds a NaN or
+an infinity reads back as NaN altogether; other blocks are not affected. The
+reference project has no counterpart (its only 8-bit form is int8).
+
+* ``quantize_token_blocks``   - activations, per token and 128 columns
+* ``rmsnorm_quant_blocks``    - (x + residual), RMSNorm, quantised (cf. runner.rmsnorm_quant)
+* ``silu_mul_quant_blocks``   - SiLU(gate) * up, quantised
+* ``quantize_weight_blocks``  - a weight, per 128 x 128 block
+* ``linear_blocks``           - the matrix product (+ bias, + residual)
+* ``Fp8BlockLinear``          - a quantised Linear (cf. w8a8.W8A8Linear)
+
+A decoder layer's MLP reads ``rmsnorm_quant_blocks`` -> ``linear_blocks``
+(packed gate/up rows) -> ``silu_mul_quant_blocks`` on the two halves ->
+``linear_blocks(..., residual=...)``. Every call runs kernels of libnpl_w8a8 on
+the current stream of its tensors' device; none synchronises, keeps a
+workspace or reads anything back, and every one can be captured into a CUDA
+graph. CUDA tensors only. Codes come and go as torch.float8_e4m3fn.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib as L
+
+BLOCK = 128
+
+_E4M3 = torch.float8_e4m3fn
+_DT16 = {torch.float16: L.NPL_F16, torch.bfloat16: L.NPL_BF16}
+_DT = {torch.float32: L.NPL_F32, **_DT16}
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    if not first.is_cuda:
+        raise ValueError("the fp8 path runs on CUDA tensors only")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+
+
+def _call(fn, device: torch.device, *args) -> None:
+    """fn(*args, stream) with ``device`` current, on its current stream."""
+    if device.index == torch.cuda.current_device():
+        L.check(fn(*args, L.stream_ptr(device)))
+    else:
+        with torch.cuda.device(device):
+            L.check(fn(*args, L.stream_ptr(device)))
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., K] as [rows, K] with contiguous columns and rows that do not
+    overlap (a copy only where the strides do not allow a view)."""
+    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    r, k = t.shape
+    if (k > 1 and t.stride(1) != 1) or (r > 1 and t.stride(0) < k):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor; a single row's is its length."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _new_codes(rows: int, k: int, device: torch.device) -> torch.Tensor:
+    """e4m3 [rows, K] whose rows start on 16-byte boundaries, as the linear reads them."""
+    if k % 16 == 0:
+        return torch.empty((rows, k), dtype=_E4M3, device=device)
+    return torch.empty((rows, -(-k // 16) * 16), dtype=_E4M3, device=device)[:, :k]
+
+
+def _activation(name: str, t: torch.Tensor, types: dict) -> int:
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise ValueError(f"{name} needs at least one column")
+    if t.dtype not in types:
+        raise ValueError(f"{name} must be one of {', '.join(str(d).replace('torch.', '') for d in types)}")
+    return types[t.dtype]
+
+
+def quantize_token_blocks(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """fp16, bf16 or fp32 [..., K] -> (codes e4m3 [..., K], scales fp32
+    [..., ceil(K / 128)])."""
+    _same_device(x)
+    dt = _activation("x", x, _DT)
+    v = _rows(x)
+    m, k = v.shape
+    q = _new_codes(m, k, x.device)
+    s = torch.empty((m, _blocks(k)), dtype=torch.float32, device=x.device)
+    if m:
+        _call(L.lib.npl_fp8_quant_rows, x.device, v.data_ptr(), dt, m, k, _ld(v), q.data_ptr(), _ld(q), s.data_ptr(),
+              s.shape[1])
+    return (q, s) if x.dim() == 2 else (q.reshape(x.shape), s.reshape(*x.shape[:-1], -1 if m else _blocks(k)))
+
+
+def quantize_weight_blocks(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """fp16, bf16 or fp32 [N, K] -> (codes e4m3 [N, K], scales fp32
+    [ceil(N / 128), ceil(K / 128)])."""
+    _same_device(weight)
+    if weight.dim() != 2 or weight.shape[0] == 0:
+        raise ValueError("weight must be [N, K] with N >= 1")
+    dt = _activation("weight", weight, _DT)
+    w = _rows(weight.detach())
+    n, k = w.shape
+    q = _new_codes(n, k, w.device)
+    s = torch.empty((_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device)
+    _call(L.lib.npl_fp8_quant_weight, w.device, w.data_ptr(), dt, n, k, _ld(w), q.data_ptr(), _ld(q), s.data_ptr(),
+          s.shape[1])
+    return q, s
+
+
+def rmsnorm_quant_blocks(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None, *,
+                         sum_out: torch.Tensor | None = None):
+    """RMSNorm (of x + residual when given) fused with the token quantiser.
+    x, residual fp16 or bf16 [M, K], weight [K], one type. Returns (codes
+    [M, K], scales [M, ceil(K / 128)], sum): the sum is x + residual in their
+    type, which the norm reads, in ``sum_out`` when given (it may be x or
+    residual itself); None without a residual. The norm stays in fp32 up to
+    the codes."""
+    _same_device(x, weight, residual, sum_out)
+    dt = _activation("x", x, _DT16)
+    if x.dim() != 2 or weight.shape != x.shape[1:] or weight.dtype != x.dtype:
+        raise ValueError("x must be [M, K] and weight [K], of one type")
+    if residual is None:
+        if sum_out is not None:
+            raise ValueError("sum_out needs a residual")
+    else:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError("residual must have the shape and type of x")
+        if sum_out is None:
+            sum_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif sum_out.shape != x.shape or sum_out.dtype != x.dtype:
+            raise ValueError("sum_out must have the shape and type of x")
+        elif sum_out is not x and sum_out is not residual and _overlap(sum_out, x, residual):
+            raise ValueError("sum_out may be x or residual itself, but not overlap them otherwise")
+        if _rows(sum_out) is not sum_out:
+            raise ValueError("sum_out needs contiguous columns and rows that do not overlap")
+    v = _rows(x)
+    r = None if residual is None else _rows(residual)
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    m, k = v.shape
+    q = _new_codes(m, k, x.device)
+    s = torch.empty((m, _blocks(k)), dtype=torch.float32, device=x.device)
+    if m:
+        _call(L.lib.npl_fp8_rmsnorm_quant, x.device, v.data_ptr(), _ld(v), L.ptr(r), 0 if r is None else _ld(r),
+              w.data_ptr(), dt, float(eps), m, k, L.ptr(sum_out), 0 if r is None else _ld(sum_out), q.data_ptr(),
+              _ld(q), s.data_ptr(), s.shape[1])
+    return q, s, sum_out
+
+
+def silu_mul_quant_blocks(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """SiLU(gate) * up of fp16 or bf16 [M, K] rows (for a packed gate/up
+    projection: its two column halves), in fp32 up to the codes. Returns
+    (codes [M, K], scales [M, ceil(K / 128)])."""
+    _same_device(gate, up)
+    dt = _activation("gate", gate, _DT16)
+    if gate.dim() != 2 or up.shape != gate.shape or up.dtype != gate.dtype:
+        raise ValueError("gate and up must be [M, K] of one shape and type")
+    g, u = _rows(gate), _rows(up)
+    m, k = g.shape
+    q = _new_codes(m, k, g.device)
+    s = torch.empty((m, _blocks(k)), dtype=torch.float32, device=g.device)
+    if m:
+        _call(L.lib.npl_fp8_silu_mul_quant, g.device, g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), dt, m, k,
+              q.data_ptr(), _ld(q), s.data_ptr(), s.shape[1])
+    return q, s
+
+
+def _overlap(out: torch.Tensor, *others: torch.Tensor) -> bool:
+    """Whether the memory spans of ``out`` and another tensor meet."""
+    def span(t):
+        n = sum((d - 1) * abs(st) for d, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    a0, a1 = span(out)
+    return any(a0 < b1 and b0 < a1 for b0, b1 in map(span, others))
+
+
+def _code_rows(name: str, q: torch.Tensor) -> None:
+    if q.dtype != _E4M3 or q.dim() != 2:
+        raise ValueError(f"{name} must be float8_e4m3fn [rows, K]")
+    if (q.shape[1] > 1 and q.stride(1) != 1) or q.data_ptr() % 16 or (q.shape[0] > 1 and q.stride(0) % 16):
+        raise ValueError(f"{name} needs contiguous columns and rows on 16-byte boundaries, as the quantisers return them")
+
+
+def _ld16(q: torch.Tensor) -> int:
+    """Row stride of codes; a single row's is its length rounded up to 16."""
+    return q.stride(0) if q.shape[0] > 1 else -(-q.shape[1] // 16) * 16
+
+
+def _scales(name: str, s: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    if s.dtype != torch.float32 or s.shape != (rows, cols):
+        raise ValueError(f"{name} must be float32 [{rows}, {cols}], got {s.dtype} {tuple(s.shape)}")
+    return _rows(s)
+
+
+def linear_blocks(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, wscale: torch.Tensor, *,
+                  bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Codes [M, K] with scales [M, ceil(K / 128)] times weight codes [N, K]
+    with scales [ceil(N / 128), ceil(K / 128)] -> [M, N] (+ bias fp32 [N])
+    (+ residual [M, N]), rounded once to ``out_dtype``: fp16 or bf16, by default
+    the type of ``out`` or ``residual``, else bf16. ``out`` may be ``residual``
+    itself."""
+    _same_device(q, scale, qweight, wscale, bias, residual, out)
+    _code_rows("q", q)
+    _code_rows("qweight", qweight)
+    m, k = q.shape
+    n = qweight.shape[0]
+    if qweight.shape[1] != k or k == 0 or n == 0:
+        raise ValueError("linear input/weight shapes do not match")
+    kb = _blocks(k)
+    sa, sw = _scales("scale", scale, m, kb), _scales("wscale", wscale, _blocks(n), kb)
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.bfloat16
+    if out_dtype not in _DT16:
+        raise ValueError("out_dtype must be float16 or bfloat16")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError("bias must be contiguous float32 [N]")
+    res = None
+    if residual is not None:
+        if residual.shape != (m, n) or residual.dtype != out_dtype:
+            raise ValueError("residual must be [M, N] of out_dtype")
+        res = _rows(residual)
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype, device=q.device)
+    else:
+        if out.shape != (m, n) or out.dtype != out_dtype:
+            raise ValueError("out must be [M, N] of out_dtype")
+        if _rows(out) is not out:
+            raise ValueError("out needs contiguous columns and rows that do not overlap")
+        if _overlap(out, q, scale, qweight, wscale, *(t for t in (bias,) if t is not None)) or (
+                residual is not None and out is not residual and _overlap(out, residual)):
+            raise ValueError("out may be residual itself, but not overlap an input otherwise")
+    if m:
+        _call(L.lib.npl_fp8_linear, q.device, q.data_ptr(), _ld16(q), sa.data_ptr(), _ld(sa), qweight.data_ptr(),
+              _ld16(qweight), sw.data_ptr(), _ld(sw), L.ptr(bias), m, n, k, L.ptr(res),
+              0 if res is None else _ld(res), out.data_ptr(), _ld(out), _DT16[out_dtype])
+    return out
+
+
+class Fp8BlockLinear:
+    """A quantised Linear: e4m3 weight codes [N, K] with fp32 scales
+    [ceil(N / 128), ceil(K / 128)] and an optional fp32 bias. Calling it
+    quantises the input's tokens and multiplies; the output has the input's
+    type (fp16 or bf16)."""
+
+    def __init__(self, qweight: torch.Tensor, wscale: torch.Tensor, bias: torch.Tensor | None = None):
+        if qweight.dtype != _E4M3 or qweight.dim() != 2 or 0 in qweight.shape:
+            raise ValueError("qweight must be float8_e4m3fn [N, K]")
+        n, k = qweight.shape
+        if wscale.shape != (_blocks(n), _blocks(k)):
+            raise ValueError(f"wscale must be [{_blocks(n)}, {_blocks(k)}], got {tuple(wscale.shape)}")
+        if k % 16 == 0 and qweight.is_contiguous() and qweight.data_ptr() % 16 == 0:
+            self.qweight = qweight
+        else:  # a checkpoint's rows, laid out once as the linear reads them
+            self.qweight = _new_codes(n, k, qweight.device)
+            self.qweight.copy_(qweight)
+        self.wscale = wscale.float().contiguous()
+        self.bias = None if bias is None else bias.float().contiguous()
+
+    @classmethod
+    def from_float(cls, weight: torch.Tensor, bias: torch.Tensor | None = None) -> "Fp8BlockLinear":
+        return cls(*quantize_weight_blocks(weight), bias)
+
+    @property
+    def out_features(self) -> int:
+        return self.qweight.shape[0]
+
+    @property
+    def in_features(self) -> int:
+        return self.qweight.shape[1]
+
+    def __call__(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        if x.dtype not in _DT16 or x.shape[-1] != self.in_features:
+            raise ValueError("x must be float16 or bfloat16 [..., in_features]")
+        q, s = quantize_token_blocks(x.reshape(-1, x.shape[-1]))
+        res = None if residual is None else residual.reshape(-1, self.out_features)
+        out = linear_blocks(q, s, self.qweight, self.wscale, bias=self.bias, residual=res, out_dtype=x.dtype)
+        return out.reshape(*x.shape[:-1], self.out_features)

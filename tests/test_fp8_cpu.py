@@ -1,0 +1,182 @@
+"""Host side of the block-scaled e4m3 path, without a GPU: the numpy oracle
+against torch's e4m3 type, the refusals of the C entries and of the Python
+calls, and the sizes and strides that the calls hand to the C entries."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import fp8 as O
+
+E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def L():
+    from nanopointllm_b200 import _lib
+    return _lib
+
+
+@pytest.fixture
+def F(monkeypatch):
+    """nanopointllm_b200.fp8 on CPU tensors: the device check is off and the
+    C call is written down instead of made."""
+    from nanopointllm_b200 import fp8
+    calls = []
+    monkeypatch.setattr(fp8, "_same_device", lambda *a: None)
+    monkeypatch.setattr(fp8, "_call", lambda fn, device, *args: calls.append((fn.__name__, args)))
+    fp8_calls = calls
+    return fp8, fp8_calls
+
+
+def test_oracle_rounds_as_the_type():
+    table = torch.arange(256, dtype=torch.int16).to(torch.uint8).view(E4M3).float().numpy()
+    fin = table[np.isfinite(table)]
+    np.testing.assert_array_equal(O.round_e4m3(fin), fin)
+    g = np.random.default_rng(0)
+    x = np.concatenate([g.normal(size=4000) * s for s in (1e-3, 0.05, 1.0, 60.0)]).astype(np.float32)
+    pos = np.sort(fin[fin >= 0]).astype(np.float32)
+    x = np.clip(np.concatenate([x, (pos[1:] + pos[:-1]) / 2]), -448, 448)  # ties among them
+    np.testing.assert_array_equal(O.round_e4m3(x), torch.from_numpy(x).to(E4M3).float().numpy())
+    assert (np.abs(O.round_e4m3(x) - x) <= O.half_step_e4m3(x)).all()
+
+
+def _buf(n=1 << 16):
+    b = ctypes.create_string_buffer(n + 16)
+    at = ctypes.addressof(b)
+    return b, at + (-at) % 16
+
+
+def test_c_entries_refuse_bad_arguments(L):
+    keep, p = _buf()
+    arg, bad = L.NPL_ERR_ARG, []
+    q = L.lib.npl_fp8_quant_rows
+    bad += [q(p, 7, 4, 256, 256, p, 256, p, 2, None),       # element type
+            q(p, 1, -1, 256, 256, p, 256, p, 2, None),      # rows
+            q(p, 1, 4, 0, 256, p, 256, p, 2, None),         # columns
+            q(p, 1, 4, 256, 255, p, 256, p, 2, None),       # rows that overlap
+            q(p, 1, 4, 256, 256, p, 255, p, 2, None),       # code stride
+            q(p, 1, 4, 256, 256, p, 256, p, 1, None),       # scale stride
+            q(None, 1, 4, 256, 256, p, 256, p, 2, None), q(p, 1, 4, 256, 256, None, 256, p, 2, None),
+            q(p, 1, 4, 256, 256, p, 256, None, 2, None),
+            q(p + 1, 1, 4, 256, 256, p, 256, p, 2, None),   # alignment of the elements
+            q(p, 1, 4, 256, 256, p, 256, p + 2, 2, None),
+            q(p, 1, 1 << 40, 256, 256, p, 256, p, 2, None), q(p, 1, 4, 1 << 40, 1 << 40, p, 1 << 40, p, 1 << 33, None)]
+    w = L.lib.npl_fp8_quant_weight
+    bad += [w(p, 9, 4, 256, 256, p, 256, p, 2, None), w(p, 1, 4, 256, 200, p, 256, p, 2, None)]
+    r = L.lib.npl_fp8_rmsnorm_quant
+    ok = dict(x=p, ldx=256, res=p, ldr=256, w=p, dt=1, eps=1e-6, rows=4, cols=256, so=p, lds=256, q=p, ldq=256, s=p,
+              ldsc=2, st=None)
+    for change in (dict(dt=0), dict(res=None), dict(so=None), dict(w=None), dict(ldr=255), dict(lds=1), dict(ldx=2)):
+        bad.append(r(*{**ok, **change}.values()))
+    s = L.lib.npl_fp8_silu_mul_quant
+    bad += [s(p, 256, p, 256, 0, 4, 256, p, 256, p, 2, None), s(p, 100, p, 256, 1, 4, 256, p, 256, p, 2, None),
+            s(p, 256, None, 256, 1, 4, 256, p, 256, p, 2, None)]
+    lin = L.lib.npl_fp8_linear
+    ok = dict(qa=p, lda=256, sa=p, ldsa=2, qw=p, ldw=256, sw=p, ldsw=2, bias=None, M=4, N=8, K=256, res=None, ldr=0,
+              out=p, ldo=8, dt=1, st=None)
+    for change in (dict(M=-1), dict(N=0), dict(K=0), dict(K=1 << 40), dict(qa=p + 8), dict(qw=p + 1), dict(lda=264),
+                   dict(ldw=250), dict(lda=240), dict(ldsa=1), dict(ldsw=1), dict(dt=0), dict(ldo=7),
+                   dict(res=p, ldr=7), dict(out=p + 1), dict(bias=p + 2), dict(out=None), dict(sw=None)):
+        bad.append(lin(*{**ok, **change}.values()))
+    assert bad == [arg] * len(bad), bad
+    assert b"npl_fp8_linear" in L.lib.npl_last_error_string()
+    # no rows: nothing to launch, no device needed
+    assert lin(*{**ok, "M": 0, "qa": None, "sa": None, "out": None}.values()) == L.NPL_OK
+    assert q(None, 1, 0, 256, 256, None, 256, None, 2, None) == L.NPL_OK
+
+
+def test_cpu_tensors_are_refused():
+    from nanopointllm_b200 import fp8
+    with pytest.raises(ValueError, match="CUDA"):
+        fp8.quantize_token_blocks(torch.zeros(2, 128, dtype=torch.float16))
+
+
+def test_quantiser_layouts(F):
+    f, calls = F
+    x = torch.zeros(6, 301, dtype=torch.float16)
+    q, s = f.quantize_token_blocks(x[:, 1:301])  # strided rows go as they are
+    name, a = calls.pop()
+    assert name == "npl_fp8_quant_rows" and a[1:5] == (f.L.NPL_F16, 6, 300, 301) and a[6] == 304 and a[8] == 3
+    assert q.shape == (6, 300) and q.stride(0) == 304 and s.shape == (6, 3)
+    q, s = f.quantize_token_blocks(torch.zeros(2, 3, 256).transpose(0, 1))
+    assert q.shape == (3, 2, 256) and s.shape == (3, 2, 2)
+    assert calls.pop()[1][1:5] == (f.L.NPL_F32, 6, 256, 256)
+    q, s = f.quantize_token_blocks(torch.zeros(1, 256, dtype=torch.bfloat16).expand(4, 256))  # broadcast rows
+    assert calls.pop()[1][4] == 256
+    q, s = f.quantize_token_blocks(torch.zeros(0, 200, dtype=torch.float16))
+    assert not calls and q.shape == (0, 200) and s.shape == (0, 2)
+    q, s = f.quantize_token_blocks(torch.zeros(0, 3, 200, dtype=torch.float16))
+    assert not calls and q.shape == (0, 3, 200) and s.shape == (0, 3, 2)
+    q, s = f.quantize_token_blocks(torch.zeros(7, 1, dtype=torch.float16))
+    assert q.shape == (7, 1) and s.shape == (7, 1) and calls.pop()[1][2:4] == (7, 1)
+    y = torch.zeros(5, 400, dtype=torch.float16)
+    f.silu_mul_quant_blocks(y[:, :200], y[:, 200:])
+    a = calls.pop()[1]
+    assert a[1] == a[3] == 400 and a[2] - a[0] == 400 and a[5:7] == (5, 200)
+
+
+def test_refusals_of_the_python_calls(F):
+    f, calls = F
+    h = torch.float16
+    x, w = torch.zeros(4, 256, dtype=h), torch.ones(256, dtype=h)
+    qa, sa = torch.zeros(4, 256).to(E4M3), torch.ones(4, 2)
+    qw, sw = torch.zeros(100, 256).to(E4M3), torch.ones(1, 2)
+    flat = torch.zeros(4096, dtype=h)
+    bad = [
+        lambda: f.quantize_token_blocks(torch.zeros(4, 0)),
+        lambda: f.quantize_token_blocks(torch.zeros(4, 8, dtype=torch.int8)),
+        lambda: f.quantize_token_blocks(torch.zeros(())),
+        lambda: f.quantize_weight_blocks(torch.zeros(256)),
+        lambda: f.quantize_weight_blocks(torch.zeros(0, 256)),
+        lambda: f.rmsnorm_quant_blocks(x.float(), w, 1e-6),
+        lambda: f.rmsnorm_quant_blocks(x, w[:128], 1e-6),
+        lambda: f.rmsnorm_quant_blocks(x, w.bfloat16(), 1e-6),
+        lambda: f.rmsnorm_quant_blocks(x, w, 1e-6, x[:3]),
+        lambda: f.rmsnorm_quant_blocks(x, w, 1e-6, sum_out=x),
+        lambda: f.rmsnorm_quant_blocks(x, w, 1e-6, x, sum_out=torch.zeros(256, 4, dtype=h).t()),
+        # a sum that overlaps its inputs without being one of them
+        lambda: f.rmsnorm_quant_blocks(flat[:1024].view(4, 256), w, 1e-6, x, sum_out=flat[8:1032].view(4, 256)),
+        lambda: f.silu_mul_quant_blocks(x, x[:, :128]),
+        lambda: f.silu_mul_quant_blocks(x.float(), x.float()),
+        lambda: f.linear_blocks(qa.float(), sa, qw, sw),
+        lambda: f.linear_blocks(qa, sa, qw[:, :128], sw),
+        lambda: f.linear_blocks(qa, sa[:, :1], qw, sw),
+        lambda: f.linear_blocks(qa, sa.double(), qw, sw),
+        lambda: f.linear_blocks(qa, sa, qw, sw, out_dtype=torch.float32),
+        lambda: f.linear_blocks(qa, sa, qw, sw, bias=torch.zeros(100, dtype=h)),
+        lambda: f.linear_blocks(qa, sa, qw, sw, bias=torch.zeros(99)),
+        lambda: f.linear_blocks(qa, sa, qw, sw, residual=torch.zeros(4, 99, dtype=h)),
+        lambda: f.linear_blocks(qa, sa, qw, sw, residual=torch.zeros(4, 100, dtype=h), out_dtype=torch.bfloat16),
+        lambda: f.linear_blocks(qa, sa, qw, sw, out=torch.zeros(100, 4, dtype=h).t()),
+        lambda: f.linear_blocks(torch.zeros(4, 264).to(E4M3)[:, 8:], sa, qw, sw),       # rows off 16 bytes
+        lambda: f.linear_blocks(torch.zeros(4, 260).to(E4M3)[:, :256], sa, qw, sw),     # stride off 16 bytes
+        lambda: f.linear_blocks(qa, sa, qw, sw, residual=flat[:400].view(4, 100), out=flat[8:408].view(4, 100)),
+        lambda: f.Fp8BlockLinear(qw, torch.ones(2, 2)),
+        lambda: f.Fp8BlockLinear(qw.float(), sw),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    assert not calls
+    # what is allowed: the residual in place, an output with a row stride, an odd K
+    res = torch.zeros(4, 100, dtype=h)
+    assert f.linear_blocks(qa, sa, qw, sw, residual=res, out=res) is res
+    wide = torch.zeros(4, 128, dtype=torch.bfloat16)
+    assert f.linear_blocks(qa, sa, qw, sw, out=wide[:, :100]).dtype == torch.bfloat16
+    assert calls[-1][1][-2] == 128
+    odd = f._new_codes(1, 77, torch.device("cpu"))
+    f.linear_blocks(odd, torch.ones(1, 1), f._new_codes(9, 77, torch.device("cpu")), torch.ones(1, 1))
+    assert calls[-1][1][1] == 80 and calls[-1][1][5] == 80 and calls[-1][1][9:12] == (1, 9, 77)
+
+
+def test_block_linear_lays_out_checkpoint_rows():
+    from nanopointllm_b200 import fp8
+    codes = torch.randn(10, 77).to(E4M3)
+    lin = fp8.Fp8BlockLinear(codes, torch.ones(1, 1))
+    assert lin.qweight.stride(0) == 80 and torch.equal(lin.qweight.float(), codes.float())
+    assert (lin.in_features, lin.out_features) == (77, 10)

@@ -1,0 +1,427 @@
+"""The block-scaled e4m3 kernels against the numpy oracle in 64 bits.
+
+Tolerances. The quantisers' own fp32 steps on given values are fixed, so
+tokens and weights are compared bit for bit. Behind RMSNorm and SiLU * up the
+fp32 values differ from the exact ones: by VAL = 2^-18 relative (RMSNorm: an
+fp32 sum of squares in chains of at most 64 additions, 64 * 2^-24 = 2^-18,
+halved by the square root, and five more roundings of 2^-24; SiLU: 1 + e^-g
+within 2 ulps, three more roundings); so a scale is within VAL + 2^-23, and a
+code within half a step of its exact quotient plus 2 VAL of it.
+Linear: every fp32 addition is off by at most 2^-23 of the running magnitude
+(2^-24 if it rounds to nearest; tensor cores may truncate), 128 inside a block
+and one more for each block, rank, bias and residual, so an output is within
+(128 + blocks + 12) * 2^-23 of the sum of magnitudes, and then half a step of
+its type. Sums that are exact in fp32 are compared bit for bit.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import fp8 as O
+
+pytestmark = pytest.mark.gpu
+
+E4M3 = torch.float8_e4m3fn
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+VAL = 2.0 ** -18
+
+
+@pytest.fixture(scope="module")
+def F(cuda_device):
+    from nanopointllm_b200 import fp8
+    return fp8
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    from nanopointllm_b200 import _lib
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+
+
+def cpu(t: torch.Tensor) -> np.ndarray:
+    return t.detach().float().cpu().numpy()
+
+
+def rand(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g) * scale
+    x[..., ::37] *= 20
+    return x.to(dtype)
+
+
+def laid_out(t: torch.Tensor, how: str, dev) -> torch.Tensor:
+    """The same values on the GPU: contiguous, with a row stride, or with rows
+    that start one element off any alignment."""
+    t = t.to(dev)
+    if how == "contiguous":
+        return t
+    pad = {"strided": (0, 24), "unaligned": (1, 2)}[how]
+    wide = torch.full((t.shape[0], t.shape[1] + sum(pad)), 7.0, dtype=t.dtype, device=dev)
+    wide[:, pad[0]:pad[0] + t.shape[1]] = t
+    return wide[:, pad[0]:pad[0] + t.shape[1]]
+
+
+SHAPES = [(1, 1), (1, 128), (3, 129), (5, 100), (7, 1000), (8, 4096), (33, 520), (300, 264)]
+
+
+@pytest.mark.parametrize("how", ["contiguous", "strided", "unaligned"])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_tokens(F, cuda_device, m, k, dtype, how):
+    x = rand((m, k), dtype, m * 1009 + k)
+    if m > 3:
+        x[2] = 0
+    q, s = F.quantize_token_blocks(laid_out(x, how, cuda_device))
+    oq, os = O.quant_fp32(cpu(x), 1)
+    assert q.dtype == E4M3 and q.shape == (m, k) and s.dtype == F32
+    np.testing.assert_array_equal(cpu(s), os)
+    np.testing.assert_array_equal(cpu(q), oq)
+
+
+@pytest.mark.parametrize("how", ["contiguous", "unaligned"])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("n,k", [(1, 1), (128, 128), (129, 257), (100, 1000), (1000, 512), (64, 4096)])
+def test_weight(F, cuda_device, n, k, dtype, how):
+    w = rand((n, k), dtype, n * 31 + k, 0.02)
+    q, s = F.quantize_weight_blocks(laid_out(w, how, cuda_device))
+    oq, os = O.quant_fp32(cpu(w), 128)
+    assert s.shape == (-(-n // 128), -(-k // 128))
+    np.testing.assert_array_equal(cpu(s), os)
+    np.testing.assert_array_equal(cpu(q), oq)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_extreme_blocks(F, cuda_device, dtype):
+    """The type's largest and smallest values, zeros of both signs, and blocks
+    that hold a NaN or an infinity, which alone read back as NaN."""
+    big, tiny = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal
+    x = rand((10, 384), dtype, 5)
+    x[0, :128] = 0.0
+    x[1, :128] = -0.0
+    x[2, 5] = big
+    x[3, :128] = tiny / 4 if dtype != F32 else tiny
+    x[4, :128], x[4, 7] = 0.0, tiny
+    x[5, 130] = float("nan")
+    x[6, 131] = float("inf")
+    x[7, 132] = float("-inf")
+    x[8, 256:] = float("inf")
+    x[9] = big
+    q, s = (cpu(t) for t in F.quantize_token_blocks(x.to(cuda_device)))
+    with np.errstate(all="ignore"):
+        oq, os = O.quant_fp32(cpu(x), 1)
+        vals = q * O.spread(s, 1, q.shape)
+    bad = np.zeros_like(vals, dtype=bool)
+    bad[5:8, 128:256] = True
+    bad[8, 256:] = True
+    assert np.isnan(vals[bad]).all() and np.isfinite(vals[~bad]).all()
+    np.testing.assert_array_equal(q[~bad], oq[~bad])
+    np.testing.assert_array_equal(s[:5], os[:5])
+    w, _ = F.quantize_weight_blocks(x[:5].to(cuda_device))
+    np.testing.assert_array_equal(cpu(w), O.quant_fp32(cpu(x[:5]), 128)[0])
+
+
+def check_codes(q, s, v, rows=1):
+    es = O.block_scales(v, rows)
+    np.testing.assert_allclose(cpu(s), es, rtol=VAL + 2.0 ** -23, atol=0)
+    want = v / O.spread(es, rows, v.shape)
+    off = np.abs(cpu(q) - want)
+    assert (off <= O.half_step_e4m3(want) + 2 * VAL * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("how", ["contiguous", "strided", "unaligned"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("m,k", SHAPES + [(2, 5000), (3, 11008), (2, 16384), (2, 20000), (1, 33000)])
+def test_rmsnorm(F, cuda_device, m, k, residual, dtype, how):
+    x, r = rand((m, k), dtype, m + k), rand((m, k), dtype, m + k + 1)
+    w = (1 + 0.1 * rand((1, k), F32, k)[0]).to(dtype)
+    if m > 3:
+        x[1], r[1] = 0, 0
+    xd = laid_out(x, how, cuda_device)
+    rd = laid_out(r, how, cuda_device) if residual else None
+    q, s, total = F.rmsnorm_quant_blocks(xd, w.to(cuda_device), 1e-6, rd)
+    t = (x.float() + r.float()).to(dtype) if residual else x
+    if residual:
+        assert torch.equal(total.cpu(), t)
+    else:
+        assert total is None
+    check_codes(q, s, O.rmsnorm(cpu(t), cpu(w), 1e-6))
+
+
+@pytest.mark.parametrize("k", [256, 4096, 20000])
+def test_rmsnorm_in_place(F, cuda_device, k):
+    """The sum in place of x or of the residual, rows past the batch untouched."""
+    x, r = rand((6, k), BF16, 1).to(cuda_device), rand((6, k), BF16, 2).to(cuda_device)
+    w = torch.ones(k, dtype=BF16, device=cuda_device)
+    q0, s0, t0 = F.rmsnorm_quant_blocks(x[:4], w, 1e-6, r[:4])
+    for into in (0, 1):
+        a, b = x.clone(), r.clone()
+        tgt = (a, b)[into][:4]
+        xs, rs = (tgt, b[:4]) if into == 0 else (a[:4], tgt)
+        q, s, t = F.rmsnorm_quant_blocks(xs, w, 1e-6, rs, sum_out=tgt)
+        assert t is tgt and torch.equal(t, t0) and torch.equal(s, s0) and torch.equal(q.float(), q0.float())
+        assert torch.equal(a[4:], x[4:]) and torch.equal(b[4:], r[4:])
+
+
+@pytest.mark.parametrize("how", ["contiguous", "strided", "unaligned"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m,k", SHAPES + [(3, 11008)])
+def test_silu_mul(F, cuda_device, m, k, dtype, how):
+    g, u = rand((m, k), dtype, m + 2 * k), rand((m, k), dtype, m + 2 * k + 1)
+    q, s = F.silu_mul_quant_blocks(laid_out(g, how, cuda_device), laid_out(u, how, cuda_device))
+    check_codes(q, s, O.silu_mul(cpu(g), cpu(u)))
+
+
+def test_silu_far_gates(F, cuda_device):
+    """Gates whose e^-g overflows or vanishes in fp32, and infinite ones."""
+    g = torch.tensor([-3e4, -120.0, -89.0, -88.0, -20.0, 0.0, 20.0, 89.0, 3e4], dtype=F16)
+    g = g.repeat(15)[:128].reshape(1, 128)
+    u = rand((1, 128), F16, 3)
+    q, s = F.silu_mul_quant_blocks(g.to(cuda_device), u.to(cuda_device))
+    check_codes(q, s, O.silu_mul(cpu(g), cpu(u)))
+    g = torch.zeros(1, 256, dtype=F16)
+    g[0, 3], g[0, 200] = float("-inf"), 1.0
+    q, s = F.silu_mul_quant_blocks(g.to(cuda_device), torch.ones(1, 256, dtype=F16, device=cuda_device))
+    vals = cpu(q) * np.repeat(cpu(s), 128, 1)
+    assert np.isnan(vals[0, :128]).all() and np.isfinite(vals[0, 128:]).all()
+
+
+def test_guarded_outputs(F, cuda_device):
+    """The C entries write their rows and columns and nothing around them."""
+    from nanopointllm_b200 import _lib as L
+    m, k, ld = 5, 300, 320
+    x = rand((m, k), F16, 9).to(cuda_device)
+    w = torch.ones(k, dtype=F16, device=cuda_device)
+    st = L.stream_ptr(cuda_device)
+
+    def guarded(call):
+        q = torch.full((m + 2, ld), 0x55, dtype=torch.uint8, device=cuda_device)
+        s = torch.full((m + 2, 5), 3.25, device=cuda_device)
+        L.check(call(q[1:], s[1:]))
+        torch.cuda.synchronize()
+        inner = torch.zeros_like(q, dtype=torch.bool)
+        inner[1:m + 1, :k] = True
+        assert (q[~inner] == 0x55).all()
+        return q[1:m + 1, :k].view(E4M3), s
+
+    q, s = guarded(lambda q, s: L.lib.npl_fp8_quant_rows(x.data_ptr(), L.NPL_F16, m, k, k, q.data_ptr(), ld,
+                                                         s.data_ptr(), 5, st))
+    assert (s[0] == 3.25).all() and (s[m + 1] == 3.25).all() and (s[1:m + 1, 3:] == 3.25).all()
+    np.testing.assert_array_equal(cpu(q), O.quant_fp32(cpu(x), 1)[0])
+    guarded(lambda q, s: L.lib.npl_fp8_silu_mul_quant(x.data_ptr(), k, x.data_ptr(), k, L.NPL_F16, m, k, q.data_ptr(),
+                                                      ld, s.data_ptr(), 5, st))
+    guarded(lambda q, s: L.lib.npl_fp8_rmsnorm_quant(x.data_ptr(), k, None, 0, w.data_ptr(), L.NPL_F16, 1e-6, m, k,
+                                                     None, 0, q.data_ptr(), ld, s.data_ptr(), 5, st))
+    q, s = guarded(lambda q, s: L.lib.npl_fp8_quant_weight(x.data_ptr(), L.NPL_F16, m, k, k, q.data_ptr(), ld,
+                                                           s.data_ptr(), 5, st))
+    assert (s[2:] == 3.25).all() and (s[1, 3:] == 3.25).all()
+
+
+# ------------------------------------------------------------------- linear
+def codes(rows, k, seed, dev, top=4):
+    """Random small whole codes, rows on 16-byte boundaries."""
+    g = torch.Generator().manual_seed(seed)
+    v = torch.randint(-top, top + 1, (rows, k), generator=g).float()
+    store = torch.zeros(rows, -(-k // 16) * 16, dtype=E4M3, device=dev)
+    store[:, :k] = v.to(dev).to(E4M3)
+    return store[:, :k]
+
+
+def powers(rows, cols, seed, dev, lo=-2, hi=1):
+    g = torch.Generator().manual_seed(seed)
+    return (2.0 ** torch.randint(lo, hi, (rows, cols), generator=g).float()).to(dev)
+
+
+LINEAR_SHAPES = [
+    (1, 1, 1), (1, 8, 16), (2, 128, 128), (8, 1000, 512), (1, 4096, 1408), (16, 100, 77), (17, 129, 129),
+    (33, 300, 640), (64, 1003, 500), (65, 257, 384), (128, 128, 256), (129, 513, 1000), (200, 640, 4096),
+    (300, 264, 132), (513, 520, 896), (1000, 1001, 272), (2100, 700, 300),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m,n,k", LINEAR_SHAPES)
+def test_linear_exact_sums(F, cuda_device, m, n, k, dtype):
+    """Whole codes under power-of-two scales: every partial sum is exact in
+    fp32 (terms are multiples of 2^-4 and sum to at most 16 K < 2^17), so the
+    result is the exact sum rounded once, whatever the order."""
+    kb, nb = -(-k // 128), -(-n // 128)
+    qa, qw = codes(m, k, 1, cuda_device), codes(n, k, 2, cuda_device)
+    sa, sw = powers(m, kb, 3, cuda_device), powers(nb, kb, 4, cuda_device)
+    bias = torch.randint(-3, 4, (n,), generator=torch.Generator().manual_seed(5)).float()
+    res = torch.randint(-9, 10, (m, n), generator=torch.Generator().manual_seed(6)).to(dtype)
+    for b, r in ((None, None), (bias, None), (bias, res)):
+        out = F.linear_blocks(qa, sa, qw, sw, bias=None if b is None else b.to(cuda_device),
+                              residual=None if r is None else r.to(cuda_device), out_dtype=dtype)
+        want, _ = O.linear(cpu(qa), cpu(sa), cpu(qw), cpu(sw), None if b is None else b.numpy(),
+                           None if r is None else cpu(r))
+        assert out.shape == (m, n) and out.dtype == dtype
+        assert torch.equal(out.cpu(), torch.from_numpy(want).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (8, 12288, 4096), (40, 1000, 11008), (200, 1100, 4100),
+                                   (560, 2000, 1000), (1500, 1300, 2048)])
+def test_linear_random(F, cuda_device, m, n, k, dtype):
+    x = rand((m, k), F32, m + n).to(cuda_device)
+    w = rand((n, k), F32, n + k, 0.02).to(cuda_device)
+    qa, sa = F.quantize_token_blocks(x)
+    qw, sw = F.quantize_weight_blocks(w)
+    res = rand((m, n), dtype, 8).to(cuda_device)
+    bias = rand((1, n), F32, 9)[0].to(cuda_device)
+    out = cpu(F.linear_blocks(qa, sa, qw, sw, bias=bias, residual=res))
+    want, mag = O.linear(cpu(qa), cpu(sa), cpu(qw), cpu(sw), cpu(bias), cpu(res))
+    tol = (128 + -(-k // 128) + 12) * 2.0 ** -23 * mag
+    half = torch.finfo(dtype).eps / 2
+    assert (np.abs(out - want) <= tol + half * (np.abs(want) + tol)).all()
+
+
+def test_linear_layouts(F, cuda_device):
+    """Strided scales, residual and output; the residual in place; columns and
+    rows around the output untouched; odd output strides."""
+    for m, n, k in ((5, 200, 300), (70, 200, 300), (300, 328, 640)):
+        kb, nb = -(-k // 128), -(-n // 128)
+        qa, qw = codes(m, k, 1, cuda_device), codes(n, k, 2, cuda_device)
+        sa, sw = powers(m, kb, 3, cuda_device), powers(nb, kb, 4, cuda_device)
+        res = torch.randint(-9, 10, (m, n), generator=torch.Generator().manual_seed(6)).to(F16).to(cuda_device)
+        want = F.linear_blocks(qa, sa, qw, sw, residual=res)
+        wide = torch.zeros(m, kb + 3, device=cuda_device)
+        wide[:, 1:kb + 1] = sa
+        turned = sw.t().contiguous().t()
+        for off, pad in ((0, 8), (1, 1), (3, 2), (8, 0)):
+            r = torch.full((m + 2, off + n + pad), 5.0, dtype=F16, device=cuda_device)
+            r[1:m + 1, off:off + n] = res
+            o = torch.full((m + 2, off + n + pad), -77.0, dtype=F16, device=cuda_device)
+            inner = torch.zeros_like(o, dtype=torch.bool)
+            inner[1:m + 1, off:off + n] = True
+            view, rv = o[1:m + 1, off:off + n], r[1:m + 1, off:off + n]
+            got = F.linear_blocks(qa, wide[:, 1:kb + 1], qw, turned, residual=rv, out=view)
+            assert got is view and torch.equal(view, want) and (o[~inner] == -77.0).all()
+            F.linear_blocks(qa, sa, qw, sw, residual=rv, out=rv)  # in place
+            assert torch.equal(rv, want) and (r[~inner] == 5.0).all()
+
+
+@pytest.mark.parametrize("m", [3, 70, 300])
+def test_linear_bad_token_stays_in_its_row(F, cuda_device, m):
+    x = rand((m, 512), F16, 1).to(cuda_device)
+    x[1, 200] = float("inf")
+    w = rand((300, 512), F16, 2, 0.02).to(cuda_device)
+    out = F.linear_blocks(*F.quantize_token_blocks(x), *F.quantize_weight_blocks(w), out_dtype=F16)
+    assert out[1].isnan().all() and out[0].isfinite().all() and out[2:].isfinite().all()
+
+
+@pytest.mark.parametrize("m", [1, 8, 64, 65, 300])
+def test_linear_repeats_bit_for_bit(F, cuda_device, m):
+    qa, sa = F.quantize_token_blocks(rand((m, 4096), F16, 1).to(cuda_device))
+    qw, sw = F.quantize_weight_blocks(rand((1000, 4096), F16, 2, 0.02).to(cuda_device))
+    first = F.linear_blocks(qa, sa, qw, sw)
+    for _ in range(20):
+        assert torch.equal(F.linear_blocks(qa, sa, qw, sw), first)
+
+
+def test_no_rows(F, cuda_device):
+    x = torch.zeros(0, 256, dtype=F16, device=cuda_device)
+    q, s = F.quantize_token_blocks(x)
+    w = torch.ones(256, dtype=F16, device=cuda_device)
+    assert F.rmsnorm_quant_blocks(x, w, 1e-6, x)[2].shape == (0, 256)
+    assert F.silu_mul_quant_blocks(x, x)[1].shape == (0, 2)
+    qw, sw = F.quantize_weight_blocks(torch.ones(100, 256, dtype=F16, device=cuda_device))
+    assert F.linear_blocks(q, s, qw, sw).shape == (0, 100)
+
+
+# ------------------------------------------------------------ used together
+def mlp_weights(F, dev, hidden, inter, dtype):
+    gu = rand((2 * inter, hidden), dtype, 11, 0.02).to(dev)
+    dn = rand((hidden, inter), dtype, 12, 0.02).to(dev)
+    nw = (1 + 0.1 * rand((1, hidden), F32, 13)[0]).to(dtype).to(dev)
+    return F.quantize_weight_blocks(gu), F.quantize_weight_blocks(dn), nw
+
+
+def mlp(F, h, delta, nw, gu, dn, inter):
+    """A decoder layer's MLP: the residual's addition and norm, packed gate/up,
+    SiLU * up, down with the residual."""
+    q, s, h = F.rmsnorm_quant_blocks(h, nw, 1e-6, delta)
+    y = F.linear_blocks(q, s, *gu, out_dtype=h.dtype)
+    a, sa = F.silu_mul_quant_blocks(y[:, :inter], y[:, inter:])
+    return F.linear_blocks(a, sa, *dn, residual=h), (q, s, h, y, a, sa)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m,hidden,inter", [(1, 512, 1024), (8, 4096, 1100), (65, 500, 1000), (300, 512, 1376)])
+def test_mlp_block(F, cuda_device, m, hidden, inter, dtype):
+    """The operators of an MLP in a row, each checked in 64 bits on what the
+    one before it gave."""
+    gu, dn, nw = mlp_weights(F, cuda_device, hidden, inter, dtype)
+    h, delta = (rand((m, hidden), dtype, i).to(cuda_device) for i in (1, 2))
+    out, (q, s, total, y, a, sa) = mlp(F, h, delta, nw, gu, dn, inter)
+    half = torch.finfo(dtype).eps / 2
+    check_codes(q, s, O.rmsnorm(cpu(total), cpu(nw), 1e-6))
+    for got, (codes_, scale), w, res in ((y, (q, s), gu, None), (out, (a, sa), dn, cpu(total))):
+        want, mag = O.linear(cpu(codes_), cpu(scale), cpu(w[0]), cpu(w[1]), None, res)
+        tol = (128 + scale.shape[1] + 12) * 2.0 ** -23 * mag
+        assert (np.abs(cpu(got) - want) <= tol + half * (np.abs(want) + tol)).all()
+    check_codes(a, sa, O.silu_mul(cpu(y[:, :inter]), cpu(y[:, inter:])))
+
+
+def test_block_linear_module(F, cuda_device):
+    w = rand((300, 500), F16, 1, 0.02).to(cuda_device)
+    x = rand((6, 500), F16, 2).to(cuda_device).reshape(2, 3, 500)
+    lin = F.Fp8BlockLinear.from_float(w, torch.ones(300, device=cuda_device))
+    out = lin(x)
+    q, s = F.quantize_token_blocks(x.reshape(6, 500))
+    want = F.linear_blocks(q, s, *F.quantize_weight_blocks(w), bias=torch.ones(300, device=cuda_device), out_dtype=F16)
+    assert out.shape == (2, 3, 300) and torch.equal(out.reshape(6, 300), want)
+    assert torch.equal(lin(x, residual=out).reshape(6, 300),
+                       F.linear_blocks(q, s, lin.qweight, lin.wscale, bias=lin.bias, residual=want))
+
+
+@pytest.mark.parametrize("m", [4, 100])
+def test_graphs_and_streams(F, cuda_device, m):
+    """The same chain captured twice, replayed by turns and at once on two
+    streams, on new inputs, gives what the eager calls give."""
+    hidden, inter = 1024, 1408
+    gu, dn, nw = mlp_weights(F, cuda_device, hidden, inter, F16)
+    ins, outs, graphs, streams = [], [], [], []
+    for i in range(2):
+        h, d = (rand((m, hidden), F16, 20 + 2 * i + j).to(cuda_device) for j in (0, 1))
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            mlp(F, h, d, nw, gu, dn, inter)
+        torch.cuda.current_stream().wait_stream(st)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out, _ = mlp(F, h, d, nw, gu, dn, inter)
+        ins.append((h, d)), outs.append(out), graphs.append(g), streams.append(st)
+    for turn in range(3):
+        for i in range(2):
+            for j in range(2):
+                ins[i][j].copy_(rand((m, hidden), F16, 100 * turn + 10 * i + j).to(cuda_device))
+        want = [mlp(F, *ins[i], nw, gu, dn, inter)[0].clone() for i in range(2)]
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], want[i])
+
+
+def test_weight_written_just_before(F, cuda_device):
+    """A weight quantised right before the product that reads it."""
+    qa, sa = F.quantize_token_blocks(rand((8, 2048), F16, 1).to(cuda_device))
+    ws = [rand((4096, 2048), F16, 2 + i, 0.02).to(cuda_device) for i in range(6)]
+    want = []
+    for w in ws:
+        qw, sw = F.quantize_weight_blocks(w)
+        torch.cuda.synchronize()
+        want.append(F.linear_blocks(qa, sa, qw, sw))
+    torch.cuda.synchronize()
+    got = [F.linear_blocks(qa, sa, *F.quantize_weight_blocks(w)) for w in ws]
+    for g, e in zip(got, want):
+        assert torch.equal(g, e)

@@ -304,65 +304,59 @@ __global__ void __launch_bounds__(kThreads)
 // Tokens are the MMA's A rows and weights its N columns here: a thread of the
 // epilogue holds one token, so a block's scale is one value per thread and 128
 // columns (one weight scale), and the update is one packed FMA for two sums.
-// Per CTA (384 threads, one CTA per SM, persistent over 128 x 256 tiles): warp
-// 0 TMA, warp 1 MMA, warps 4-7 and 8-11 the epilogue of 128 columns each, with
-// all of its sums (128 a thread) in registers: the first warpgroup hands most
-// of its registers to the other two. Two 256-column accumulators fill TMEM:
-// the MMAs of a block run while the epilogue adds up the one before.
-constexpr int kPM = 128;   // tokens per tile
+//
+// Two CTAs of a cluster share a tile of 256 tokens x 256 weight rows
+// (cta_group::2): each loads 128 rows of both, CTA 0 issues the MMAs for both,
+// and each holds the accumulator of its 128 tokens. An SM takes in about 58
+// bytes a cycle from L2 (measured), and a block's MMAs run 512 cycles; a CTA
+// of its own with a 128 x 256 tile needs 48 KB for a block and waits for them,
+// one of a pair 32 KB.
+//
+// Per CTA (384 threads, one CTA per SM, persistent): warp 0 TMA, warp 1 MMA,
+// warps 2-3 the scales, two warpgroups the epilogue of 128 columns each, with
+// all of its sums in registers (128 a thread; the first warpgroup hands most
+// of its registers to the other two). Two 256-column accumulators fill TMEM:
+// the MMAs of a block run while the epilogue adds up the one before, so the
+// block's whole round (MMAs, hand-over, TMEM loads, hand-back) has to fit into
+// the time of two blocks' MMAs. What counts there is instructions: four
+// warpgroups of 64 columns spend as many on waiting and scales as on sums.
+// The scales' products go through shared memory, 8 blocks at a time: read by
+// the threads that use them, every load would touch 32 rows, and these loads
+// alone took as long as the MMAs.
+constexpr int kPM = 128;   // tokens per CTA
 constexpr int kPN = 256;   // weight rows per tile
-constexpr int kPThreads = 384;
-// 168 a thread at launch; 48 + 2 * 224 <= 3 * 168
-constexpr int kPRegsFew = 48, kPRegsMany = 224;
-constexpr int kPStages = 4;
-constexpr uint32_t kPStageX = kPM * kBlockK, kPStageW = kPN * kBlockK;
+constexpr int kPGroups = 2;                           // epilogue warpgroups
+constexpr int kPGroupCols = kPN / kPGroups;           // 128: one weight scale
+constexpr int kPThreads = 128 + 128 * kPGroups;
+// 168 a thread at launch (65536 / 384); 56 + 2 * 224 = 3 * 168
+constexpr int kPRegsFew = 56, kPRegsMany = 224;
+constexpr int kPStages = 5;
+constexpr uint32_t kPStageX = kPM * kBlockK, kPStageW = kPN / 2 * kBlockK;
 constexpr uint32_t kPStage = kPStageX + kPStageW;
 constexpr int kPOutCols = 64;                         // columns staged at a time by a warpgroup
 constexpr uint32_t kPOut = kPM * kPOutCols * 2;       // 16 KB
-constexpr int kPSmem = kPStages * (int)kPStage + 2 * (int)kPOut + 1024;
+constexpr int kPScaleBlocks = 8;                      // blocks of scales loaded at a time
+constexpr int kPScaleLd = kPM + 4;                    // 4 (mod 32): 8 blocks x 4 tokens of a warp hit 32 banks
+constexpr int kPSmem = kPStages * (int)kPStage + kPGroups * (int)kPOut + 1024;
 
 struct PrefillCtl {
-  uint64_t full[kPStages];
+  uint64_t full[kPStages];   // CTA 0's: both CTAs' loads of a stage
   uint64_t empty[kPStages];
   uint64_t tfull[2];
-  uint64_t tempty[2];
+  uint64_t tempty[2];        // CTA 0's: both CTAs' epilogue warps
+  uint64_t sfull[2];
+  uint64_t sempty[2];
   uint64_t teardown;
   uint32_t tmem_base;
+  __align__(16) float scale[2][kPGroups][kPScaleBlocks][kPScaleLd];
 };
 
-__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-
-// tcgen05.wait::ld that the loaded registers pass through, so that no use of
-// them can be moved before it.
-__device__ __forceinline__ void tmem_wait_regs(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                 "+r"(r[15])::"memory");
-}
-
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-  return v;
-}
-
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-
-// Two fp32 FMAs in one instruction.
-__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b) {
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+// acc += d * s. Volatile, like tcgen05.ld and its wait: it stays behind the
+// wait for d. (The packed fma.rn.f32x2 has the same rate on B200, 128 FMAs a
+// cycle and SM, and its operand pairs cost moves: 1810 us against 1511 for
+// 16000 x 22016 x 4096.)
+__device__ __forceinline__ void fma_after_ld(float& acc, uint32_t d, float s) {
+  asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(__uint_as_float(d)), "f"(s));
 }
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* smem, int c0, int c1) {
@@ -377,9 +371,72 @@ __device__ __forceinline__ void tma_store_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
+// TMA load into this CTA's shared memory, counted on a barrier of either CTA
+// of the pair (a shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map, int c0, int c1,
+                                                 uint32_t bar_cluster, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint"
+      " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar_cluster), "l"(policy)
+      : "memory");
+}
+
+// The pair's MMA: 256 x N, rows 0-127 in CTA 0's TMEM, the others in CTA 1's.
+template <bool kAccumulate>
+__device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "n"((int)kAccumulate)
+      : "memory");
+}
+
+// One lane of the warp, the same each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
+// Completion of the MMAs issued so far arrives on this barrier in both CTAs.
+__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// One arrival on a barrier of either CTA of the pair. It carries no ordinary
+// memory from CTA to CTA (TMEM reads are ordered by the tcgen05 fences), so it
+// and the waits need no cluster scope, which costs a fence each: with it a
+// block took 1.4 us.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t bar_cluster) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+
+// Byte offset of 16-byte chunk `ch` of row `row` in a staged box of 128-byte
+// rows: the 128-byte swizzle of the output's tensor map.
+__device__ __forceinline__ int staged(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
+
+// mbar_wait bounded by a count of polls (each takes 20 ns or more), without
+// the clock: fewer instructions where every block waits.
+__device__ __forceinline__ bool poll_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+  for (int i = 0; i < (1 << 25); ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  if (status) atomicExch(status, code);
+  return false;
+}
+
 // Tile t -> (token tile, weight tile): groups of raster_g token tiles, the
 // token tile running fastest, so that the tiles in flight at one time share
-// raster_g token tiles and 148 / raster_g weight tiles in L2.
+// raster_g token tiles and 74 / raster_g weight tiles in L2.
 __device__ __forceinline__ void prefill_tile(const Fp8LinearArgs& p, int t, int& m_tile, int& n_tile) {
   const int span = p.raster_g * p.n_tiles;
   const int grp = t / span, r = t - grp * span;
@@ -400,7 +457,7 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kPThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
     fp8_linear_prefill_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                               const __grid_constant__ CUtensorMap tmap_out, const Fp8LinearArgs p) {
   extern __shared__ unsigned char smem_raw[];
@@ -408,10 +465,12 @@ __global__ void __launch_bounds__(kPThreads, 1)
                                                          ~uintptr_t(1023));
   unsigned char* staging = ring + kPStages * kPStage;
   __shared__ PrefillCtl c;
-  constexpr uint32_t kIdesc = idesc_e4m3(kPM, kPN);
+  constexpr uint32_t kIdesc = idesc_e4m3(2 * kPM, kPN);
   constexpr uint32_t kTmemCols = 2 * kPN;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = p.m_tiles * p.n_tiles;
+  const int rank = (int)(blockIdx.x & 1u);
+  const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tmap_x);
@@ -423,17 +482,23 @@ __global__ void __launch_bounds__(kPThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c.tfull[i], 1);
-      mbar_init(&c.tempty[i], 8);
+      mbar_init(&c.tempty[i], 2 * 4 * kPGroups);
+      mbar_init(&c.sfull[i], 64);
+      mbar_init(&c.sempty[i], 4 * kPGroups);
     }
     mbar_init(&c.teardown, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(&c.tmem_base, kTmemCols);
-    tmem_relinquish();
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem_base)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  cluster_arrive_release();  // both CTAs' barriers and TMEM are ready
+  cluster_wait_acquire();
   tc_fence_after();
   const uint32_t tmem_base = c.tmem_base;
   pdl_wait();
@@ -446,7 +511,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
       int stage = 0, loads = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      for (int t = pair; ok && t < tiles; t += pairs) {
         int m_tile, n_tile;
         prefill_tile(p, t, m_tile, n_tile);
         for (int kb = 0; kb < p.k_blocks; ++kb) {
@@ -455,9 +520,10 @@ __global__ void __launch_bounds__(kPThreads, 1)
             break;
           }
           unsigned char* at = ring + (size_t)stage * kPStage;
-          mbar_arrive_expect_tx(&c.full[stage], kPStage);
-          tma_load_2d(at, &tmap_x, kb * kBlockK, m_tile * kPM, &c.full[stage], pol);
-          tma_load_2d(at + kPStageX, &tmap_w, kb * kBlockK, n_tile * kPN, &c.full[stage], pol);
+          if (rank == 0) mbar_arrive_expect_tx(&c.full[stage], 2 * kPStage);
+          const uint32_t bar = cluster_map(&c.full[stage], 0);
+          tma_load_2d_pair(at, &tmap_x, kb * kBlockK, (2 * m_tile + rank) * kPM, bar, pol);
+          tma_load_2d_pair(at + kPStageX, &tmap_w, kb * kBlockK, n_tile * kPN + rank * (kPN / 2), bar, pol);
           loads = min(loads + 1, kPStages);
           if (++stage == kPStages) {
             stage = 0;
@@ -465,103 +531,147 @@ __global__ void __launch_bounds__(kPThreads, 1)
           }
         }
       }
-      for (int i = 0; i < loads; ++i)  // every issued load lands before the ring is released
-        mbar_wait(&c.full[i], i < stage ? phase : phase ^ 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
-    } else if (warp == 1 && lane == 0) {
+      // every load is read by its MMAs (or, where those gave up, has landed)
+      // before the ring is released
+      for (int i = 0; i < loads; ++i) {
+        const uint32_t last = i < stage ? phase : phase ^ 1;
+        if (!mbar_wait(&c.empty[i], last, p.status, NPL_DEV_TIMEOUT_TEARDOWN) && rank == 0)
+          mbar_wait(&c.full[i], last, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+      }
+    } else if (warp == 1) {
+      // The whole warp runs this loop and one lane issues: addresses and
+      // descriptors then stay in uniform registers, which tcgen05.mma reads.
+      // From one lane's branch each is moved there first, and issuing a block
+      // took 650 cycles.
+      const bool issuer = elect_one();
+      const uint64_t desc0 = sdesc_k_sw128(smem_u32(ring));
       int stage = 0;
       uint32_t phase = 0, it = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      bool ok = rank == 0;
+      for (int t = pair; ok && t < tiles; t += pairs) {
         for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
           const uint32_t buf = it & 1;
-          if (!mbar_wait(&c.tempty[buf], ((it >> 1) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA) ||
-              !mbar_wait(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA)) {
+          if (!poll_wait(&c.tempty[buf], ((it >> 1) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA) ||
+              !poll_wait(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a0 = smem_u32(ring + (size_t)stage * kPStage), b0 = a0 + kPStageX;
+          const uint64_t a = desc0 + (uint32_t)stage * (kPStage >> 4), b = a + (kPStageX >> 4);
+          const uint32_t d = tmem_base + buf * kPN;
+          if (issuer) {
+            mma_e4m3_pair<false>(d, a, b, kIdesc);
 #pragma unroll
-          for (int kk = 0; kk < kBlockK / 32; ++kk)
-            mma_e4m3(tmem_base + buf * kPN, sdesc_k_sw128(a0 + kk * 32), sdesc_k_sw128(b0 + kk * 32), kIdesc,
-                     kk > 0 ? 1u : 0u);
-          tc_commit(&c.empty[stage]);
-          tc_commit(&c.tfull[buf]);
+            for (int kk = 1; kk < kBlockK / 32; ++kk) mma_e4m3_pair<true>(d, a + kk * 2, b + kk * 2, kIdesc);
+            tc_commit_pair(&c.tfull[buf]);
+            tc_commit_pair(&c.empty[stage]);
+          }
+          __syncwarp();
           if (++stage == kPStages) {
             stage = 0;
             phase ^= 1;
           }
         }
       }
-      tc_commit(&c.teardown);  // all MMAs complete before TMEM is freed
-      mbar_wait(&c.teardown, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+      // all MMAs complete, in both CTAs' view, before TMEM is freed
+      if (rank == 0 && issuer) tc_commit_pair(&c.teardown);
+      poll_wait(&c.teardown, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+      __syncwarp();
+    } else if (warp >= 2) {
+      // 8 blocks x 4 tokens per load of a warp, transposed into shared memory
+      const int kk = lane & 7, r0 = (warp - 2) * 4 + (lane >> 3);
+      uint32_t chunk = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < tiles; t += pairs) {
+        int m_tile, n_tile;
+        prefill_tile(p, t, m_tile, n_tile);
+        const int m0 = (2 * m_tile + rank) * kPM;
+        const float* sw0 = p.sw + (long long)(2 * n_tile) * p.ld_sw;
+        const bool two = (2 * n_tile + 1) * kTileN < p.N;  // the tile's second half has weight rows
+        for (int kb = kk; kb - kk < p.k_blocks; kb += kPScaleBlocks, ++chunk) {
+          const uint32_t buf = chunk & 1;
+          const bool in = kb < p.k_blocks;
+          const float w0 = in ? sw0[kb] : 0.f, w1 = in && two ? sw0[p.ld_sw + kb] : 0.f;
+          if (!mbar_wait(&c.sempty[buf], ((chunk >> 1) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
+            ok = false;
+            break;
+          }
+#pragma unroll 8
+          for (int r = r0; r < kPM; r += 8) {
+            const float a = (in && m0 + r < p.M) ? p.sa[(long long)(m0 + r) * p.ld_sa + kb] : 0.f;
+            c.scale[buf][0][kk][r] = __fmul_rn(a, w0);
+            c.scale[buf][1][kk][r] = __fmul_rn(a, w1);
+          }
+          mbar_arrive(&c.sfull[buf]);
+        }
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPRegsMany));
     const int group = (warp - 4) >> 2;  // columns [128 group, 128 group + 128) of the tile
     const int row = (warp & 3) * 32 + lane;
-    const bool elected = (int)threadIdx.x == 128 + 128 * group;
+    const bool elected = (threadIdx.x & 127) == 0;
     unsigned char* stg = staging + group * kPOut;
     auto group_bar = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
     const T* res = static_cast<const T*>(p.residual);
     T* out = static_cast<T*>(p.out);
-    uint32_t it = 0;
+    const uint32_t tempty0 = cluster_map(&c.tempty[0], 0), tempty1 = cluster_map(&c.tempty[1], 0);
+    const uint32_t taddr0 = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + group * kPGroupCols;
+    uint32_t it = 0, chunk = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+    for (int t = pair; ok && t < tiles; t += pairs) {
       int m_tile, n_tile;
       prefill_tile(p, t, m_tile, n_tile);
-      const int m = m_tile * kPM + row;
-      const int n0 = n_tile * kPN + group * 128;
-      const bool live = m < p.M && n0 < p.N;
-      const float* sa = p.sa + (live ? (long long)m * p.ld_sa : 0);
-      const float* sw = p.sw + (live ? (long long)(n0 / kTileN) * p.ld_sw : 0);
-      uint64_t acc[64];
+      const int m_base = (2 * m_tile + rank) * kPM, m = m_base + row;
+      const int n0 = n_tile * kPN + group * kPGroupCols;
+      float acc[kPGroupCols];
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = 0;
-      float s_next = live ? __fmul_rn(sa[0], sw[0]) : 0.f;
-      for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-        const uint32_t buf = it & 1;
-        const uint32_t sbits = __float_as_uint(s_next);
-        const uint64_t s2 = pack2(sbits, sbits);
-        if (live && kb + 1 < p.k_blocks) s_next = __fmul_rn(sa[kb + 1], sw[kb + 1]);
-        if (!mbar_wait(&c.tfull[buf], (it >> 1) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + buf * kPN + group * 128;
-        uint32_t d[2][16];
-        tmem_ld_x16(taddr, d[0]);
-        tmem_wait_regs(d[0]);
+      for (int j = 0; j < kPGroupCols; ++j) acc[j] = 0.f;
+      for (int kb = 0; ok && kb < p.k_blocks; kb += kPScaleBlocks, ++chunk) {
+        const uint32_t sbuf = chunk & 1;
+        ok = poll_wait(&c.sfull[sbuf], (chunk >> 1) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
+        const int kn = min(kPScaleBlocks, p.k_blocks - kb);
+        const float* scale = &c.scale[sbuf][group][0][row];
+        for (int kk = 0; ok && kk < kn; ++kk, ++it, scale += kPScaleLd) {
+          const uint32_t buf = it & 1;
+          const float s = *scale;
+          if (!poll_wait(&c.tfull[buf], (it >> 1) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t taddr = taddr0 + buf * kPN;
+          uint32_t d[2][32];
+          tmem_ld_x32(taddr, d[0]);
+          tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          if (q < 7) tmem_ld_x16(taddr + (q + 1) * 16, d[(q + 1) & 1]);
+          for (int q = 0; q < kPGroupCols / 32; ++q) {
+            if (q + 1 < kPGroupCols / 32) tmem_ld_x32(taddr + (q + 1) * 32, d[(q + 1) & 1]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) fma2(acc[q * 8 + j], pack2(d[q & 1][2 * j], d[q & 1][2 * j + 1]), s2);
-          if (q < 7) tmem_wait_regs(d[(q + 1) & 1]);
-          if (q == 6) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&c.tempty[buf]);
+            for (int j = 0; j < 32; ++j) fma_after_ld(acc[q * 32 + j], d[q & 1][j], s);
+            if (q + 1 < kPGroupCols / 32) tmem_wait_ld();
+            if (q + 2 == kPGroupCols / 32) {  // the accumulator is read
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_pair(buf ? tempty1 : tempty0);
+            }
           }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c.sempty[sbuf]);  // the chunk of scales is read
       }
       if (!ok) break;
       // bias, residual, rounding; 64 columns at a time through shared memory
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kPGroupCols / kPOutCols; ++h) {
         const int nh = n0 + h * kPOutCols;
         if (elected) tma_store_wait_read();
         group_bar();  // the staging buffer is free
 #pragma unroll
-        for (int ch = 0; ch < 8; ++ch) {
+        for (int ch = 0; ch < kPOutCols / 8; ++ch) {
           float v[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack2(acc[h * 32 + ch * 4 + j]);
-            v[2 * j] = f.x;
-            v[2 * j + 1] = f.y;
-          }
+          for (int j = 0; j < 8; ++j) v[j] = acc[h * kPOutCols + ch * 8 + j];
           const int n = nh + ch * 8;
           if (p.bias) {
 #pragma unroll
@@ -587,23 +697,22 @@ __global__ void __launch_bounds__(kPThreads, 1)
           o.y = narrow2<T>(v[2], v[3]);
           o.z = narrow2<T>(v[4], v[5]);
           o.w = narrow2<T>(v[6], v[7]);
-          // the 128-byte swizzle of the output's tensor map
-          *reinterpret_cast<uint4*>(stg + row * 128 + ((ch ^ (row & 7)) << 4)) = o;
+          *reinterpret_cast<uint4*>(stg + staged(row, ch)) = o;
         }
         if (p.tma_out) {
           fence_proxy_async_smem();
           group_bar();
-          if (elected && nh < p.N) tma_store_2d(&tmap_out, stg, nh, m_tile * kPM);
+          if (elected && nh < p.N && m_base < p.M) tma_store_2d(&tmap_out, stg, nh, m_base);
         } else {  // rows that TMA cannot store: element by element, 32 columns a warp
           group_bar();
           for (int r = (warp & 3); r < kPM; r += 4) {
-            const long long mr = (long long)m_tile * kPM + r;
+            const long long mr = (long long)m_base + r;
             if (mr >= p.M) break;
 #pragma unroll
             for (int e = lane; e < kPOutCols; e += 32)
               if (nh + e < p.N)
                 out[mr * p.ld_out + nh + e] =
-                    *reinterpret_cast<const T*>(stg + r * 128 + (((e >> 3) ^ (r & 7)) << 4) + (e & 7) * 2);
+                    *reinterpret_cast<const T*>(stg + staged(r, e >> 3) + (e & 7) * 2);
           }
         }
       }
@@ -613,9 +722,11 @@ __global__ void __launch_bounds__(kPThreads, 1)
 
   tc_fence_before();
   __syncthreads();
+  cluster_arrive_release();  // neither CTA's shared memory or TMEM is given up while the pair uses it
+  cluster_wait_acquire();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, kTmemCols);
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
   }
 }
 
@@ -701,23 +812,23 @@ template <typename T>
 int launch_prefill(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
   CUtensorMap tx, tw, to;
   if (int rc = code_map(&tx, o.qa, p.M, o.K, o.lda, kPM)) return rc;
-  if (int rc = code_map(&tw, o.qw, p.N, o.K, o.ldw, kPN)) return rc;
+  if (int rc = code_map(&tw, o.qw, p.N, o.K, o.ldw, kPN / 2)) return rc;
   p.tma_out = aligned16(p.out) && p.ld_out % 8 == 0;
   p.vec_res = aligned16(p.residual) && p.ld_res % 8 == 0;
   to = tx;
   if (p.tma_out)
     if (int rc = out_map(&to, p.out, o.out_dtype, p.M, p.N, p.ld_out)) return rc;
-  p.m_tiles = (p.M + kPM - 1) / kPM;
+  p.m_tiles = (p.M + 2 * kPM - 1) / (2 * kPM);
   p.n_tiles = (p.N + kPN - 1) / kPN;
   const long long tiles = (long long)p.m_tiles * p.n_tiles;
   if (tiles > 1ll << 30)
     return fail(NPL_ERR_UNSUPPORTED, "npl_fp8_linear: M=%d N=%d has too many tiles", p.M, p.N);
-  p.raster_g = std::min(16, p.m_tiles);
+  p.raster_g = std::min(8, p.m_tiles);
   auto kern = fp8_linear_prefill_kernel<T>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPSmem) != cudaSuccess)
     return launch_status("npl_fp8_linear: smem attribute");
-  return launch_pdl("npl_fp8_linear", kern, dim3((unsigned)std::min<long long>(tiles, num_sms())), dim3(kPThreads),
-                    (size_t)kPSmem, st, tx, tw, to, p);
+  return launch_pdl("npl_fp8_linear", kern, dim3(2 * (unsigned)std::min<long long>(tiles, num_sms() / 2)),
+                    dim3(kPThreads), (size_t)kPSmem, st, tx, tw, to, p);
 }
 
 template <typename T>

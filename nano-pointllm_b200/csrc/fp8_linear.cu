@@ -551,8 +551,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
       for (int t = pair; ok && t < tiles; t += pairs) {
         for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
           const uint32_t buf = it & 1;
-          if (!poll_wait(&c.tempty[buf], ((it >> 1) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA) ||
-              !poll_wait(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA)) {
+          if (!poll_wait(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA) ||
+              !poll_wait(&c.tempty[buf], ((it >> 1) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA)) {
             ok = false;
             break;
           }
@@ -642,19 +642,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
           tc_fence_after();
           const uint32_t taddr = taddr0 + buf * kPN;
           uint32_t d[2][32];
-          tmem_ld_x32(taddr, d[0]);
-          tmem_wait_ld();
 #pragma unroll
-          for (int q = 0; q < kPGroupCols / 32; ++q) {
-            if (q + 1 < kPGroupCols / 32) tmem_ld_x32(taddr + (q + 1) * 32, d[(q + 1) & 1]);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) fma_after_ld(acc[q * 32 + j], d[q & 1][j], s);
-            if (q + 1 < kPGroupCols / 32) tmem_wait_ld();
-            if (q + 2 == kPGroupCols / 32) {  // the accumulator is read
+          for (int q = 0; q < kPGroupCols; q += 64) {
+            tmem_ld_x32(taddr + q, d[0]);
+            tmem_ld_x32(taddr + q + 32, d[1]);
+            tmem_wait_ld();
+            if (q + 64 == kPGroupCols) {  // the accumulator is read: its next MMAs may start
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive_pair(buf ? tempty1 : tempty0);
             }
+#pragma unroll
+            for (int j = 0; j < 64; ++j) fma_after_ld(acc[q + j], d[j >> 5][j & 31], s);
           }
         }
         __syncwarp();

@@ -71,29 +71,80 @@ __device__ __forceinline__ void widen8(const Raw8<T>& r, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = to_f32(r.e[i]);
 }
 
-// max that returns NaN when either operand is NaN (fmaxf drops it)
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
+// max |v| is taken on the bit patterns without their sign: they order like the
+// magnitudes, an infinity above every number and a NaN above infinity, so a
+// NaN is never lost. A key is such a pattern, of fp32 or of a 16-bit type.
+template <typename T>
+__device__ __forceinline__ float key_value(uint32_t key);
+template <>
+__device__ __forceinline__ float key_value<float>(uint32_t key) { return __uint_as_float(key); }
+template <>
+__device__ __forceinline__ float key_value<__half>(uint32_t key) {
+  return __half2float(__ushort_as_half((unsigned short)key));
 }
+template <>
+__device__ __forceinline__ float key_value<__nv_bfloat16>(uint32_t key) { return __uint_as_float(key << 16); }
 
-__device__ __forceinline__ float absmax8(const float (&v)[8]) {
-  float a = fabsf(v[0]);
+__device__ __forceinline__ uint32_t key8(const float (&v)[8]) {
+  uint32_t a = __float_as_uint(v[0]) & 0x7fffffffu;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) a = max_nan(a, fabsf(v[i]));
+  for (int i = 1; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);
   return a;
 }
 
-// Over the 16 lanes that share a block; every lane receives the result.
-__device__ __forceinline__ float group_max(float a) {
-#pragma unroll
-  for (int o = kGroup / 2; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-  return a;
+template <typename T>
+__device__ __forceinline__ uint32_t key8(const Raw8<T>& r) {
+  if constexpr (sizeof(T) == 4) {
+    return key8(r.e);
+  } else {  // two 16-bit patterns at a time
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                                __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16);
+  }
+}
+
+__device__ __forceinline__ uint32_t max_xor(uint32_t own, uint32_t sent, int o) {
+  return max(own, __shfl_xor_sync(0xffffffffu, sent, o));
+}
+
+// The largest key of U blocks (1, 2 or 4) over the 16 lanes that share them.
+// Halving the blocks with each exchange costs 4, 4 or 5 shuffles instead of
+// 4 U, and leaves lane l with block own_block<U>(l), whose scale it then works
+// out for the other lanes too.
+template <int U>
+__device__ __forceinline__ int own_block(int lane) { return U == 4 ? (lane >> 2) & 3 : U == 2 ? (lane >> 3) & 1 : 0; }
+
+template <int U>
+__device__ __forceinline__ uint32_t block_key(const uint32_t (&k)[U], int lane) {
+  uint32_t m;
+  if constexpr (U == 4) {
+    const bool hi = lane & 8, mid = lane & 4;
+    const uint32_t a = max_xor(hi ? k[2] : k[0], hi ? k[0] : k[2], 8);
+    const uint32_t b = max_xor(hi ? k[3] : k[1], hi ? k[1] : k[3], 8);
+    m = max_xor(mid ? b : a, mid ? a : b, 4);
+  } else if constexpr (U == 2) {
+    const bool hi = lane & 8;
+    m = max_xor(hi ? k[1] : k[0], hi ? k[0] : k[1], 8);
+    m = max_xor(m, m, 4);
+  } else {
+    m = max_xor(k[0], k[0], 8);
+    m = max_xor(m, m, 4);
+  }
+  m = max_xor(m, m, 2);
+  return max_xor(m, m, 1);
+}
+
+// Block u's value of `v`, held by the lanes whose own_block is u.
+template <int U>
+__device__ __forceinline__ float from_block(float v, int u) {
+  return U == 1 ? v : __shfl_sync(0xffffffffu, v, (int)(threadIdx.x & 16) + u * (kGroup / U));
 }
 
 __device__ __forceinline__ float block_scale(float absmax) {
-  return max_nan(__fdiv_rn(absmax, kE4m3Max), kScaleMin);
+  // absmax >= 0 or NaN: the comparison keeps a NaN
+  const float s = __fdiv_rn(absmax, kE4m3Max);
+  return s < kScaleMin ? kScaleMin : s;
 }
 
 __device__ __forceinline__ uint2 codes8(const float (&v)[8], float inv) {
@@ -121,20 +172,32 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, uint2 q, int n) {
     if (i < n) dst[i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
 }
 
-// Where the quantised values come from.
+// Where the quantised values come from: what a thread loads for its 8 columns,
+// what it keeps of them, their key and the fp32 values.
 template <typename T, bool kVec>
 struct RowSource {  // the row itself
+  using Elem = T;
   using Raw = Raw8<T>;
+  using Kept = Raw8<T>;
   const T* x;
   long long ldx;
   __device__ __forceinline__ Raw load(int row, int col, int n) const { return load8<kVec>(x + row * ldx + col, n); }
-  __device__ __forceinline__ static void values(const Raw& r, float (&v)[8]) { widen8(r, v); }
+  __device__ __forceinline__ static Kept keep(const Raw& r) { return r; }
+  __device__ __forceinline__ static uint32_t key(const Kept& k) { return key8(k); }
+  __device__ __forceinline__ static void values(const Kept& k, float (&v)[8]) { widen8(k, v); }
 };
 
+// silu(g) up = g / (1 + e^-g) up in fp32. With t = e^-|g| <= 1 it is
+// (g < 0 ? g t : g) / (1 + t): nothing overflows, and 1 + t in [1, 2] has a
+// fast reciprocal (1 ulp) without special cases.
 template <typename T, bool kVec>
-struct SiluSource {  // silu(gate) * up = gate / (1 + e^-gate) * up, fp32
+struct SiluSource {
+  using Elem = float;
   struct Raw {
     Raw8<T> g, u;
+  };
+  struct Kept {
+    float v[8];
   };
   const T* gate;
   const T* up;
@@ -142,12 +205,23 @@ struct SiluSource {  // silu(gate) * up = gate / (1 + e^-gate) * up, fp32
   __device__ __forceinline__ Raw load(int row, int col, int n) const {
     return {load8<kVec>(gate + row * ld_gate + col, n), load8<kVec>(up + row * ld_up + col, n)};
   }
-  __device__ __forceinline__ static void values(const Raw& r, float (&v)[8]) {
+  __device__ __forceinline__ static Kept keep(const Raw& r) {
+    Kept k;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float g = to_f32(r.g.e[i]);
-      v[i] = __fmul_rn(__fdiv_rn(g, __fadd_rn(1.0f, expf(-g))), to_f32(r.u.e[i]));
+      const float t = expf(-fabsf(g));
+      float inv;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(__fadd_rn(1.0f, t)));
+      const float num = g >= 0.f ? g : __fmul_rn(g, t);
+      k.v[i] = __fmul_rn(__fmul_rn(num, inv), to_f32(r.u.e[i]));
     }
+    return k;
+  }
+  __device__ __forceinline__ static uint32_t key(const Kept& k) { return key8(k.v); }
+  __device__ __forceinline__ static void values(const Kept& k, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k.v[i];
   }
 };
 
@@ -159,39 +233,56 @@ struct CodeSink {
 };
 
 constexpr int kQuantThreads = 256;
-constexpr int kUnroll = 4;  // blocks per 16-thread group
-constexpr int kNormThreads = 512;
+constexpr int kNormThreads = 1024;
 
-// Blocks are numbered row by row; a CTA takes 16 * kUnroll consecutive ones.
-template <typename Source, bool kVecQ>
-__global__ void __launch_bounds__(kQuantThreads) fp8_quant_kernel(const Source src, const CodeSink out, int rows,
-                                                                  int cols, int k_blocks) {
+// A warp takes 2 U consecutive blocks of a row, each of its two 16-lane groups
+// every other one, all loads before the first store, which the compiler would
+// not move them across. The bound on registers keeps 24 to 40 warps, and 80 KB
+// of loads or more, in flight on an SM.
+template <typename Source, int U, bool kVecQ>
+__global__ void __launch_bounds__(kQuantThreads, sizeof(typename Source::Raw) > 16 ? 3 : 5)
+    fp8_quant_kernel(const Source src, const CodeSink out, int rows, int cols, unsigned spans) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x % kGroup, group = threadIdx.x / kGroup;
-  constexpr int kGroups = kQuantThreads / kGroup;
-  const unsigned total = (unsigned)rows * (unsigned)k_blocks;
+  const int lane = threadIdx.x % kGroup;
+  const unsigned item = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);  // (row, span of 2 U blocks)
+  const int row = (int)(item / spans);
+  if (row >= rows) return;  // whole warps
+  const int kb0 = (int)(item - (unsigned)row * spans) * (2 * U) + (int)(threadIdx.x & 31) / kGroup;
+  const int col0 = kb0 * kBlock + lane * kVecCols;
+  typename Source::Raw raw[U];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const unsigned item = (blockIdx.x * kUnroll + u) * kGroups + group;
-    const bool in = item < total;
-    const int row = in ? (int)(item / (unsigned)k_blocks) : 0;
-    const int kb = (int)(item - (unsigned)row * (unsigned)k_blocks);
-    const int col = kb * kBlock + lane * kVecCols;
-    const int n = in ? min(8, max(0, cols - col)) : 0;
-    const typename Source::Raw raw = src.load(row, n > 0 ? col : 0, n);
+  for (int u = 0; u < U; ++u) {
+    const int col = col0 + u * (2 * kBlock);
+    raw[u] = src.load(row, col < cols ? col : 0, cols - col);
+  }
+  typename Source::Kept kept[U];
+  uint32_t key[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    kept[u] = Source::keep(raw[u]);
+    key[u] = Source::key(kept[u]);
+  }
+  const float s = block_scale(key_value<typename Source::Elem>(block_key<U>(key, lane)));
+  const float inv = __frcp_rn(s);
+  {
+    const int kb = kb0 + 2 * own_block<U>(lane);
+    if (lane % (kGroup / U) == 0 && kb * kBlock < cols) out.scale[row * out.ld_scale + kb] = s;
+  }
+  uint8_t* q = out.q + row * out.ldq;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float inv_u = from_block<U>(inv, u);
+    const int col = col0 + u * (2 * kBlock);
     float v[8];
-    Source::values(raw, v);
-    const float s = block_scale(group_max(absmax8(v)));
-    const uint2 q = codes8(v, __frcp_rn(s));
-    if (n > 0) store_codes<kVecQ>(out.q + row * out.ldq + col, q, n);
-    if (in && lane == 0) out.scale[row * out.ld_scale + kb] = s;
+    Source::values(kept[u], v);
+    if (col < cols) store_codes<kVecQ>(q + col, codes8(v, inv_u), cols - col);
   }
 }
 
 // (x + residual) -> RMSNorm -> codes; one CTA per row. kChunks > 0: the row
-// stays in registers, kChunks * 8 columns a thread; 0: any length, the row is
-// read again for the second half.
+// stays in registers as T, kChunks * 8 columns a thread; 0: any length, the
+// row is read again for the second half.
 template <typename T, int kChunks, bool kVec, bool kVecQ>
 __global__ void __launch_bounds__(kNormThreads)
     fp8_rmsnorm_kernel(const T* x, long long ldx, const T* res, long long ld_res, const T* __restrict__ w, float eps,
@@ -200,25 +291,22 @@ __global__ void __launch_bounds__(kNormThreads)
   pdl_wait();
   pdl_trigger();
   const long long row = blockIdx.x;
+  const int lane = threadIdx.x % kGroup;
   const int step = (int)blockDim.x * kVecCols;
-  const int chunks = kChunks > 0 ? kChunks : (cols + step - 1) / step;
   constexpr int kKeep = kChunks > 0 ? kChunks : 1;
-  float keep[kKeep][8];
+  Raw8<T> keep[kKeep], other[kKeep];
   float ss = 0.f;
-  auto one = [&](int c, float(&v)[8]) {
-    const int col = c * step + (int)threadIdx.x * kVecCols;
-    const int n = min(8, max(0, cols - col));
-    const int at = n > 0 ? col : 0;
-    widen8(load8<kVec>(x + row * ldx + at, n), v);
+  // the sum as it is stored, and its squares: the norm is that of the stored sum
+  auto add = [&](int col, Raw8<T>& t, const Raw8<T>& r) {
+    const int n = cols - col;
+    float v[8];
+    widen8(t, v);
     if (res) {
-      float r[8];
-      widen8(load8<kVec>(res + row * ld_res + at, n), r);
-      Raw8<T> t;
+      float rv[8];
+      widen8(r, rv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {  // rounded as it is stored: the norm is that of the stored sum
-        t.e[i] = from_f32<T>(__fadd_rn(v[i], r[i]));
-        v[i] = to_f32(t.e[i]);
-      }
+      for (int i = 0; i < 8; ++i) t.e[i] = from_f32<T>(__fadd_rn(v[i], rv[i]));
+      widen8(t, v);
       if (kVec && n >= 8) {
         *reinterpret_cast<uint4*>(sum_out + row * ld_sum + col) = *reinterpret_cast<const uint4*>(&t);
       } else {
@@ -230,49 +318,74 @@ __global__ void __launch_bounds__(kNormThreads)
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = __fmaf_rn(v[i], v[i], ss);
   };
+  auto fetch = [&](const T* p, long long ld, int col) {
+    return load8<kVec>(p + row * ld + (col < cols ? col : 0), cols - col);
+  };
+  const int col0 = (int)threadIdx.x * kVecCols;
   if constexpr (kChunks > 0) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) one(c, keep[c]);
-  } else {
-    for (int c = 0; c < chunks; ++c) one(c, keep[0]);
-  }
-  ss = block_sum(ss, red);
-  const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)cols), eps)));
-  // The second reading takes the stored sum where there is one: it may have
-  // replaced x or the residual.
-  const T* again = res ? sum_out + row * ld_sum : x + row * ldx;
-#pragma unroll
-  for (int c = 0; c < chunks; ++c) {
-    const int col = c * step + (int)threadIdx.x * kVecCols;
-    const int n = min(8, max(0, cols - col));
-    const int at = n > 0 ? col : 0;
-    float v[8], wv[8];
-    widen8(load8<kVec>(w + at, n), wv);
-    if constexpr (kChunks > 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = keep[c][i];
-    } else {
-      widen8(load8<kVec>(again + at, n), v);
+    for (int c = 0; c < kChunks; ++c) {
+      keep[c] = fetch(x, ldx, col0 + c * step);
+      if (res) other[c] = fetch(res, ld_res, col0 + c * step);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn(v[i], r), wv[i]);
-    const float s = block_scale(group_max(absmax8(v)));
-    const uint2 q = codes8(v, __frcp_rn(s));
-    if (n > 0) {
-      store_codes<kVecQ>(out.q + row * out.ldq + col, q, n);
-      if (threadIdx.x % kGroup == 0) out.scale[row * out.ld_scale + col / kBlock] = s;
+    for (int c = 0; c < kChunks; ++c) add(col0 + c * step, keep[c], other[c]);
+  } else {
+    for (int col = col0; col < cols; col += step) {
+      keep[0] = fetch(x, ldx, col);
+      if (res) other[0] = fetch(res, ld_res, col);
+      add(col, keep[0], other[0]);
+    }
+  }
+  if constexpr (kChunks > 0) {  // the norm's weights, on their way while the sums are joined
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) other[c] = fetch(w, 0, col0 + c * step);
+  }
+  ss = warp_sum(ss);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
+  __syncthreads();
+  ss = warp_sum((threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0.f);
+  const float r = rsqrtf(__fadd_rn(__fdividef(ss, (float)cols), eps));  // both within 2 ulps
+  // kChunks blocks at a time; the second reading takes the stored sum where
+  // there is one: it may have replaced x or the residual
+  for (int base = 0; base < cols; base += kKeep * step) {
+    float v[kKeep][8];
+    uint32_t key[kKeep];
+#pragma unroll
+    for (int c = 0; c < kKeep; ++c) {
+      if constexpr (kChunks == 0) {
+        keep[0] = res ? fetch(sum_out, ld_sum, base + col0) : fetch(x, ldx, base + col0);
+        other[0] = fetch(w, 0, base + col0);
+      }
+      float wv[8];
+      widen8(keep[c], v[c]);
+      widen8(other[c], wv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[c][i] = __fmul_rn(__fmul_rn(v[c][i], r), wv[i]);
+      key[c] = key8(v[c]);
+    }
+    const float s = block_scale(__uint_as_float(block_key<kKeep>(key, lane)));
+    const float inv = __frcp_rn(s);
+#pragma unroll
+    for (int c = 0; c < kKeep; ++c) {
+      const float inv_c = from_block<kKeep>(inv, c);
+      const int col = base + col0 + c * step;
+      if (col < cols) store_codes<kVecQ>(out.q + row * out.ldq + col, codes8(v[c], inv_c), cols - col);
+      if (lane == c * (kGroup / kKeep) && col - lane * kVecCols < cols)
+        out.scale[row * out.ld_scale + col / kBlock] = s;
     }
   }
 }
 
-// One 128 x 128 weight block per CTA: 16 threads across, 16 rows at a time,
+// One 128 x 128 weight block per CTA: 16 threads across, 32 rows at a time,
 // the block held in registers between its maximum and its codes.
-constexpr int kWeightRows = kQuantThreads / kGroup;
+constexpr int kWeightThreads = 512;
+constexpr int kWeightRows = kWeightThreads / kGroup;
 
 template <typename T, bool kVec, bool kVecQ>
-__global__ void __launch_bounds__(kQuantThreads) fp8_quant_weight_kernel(const T* __restrict__ w, long long ldw,
+__global__ void __launch_bounds__(kWeightThreads) fp8_quant_weight_kernel(const T* __restrict__ w, long long ldw,
                                                                          int rows, int cols, const CodeSink out) {
-  __shared__ float red[32];
+  __shared__ uint32_t red[kWeightThreads / 32];
   pdl_wait();
   constexpr int kSteps = kBlock / kWeightRows;
   const int nb = blockIdx.x, kb = blockIdx.y;
@@ -286,21 +399,14 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_quant_weight_kernel(const T
     const bool in = row < rows && n > 0;
     raw[i] = load8<kVec>(w + (in ? (long long)row * ldw + col : 0), in ? n : 0);
   }
-  float a = 0.f;
+  uint32_t a = 0;
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    float v[8];
-    widen8(raw[i], v);
-    a = max_nan(a, absmax8(v));
-  }
-  a = group_max(a);
-  a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 16));
+  for (int i = 0; i < kSteps; ++i) a = max(a, key8(raw[i]));
+  a = __reduce_max_sync(0xffffffffu, a);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
   __syncthreads();
-  a = red[0];
-#pragma unroll
-  for (int i = 1; i < kQuantThreads / 32; ++i) a = max_nan(a, red[i]);
-  const float s = block_scale(a);
+  a = __reduce_max_sync(0xffffffffu, red[threadIdx.x & (kWeightThreads / 32 - 1)]);
+  const float s = block_scale(key_value<T>(a));
   const float inv = __frcp_rn(s);
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
@@ -358,26 +464,38 @@ bool vec_codes(const CodeSink& o) {
   return (reinterpret_cast<uintptr_t>(o.q) & 7u) == 0 && o.ldq % 8 == 0;
 }
 
+template <typename Source, int U>
+int launch_quant_spans(const char* what, const Source& src, const CodeSink& out, int rows, int cols, cudaStream_t st) {
+  const long long spans = (cols + 2 * U * kBlock - 1) / (2 * U * kBlock);
+  constexpr int per_cta = kQuantThreads / 32;
+  const long long ctas = (rows * spans + per_cta - 1) / per_cta;
+  if (ctas * per_cta > kMaxInt) return fail(NPL_ERR_UNSUPPORTED, "%s: rows=%d cols=%d is too large", what, rows, cols);
+  return launch_pdl(what, vec_codes(out) ? fp8_quant_kernel<Source, U, true> : fp8_quant_kernel<Source, U, false>,
+                    dim3((unsigned)ctas), dim3(kQuantThreads), 0, st, src, out, rows, cols, (unsigned)spans);
+}
+
+// Four blocks a thread, except where the rows are short (half of the warps'
+// lanes or more would idle) or so few that one block a thread fits on the SMs
+// at once (8 x 4096: X us against Y with four).
 template <typename Source>
 int launch_quant(const char* what, const Source& src, const CodeSink& out, int rows, int cols, cudaStream_t st) {
-  const long long kb = (cols + kBlock - 1) / kBlock;
-  const long long total = rows * kb;
-  if (total > kMaxInt) return fail(NPL_ERR_UNSUPPORTED, "%s: %lld blocks (at most 2^31 - 1)", what, total);
-  constexpr int per_cta = kQuantThreads / kGroup * kUnroll;
-  const dim3 grid((unsigned)((total + per_cta - 1) / per_cta));
-  return launch_pdl(what, vec_codes(out) ? fp8_quant_kernel<Source, true> : fp8_quant_kernel<Source, false>, grid,
-                    dim3(kQuantThreads), 0, st, src, out, rows, cols, (int)kb);
+  const long long blocks = (long long)rows * ((cols + kBlock - 1) / kBlock);
+  if (cols <= 4 * kBlock || blocks <= 64ll * num_sms()) return launch_quant_spans<Source, 1>(what, src, out, rows, cols, st);
+  return launch_quant_spans<Source, 4>(what, src, out, rows, cols, st);
 }
 
 template <typename T, bool kVec, bool kVecQ>
 int launch_rmsnorm(const T* x, long long ldx, const T* res, long long ld_res, const T* w, float eps, int rows,
                    int cols, T* sum_out, long long ld_sum, const CodeSink& out, cudaStream_t st) {
+  // Few rows: one chunk a thread, the shortest way through a row. More rows
+  // than run at once: two, which halves the share of the two barriers and of
+  // the scales (16000 x 4096: X us against Y).
   const int lanes = (cols + kVecCols - 1) / kVecCols;
-  const int threads = std::min(kNormThreads, (lanes + 31) / 32 * 32);
+  const int want = lanes <= kNormThreads && rows <= 2 * num_sms() ? 1 : 2;
+  const int threads = std::min(kNormThreads, (lanes + 32 * want - 1) / (32 * want) * 32);
   const int chunks = (lanes + threads - 1) / threads;
   auto kern = chunks <= 1   ? fp8_rmsnorm_kernel<T, 1, kVec, kVecQ>
               : chunks <= 2 ? fp8_rmsnorm_kernel<T, 2, kVec, kVecQ>
-              : chunks <= 4 ? fp8_rmsnorm_kernel<T, 4, kVec, kVecQ>
                             : fp8_rmsnorm_kernel<T, 0, kVec, kVecQ>;
   return launch_pdl("npl_fp8_rmsnorm_quant", kern, dim3((unsigned)rows), dim3((unsigned)threads), 0, st, x, ldx, res,
                     ld_res, w, eps, cols, sum_out, ld_sum, out);
@@ -472,7 +590,7 @@ extern "C" int npl_fp8_quant_weight(const void* w, int w_dtype, int64_t rows, in
     using T = decltype(t);
     auto kern = vec ? (vecq ? fp8_quant_weight_kernel<T, true, true> : fp8_quant_weight_kernel<T, true, false>)
                     : (vecq ? fp8_quant_weight_kernel<T, false, true> : fp8_quant_weight_kernel<T, false, false>);
-    return launch_pdl(what, kern, dim3((unsigned)nb, (unsigned)kb), dim3(kQuantThreads), 0,
+    return launch_pdl(what, kern, dim3((unsigned)nb, (unsigned)kb), dim3(kWeightThreads), 0,
                       static_cast<cudaStream_t>(stream), static_cast<const T*>(w), ldw, (int)rows, (int)cols, out);
   });
 }

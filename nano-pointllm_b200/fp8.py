@@ -47,26 +47,34 @@ def _blocks(n: int) -> int:
 
 
 def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
-    if not first.is_cuda:
+    d = first.get_device()
+    if d < 0:
         raise ValueError("the fp8 path runs on CUDA tensors only")
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != d:
             raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
 
 
 def _call(fn, device: torch.device, *args) -> None:
-    """fn(*args, stream) with ``device`` current, on its current stream."""
-    if device.index == torch.cuda.current_device():
-        L.check(fn(*args, L.stream_ptr(device)))
+    """fn(*args, stream) with ``device`` current, on its current stream. (The
+    raw queries: a call on a few rows is bound by the host, and
+    torch.cuda.current_stream alone takes as long as the kernel.)"""
+    i = device.index
+    if i == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
-        with torch.cuda.device(device):
-            L.check(fn(*args, L.stream_ptr(device)))
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        L.check(rc)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., K] as [rows, K] with contiguous columns and rows that do not
     overlap (a copy only where the strides do not allow a view)."""
     t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if t.is_contiguous():
+        return t
     r, k = t.shape
     if (k > 1 and t.stride(1) != 1) or (r > 1 and t.stride(0) < k):
         t = t.contiguous()
@@ -74,15 +82,17 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _ld(t: torch.Tensor) -> int:
-    """Row stride of a 2-D tensor; a single row's is its length."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    """Row stride of a 2-D tensor; a single row's is its length at least."""
+    return max(t.stride(0), t.shape[1])
 
 
 def _new_codes(rows: int, k: int, device: torch.device) -> torch.Tensor:
     """e4m3 [rows, K] whose rows start on 16-byte boundaries, as the linear reads them."""
-    if k % 16 == 0:
-        return torch.empty((rows, k), dtype=_E4M3, device=device)
-    return torch.empty((rows, -(-k // 16) * 16), dtype=_E4M3, device=device)[:, :k]
+    return torch.empty_strided((rows, k), (-(-k // 16) * 16, 1), dtype=_E4M3, device=device)
+
+
+def _new_scales(rows: int, blocks: int, device: torch.device) -> torch.Tensor:
+    return torch.empty_strided((rows, blocks), (blocks, 1), dtype=torch.float32, device=device)
 
 
 def _activation(name: str, t: torch.Tensor, types: dict) -> int:
@@ -100,12 +110,11 @@ def quantize_token_blocks(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     dt = _activation("x", x, _DT)
     v = _rows(x)
     m, k = v.shape
-    q = _new_codes(m, k, x.device)
-    s = torch.empty((m, _blocks(k)), dtype=torch.float32, device=x.device)
+    dev, kb = x.device, _blocks(k)
+    q, s = _new_codes(m, k, dev), _new_scales(m, kb, dev)
     if m:
-        _call(L.lib.npl_fp8_quant_rows, x.device, v.data_ptr(), dt, m, k, _ld(v), q.data_ptr(), _ld(q), s.data_ptr(),
-              s.shape[1])
-    return (q, s) if x.dim() == 2 else (q.reshape(x.shape), s.reshape(*x.shape[:-1], -1 if m else _blocks(k)))
+        _call(L.lib.npl_fp8_quant_rows, dev, v.data_ptr(), dt, m, k, _ld(v), q.data_ptr(), q.stride(0), s.data_ptr(), kb)
+    return (q, s) if x.dim() == 2 else (q.reshape(x.shape), s.reshape(*x.shape[:-1], kb))
 
 
 def quantize_weight_blocks(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -117,10 +126,9 @@ def quantize_weight_blocks(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Te
     dt = _activation("weight", weight, _DT)
     w = _rows(weight.detach())
     n, k = w.shape
-    q = _new_codes(n, k, w.device)
-    s = torch.empty((_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device)
-    _call(L.lib.npl_fp8_quant_weight, w.device, w.data_ptr(), dt, n, k, _ld(w), q.data_ptr(), _ld(q), s.data_ptr(),
-          s.shape[1])
+    dev, kb = w.device, _blocks(k)
+    q, s = _new_codes(n, k, dev), _new_scales(_blocks(n), kb, dev)
+    _call(L.lib.npl_fp8_quant_weight, dev, w.data_ptr(), dt, n, k, _ld(w), q.data_ptr(), q.stride(0), s.data_ptr(), kb)
     return q, s
 
 
@@ -143,7 +151,7 @@ def rmsnorm_quant_blocks(x: torch.Tensor, weight: torch.Tensor, eps: float, resi
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError("residual must have the shape and type of x")
         if sum_out is None:
-            sum_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            sum_out = torch.empty_strided(x.shape, (x.shape[1], 1), dtype=x.dtype, device=x.device)
         elif sum_out.shape != x.shape or sum_out.dtype != x.dtype:
             raise ValueError("sum_out must have the shape and type of x")
         elif sum_out is not x and sum_out is not residual and _overlap(sum_out, x, residual):
@@ -154,12 +162,12 @@ def rmsnorm_quant_blocks(x: torch.Tensor, weight: torch.Tensor, eps: float, resi
     r = None if residual is None else _rows(residual)
     w = weight if weight.is_contiguous() else weight.contiguous()
     m, k = v.shape
-    q = _new_codes(m, k, x.device)
-    s = torch.empty((m, _blocks(k)), dtype=torch.float32, device=x.device)
+    dev, kb = x.device, _blocks(k)
+    q, s = _new_codes(m, k, dev), _new_scales(m, kb, dev)
     if m:
-        _call(L.lib.npl_fp8_rmsnorm_quant, x.device, v.data_ptr(), _ld(v), L.ptr(r), 0 if r is None else _ld(r),
+        _call(L.lib.npl_fp8_rmsnorm_quant, dev, v.data_ptr(), _ld(v), L.ptr(r), 0 if r is None else _ld(r),
               w.data_ptr(), dt, float(eps), m, k, L.ptr(sum_out), 0 if r is None else _ld(sum_out), q.data_ptr(),
-              _ld(q), s.data_ptr(), s.shape[1])
+              q.stride(0), s.data_ptr(), kb)
     return q, s, sum_out
 
 
@@ -173,11 +181,11 @@ def silu_mul_quant_blocks(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.T
         raise ValueError("gate and up must be [M, K] of one shape and type")
     g, u = _rows(gate), _rows(up)
     m, k = g.shape
-    q = _new_codes(m, k, g.device)
-    s = torch.empty((m, _blocks(k)), dtype=torch.float32, device=g.device)
+    dev, kb = g.device, _blocks(k)
+    q, s = _new_codes(m, k, dev), _new_scales(m, kb, dev)
     if m:
-        _call(L.lib.npl_fp8_silu_mul_quant, g.device, g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), dt, m, k,
-              q.data_ptr(), _ld(q), s.data_ptr(), s.shape[1])
+        _call(L.lib.npl_fp8_silu_mul_quant, dev, g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), dt, m, k, q.data_ptr(),
+              q.stride(0), s.data_ptr(), kb)
     return q, s
 
 
@@ -237,7 +245,7 @@ def linear_blocks(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w
             raise ValueError("residual must be [M, N] of out_dtype")
         res = _rows(residual)
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype, device=q.device)
+        out = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=q.device)
     else:
         if out.shape != (m, n) or out.dtype != out_dtype:
             raise ValueError("out must be [M, N] of out_dtype")

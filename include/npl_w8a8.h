@@ -417,7 +417,7 @@ int npl_fp8_quant_rows(const void* x, int x_dtype, int64_t rows, int64_t cols, i
                        float* scale, int64_t ld_scale, void* stream);
 
 /* A weight per 128 x 128 block: scale fp32 [ceil(rows / 128), ceil(cols /
- * 128)]. w_dtype may be NPL_F32; cols <= 65535 * 128. */
+ * 128)]. w_dtype may be NPL_F32. */
 int npl_fp8_quant_weight(const void* w, int w_dtype, int64_t rows, int64_t cols, int64_t ldw, uint8_t* q, int64_t ldq,
                          float* scale, int64_t ld_scale, void* stream);
 

@@ -78,14 +78,34 @@ struct Fp8Ctl {
 };
 
 // D[tmem] (+)= A[smem] * B[smem]^T, e4m3 x e4m3 -> fp32 (kind::f8f6f4).
-__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                         uint32_t accumulate) {
+template <bool kAccumulate>
+__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "l"(adesc), "l"(bdesc), "r"(idesc), "n"((int)kAccumulate)
       : "memory");
+}
+
+// One lane of the warp, the same each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
+// mbar_wait bounded by a count of polls (each takes 20 ns or more), without
+// the clock: fewer instructions where every block waits.
+__device__ __forceinline__ bool poll_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+  for (int i = 0; i < (1 << 25); ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  if (status) atomicExch(status, code);
+  return false;
 }
 
 // Instruction descriptor of kind::f8f6f4: fp32 accumulator (c_format [4,6) =
@@ -153,7 +173,6 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = c.tmem_base;
-  pdl_wait();
   pdl_trigger();
 
   const int quarter = warp & 3;  // TMEM lanes this warp may access
@@ -166,12 +185,23 @@ __global__ void __launch_bounds__(kThreads)
     if (lane == 0) {
       const uint64_t pol_w = policy_evict_first();
       const uint64_t pol_x = policy_evict_last();
+      auto load_w = [&](int kb, int stage) {
+        mbar_arrive_expect_tx(&c.full[stage], kStageW + kStageX);
+        tma_load_2d(ring_w + (size_t)stage * kStageW, &tmap_w, kb * kBlockK, n_tile * kTileN, &c.full[stage], pol_w);
+      };
+      // Weights do not depend on the kernels before this one on its stream
+      // (npl_fp8_quant_weight lets this one start only when its codes are
+      // visible), so the ring is filled with them before the wait.
+      const int ahead = min(p.stages, kb1 - kb0);
+      for (int i = 0; i < ahead; ++i) load_w(kb0 + i, i);
+      pdl_wait();
       int stage = 0, loads = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&c.empty[stage], phase ^ 1, p.status, NPL_DEV_TIMEOUT_TMA)) break;
-        mbar_arrive_expect_tx(&c.full[stage], kStageW + kStageX);
-        tma_load_2d(ring_w + (size_t)stage * kStageW, &tmap_w, kb * kBlockK, n_tile * kTileN, &c.full[stage], pol_w);
+        if (loads >= ahead) {
+          if (!mbar_wait(&c.empty[stage], phase ^ 1, p.status, NPL_DEV_TIMEOUT_TMA)) break;
+          load_w(kb, stage);
+        }
         tma_load_2d(ring_x + (size_t)stage * kStageX, &tmap_x, kb * kBlockK, m_tile * NT, &c.full[stage], pol_x);
         ++loads;
         if (++stage == p.stages) {
@@ -185,32 +215,38 @@ __global__ void __launch_bounds__(kThreads)
         mbar_wait(&c.full[i], i < stage ? phase : phase ^ 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, buf = i % kAccBufs;
-        if (!mbar_wait(&c.tempty[buf], ((i / kAccBufs) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA)) break;
-        if (!mbar_wait(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA)) break;
-        tc_fence_after();
-        const uint32_t a0 = smem_u32(ring_w + (size_t)stage * kStageW);
-        const uint32_t b0 = smem_u32(ring_x + (size_t)stage * kStageX);
-        const uint32_t d = tmem_base + (uint32_t)(buf * NT);
+    // The whole warp runs this loop and one lane issues, so that descriptors
+    // stay in uniform registers (see the prefill kernel).
+    const bool issuer = elect_one();
+    const uint64_t desc_w = sdesc_k_sw128(smem_u32(ring_w)), desc_x = sdesc_k_sw128(smem_u32(ring_x));
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int i = kb - kb0, buf = i % kAccBufs;
+      if (!poll_wait(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA)) break;
+      if (!poll_wait(&c.tempty[buf], ((i / kAccBufs) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA)) break;
+      tc_fence_after();
+      const uint64_t a = desc_w + (uint32_t)stage * (kStageW >> 4), b = desc_x + (uint32_t)stage * (kStageX >> 4);
+      const uint32_t d = tmem_base + (uint32_t)(buf * NT);
+      if (issuer) {
+        mma_e4m3<false>(d, a, b, kIdesc);
 #pragma unroll
-        for (int kk = 0; kk < kBlockK / 32; ++kk)
-          mma_e4m3(d, sdesc_k_sw128(a0 + kk * 32), sdesc_k_sw128(b0 + kk * 32), kIdesc, kk > 0 ? 1u : 0u);
-        tc_commit(&c.empty[stage]);
+        for (int kk = 1; kk < kBlockK / 32; ++kk) mma_e4m3<true>(d, a + kk * 2, b + kk * 2, kIdesc);
         tc_commit(&c.tfull[buf]);
-        if (++stage == p.stages) {
-          stage = 0;
-          phase ^= 1;
-        }
+        tc_commit(&c.empty[stage]);
       }
-      // all MMAs issued by this thread complete before the ring and TMEM are given up
-      tc_commit(&c.teardown);
-      mbar_wait(&c.teardown, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+      __syncwarp();
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
+    // all MMAs issued complete before the ring and TMEM are given up
+    if (issuer) tc_commit(&c.teardown);
+    poll_wait(&c.teardown, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+    __syncwarp();
   } else {
+    pdl_wait();
     // Lanes hold the scales of tokens lane and lane + 32 of the next block.
     constexpr int kPer = (NT + 31) / 32;
     float next[kPer], next_sw;
@@ -393,17 +429,6 @@ __device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t adesc, u
       : "memory");
 }
 
-// One lane of the warp, the same each time.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t one;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(one));
-  return one != 0;
-}
-
 // Completion of the MMAs issued so far arrives on this barrier in both CTAs.
 __device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
   asm volatile(
@@ -424,15 +449,6 @@ __device__ __forceinline__ void mbar_arrive_pair(uint32_t bar_cluster) {
 // Byte offset of 16-byte chunk `ch` of row `row` in a staged box of 128-byte
 // rows: the 128-byte swizzle of the output's tensor map.
 __device__ __forceinline__ int staged(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
-
-// mbar_wait bounded by a count of polls (each takes 20 ns or more), without
-// the clock: fewer instructions where every block waits.
-__device__ __forceinline__ bool poll_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
-  for (int i = 0; i < (1 << 25); ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  if (status) atomicExch(status, code);
-  return false;
-}
 
 // Tile t -> (token tile, weight tile): groups of raster_g token tiles, the
 // token tile running fastest, so that the tiles in flight at one time share

@@ -15,11 +15,12 @@
 // infinity gets a non-finite scale, and all its values read back as NaN.
 //
 // Every kernel is one pass over its input: the block stays in registers
-// between the maximum and the codes, 8 columns a thread, 16 threads a block.
+// between the maximum and the codes, 16 columns a thread, 8 threads a block.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "npl_common.cuh"
 
@@ -27,14 +28,11 @@ namespace npl {
 namespace {
 
 constexpr int kBlock = 128;       // columns (and weight rows) per scale
-constexpr int kVecCols = 8;       // columns per thread
-constexpr int kGroup = kBlock / kVecCols;  // threads per block of a row
+constexpr int kCols = 16;         // columns per thread
+constexpr int kGroup = kBlock / kCols;  // threads per block of a row
 constexpr float kE4m3Max = 448.0f;
 constexpr float kScaleMin = 0x1p-126f;
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
 template <>
@@ -42,38 +40,82 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 8 consecutive elements as they lie in memory.
+// 16 consecutive elements as they lie in memory.
 template <typename T>
-struct alignas(16) Raw8 {
-  T e[8];
+struct alignas(16) Raw {
+  T e[kCols];
+  static constexpr int kWords = kCols * (int)sizeof(T) / 4;
 };
 
-// The first n of 8 consecutive elements at p (zeros after them). kVec: p is
-// 16-byte aligned, and 8 elements are loaded at once.
-template <bool kVec, typename T>
-__device__ __forceinline__ Raw8<T> load8(const T* p, int n) {
-  Raw8<T> r;
-  if (kVec && n >= 8) {
-    const uint4* s = reinterpret_cast<const uint4*>(p);
-    uint4* d = reinterpret_cast<uint4*>(&r);
+// How rows can be accessed: their alignment in bytes (32, 16, or that of an element).
+enum Access { kElements = 0, kBy16 = 1, kBy32 = 2 };
+
+__device__ __forceinline__ void ld32(const void* p, uint32_t* r) {  // one 256-bit load
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p));
+}
+
+// The first n of 16 consecutive elements at p (zeros after them).
+template <int kAccess, typename T>
+__device__ __forceinline__ Raw<T> load16(const T* p, int n) {
+  Raw<T> r;
+  if (kAccess != kElements && n >= kCols) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+    if constexpr (kAccess == kBy32) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(Raw8<T>) / 16; ++i) d[i] = s[i];
+      for (int i = 0; i < Raw<T>::kWords; i += 8) ld32(reinterpret_cast<const uint32_t*>(p) + i, w + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < Raw<T>::kWords; i += 4)
+        *reinterpret_cast<uint4*>(w + i) = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+    }
     return r;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r.e[i] = i < n ? p[i] : T(0.0f);
+  for (int i = 0; i < kCols; ++i) r.e[i] = i < n ? p[i] : T(0.0f);
   return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void widen8(const Raw8<T>& r, float (&v)[8]) {
+template <int kAccess, typename T>
+__device__ __forceinline__ void store16(T* p, const Raw<T>& r, int n) {
+  if (kAccess != kElements && n >= kCols) {
+    const uint4* w = reinterpret_cast<const uint4*>(&r);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_f32(r.e[i]);
+    for (int i = 0; i < Raw<T>::kWords / 4; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kCols; ++i)
+    if (i < n) p[i] = r.e[i];
 }
 
-// max |v| is taken on the bit patterns without their sign: they order like the
-// magnitudes, an infinity above every number and a NaN above infinity, so a
-// NaN is never lost. A key is such a pattern, of fp32 or of a 16-bit type.
+__device__ __forceinline__ void widen(const Raw<float>& r, float (&v)[kCols]) {
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) v[i] = r.e[i];
+}
+__device__ __forceinline__ void widen(const Raw<__half>& r, float (&v)[kCols]) {
+  const __half2* h = reinterpret_cast<const __half2*>(&r);
+#pragma unroll
+  for (int i = 0; i < kCols / 2; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void widen(const Raw<__nv_bfloat16>& r, float (&v)[kCols]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < kCols / 2; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// A key is max |v| as a bit pattern, of fp32 or of a 16-bit type. Patterns
+// without a sign order like the magnitudes, an infinity above every number
+// and a NaN above infinity; with the NaN-propagating max of a thread's own
+// values a NaN is never lost.
 template <typename T>
 __device__ __forceinline__ float key_value(uint32_t key);
 template <>
@@ -85,22 +127,37 @@ __device__ __forceinline__ float key_value<__half>(uint32_t key) {
 template <>
 __device__ __forceinline__ float key_value<__nv_bfloat16>(uint32_t key) { return __uint_as_float(key << 16); }
 
-__device__ __forceinline__ uint32_t key8(const float (&v)[8]) {
-  uint32_t a = __float_as_uint(v[0]) & 0x7fffffffu;
-#pragma unroll
-  for (int i = 1; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);
-  return a;
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+__device__ __forceinline__ __half2 max_abs(__half2 a, __half2 b) { return __hmax2_nan(__habs2(a), __habs2(b)); }
+__device__ __forceinline__ __nv_bfloat162 max_abs(__nv_bfloat162 a, __nv_bfloat162 b) {
+  return __hmax2_nan(__habs2(a), __habs2(b));
+}
+
+template <typename V, int N>
+__device__ __forceinline__ V max_abs_all(const V* v) {
+  if constexpr (N == 1)
+    return v[0];
+  else
+    return max_abs(max_abs_all<V, N / 2>(v), max_abs_all<V, N / 2>(v + N / 2));
+}
+
+__device__ __forceinline__ uint32_t key_of(const float (&v)[kCols]) {
+  return __float_as_uint(max_abs_all<float, kCols>(v));
 }
 
 template <typename T>
-__device__ __forceinline__ uint32_t key8(const Raw8<T>& r) {
+__device__ __forceinline__ uint32_t key_of(const Raw<T>& r) {
   if constexpr (sizeof(T) == 4) {
-    return key8(r.e);
-  } else {  // two 16-bit patterns at a time
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
-    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
-                                __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-    return max(m & 0xffffu, m >> 16);
+    return key_of(r.e);
+  } else {
+    using Pair = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const Pair m = max_abs_all<Pair, kCols / 2>(reinterpret_cast<const Pair*>(&r));
+    const uint32_t bits = *reinterpret_cast<const uint32_t*>(&m);
+    return max(bits & 0xffffu, bits >> 16);
   }
 }
 
@@ -108,29 +165,20 @@ __device__ __forceinline__ uint32_t max_xor(uint32_t own, uint32_t sent, int o) 
   return max(own, __shfl_xor_sync(0xffffffffu, sent, o));
 }
 
-// The largest key of U blocks (1, 2 or 4) over the 16 lanes that share them.
-// Halving the blocks with each exchange costs 4, 4 or 5 shuffles instead of
-// 4 U, and leaves lane l with block own_block<U>(l), whose scale it then works
-// out for the other lanes too.
+// The largest key of U blocks (1 or 2) over the 8 lanes that share them. With
+// two, half of the lanes go on with each after the first exchange: 3 shuffles
+// instead of 6, and lane l is left with block own_block<U>(l), whose scale it
+// works out for the other lanes too.
 template <int U>
-__device__ __forceinline__ int own_block(int lane) { return U == 4 ? (lane >> 2) & 3 : U == 2 ? (lane >> 3) & 1 : 0; }
+__device__ __forceinline__ int own_block(int lane) { return U == 2 ? (lane >> 2) & 1 : 0; }
 
 template <int U>
 __device__ __forceinline__ uint32_t block_key(const uint32_t (&k)[U], int lane) {
   uint32_t m;
-  if constexpr (U == 4) {
-    const bool hi = lane & 8, mid = lane & 4;
-    const uint32_t a = max_xor(hi ? k[2] : k[0], hi ? k[0] : k[2], 8);
-    const uint32_t b = max_xor(hi ? k[3] : k[1], hi ? k[1] : k[3], 8);
-    m = max_xor(mid ? b : a, mid ? a : b, 4);
-  } else if constexpr (U == 2) {
-    const bool hi = lane & 8;
-    m = max_xor(hi ? k[1] : k[0], hi ? k[0] : k[1], 8);
-    m = max_xor(m, m, 4);
-  } else {
-    m = max_xor(k[0], k[0], 8);
-    m = max_xor(m, m, 4);
-  }
+  if constexpr (U == 2)
+    m = max_xor(lane & 4 ? k[1] : k[0], lane & 4 ? k[0] : k[1], 4);
+  else
+    m = max_xor(k[0], k[0], 4);
   m = max_xor(m, m, 2);
   return max_xor(m, m, 1);
 }
@@ -138,7 +186,7 @@ __device__ __forceinline__ uint32_t block_key(const uint32_t (&k)[U], int lane) 
 // Block u's value of `v`, held by the lanes whose own_block is u.
 template <int U>
 __device__ __forceinline__ float from_block(float v, int u) {
-  return U == 1 ? v : __shfl_sync(0xffffffffu, v, (int)(threadIdx.x & 16) + u * (kGroup / U));
+  return U == 1 ? v : __shfl_sync(0xffffffffu, v, (int)(threadIdx.x & 24) + u * (kGroup / U));
 }
 
 __device__ __forceinline__ float block_scale(float absmax) {
@@ -147,81 +195,83 @@ __device__ __forceinline__ float block_scale(float absmax) {
   return s < kScaleMin ? kScaleMin : s;
 }
 
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float inv) {
-  uint32_t w[2];
+__device__ __forceinline__ uint4 codes16(const float (&v)[kCols], float inv) {
+  uint32_t w[4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < 4; ++h) {
     const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(
         make_float2(__fmul_rn(v[4 * h], inv), __fmul_rn(v[4 * h + 1], inv)), __NV_SATFINITE, __NV_E4M3);
     const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(
         make_float2(__fmul_rn(v[4 * h + 2], inv), __fmul_rn(v[4 * h + 3], inv)), __NV_SATFINITE, __NV_E4M3);
     w[h] = (uint32_t)lo | ((uint32_t)hi << 16);
   }
-  return make_uint2(w[0], w[1]);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Stores the first n of 8 codes; kVecQ: dst is 8-byte aligned.
+// Stores the first n of 16 codes; kVecQ: dst is 16-byte aligned.
 template <bool kVecQ>
-__device__ __forceinline__ void store_codes(uint8_t* dst, uint2 q, int n) {
-  if (kVecQ && n >= 8) {
-    *reinterpret_cast<uint2*>(dst) = q;
+__device__ __forceinline__ void store_codes(uint8_t* dst, uint4 q, int n) {
+  if (kVecQ && n >= kCols) {
+    *reinterpret_cast<uint4*>(dst) = q;
     return;
   }
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) dst[i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+  for (int i = 0; i < kCols; ++i)
+    if (i < n) dst[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
 }
 
-// Where the quantised values come from: what a thread loads for its 8 columns,
+// Where the quantised values come from: what a thread loads for its columns,
 // what it keeps of them, their key and the fp32 values.
-template <typename T, bool kVec>
+template <typename T, int kAccess>
 struct RowSource {  // the row itself
   using Elem = T;
-  using Raw = Raw8<T>;
-  using Kept = Raw8<T>;
+  using Loaded = Raw<T>;
+  using Kept = Raw<T>;
   const T* x;
   long long ldx;
-  __device__ __forceinline__ Raw load(int row, int col, int n) const { return load8<kVec>(x + row * ldx + col, n); }
-  __device__ __forceinline__ static Kept keep(const Raw& r) { return r; }
-  __device__ __forceinline__ static uint32_t key(const Kept& k) { return key8(k); }
-  __device__ __forceinline__ static void values(const Kept& k, float (&v)[8]) { widen8(k, v); }
+  __device__ __forceinline__ Loaded load(int row, int col, int n) const {
+    return load16<kAccess>(x + row * ldx + col, n);
+  }
+  __device__ __forceinline__ static Kept keep(const Loaded& r) { return r; }
+  __device__ __forceinline__ static uint32_t key(const Kept& k) { return key_of(k); }
+  __device__ __forceinline__ static void values(const Kept& k, float (&v)[kCols]) { widen(k, v); }
 };
 
-// silu(g) up = g / (1 + e^-g) up in fp32. With t = e^-|g| <= 1 it is
-// (g < 0 ? g t : g) / (1 + t): nothing overflows, and 1 + t in [1, 2] has a
-// fast reciprocal (1 ulp) without special cases.
-template <typename T, bool kVec>
+// silu(g) up = g / (1 + e^-g) up in fp32, within a few ulps. For g below
+// -87.3, where it is under 1e-36, the approximate reciprocal gives 0.
+template <typename T, int kAccess>
 struct SiluSource {
   using Elem = float;
-  struct Raw {
-    Raw8<T> g, u;
+  struct Loaded {
+    Raw<T> g, u;
   };
   struct Kept {
-    float v[8];
+    float v[kCols];
   };
   const T* gate;
   const T* up;
   long long ld_gate, ld_up;
-  __device__ __forceinline__ Raw load(int row, int col, int n) const {
-    return {load8<kVec>(gate + row * ld_gate + col, n), load8<kVec>(up + row * ld_up + col, n)};
+  __device__ __forceinline__ Loaded load(int row, int col, int n) const {
+    return {load16<kAccess>(gate + row * ld_gate + col, n), load16<kAccess>(up + row * ld_up + col, n)};
   }
-  __device__ __forceinline__ static Kept keep(const Raw& r) {
+  __device__ __forceinline__ static Kept keep(const Loaded& r) {
     Kept k;
+    float up[kCols];
+    widen(r.g, k.v);
+    widen(r.u, up);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float g = to_f32(r.g.e[i]);
-      const float t = expf(-fabsf(g));
-      float inv;
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(__fadd_rn(1.0f, t)));
-      const float num = g >= 0.f ? g : __fmul_rn(g, t);
-      k.v[i] = __fmul_rn(__fmul_rn(num, inv), to_f32(r.u.e[i]));
+    for (int i = 0; i < kCols; ++i) {
+      float sig;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sig) : "f"(__fadd_rn(1.0f, expf(-k.v[i]))));
+      k.v[i] = __fmul_rn(__fmul_rn(k.v[i], sig), up[i]);
     }
     return k;
   }
-  __device__ __forceinline__ static uint32_t key(const Kept& k) { return key8(k.v); }
-  __device__ __forceinline__ static void values(const Kept& k, float (&v)[8]) {
+  __device__ __forceinline__ static uint32_t key(const Kept& k) { return key_of(k.v); }
+  __device__ __forceinline__ static void values(const Kept& k, float (&v)[kCols]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k.v[i];
+    for (int i = 0; i < kCols; ++i) v[i] = k.v[i];
   }
 };
 
@@ -233,27 +283,26 @@ struct CodeSink {
 };
 
 constexpr int kQuantThreads = 256;
-constexpr int kNormThreads = 1024;
+constexpr int kNormThreads = 512;
 
-// A warp takes 2 U consecutive blocks of a row, each of its two 16-lane groups
-// every other one, all loads before the first store, which the compiler would
-// not move them across. The bound on registers keeps 24 to 40 warps, and 80 KB
-// of loads or more, in flight on an SM.
+// A warp takes 4 U consecutive blocks of a row, each of its four 8-lane groups
+// every fourth, all loads before the first store, which the compiler would not
+// move them across.
 template <typename Source, int U, bool kVecQ>
-__global__ void __launch_bounds__(kQuantThreads, sizeof(typename Source::Raw) > 16 ? 3 : 5)
+__global__ void __launch_bounds__(kQuantThreads, sizeof(typename Source::Loaded) > 32 ? 4 : 5)
     fp8_quant_kernel(const Source src, const CodeSink out, int rows, int cols, unsigned spans) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x % kGroup;
-  const unsigned item = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);  // (row, span of 2 U blocks)
+  const unsigned item = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);  // (row, span of 4 U blocks)
   const int row = (int)(item / spans);
   if (row >= rows) return;  // whole warps
-  const int kb0 = (int)(item - (unsigned)row * spans) * (2 * U) + (int)(threadIdx.x & 31) / kGroup;
-  const int col0 = kb0 * kBlock + lane * kVecCols;
-  typename Source::Raw raw[U];
+  const int kb0 = (int)(item - (unsigned)row * spans) * (4 * U) + (int)(threadIdx.x & 31) / kGroup;
+  const int col0 = kb0 * kBlock + lane * kCols;
+  typename Source::Loaded raw[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int col = col0 + u * (2 * kBlock);
+    const int col = col0 + u * (4 * kBlock);
     raw[u] = src.load(row, col < cols ? col : 0, cols - col);
   }
   typename Source::Kept kept[U];
@@ -265,143 +314,109 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(typename Source::Raw) > 
   }
   const float s = block_scale(key_value<typename Source::Elem>(block_key<U>(key, lane)));
   const float inv = __frcp_rn(s);
-  {
-    const int kb = kb0 + 2 * own_block<U>(lane);
-    if (lane % (kGroup / U) == 0 && kb * kBlock < cols) out.scale[row * out.ld_scale + kb] = s;
-  }
-  uint8_t* q = out.q + row * out.ldq;
+  const int kb = kb0 + 4 * own_block<U>(lane);
+  if (lane % (kGroup / U) == 0 && kb * kBlock < cols) out.scale[row * out.ld_scale + kb] = s;
+  uint8_t* q = out.q + row * out.ldq + col0;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const float inv_u = from_block<U>(inv, u);
-    const int col = col0 + u * (2 * kBlock);
-    float v[8];
+    float v[kCols];
     Source::values(kept[u], v);
-    if (col < cols) store_codes<kVecQ>(q + col, codes8(v, inv_u), cols - col);
+    const int n = cols - col0 - u * (4 * kBlock);
+    if (n > 0) store_codes<kVecQ>(q + u * (4 * kBlock), codes16(v, inv_u), n);
   }
 }
 
-// (x + residual) -> RMSNorm -> codes; one CTA per row. kChunks > 0: the row
-// stays in registers as T, kChunks * 8 columns a thread; 0: any length, the
-// row is read again for the second half.
-template <typename T, int kChunks, bool kVec, bool kVecQ>
-__global__ void __launch_bounds__(kNormThreads)
+// (x + residual) -> RMSNorm -> codes; one CTA per row. kMaxThreads > 0: the row
+// stays in registers, 16 columns a thread, with as many registers as the longest
+// row's threads leave (up to 704 threads two CTAs share an SM: 16000 x 11008
+// with residual takes 273 us, one CTA an SM 358); 0: the row, of any length, is
+// read again for the second half.
+template <typename T, int kMaxThreads, int kAccess, bool kVecQ>
+__global__ void __launch_bounds__(kMaxThreads ? kMaxThreads : kNormThreads, kMaxThreads == 704 ? 2 : 1)
     fp8_rmsnorm_kernel(const T* x, long long ldx, const T* res, long long ld_res, const T* __restrict__ w, float eps,
                        int cols, T* sum_out, long long ld_sum, const CodeSink out) {  // sum_out may be x or res
+  constexpr bool kInRegs = kMaxThreads > 0;
   __shared__ float red[32];
   pdl_wait();
   pdl_trigger();
   const long long row = blockIdx.x;
   const int lane = threadIdx.x % kGroup;
-  const int step = (int)blockDim.x * kVecCols;
-  constexpr int kKeep = kChunks > 0 ? kChunks : 1;
-  Raw8<T> keep[kKeep], other[kKeep];
-  float ss = 0.f;
-  // the sum as it is stored, and its squares: the norm is that of the stored sum
-  auto add = [&](int col, Raw8<T>& t, const Raw8<T>& r) {
-    const int n = cols - col;
-    float v[8];
-    widen8(t, v);
-    if (res) {
-      float rv[8];
-      widen8(r, rv);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t.e[i] = from_f32<T>(__fadd_rn(v[i], rv[i]));
-      widen8(t, v);
-      if (kVec && n >= 8) {
-        *reinterpret_cast<uint4*>(sum_out + row * ld_sum + col) = *reinterpret_cast<const uint4*>(&t);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < n) sum_out[row * ld_sum + col + i] = t.e[i];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss = __fmaf_rn(v[i], v[i], ss);
-  };
+  const int step = (int)blockDim.x * kCols;
+  const int col0 = (int)threadIdx.x * kCols;
   auto fetch = [&](const T* p, long long ld, int col) {
-    return load8<kVec>(p + row * ld + (col < cols ? col : 0), cols - col);
+    return load16<kAccess>(p + row * ld + (col < cols ? col : 0), cols - col);
   };
-  const int col0 = (int)threadIdx.x * kVecCols;
-  if constexpr (kChunks > 0) {
+  Raw<T> kept, other;
+  float ss = 0.f;
+  for (int col = col0; kInRegs || col < cols; col += step) {
+    kept = fetch(x, ldx, col);
+    if (res) other = fetch(res, ld_res, col);
+    float v[kCols];
+    widen(kept, v);
+    if (res) {  // rounded as it is stored: the norm is that of the stored sum
+      float r[kCols];
+      widen(other, r);
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      keep[c] = fetch(x, ldx, col0 + c * step);
-      if (res) other[c] = fetch(res, ld_res, col0 + c * step);
+      for (int i = 0; i < kCols; ++i) kept.e[i] = from_f32<T>(__fadd_rn(v[i], r[i]));
+      widen(kept, v);
+      store16<kAccess>(sum_out + row * ld_sum + (col < cols ? col : 0), kept, cols - col);
     }
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) add(col0 + c * step, keep[c], other[c]);
-  } else {
-    for (int col = col0; col < cols; col += step) {
-      keep[0] = fetch(x, ldx, col);
-      if (res) other[0] = fetch(res, ld_res, col);
-      add(col, keep[0], other[0]);
-    }
+    for (int i = 0; i < kCols; ++i) ss = __fmaf_rn(v[i], v[i], ss);
+    if (kInRegs) break;
   }
-  if constexpr (kChunks > 0) {  // the norm's weights, on their way while the sums are joined
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) other[c] = fetch(w, 0, col0 + c * step);
-  }
+  if (kInRegs) other = fetch(w, 0, col0);  // on its way while the sums are joined
   ss = warp_sum(ss);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
   __syncthreads();
   ss = warp_sum((threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0.f);
   const float r = rsqrtf(__fadd_rn(__fdividef(ss, (float)cols), eps));  // both within 2 ulps
-  // kChunks blocks at a time; the second reading takes the stored sum where
-  // there is one: it may have replaced x or the residual
-  for (int base = 0; base < cols; base += kKeep * step) {
-    float v[kKeep][8];
-    uint32_t key[kKeep];
-#pragma unroll
-    for (int c = 0; c < kKeep; ++c) {
-      if constexpr (kChunks == 0) {
-        keep[0] = res ? fetch(sum_out, ld_sum, base + col0) : fetch(x, ldx, base + col0);
-        other[0] = fetch(w, 0, base + col0);
-      }
-      float wv[8];
-      widen8(keep[c], v[c]);
-      widen8(other[c], wv);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[c][i] = __fmul_rn(__fmul_rn(v[c][i], r), wv[i]);
-      key[c] = key8(v[c]);
+  for (int base = 0; base < cols; base += step) {
+    const int col = base + col0;
+    if (!kInRegs) {  // the stored sum, where there is one: it may have replaced x or the residual
+      kept = res ? fetch(sum_out, ld_sum, col) : fetch(x, ldx, col);
+      other = fetch(w, 0, col);
     }
-    const float s = block_scale(__uint_as_float(block_key<kKeep>(key, lane)));
-    const float inv = __frcp_rn(s);
+    float v[kCols], wv[kCols];
+    widen(kept, v);
+    widen(other, wv);
 #pragma unroll
-    for (int c = 0; c < kKeep; ++c) {
-      const float inv_c = from_block<kKeep>(inv, c);
-      const int col = base + col0 + c * step;
-      if (col < cols) store_codes<kVecQ>(out.q + row * out.ldq + col, codes8(v[c], inv_c), cols - col);
-      if (lane == c * (kGroup / kKeep) && col - lane * kVecCols < cols)
-        out.scale[row * out.ld_scale + col / kBlock] = s;
+    for (int i = 0; i < kCols; ++i) v[i] = __fmul_rn(__fmul_rn(v[i], r), wv[i]);
+    const uint32_t key[1] = {key_of(v)};
+    const float s = block_scale(__uint_as_float(block_key<1>(key, lane)));
+    if (col < cols) {
+      store_codes<kVecQ>(out.q + row * out.ldq + col, codes16(v, __frcp_rn(s)), cols - col);
+      if (lane == 0) out.scale[row * out.ld_scale + col / kBlock] = s;
     }
   }
 }
 
-// One 128 x 128 weight block per CTA: 16 threads across, 32 rows at a time,
-// the block held in registers between its maximum and its codes.
-constexpr int kWeightThreads = 512;
+// One 128 x 128 weight block per CTA: 8 threads across, 32 rows at a time, the
+// block held in registers between its maximum and its codes.
+constexpr int kWeightThreads = 256;
 constexpr int kWeightRows = kWeightThreads / kGroup;
 
-template <typename T, bool kVec, bool kVecQ>
-__global__ void __launch_bounds__(kWeightThreads) fp8_quant_weight_kernel(const T* __restrict__ w, long long ldw,
-                                                                         int rows, int cols, const CodeSink out) {
+template <typename T, int kAccess, bool kVecQ>
+__global__ void __launch_bounds__(kWeightThreads, 3) fp8_quant_weight_kernel(const T* __restrict__ w, long long ldw,
+                                                                          int rows, int cols, int k_blocks,
+                                                                          const CodeSink out) {
   __shared__ uint32_t red[kWeightThreads / 32];
   pdl_wait();
   constexpr int kSteps = kBlock / kWeightRows;
-  const int nb = blockIdx.x, kb = blockIdx.y;
-  const int col = kb * kBlock + (int)(threadIdx.x % kGroup) * kVecCols;
-  const int n = min(8, max(0, cols - col));
+  const int nb = (int)(blockIdx.x / (unsigned)k_blocks), kb = (int)(blockIdx.x - (unsigned)nb * (unsigned)k_blocks);
+  const int col = kb * kBlock + (int)(threadIdx.x % kGroup) * kCols;
   const int row0 = nb * kBlock + (int)threadIdx.x / kGroup;
-  Raw8<T> raw[kSteps];
+  Raw<T> raw[kSteps];
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int row = row0 + i * kWeightRows;
-    const bool in = row < rows && n > 0;
-    raw[i] = load8<kVec>(w + (in ? (long long)row * ldw + col : 0), in ? n : 0);
+    const bool in = row < rows && col < cols;
+    raw[i] = load16<kAccess>(w + (in ? (long long)row * ldw + col : 0), in ? cols - col : 0);
   }
   uint32_t a = 0;
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) a = max(a, key8(raw[i]));
+  for (int i = 0; i < kSteps; ++i) a = max(a, key_of(raw[i]));
   a = __reduce_max_sync(0xffffffffu, a);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
   __syncthreads();
@@ -411,9 +426,10 @@ __global__ void __launch_bounds__(kWeightThreads) fp8_quant_weight_kernel(const 
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int row = row0 + i * kWeightRows;
-    float v[8];
-    widen8(raw[i], v);
-    if (row < rows && n > 0) store_codes<kVecQ>(out.q + (long long)row * out.ldq + col, codes8(v, inv), n);
+    float v[kCols];
+    widen(raw[i], v);
+    if (row < rows && col < cols)
+      store_codes<kVecQ>(out.q + (long long)row * out.ldq + col, codes16(v, inv), cols - col);
   }
   if (threadIdx.x == 0) out.scale[(long long)nb * out.ld_scale + kb] = s;
   pdl_trigger_after_writes();
@@ -424,9 +440,18 @@ constexpr long long kMaxInt = 2147483647ll;
 
 int elem_size(int dtype) { return dtype == NPL_F32 ? 4 : 2; }
 
-// Whether all rows, `ld` elements apart from `p` on, start on 16-byte boundaries.
-bool vec_rows(const void* p, long long rows, long long ld, int dtype) {
-  return aligned16(p) && (rows == 1 || (ld * elem_size(dtype)) % 16 == 0);
+// How all rows, `ld` elements apart from `p` on, can be accessed.
+int row_access(const void* p, long long rows, long long ld, int dtype) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | (rows == 1 ? 0 : (uintptr_t)(ld * elem_size(dtype)));
+  return bits % 32 == 0 ? kBy32 : bits % 16 == 0 ? kBy16 : kElements;
+}
+
+// fn(std::integral_constant<int, access>())
+template <typename Fn>
+int by_access(int access, Fn&& fn) {
+  if (access == kBy32) return fn(std::integral_constant<int, kBy32>());
+  if (access == kBy16) return fn(std::integral_constant<int, kBy16>());
+  return fn(std::integral_constant<int, kElements>());
 }
 
 int check_codes(const char* what, long long rows, long long cols, const void* q, long long ldq, const void* scale,
@@ -461,12 +486,12 @@ int by_type(int dtype, Fn&& fn) {
 }
 
 bool vec_codes(const CodeSink& o) {
-  return (reinterpret_cast<uintptr_t>(o.q) & 7u) == 0 && o.ldq % 8 == 0;
+  return aligned16(o.q) && o.ldq % 16 == 0;
 }
 
 template <typename Source, int U>
 int launch_quant_spans(const char* what, const Source& src, const CodeSink& out, int rows, int cols, cudaStream_t st) {
-  const long long spans = (cols + 2 * U * kBlock - 1) / (2 * U * kBlock);
+  const long long spans = (cols + 4 * U * kBlock - 1) / (4 * U * kBlock);
   constexpr int per_cta = kQuantThreads / 32;
   const long long ctas = (rows * spans + per_cta - 1) / per_cta;
   if (ctas * per_cta > kMaxInt) return fail(NPL_ERR_UNSUPPORTED, "%s: rows=%d cols=%d is too large", what, rows, cols);
@@ -474,29 +499,27 @@ int launch_quant_spans(const char* what, const Source& src, const CodeSink& out,
                     dim3((unsigned)ctas), dim3(kQuantThreads), 0, st, src, out, rows, cols, (unsigned)spans);
 }
 
-// Four blocks a thread, except where the rows are short (half of the warps'
-// lanes or more would idle) or so few that one block a thread fits on the SMs
-// at once (8 x 4096: X us against Y with four).
+// Two blocks a thread where a thread's loads are 32 bytes, except where the
+// rows are short (half of the warps' lanes or more would idle) or so few that
+// one block a thread fits on the SMs at once (8 x 4096: X us against Y).
 template <typename Source>
 int launch_quant(const char* what, const Source& src, const CodeSink& out, int rows, int cols, cudaStream_t st) {
+  constexpr int U = sizeof(typename Source::Loaded) > 32 ? 1 : 2;
   const long long blocks = (long long)rows * ((cols + kBlock - 1) / kBlock);
-  if (cols <= 4 * kBlock || blocks <= 64ll * num_sms()) return launch_quant_spans<Source, 1>(what, src, out, rows, cols, st);
-  return launch_quant_spans<Source, 4>(what, src, out, rows, cols, st);
+  if (cols <= 4 * kBlock || blocks <= 128ll * num_sms())
+    return launch_quant_spans<Source, 1>(what, src, out, rows, cols, st);
+  return launch_quant_spans<Source, U>(what, src, out, rows, cols, st);
 }
 
-template <typename T, bool kVec, bool kVecQ>
+template <typename T, int kAccess, bool kVecQ>
 int launch_rmsnorm(const T* x, long long ldx, const T* res, long long ld_res, const T* w, float eps, int rows,
                    int cols, T* sum_out, long long ld_sum, const CodeSink& out, cudaStream_t st) {
-  // Few rows: one chunk a thread, the shortest way through a row. More rows
-  // than run at once: two, which halves the share of the two barriers and of
-  // the scales (16000 x 4096: X us against Y).
-  const int lanes = (cols + kVecCols - 1) / kVecCols;
-  const int want = lanes <= kNormThreads && rows <= 2 * num_sms() ? 1 : 2;
-  const int threads = std::min(kNormThreads, (lanes + 32 * want - 1) / (32 * want) * 32);
-  const int chunks = (lanes + threads - 1) / threads;
-  auto kern = chunks <= 1   ? fp8_rmsnorm_kernel<T, 1, kVec, kVecQ>
-              : chunks <= 2 ? fp8_rmsnorm_kernel<T, 2, kVec, kVecQ>
-                            : fp8_rmsnorm_kernel<T, 0, kVec, kVecQ>;
+  const int lanes = (cols + kCols - 1) / kCols;
+  const int threads = lanes <= 1024 ? (lanes + 31) / 32 * 32 : kNormThreads;
+  auto kern = lanes <= 512    ? fp8_rmsnorm_kernel<T, 512, kAccess, kVecQ>
+              : lanes <= 704  ? fp8_rmsnorm_kernel<T, 704, kAccess, kVecQ>
+              : lanes <= 1024 ? fp8_rmsnorm_kernel<T, 1024, kAccess, kVecQ>
+                              : fp8_rmsnorm_kernel<T, 0, kAccess, kVecQ>;
   return launch_pdl("npl_fp8_rmsnorm_quant", kern, dim3((unsigned)rows), dim3((unsigned)threads), 0, st, x, ldx, res,
                     ld_res, w, eps, cols, sum_out, ld_sum, out);
 }
@@ -518,9 +541,9 @@ extern "C" int npl_fp8_quant_rows(const void* x, int x_dtype, int64_t rows, int6
     using T = decltype(t);
     const T* p = static_cast<const T*>(x);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (vec_rows(x, rows, ldx, x_dtype))
-      return launch_quant(what, RowSource<T, true>{p, ldx}, out, (int)rows, (int)cols, st);
-    return launch_quant(what, RowSource<T, false>{p, ldx}, out, (int)rows, (int)cols, st);
+    return by_access(row_access(x, rows, ldx, x_dtype), [&](auto a) {
+      return launch_quant(what, RowSource<T, a.value>{p, ldx}, out, (int)rows, (int)cols, st);
+    });
   });
 }
 
@@ -539,9 +562,10 @@ extern "C" int npl_fp8_silu_mul_quant(const void* gate, int64_t ld_gate, const v
     const T* g = static_cast<const T*>(gate);
     const T* u = static_cast<const T*>(up);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (vec_rows(gate, rows, ld_gate, dtype) && vec_rows(up, rows, ld_up, dtype))
-      return launch_quant(what, SiluSource<T, true>{g, u, ld_gate, ld_up}, out, (int)rows, (int)cols, st);
-    return launch_quant(what, SiluSource<T, false>{g, u, ld_gate, ld_up}, out, (int)rows, (int)cols, st);
+    const int access = std::min(row_access(gate, rows, ld_gate, dtype), row_access(up, rows, ld_up, dtype));
+    return by_access(access, [&](auto a) {
+      return launch_quant(what, SiluSource<T, a.value>{g, u, ld_gate, ld_up}, out, (int)rows, (int)cols, st);
+    });
   };
   return dtype == NPL_F16 ? go(__half()) : go(__nv_bfloat16());
 }
@@ -562,15 +586,17 @@ extern "C" int npl_fp8_rmsnorm_quant(const void* x, int64_t ldx, const void* res
   if (rows == 0) return NPL_OK;
   if (int rc = check_device()) return rc;
   const CodeSink out{q, ldq, scale, ld_scale};
-  const bool vec = vec_rows(x, rows, ldx, dtype) && aligned16(weight) &&
-                   (!residual || (vec_rows(residual, rows, ld_res, dtype) && vec_rows(sum_out, rows, ld_sum, dtype)));
+  int access = std::min(row_access(x, rows, ldx, dtype), row_access(weight, 1, cols, dtype));
+  if (residual)
+    access = std::min(access, std::min(row_access(residual, rows, ld_res, dtype), row_access(sum_out, rows, ld_sum, dtype)));
   const bool vecq = vec_codes(out);
   auto go = [&](auto t) {
     using T = decltype(t);
-    auto* fn = vec ? (vecq ? launch_rmsnorm<T, true, true> : launch_rmsnorm<T, true, false>)
-                   : (vecq ? launch_rmsnorm<T, false, true> : launch_rmsnorm<T, false, false>);
-    return fn(static_cast<const T*>(x), ldx, static_cast<const T*>(residual), ld_res, static_cast<const T*>(weight),
-              eps, (int)rows, (int)cols, static_cast<T*>(sum_out), ld_sum, out, static_cast<cudaStream_t>(stream));
+    return by_access(access, [&](auto a) {
+      auto* fn = vecq ? launch_rmsnorm<T, a.value, true> : launch_rmsnorm<T, a.value, false>;
+      return fn(static_cast<const T*>(x), ldx, static_cast<const T*>(residual), ld_res, static_cast<const T*>(weight),
+                eps, (int)rows, (int)cols, static_cast<T*>(sum_out), ld_sum, out, static_cast<cudaStream_t>(stream));
+    });
   };
   return dtype == NPL_F16 ? go(__half()) : go(__nv_bfloat16());
 }
@@ -583,14 +609,16 @@ extern "C" int npl_fp8_quant_weight(const void* w, int w_dtype, int64_t rows, in
   if (rows == 0) return NPL_OK;
   if (int rc = check_device()) return rc;
   const long long nb = (rows + kBlock - 1) / kBlock, kb = (cols + kBlock - 1) / kBlock;
-  if (kb > 65535) return fail(NPL_ERR_UNSUPPORTED, "%s: %lld columns (at most 65535 blocks)", what, (long long)cols);
+  if (nb * kb > kMaxInt) return fail(NPL_ERR_UNSUPPORTED, "%s: %lld blocks (at most 2^31 - 1)", what, nb * kb);
   const CodeSink out{q, ldq, scale, ld_scale};
-  const bool vec = vec_rows(w, rows, ldw, w_dtype), vecq = vec_codes(out);
+  const bool vecq = vec_codes(out);
   return by_type(w_dtype, [&](auto t) {
     using T = decltype(t);
-    auto kern = vec ? (vecq ? fp8_quant_weight_kernel<T, true, true> : fp8_quant_weight_kernel<T, true, false>)
-                    : (vecq ? fp8_quant_weight_kernel<T, false, true> : fp8_quant_weight_kernel<T, false, false>);
-    return launch_pdl(what, kern, dim3((unsigned)nb, (unsigned)kb), dim3(kWeightThreads), 0,
-                      static_cast<cudaStream_t>(stream), static_cast<const T*>(w), ldw, (int)rows, (int)cols, out);
+    return by_access(row_access(w, rows, ldw, w_dtype), [&](auto a) {
+      auto kern = vecq ? fp8_quant_weight_kernel<T, a.value, true> : fp8_quant_weight_kernel<T, a.value, false>;
+      return launch_pdl(what, kern, dim3((unsigned)(nb * kb)), dim3(kWeightThreads), 0,
+                        static_cast<cudaStream_t>(stream), static_cast<const T*>(w), ldw, (int)rows, (int)cols, (int)kb,
+                        out);
+    });
   });
 }

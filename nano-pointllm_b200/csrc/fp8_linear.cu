@@ -16,9 +16,11 @@
 // Per decode CTA (192 threads):
 //   warp 0     TMA producer: weight tile [128 x 128 B] and token tile
 //              [NT x 128 B] per block, 128-byte swizzle, a ring of stages
-//   warp 1     TMEM owner + MMA issuer: 4 MMAs of K = 32 per block into a ring
-//              of 4 accumulators
-//   warps 2-5  TMEM lane = weight row, column = token: acc += (sa sw) * D
+//   warp 1     TMEM owner + MMA issuer: 4 MMAs of K = 32 per block, a ring of
+//              4 units of 64 columns, which hold 64 / NT blocks each
+//   warps 2-5  TMEM lane = weight row, column = token: acc += (sa sw) * D, a
+//              unit at a time (waiting for every block of 16 tokens took longer
+//              than adding it up)
 //
 // Split over K: the S CTAs of a thread-block cluster share a tile's blocks.
 // Each leaves its fp32 sums in its own shared memory; after a cluster barrier
@@ -43,8 +45,10 @@ constexpr int kTileN = 128;   // weight rows per tile (MMA M) and per scale
 constexpr int kBlockK = 128;  // columns per scale = bytes per stage row (one 128-byte swizzle atom)
 constexpr int kThreads = 192;
 constexpr int kMaxStages = 6;
-constexpr int kAccBufs = 4;
+constexpr int kUnitCols = 64;  // TMEM columns handed over at a time: 64 / NT blocks
+constexpr int kUnits = 4;     // TMEM ring: 256 columns
 constexpr int kMaxSplit = 8;
+constexpr int kScaleBlocks = 32;  // blocks whose scales a decode CTA holds at a time
 
 struct Fp8LinearArgs {
   int M, N;
@@ -71,8 +75,8 @@ struct Fp8LinearArgs {
 struct Fp8Ctl {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
-  uint64_t tfull[kAccBufs];
-  uint64_t tempty[kAccBufs];
+  uint64_t tfull[kUnits];
+  uint64_t tempty[kUnits];
   uint64_t teardown;
   uint32_t tmem_base;
 };
@@ -115,6 +119,21 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// acc += d * s. Volatile, like tcgen05.ld and its wait: it stays behind the
+// wait for d. (The packed fma.rn.f32x2 has the same rate on B200, 128 FMAs a
+// cycle and SM, and its operand pairs cost moves: 1810 us against 1511 for
+// 16000 x 22016 x 4096.)
+__device__ __forceinline__ void fma_after_ld(float& acc, uint32_t d, float s) {
+  asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(__uint_as_float(d)), "f"(s));
+}
+
+__device__ __forceinline__ void lds128(const float* p, float* v) {
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+               : "r"(smem_u32(p))
+               : "memory");
+}
+
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -126,8 +145,6 @@ __device__ __forceinline__ float wide(__nv_bfloat16 v) { return __bfloat162float
 __device__ __forceinline__ void narrow(float v, __half& o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void narrow(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
-__host__ __device__ constexpr uint32_t tmem_cols_for(int nt) { return (uint32_t)(kAccBufs * nt); }
-
 // T: element type of residual and out; NT: tokens per tile.
 template <typename T, int NT>
 __global__ void __launch_bounds__(kThreads)
@@ -137,12 +154,13 @@ __global__ void __launch_bounds__(kThreads)
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                          ~uintptr_t(1023));
   __shared__ Fp8Ctl c;
-  __shared__ __align__(16) float s_scale[4][2][NT];  // per epilogue warp, double buffered
+  __shared__ __align__(16) float s_scale[kScaleBlocks][NT + 4];  // the tokens' scales times the weight's, by block
+  constexpr int U = kUnitCols / NT;  // blocks per unit
   constexpr uint32_t kStageW = kTileN * kBlockK, kStageX = NT * kBlockK;
   unsigned char* ring_w = base;
   unsigned char* ring_x = base + (size_t)p.stages * kStageW;
   constexpr uint32_t kIdesc = idesc_e4m3(kTileN, NT);
-  constexpr uint32_t kTmemCols = tmem_cols_for(NT);
+  constexpr uint32_t kTmemCols = kUnits * kUnitCols;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)(blockIdx.x % (unsigned)p.split);
@@ -158,7 +176,7 @@ __global__ void __launch_bounds__(kThreads)
       mbar_init(&c.full[i], 1);
       mbar_init(&c.empty[i], 1);
     }
-    for (int i = 0; i < kAccBufs; ++i) {
+    for (int i = 0; i < kUnits; ++i) {
       mbar_init(&c.tfull[i], 1);
       mbar_init(&c.tempty[i], 4);
     }
@@ -182,38 +200,43 @@ __global__ void __launch_bounds__(kThreads)
   for (int j = 0; j < NT; ++j) acc[j] = 0.f;
 
   if (warp == 0) {
-    if (lane == 0) {
-      const uint64_t pol_w = policy_evict_first();
-      const uint64_t pol_x = policy_evict_last();
-      auto load_w = [&](int kb, int stage) {
+    // As warp 1, all lanes run the loop and one issues: the copies' operands
+    // stay in uniform registers.
+    const bool issuer = elect_one();
+    const uint64_t pol_w = policy_evict_first();
+    const uint64_t pol_x = policy_evict_last();
+    auto load_w = [&](int kb, int stage) {
+      if (issuer) {
         mbar_arrive_expect_tx(&c.full[stage], kStageW + kStageX);
         tma_load_2d(ring_w + (size_t)stage * kStageW, &tmap_w, kb * kBlockK, n_tile * kTileN, &c.full[stage], pol_w);
-      };
-      // Weights do not depend on the kernels before this one on its stream
-      // (npl_fp8_quant_weight lets this one start only when its codes are
-      // visible), so the ring is filled with them before the wait.
-      const int ahead = min(p.stages, kb1 - kb0);
-      for (int i = 0; i < ahead; ++i) load_w(kb0 + i, i);
-      pdl_wait();
-      int stage = 0, loads = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (loads >= ahead) {
-          if (!mbar_wait(&c.empty[stage], phase ^ 1, p.status, NPL_DEV_TIMEOUT_TMA)) break;
-          load_w(kb, stage);
-        }
-        tma_load_2d(ring_x + (size_t)stage * kStageX, &tmap_x, kb * kBlockK, m_tile * NT, &c.full[stage], pol_x);
-        ++loads;
-        if (++stage == p.stages) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
-      // every issued load lands before the ring is used again or released:
-      // stage i was last loaded with the parity of that load
-      for (int i = 0; i < min(loads, p.stages); ++i)
-        mbar_wait(&c.full[i], i < stage ? phase : phase ^ 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+    };
+    // Weights do not depend on the kernels before this one on its stream
+    // (npl_fp8_quant_weight lets this one start only when its codes are
+    // visible), so the ring is filled with them before the wait.
+    const int ahead = min(p.stages, kb1 - kb0);
+    for (int i = 0; i < ahead; ++i) load_w(kb0 + i, i);
+    pdl_wait();
+    int stage = 0, loads = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (loads >= ahead) {
+        if (!poll_wait(&c.empty[stage], phase ^ 1, p.status, NPL_DEV_TIMEOUT_TMA)) break;
+        load_w(kb, stage);
+      }
+      if (issuer)
+        tma_load_2d(ring_x + (size_t)stage * kStageX, &tmap_x, kb * kBlockK, m_tile * NT, &c.full[stage], pol_x);
+      ++loads;
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
+    // every issued load lands before the ring is used again or released: stage
+    // i was last loaded with the parity of that load
+    for (int i = 0; i < min(loads, p.stages); ++i)
+      poll_wait(&c.full[i], i < stage ? phase : phase ^ 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+    __syncwarp();
   } else if (warp == 1) {
     // The whole warp runs this loop and one lane issues, so that descriptors
     // stay in uniform registers (see the prefill kernel).
@@ -222,17 +245,17 @@ __global__ void __launch_bounds__(kThreads)
     int stage = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      const int i = kb - kb0, buf = i % kAccBufs;
+      const int i = kb - kb0, unit = i / U, buf = unit % kUnits, u = i % U;
       if (!poll_wait(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA)) break;
-      if (!poll_wait(&c.tempty[buf], ((i / kAccBufs) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA)) break;
+      if (u == 0 && !poll_wait(&c.tempty[buf], ((unit / kUnits) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA)) break;
       tc_fence_after();
       const uint64_t a = desc_w + (uint32_t)stage * (kStageW >> 4), b = desc_x + (uint32_t)stage * (kStageX >> 4);
-      const uint32_t d = tmem_base + (uint32_t)(buf * NT);
+      const uint32_t d = tmem_base + (uint32_t)(buf * kUnitCols + u * NT);
       if (issuer) {
         mma_e4m3<false>(d, a, b, kIdesc);
 #pragma unroll
         for (int kk = 1; kk < kBlockK / 32; ++kk) mma_e4m3<true>(d, a + kk * 2, b + kk * 2, kIdesc);
-        tc_commit(&c.tfull[buf]);
+        if (u == U - 1 || kb + 1 == kb1) tc_commit(&c.tfull[buf]);
         tc_commit(&c.empty[stage]);
       }
       __syncwarp();
@@ -247,42 +270,58 @@ __global__ void __launch_bounds__(kThreads)
     __syncwarp();
   } else {
     pdl_wait();
-    // Lanes hold the scales of tokens lane and lane + 32 of the next block.
-    constexpr int kPer = (NT + 31) / 32;
-    float next[kPer], next_sw;
-    auto fetch = [&](int kb) {
-      next_sw = p.sw[(long long)n_tile * p.ld_sw + kb];
+    bool ok = true;
+    int unit = 0;
+    for (int kc = kb0; ok && kc < kb1; kc += kScaleBlocks) {
+      // The scales of the next kScaleBlocks blocks: a warp reads a token's with
+      // one load, all loads of a thread at once.
+      {
+        const int b = kc + lane;
+        const float w = b < kb1 ? p.sw[(long long)n_tile * p.ld_sw + b] : 0.f;
+        float a[NT / 4];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int m = m_tile * NT + lane + 32 * i;
-        next[i] = (lane + 32 * i < NT && m < p.M) ? p.sa[(long long)m * p.ld_sa + kb] : 0.f;
+        for (int i = 0; i < NT / 4; ++i) {
+          const int m = m_tile * NT + 4 * i + quarter;
+          a[i] = b < kb1 && m < p.M ? p.sa[(long long)m * p.ld_sa + b] : 0.f;
+        }
+        if (kc > kb0) asm volatile("bar.sync 1, 128;" ::: "memory");  // the scales before are read
+#pragma unroll
+        for (int i = 0; i < NT / 4; ++i) s_scale[lane][4 * i + quarter] = __fmul_rn(a[i], w);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
       }
-    };
-    if (kb0 < kb1) fetch(kb0);
-    for (int kb = kb0; kb < kb1; ++kb) {
-      const int i = kb - kb0, buf = i % kAccBufs;
-      float* sc = s_scale[quarter][i & 1];
+      const int kn = min(kScaleBlocks, kb1 - kc);
+      for (int k = 0; k < kn; k += U, ++unit) {
+        const int buf = unit % kUnits;
+        if (!poll_wait(&c.tfull[buf], (unit / kUnits) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * kUnitCols);
 #pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        if (lane + 32 * e < NT) sc[lane + 32 * e] = __fmul_rn(next[e], next_sw);
-      __syncwarp();
-      if (kb + 1 < kb1) fetch(kb + 1);
-      if (!mbar_wait(&c.tfull[buf], (i / kAccBufs) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) break;
-      tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * NT);
+        for (int h = 0; h < 2; ++h) {
+          float sc[32];  // loaded ahead of their uses
 #pragma unroll
-      for (int c0 = 0; c0 < NT; c0 += 16) {
-        int32_t d[2][8];
-        tmem_ld_x8(taddr + c0, d[0]);
-        tmem_ld_x8(taddr + c0 + 8, d[1]);
-        tmem_wait_ld();
+          for (int q = 0; q < 32; q += 4) {
+            const int at = 32 * h + q;
+            lds128(&s_scale[k + at / NT][at % NT], sc + q);
+          }
+          uint32_t d[32];
+          tmem_ld_x32(taddr + 32 * h, d);
+          tmem_wait_ld();
+          if (h == 1) {  // the unit is read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c.tempty[buf]);
+          }
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          acc[c0 + j] = __fmaf_rn(__int_as_float(d[j / 8][j % 8]), sc[c0 + j], acc[c0 + j]);
+          for (int q = 0; q < 32; ++q) {
+            const int at = 32 * h + q;  // block at / NT, which a last unit may lack: what TMEM holds there is not used
+            if (at % NT == 0 && k + at / NT >= kn) break;
+            fma_after_ld(acc[at % NT], d[q], sc[q]);
+          }
+        }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c.tempty[buf]);
     }
   }
 
@@ -317,11 +356,14 @@ __global__ void __launch_bounds__(kThreads)
     };
     if (p.split > 1) {
       for (int j = j0; j < j1; ++j) {
-        float v = 0.f;
-        for (int r = 0; r < p.split; ++r) {
-          const float x = ld_cluster_f32(cluster_map(part + j * kTileN + row, (uint32_t)r));
-          v = r == 0 ? x : __fadd_rn(v, x);
-        }
+        float x[kMaxSplit];  // all ranks' loads at once
+#pragma unroll
+        for (int r = 0; r < kMaxSplit; ++r)
+          if (r < p.split) x[r] = ld_cluster_f32(cluster_map(part + j * kTileN + row, (uint32_t)r));
+        float v = x[0];
+#pragma unroll
+        for (int r = 1; r < kMaxSplit; ++r)
+          if (r < p.split) v = __fadd_rn(v, x[r]);
         finish(j, v);
       }
     } else {
@@ -386,14 +428,6 @@ struct PrefillCtl {
   uint32_t tmem_base;
   __align__(16) float scale[2][kPGroups][kPScaleBlocks][kPScaleLd];
 };
-
-// acc += d * s. Volatile, like tcgen05.ld and its wait: it stays behind the
-// wait for d. (The packed fma.rn.f32x2 has the same rate on B200, 128 FMAs a
-// cycle and SM, and its operand pairs cost moves: 1810 us against 1511 for
-// 16000 x 22016 x 4096.)
-__device__ __forceinline__ void fma_after_ld(float& acc, uint32_t d, float s) {
-  asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(__uint_as_float(d)), "f"(s));
-}
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* smem, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
@@ -797,8 +831,13 @@ int launch_decode(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
   const int smem = std::max(p.stages * stage + 1024, kDecodeSmemMin);
   const long long m_tiles = (p.M + NT - 1) / NT;
   const long long tiles = m_tiles * p.n_tiles;
-  p.split = 1;
-  while (p.split < kMaxSplit && tiles * p.split * 2 <= 2ll * num_sms() && p.split * 2 <= p.k_blocks) p.split *= 2;
+  // As many CTAs per tile as keep 1.75 CTAs an SM (beyond it not all clusters
+  // run at once: 96 tiles of 32 blocks take 12.0 us unsplit, 13.9 two-way, 17.9
+  // three-way; 76 tiles 12.4, 13.0, 10.8, 15.3 four-way) and two blocks a CTA.
+  // Two CTAs cost more to join than they save at any size tried (8 x 5120..16384
+  // x 4096).
+  p.split = (int)std::max(1ll, std::min({(long long)kMaxSplit, 7ll * num_sms() / (4 * tiles), (long long)p.k_blocks / 2}));
+  if (p.split == 2) p.split = 1;
   if (tiles * p.split > 2147483647ll)
     return fail(NPL_ERR_UNSUPPORTED, "npl_fp8_linear: M=%d N=%d has too many tiles", p.M, p.N);
   auto kern = fp8_linear_decode_kernel<T, NT>;

@@ -413,8 +413,8 @@ constexpr uint32_t kPStageX = kPM * kBlockK, kPStageW = kPN / 2 * kBlockK;
 constexpr uint32_t kPStage = kPStageX + kPStageW;
 constexpr int kPOutCols = 64;                         // columns staged at a time by a warpgroup
 constexpr uint32_t kPOut = kPM * kPOutCols * 2;       // 16 KB
-constexpr int kPScaleBlocks = 8;                      // blocks of scales loaded at a time
-constexpr int kPScaleLd = kPM + 4;                    // 4 (mod 32): 8 blocks x 4 tokens of a warp hit 32 banks
+constexpr int kPScaleBlocks = 8;                     // blocks of scales loaded at a time
+constexpr int kPScaleLd = kPM + 4;                    // a warp's 8 blocks x 4 tokens hit 32 banks
 constexpr int kPSmem = kPStages * (int)kPStage + kPGroups * (int)kPOut + 1024;
 
 struct PrefillCtl {
@@ -463,12 +463,13 @@ __device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t adesc, u
       : "memory");
 }
 
-// Completion of the MMAs issued so far arrives on this barrier in both CTAs.
-__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
+// Completion of the MMAs issued so far arrives on this barrier in both CTAs
+// (`mask`: their ranks in the cluster, as bits).
+__device__ __forceinline__ void tc_commit_pair(uint64_t* bar, uint16_t mask) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"(mask)
       : "memory");
 }
 
@@ -506,8 +507,9 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
   return u;
 }
 
-template <typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
+// kSplit: pairs per tile, which share its blocks (1 or 2).
+template <typename T, int kSplit>
+__global__ void __launch_bounds__(kPThreads, 1)
     fp8_linear_prefill_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                               const __grid_constant__ CUtensorMap tmap_out, const Fp8LinearArgs p) {
   extern __shared__ unsigned char smem_raw[];
@@ -519,8 +521,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
   constexpr uint32_t kTmemCols = 2 * kPN;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = p.m_tiles * p.n_tiles;
-  const int rank = (int)(blockIdx.x & 1u);
-  const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+  constexpr int cluster_size = 2 * kSplit;
+  const int cluster_rank = (int)(blockIdx.x % (unsigned)cluster_size);
+  const int rank = cluster_rank & 1;                   // in the pair
+  const uint32_t leader = kSplit == 1 ? 0 : (uint32_t)cluster_rank & ~1u;  // the pair's CTA 0
+  const uint16_t both = (uint16_t)(3u << leader);
+  const int part = kSplit == 1 ? 0 : cluster_rank >> 1;  // of the tile's blocks
+  const int kb0 = (int)((long long)part * p.k_blocks / kSplit);
+  const int kb1 = (int)((long long)(part + 1) * p.k_blocks / kSplit);
+  const int cluster = (int)(blockIdx.x / (unsigned)cluster_size), clusters = (int)(gridDim.x / (unsigned)cluster_size);
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tmap_x);
@@ -561,17 +570,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
       int stage = 0, loads = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = pair; ok && t < tiles; t += pairs) {
+      for (int t = cluster; ok && t < tiles; t += clusters) {
         int m_tile, n_tile;
         prefill_tile(p, t, m_tile, n_tile);
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&c.empty[stage], phase ^ 1, p.status, NPL_DEV_TIMEOUT_TMA)) {
             ok = false;
             break;
           }
           unsigned char* at = ring + (size_t)stage * kPStage;
           if (rank == 0) mbar_arrive_expect_tx(&c.full[stage], 2 * kPStage);
-          const uint32_t bar = cluster_map(&c.full[stage], 0);
+          const uint32_t bar = cluster_map(&c.full[stage], leader);
           tma_load_2d_pair(at, &tmap_x, kb * kBlockK, (2 * m_tile + rank) * kPM, bar, pol);
           tma_load_2d_pair(at + kPStageX, &tmap_w, kb * kBlockK, n_tile * kPN + rank * (kPN / 2), bar, pol);
           loads = min(loads + 1, kPStages);
@@ -598,8 +607,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
       int stage = 0;
       uint32_t phase = 0, it = 0;
       bool ok = rank == 0;
-      for (int t = pair; ok && t < tiles; t += pairs) {
-        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+      for (int t = cluster; ok && t < tiles; t += clusters) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const uint32_t buf = it & 1;
           if (!poll_wait(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA) ||
               !poll_wait(&c.tempty[buf], ((it >> 1) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA)) {
@@ -613,8 +622,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
             mma_e4m3_pair<false>(d, a, b, kIdesc);
 #pragma unroll
             for (int kk = 1; kk < kBlockK / 32; ++kk) mma_e4m3_pair<true>(d, a + kk * 2, b + kk * 2, kIdesc);
-            tc_commit_pair(&c.tfull[buf]);
-            tc_commit_pair(&c.empty[stage]);
+            tc_commit_pair(&c.tfull[buf], both);
+            tc_commit_pair(&c.empty[stage], both);
           }
           __syncwarp();
           if (++stage == kPStages) {
@@ -624,33 +633,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
         }
       }
       // all MMAs complete, in both CTAs' view, before TMEM is freed
-      if (rank == 0 && issuer) tc_commit_pair(&c.teardown);
+      if (rank == 0 && issuer) tc_commit_pair(&c.teardown, both);
       poll_wait(&c.teardown, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
       __syncwarp();
     } else if (warp >= 2) {
-      // 8 blocks x 4 tokens per load of a warp, transposed into shared memory
-      const int kk = lane & 7, r0 = (warp - 2) * 4 + (lane >> 3);
+      // A load of a warp reads kPScaleBlocks blocks of 32 / kPScaleBlocks tokens;
+      // transposed into shared memory. Eight loads before the first store: the
+      // compiler does not move them across.
+      constexpr int kRows = 32 / kPScaleBlocks, kStep = 2 * kRows;
+      const int kk = lane % kPScaleBlocks, r0 = (warp - 2) * kRows + lane / kPScaleBlocks;
       uint32_t chunk = 0;
       bool ok = true;
-      for (int t = pair; ok && t < tiles; t += pairs) {
+      for (int t = cluster; ok && t < tiles; t += clusters) {
         int m_tile, n_tile;
         prefill_tile(p, t, m_tile, n_tile);
         const int m0 = (2 * m_tile + rank) * kPM;
         const float* sw0 = p.sw + (long long)(2 * n_tile) * p.ld_sw;
         const bool two = (2 * n_tile + 1) * kTileN < p.N;  // the tile's second half has weight rows
-        for (int kb = kk; kb - kk < p.k_blocks; kb += kPScaleBlocks, ++chunk) {
+        for (int kb = kb0 + kk; kb - kk < kb1; kb += kPScaleBlocks, ++chunk) {
           const uint32_t buf = chunk & 1;
-          const bool in = kb < p.k_blocks;
+          const bool in = kb < kb1;
           const float w0 = in ? sw0[kb] : 0.f, w1 = in && two ? sw0[p.ld_sw + kb] : 0.f;
           if (!mbar_wait(&c.sempty[buf], ((chunk >> 1) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
             ok = false;
             break;
           }
-#pragma unroll 8
-          for (int r = r0; r < kPM; r += 8) {
-            const float a = (in && m0 + r < p.M) ? p.sa[(long long)(m0 + r) * p.ld_sa + kb] : 0.f;
-            c.scale[buf][0][kk][r] = __fmul_rn(a, w0);
-            c.scale[buf][1][kk][r] = __fmul_rn(a, w1);
+          for (int r = r0; r < kPM; r += 8 * kStep) {
+            float a[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int m = m0 + r + i * kStep;
+              a[i] = in && m < p.M ? p.sa[(long long)m * p.ld_sa + kb] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              c.scale[buf][0][kk][r + i * kStep] = __fmul_rn(a[i], w0);
+              c.scale[buf][1][kk][r + i * kStep] = __fmul_rn(a[i], w1);
+            }
           }
           mbar_arrive(&c.sfull[buf]);
         }
@@ -665,11 +684,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
     auto group_bar = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
     const T* res = static_cast<const T*>(p.residual);
     T* out = static_cast<T*>(p.out);
-    const uint32_t tempty0 = cluster_map(&c.tempty[0], 0), tempty1 = cluster_map(&c.tempty[1], 0);
+    const uint32_t tempty0 = cluster_map(&c.tempty[0], leader), tempty1 = cluster_map(&c.tempty[1], leader);
     const uint32_t taddr0 = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + group * kPGroupCols;
     uint32_t it = 0, chunk = 0;
     bool ok = true;
-    for (int t = pair; ok && t < tiles; t += pairs) {
+    for (int t = cluster; ok && t < tiles; t += clusters) {
       int m_tile, n_tile;
       prefill_tile(p, t, m_tile, n_tile);
       const int m_base = (2 * m_tile + rank) * kPM, m = m_base + row;
@@ -677,10 +696,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
       float acc[kPGroupCols];
 #pragma unroll
       for (int j = 0; j < kPGroupCols; ++j) acc[j] = 0.f;
-      for (int kb = 0; ok && kb < p.k_blocks; kb += kPScaleBlocks, ++chunk) {
+      for (int kb = kb0; ok && kb < kb1; kb += kPScaleBlocks, ++chunk) {
         const uint32_t sbuf = chunk & 1;
         ok = poll_wait(&c.sfull[sbuf], (chunk >> 1) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
-        const int kn = min(kPScaleBlocks, p.k_blocks - kb);
+        const int kn = min(kPScaleBlocks, kb1 - kb);
         const float* scale = &c.scale[sbuf][group][0][row];
         for (int kk = 0; ok && kk < kn; ++kk, ++it, scale += kPScaleLd) {
           const uint32_t buf = it & 1;
@@ -709,11 +728,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&c.sempty[sbuf]);  // the chunk of scales is read
       }
+      int boxes = kPGroupCols / kPOutCols, n_out = n0;
+      if constexpr (kSplit > 1) {
+        // The sums of this CTA's blocks go to its ring, which its last MMAs are
+        // done with, [column][token]; after the barrier the CTAs of one rank add
+        // those of parts 0, 1 for 128 columns each, 64 a warpgroup.
+        static_assert(kSplit * kPGroups * kPOutCols == kPN);
+        float* sums = reinterpret_cast<float*>(ring);
+        if (ok) {
+#pragma unroll
+          for (int j = 0; j < kPGroupCols; ++j) sums[(group * kPGroupCols + j) * kPM + row] = acc[j];
+        }
+        cluster_arrive_release();
+        cluster_wait_acquire();
+        const int col = (part * kPGroups + group) * kPOutCols;
+        boxes = 1;
+        n_out = n_tile * kPN + col;
+        if (ok) {
+          uint32_t from[kSplit];
+#pragma unroll
+          for (int q = 0; q < kSplit; ++q) from[q] = cluster_map(sums + col * kPM + row, (uint32_t)(2 * q + rank));
+#pragma unroll
+          for (int j = 0; j < kPOutCols; ++j) {
+            float v = ld_cluster_f32(from[0] + j * kPM * 4);
+#pragma unroll
+            for (int q = 1; q < kSplit; ++q) v = __fadd_rn(v, ld_cluster_f32(from[q] + j * kPM * 4));
+            acc[j] = v;
+          }
+        }
+      }
       if (!ok) break;
       // bias, residual, rounding; 64 columns at a time through shared memory
 #pragma unroll
       for (int h = 0; h < kPGroupCols / kPOutCols; ++h) {
-        const int nh = n0 + h * kPOutCols;
+        if (h >= boxes) break;
+        const int nh = n_out + h * kPOutCols;
         if (elected) tma_store_wait_read();
         group_bar();  // the staging buffer is free
 #pragma unroll
@@ -768,10 +817,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
     }
     if (elected) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
+  if (kSplit > 1 && warp < 4) {  // the epilogue warps' barrier over the sums
+    cluster_arrive_release();
+    cluster_wait_acquire();
+  }
 
   tc_fence_before();
   __syncthreads();
-  cluster_arrive_release();  // neither CTA's shared memory or TMEM is given up while the pair uses it
+  cluster_arrive_release();  // no CTA's shared memory or TMEM is given up while another uses it
   cluster_wait_acquire();
   if (warp == 1) {
     tc_fence_after();
@@ -821,6 +874,16 @@ struct Operands {
 constexpr int kDecodeSmemMin = 78 * 1024;
 constexpr int kDecodeSmemMax = 110 * 1024;
 
+// CTAs that share a decode tile: as many as keep 1.75 CTAs an SM (beyond it not
+// all clusters run at once: 96 tiles of 32 blocks take 12.0 us unsplit, 13.9
+// two-way, 17.9 three-way; 76 tiles 12.4, 13.0, 10.8, 15.3 four-way) and two
+// blocks a CTA. Two CTAs cost more to join than they save at any size tried (8 x
+// 5120..16384 x 4096).
+int decode_split(long long tiles, int k_blocks) {
+  const long long s = std::min({(long long)kMaxSplit, 7ll * num_sms() / (4 * tiles), (long long)k_blocks / 2});
+  return s <= 2 ? 1 : (int)s;
+}
+
 template <typename T, int NT>
 int launch_decode(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
   CUtensorMap tw, tx;
@@ -831,13 +894,7 @@ int launch_decode(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
   const int smem = std::max(p.stages * stage + 1024, kDecodeSmemMin);
   const long long m_tiles = (p.M + NT - 1) / NT;
   const long long tiles = m_tiles * p.n_tiles;
-  // As many CTAs per tile as keep 1.75 CTAs an SM (beyond it not all clusters
-  // run at once: 96 tiles of 32 blocks take 12.0 us unsplit, 13.9 two-way, 17.9
-  // three-way; 76 tiles 12.4, 13.0, 10.8, 15.3 four-way) and two blocks a CTA.
-  // Two CTAs cost more to join than they save at any size tried (8 x 5120..16384
-  // x 4096).
-  p.split = (int)std::max(1ll, std::min({(long long)kMaxSplit, 7ll * num_sms() / (4 * tiles), (long long)p.k_blocks / 2}));
-  if (p.split == 2) p.split = 1;
+  p.split = decode_split(tiles, p.k_blocks);
   if (tiles * p.split > 2147483647ll)
     return fail(NPL_ERR_UNSUPPORTED, "npl_fp8_linear: M=%d N=%d has too many tiles", p.M, p.N);
   auto kern = fp8_linear_decode_kernel<T, NT>;
@@ -878,19 +935,30 @@ int launch_prefill(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
   if (tiles > 1ll << 30)
     return fail(NPL_ERR_UNSUPPORTED, "npl_fp8_linear: M=%d N=%d has too many tiles", p.M, p.N);
   p.raster_g = std::min(8, p.m_tiles);
-  auto kern = fp8_linear_prefill_kernel<T>;
+  // Few tiles: two pairs share one where all run at once and have 8 blocks
+  // each or more (512 x 4096 x 11008: 30.4 us against 45.2; 256 x 4096 x 1024,
+  // with 4 blocks each, 10.2 against 9.4). Four pairs, clusters of 8 CTAs with an
+  // SM each, take 29 us where two take 16 (256 x 4096 x 4096).
+  const int pairs = num_sms() / 2;
+  const bool split = 2 * tiles <= pairs && p.k_blocks >= 16;
+  auto kern = split ? fp8_linear_prefill_kernel<T, 2> : fp8_linear_prefill_kernel<T, 1>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPSmem) != cudaSuccess)
     return launch_status("npl_fp8_linear: smem attribute");
-  return launch_pdl("npl_fp8_linear", kern, dim3(2 * (unsigned)std::min<long long>(tiles, num_sms() / 2)),
-                    dim3(kPThreads), (size_t)kPSmem, st, tx, tw, to, p);
+  const unsigned clusters = (unsigned)std::min<long long>(tiles, pairs), size = split ? 4 : 2;
+  return launch_pdl_cluster("npl_fp8_linear", kern, dim3(clusters * size), dim3(kPThreads), (size_t)kPSmem, st, size, tx,
+                            tw, to, p);
 }
 
+// Decode tiles up to 64 tokens. Two rows of them, up to 128 tokens, as long as
+// they still split three ways (128 x 4096 x 4096: 12.1 us against 15.3 with
+// prefill tiles; 128 x 12288 x 4096, which does not split: 21.0 against 20.1;
+// four rows, 200 x 4096 x 4096: 20.0 against 15.5).
 template <typename T>
 int launch(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
-  if (p.M > 64) return launch_prefill<T>(o, p, st);
   if (p.M <= 16) return launch_decode<T, 16>(o, p, st);
   if (p.M <= 32) return launch_decode<T, 32>(o, p, st);
-  return launch_decode<T, 64>(o, p, st);
+  if (p.M <= 64 || (p.M <= 128 && decode_split(2ll * p.n_tiles, p.k_blocks) >= 3)) return launch_decode<T, 64>(o, p, st);
+  return launch_prefill<T>(o, p, st);
 }
 
 }  // namespace

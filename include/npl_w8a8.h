@@ -405,8 +405,10 @@ int npl_tp_allreduce_dequant(const npl_tp_peers* peers, const int32_t* acc, int 
  * Sizes and strides are 64-bit, strides in elements between rows (>= the row's
  * length; the columns of a row are contiguous). Any sizes: no row or column
  * count has to be a multiple of anything, inputs need the alignment of their
- * elements only (16-byte aligned rows are faster). Nothing beyond the given
- * rows and columns is read or written. rows == 0 launches nothing.
+ * elements only (32-byte aligned rows are fastest). Nothing outside the given
+ * rows and columns is written, and nothing before the first or after the last
+ * element read (unaligned rows are read with what lies between them). rows == 0
+ * launches nothing.
  * q: e4m3 codes [rows, cols], stride ldq. scale: fp32 [rows, ceil(cols /
  * 128)], stride ld_scale. dtype: NPL_F16 or NPL_BF16, and NPL_F32 where said.
  * No workspace: calls on different streams share nothing.

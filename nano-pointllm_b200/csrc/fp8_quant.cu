@@ -56,9 +56,39 @@ __device__ __forceinline__ void ld32(const void* p, uint32_t* r) {  // one 256-b
                : "l"(p));
 }
 
-// The first n of 16 consecutive elements at p (zeros after them).
+// 16 consecutive elements at any p: the aligned 16-byte words around them,
+// shifted into place. [lo, hi) bounds what may be read; false where the words
+// do not lie in it. Element by element 1000 x 5003 fp16 took X us, so Y.
+template <typename T>
+__device__ __forceinline__ bool load_shifted(const T* p, const T* lo, const T* hi, Raw<T>& r) {
+  constexpr int W = Raw<T>::kWords;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const uint32_t off = (uint32_t)at & 15u;
+  const uint4* from = reinterpret_cast<const uint4*>(at - off);
+  if (from < reinterpret_cast<const uint4*>(lo) || from + (W / 4 + 1) > reinterpret_cast<const uint4*>(hi)) return false;
+  uint32_t w[W + 4];
+#pragma unroll
+  for (int i = 0; i < W / 4 + 1; ++i) {
+    const uint4 x = from[i];
+    w[4 * i] = x.x;
+    w[4 * i + 1] = x.y;
+    w[4 * i + 2] = x.z;
+    w[4 * i + 3] = x.w;
+  }
+#pragma unroll
+  for (int i = 0; i < W + 3; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < W + 1; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+  uint32_t* out = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < W; ++i) out[i] = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], (off & 2) * 8) : w[i];
+  return true;
+}
+
+// The first n of 16 consecutive elements at p (zeros after them) of a tensor
+// that lies in [lo, hi).
 template <int kAccess, typename T>
-__device__ __forceinline__ Raw<T> load16(const T* p, int n) {
+__device__ __forceinline__ Raw<T> load16(const T* p, int n, const T* lo, const T* hi) {
   Raw<T> r;
   if (kAccess != kElements && n >= kCols) {
     uint32_t* w = reinterpret_cast<uint32_t*>(&r);
@@ -72,14 +102,16 @@ __device__ __forceinline__ Raw<T> load16(const T* p, int n) {
     }
     return r;
   }
+  if (kAccess == kElements && n >= kCols && load_shifted(p, lo, hi, r)) return r;
 #pragma unroll
   for (int i = 0; i < kCols; ++i) r.e[i] = i < n ? p[i] : T(0.0f);
   return r;
 }
 
-template <int kAccess, typename T>
-__device__ __forceinline__ void store16(T* p, const Raw<T>& r, int n) {
-  if (kAccess != kElements && n >= kCols) {
+// The first n of 16 elements; by16: p is 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const Raw<T>& r, int n, bool by16) {
+  if (by16 && n >= kCols) {
     const uint4* w = reinterpret_cast<const uint4*>(&r);
 #pragma unroll
     for (int i = 0; i < Raw<T>::kWords / 4; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
@@ -230,8 +262,9 @@ struct RowSource {  // the row itself
   using Kept = Raw<T>;
   const T* x;
   long long ldx;
+  const T* end;
   __device__ __forceinline__ Loaded load(int row, int col, int n) const {
-    return load16<kAccess>(x + row * ldx + col, n);
+    return load16<kAccess>(x + row * ldx + col, n, x, end);
   }
   __device__ __forceinline__ static Kept keep(const Loaded& r) { return r; }
   __device__ __forceinline__ static uint32_t key(const Kept& k) { return key_of(k); }
@@ -252,8 +285,10 @@ struct SiluSource {
   const T* gate;
   const T* up;
   long long ld_gate, ld_up;
+  const T *gate_end, *up_end;
   __device__ __forceinline__ Loaded load(int row, int col, int n) const {
-    return {load16<kAccess>(gate + row * ld_gate + col, n), load16<kAccess>(up + row * ld_up + col, n)};
+    return {load16<kAccess>(gate + row * ld_gate + col, n, gate, gate_end),
+            load16<kAccess>(up + row * ld_up + col, n, up, up_end)};
   }
   __device__ __forceinline__ static Kept keep(const Loaded& r) {
     Kept k;
@@ -335,7 +370,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(typename Source::Loaded)
 template <typename T, int kMaxThreads, int kAccess, bool kVecQ>
 __global__ void __launch_bounds__(kMaxThreads ? kMaxThreads : kNormThreads, kMaxThreads == 704 ? 2 : 1)
     fp8_rmsnorm_kernel(const T* x, long long ldx, const T* res, long long ld_res, const T* __restrict__ w, float eps,
-                       int cols, T* sum_out, long long ld_sum, const CodeSink out) {  // sum_out may be x or res
+                       int cols, T* sum_out, long long ld_sum, bool sum_by16, const CodeSink out) {  // sum_out may be x or res
   constexpr bool kInRegs = kMaxThreads > 0;
   __shared__ float red[32];
   pdl_wait();
@@ -344,8 +379,9 @@ __global__ void __launch_bounds__(kMaxThreads ? kMaxThreads : kNormThreads, kMax
   const int lane = threadIdx.x % kGroup;
   const int step = (int)blockDim.x * kCols;
   const int col0 = (int)threadIdx.x * kCols;
+  // the rows of p end with the last CTA's; w, with ld 0, is one row
   auto fetch = [&](const T* p, long long ld, int col) {
-    return load16<kAccess>(p + row * ld + (col < cols ? col : 0), cols - col);
+    return load16<kAccess>(p + row * ld + (col < cols ? col : 0), cols - col, p, p + (gridDim.x - 1) * ld + cols);
   };
   Raw<T> kept, other;
   float ss = 0.f;
@@ -360,7 +396,7 @@ __global__ void __launch_bounds__(kMaxThreads ? kMaxThreads : kNormThreads, kMax
 #pragma unroll
       for (int i = 0; i < kCols; ++i) kept.e[i] = from_f32<T>(__fadd_rn(v[i], r[i]));
       widen(kept, v);
-      store16<kAccess>(sum_out + row * ld_sum + (col < cols ? col : 0), kept, cols - col);
+      store16(sum_out + row * ld_sum + (col < cols ? col : 0), kept, cols - col, sum_by16);
     }
 #pragma unroll
     for (int i = 0; i < kCols; ++i) ss = __fmaf_rn(v[i], v[i], ss);
@@ -412,7 +448,8 @@ __global__ void __launch_bounds__(kWeightThreads, 3) fp8_quant_weight_kernel(con
   for (int i = 0; i < kSteps; ++i) {
     const int row = row0 + i * kWeightRows;
     const bool in = row < rows && col < cols;
-    raw[i] = load16<kAccess>(w + (in ? (long long)row * ldw + col : 0), in ? cols - col : 0);
+    raw[i] = load16<kAccess>(w + (in ? (long long)row * ldw + col : 0), in ? cols - col : 0, w,
+                             w + (long long)(rows - 1) * ldw + cols);
   }
   uint32_t a = 0;
 #pragma unroll
@@ -513,7 +550,7 @@ int launch_quant(const char* what, const Source& src, const CodeSink& out, int r
 
 template <typename T, int kAccess, bool kVecQ>
 int launch_rmsnorm(const T* x, long long ldx, const T* res, long long ld_res, const T* w, float eps, int rows,
-                   int cols, T* sum_out, long long ld_sum, const CodeSink& out, cudaStream_t st) {
+                   int cols, T* sum_out, long long ld_sum, bool sum_by16, const CodeSink& out, cudaStream_t st) {
   const int lanes = (cols + kCols - 1) / kCols;
   const int threads = lanes <= 1024 ? (lanes + 31) / 32 * 32 : kNormThreads;
   auto kern = lanes <= 512    ? fp8_rmsnorm_kernel<T, 512, kAccess, kVecQ>
@@ -521,7 +558,7 @@ int launch_rmsnorm(const T* x, long long ldx, const T* res, long long ld_res, co
               : lanes <= 1024 ? fp8_rmsnorm_kernel<T, 1024, kAccess, kVecQ>
                               : fp8_rmsnorm_kernel<T, 0, kAccess, kVecQ>;
   return launch_pdl("npl_fp8_rmsnorm_quant", kern, dim3((unsigned)rows), dim3((unsigned)threads), 0, st, x, ldx, res,
-                    ld_res, w, eps, cols, sum_out, ld_sum, out);
+                    ld_res, w, eps, cols, sum_out, ld_sum, sum_by16, out);
 }
 
 }  // namespace
@@ -542,7 +579,7 @@ extern "C" int npl_fp8_quant_rows(const void* x, int x_dtype, int64_t rows, int6
     const T* p = static_cast<const T*>(x);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return by_access(row_access(x, rows, ldx, x_dtype), [&](auto a) {
-      return launch_quant(what, RowSource<T, a.value>{p, ldx}, out, (int)rows, (int)cols, st);
+      return launch_quant(what, RowSource<T, a.value>{p, ldx, p + (rows - 1) * ldx + cols}, out, (int)rows, (int)cols, st);
     });
   });
 }
@@ -564,7 +601,8 @@ extern "C" int npl_fp8_silu_mul_quant(const void* gate, int64_t ld_gate, const v
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int access = std::min(row_access(gate, rows, ld_gate, dtype), row_access(up, rows, ld_up, dtype));
     return by_access(access, [&](auto a) {
-      return launch_quant(what, SiluSource<T, a.value>{g, u, ld_gate, ld_up}, out, (int)rows, (int)cols, st);
+      const SiluSource<T, a.value> src{g, u, ld_gate, ld_up, g + (rows - 1) * ld_gate + cols, u + (rows - 1) * ld_up + cols};
+      return launch_quant(what, src, out, (int)rows, (int)cols, st);
     });
   };
   return dtype == NPL_F16 ? go(__half()) : go(__nv_bfloat16());
@@ -587,15 +625,19 @@ extern "C" int npl_fp8_rmsnorm_quant(const void* x, int64_t ldx, const void* res
   if (int rc = check_device()) return rc;
   const CodeSink out{q, ldq, scale, ld_scale};
   int access = std::min(row_access(x, rows, ldx, dtype), row_access(weight, 1, cols, dtype));
-  if (residual)
-    access = std::min(access, std::min(row_access(residual, rows, ld_res, dtype), row_access(sum_out, rows, ld_sum, dtype)));
+  // the row that is not kept in registers is read back from the sum
+  if (residual) access = std::min(access, row_access(residual, rows, ld_res, dtype));
+  const bool sum_by16 = residual && row_access(sum_out, rows, ld_sum, dtype) >= kBy16;
+  if (residual && (cols + kCols - 1) / kCols > 1024)
+    access = std::min(access, row_access(sum_out, rows, ld_sum, dtype));
   const bool vecq = vec_codes(out);
   auto go = [&](auto t) {
     using T = decltype(t);
     return by_access(access, [&](auto a) {
       auto* fn = vecq ? launch_rmsnorm<T, a.value, true> : launch_rmsnorm<T, a.value, false>;
       return fn(static_cast<const T*>(x), ldx, static_cast<const T*>(residual), ld_res, static_cast<const T*>(weight),
-                eps, (int)rows, (int)cols, static_cast<T*>(sum_out), ld_sum, out, static_cast<cudaStream_t>(stream));
+                eps, (int)rows, (int)cols, static_cast<T*>(sum_out), ld_sum, sum_by16, out,
+                static_cast<cudaStream_t>(stream));
     });
   };
   return dtype == NPL_F16 ? go(__half()) : go(__nv_bfloat16());

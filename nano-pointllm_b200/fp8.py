@@ -81,11 +81,6 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _ld(t: torch.Tensor) -> int:
-    """Row stride of a 2-D tensor; a single row's is its length at least."""
-    return max(t.stride(0), t.shape[1])
-
-
 def _new_codes(rows: int, k: int, device: torch.device) -> torch.Tensor:
     """e4m3 [rows, K] whose rows start on 16-byte boundaries, as the linear reads them."""
     return torch.empty_strided((rows, k), (-(-k // 16) * 16, 1), dtype=_E4M3, device=device)
@@ -113,7 +108,7 @@ def quantize_token_blocks(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     dev, kb = x.device, _blocks(k)
     q, s = _new_codes(m, k, dev), _new_scales(m, kb, dev)
     if m:
-        _call(L.lib.npl_fp8_quant_rows, dev, v.data_ptr(), dt, m, k, _ld(v), q.data_ptr(), q.stride(0), s.data_ptr(), kb)
+        _call(L.lib.npl_fp8_quant_rows, dev, v.data_ptr(), dt, m, k, v.stride(0), q.data_ptr(), q.stride(0), s.data_ptr(), kb)
     return (q, s) if x.dim() == 2 else (q.reshape(x.shape), s.reshape(*x.shape[:-1], kb))
 
 
@@ -128,7 +123,7 @@ def quantize_weight_blocks(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Te
     n, k = w.shape
     dev, kb = w.device, _blocks(k)
     q, s = _new_codes(n, k, dev), _new_scales(_blocks(n), kb, dev)
-    _call(L.lib.npl_fp8_quant_weight, dev, w.data_ptr(), dt, n, k, _ld(w), q.data_ptr(), q.stride(0), s.data_ptr(), kb)
+    _call(L.lib.npl_fp8_quant_weight, dev, w.data_ptr(), dt, n, k, w.stride(0), q.data_ptr(), q.stride(0), s.data_ptr(), kb)
     return q, s
 
 
@@ -138,8 +133,8 @@ def rmsnorm_quant_blocks(x: torch.Tensor, weight: torch.Tensor, eps: float, resi
     x, residual fp16 or bf16 [M, K], weight [K], one type. Returns (codes
     [M, K], scales [M, ceil(K / 128)], sum): the sum is x + residual in their
     type, which the norm reads, in ``sum_out`` when given (it may be x or
-    residual itself); None without a residual. The norm stays in fp32 up to
-    the codes."""
+    residual itself), else in new rows that start 32 bytes aligned; None
+    without a residual. The norm stays in fp32 up to the codes."""
     _same_device(x, weight, residual, sum_out)
     dt = _activation("x", x, _DT16)
     if x.dim() != 2 or weight.shape != x.shape[1:] or weight.dtype != x.dtype:
@@ -151,7 +146,8 @@ def rmsnorm_quant_blocks(x: torch.Tensor, weight: torch.Tensor, eps: float, resi
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError("residual must have the shape and type of x")
         if sum_out is None:
-            sum_out = torch.empty_strided(x.shape, (x.shape[1], 1), dtype=x.dtype, device=x.device)
+            k = x.shape[1]
+            sum_out = torch.empty_strided(x.shape, (-(-k // 16) * 16, 1), dtype=x.dtype, device=x.device)
         elif sum_out.shape != x.shape or sum_out.dtype != x.dtype:
             raise ValueError("sum_out must have the shape and type of x")
         elif sum_out is not x and sum_out is not residual and _overlap(sum_out, x, residual):
@@ -165,8 +161,8 @@ def rmsnorm_quant_blocks(x: torch.Tensor, weight: torch.Tensor, eps: float, resi
     dev, kb = x.device, _blocks(k)
     q, s = _new_codes(m, k, dev), _new_scales(m, kb, dev)
     if m:
-        _call(L.lib.npl_fp8_rmsnorm_quant, dev, v.data_ptr(), _ld(v), L.ptr(r), 0 if r is None else _ld(r),
-              w.data_ptr(), dt, float(eps), m, k, L.ptr(sum_out), 0 if r is None else _ld(sum_out), q.data_ptr(),
+        _call(L.lib.npl_fp8_rmsnorm_quant, dev, v.data_ptr(), v.stride(0), L.ptr(r), 0 if r is None else r.stride(0),
+              w.data_ptr(), dt, float(eps), m, k, L.ptr(sum_out), 0 if r is None else sum_out.stride(0), q.data_ptr(),
               q.stride(0), s.data_ptr(), kb)
     return q, s, sum_out
 
@@ -184,7 +180,7 @@ def silu_mul_quant_blocks(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.T
     dev, kb = g.device, _blocks(k)
     q, s = _new_codes(m, k, dev), _new_scales(m, kb, dev)
     if m:
-        _call(L.lib.npl_fp8_silu_mul_quant, dev, g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), dt, m, k, q.data_ptr(),
+        _call(L.lib.npl_fp8_silu_mul_quant, dev, g.data_ptr(), g.stride(0), u.data_ptr(), u.stride(0), dt, m, k, q.data_ptr(),
               q.stride(0), s.data_ptr(), kb)
     return q, s
 
@@ -198,22 +194,24 @@ def _overlap(out: torch.Tensor, *others: torch.Tensor) -> bool:
     return any(a0 < b1 and b0 < a1 for b0, b1 in map(span, others))
 
 
-def _code_rows(name: str, q: torch.Tensor) -> None:
-    if q.dtype != _E4M3 or q.dim() != 2:
+def _code_rows(name: str, q: torch.Tensor) -> tuple[int, int, int]:
+    """(rows, K, row stride) of codes; a single row's stride is K rounded up to 16."""
+    if q.dtype is not _E4M3 or q.dim() != 2:
         raise ValueError(f"{name} must be float8_e4m3fn [rows, K]")
-    if (q.shape[1] > 1 and q.stride(1) != 1) or q.data_ptr() % 16 or (q.shape[0] > 1 and q.stride(0) % 16):
+    rows, k = q.shape
+    ld, step = q.stride()
+    if rows <= 1:
+        ld = -(-k // 16) * 16
+    if (step != 1 and k > 1) or (ld | q.data_ptr()) & 15 or ld < k:
         raise ValueError(f"{name} needs contiguous columns and rows on 16-byte boundaries, as the quantisers return them")
+    return rows, k, ld
 
 
-def _ld16(q: torch.Tensor) -> int:
-    """Row stride of codes; a single row's is its length rounded up to 16."""
-    return q.stride(0) if q.shape[0] > 1 else -(-q.shape[1] // 16) * 16
-
-
-def _scales(name: str, s: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
-    if s.dtype != torch.float32 or s.shape != (rows, cols):
+def _scales(name: str, s: torch.Tensor, rows: int, cols: int) -> tuple[torch.Tensor, int]:
+    if s.dtype is not torch.float32 or s.shape != (rows, cols):
         raise ValueError(f"{name} must be float32 [{rows}, {cols}], got {s.dtype} {tuple(s.shape)}")
-    return _rows(s)
+    s = _rows(s)
+    return s, s.stride(0) if rows > 1 else cols
 
 
 def linear_blocks(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, wscale: torch.Tensor, *,
@@ -225,14 +223,13 @@ def linear_blocks(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w
     the type of ``out`` or ``residual``, else bf16. ``out`` may be ``residual``
     itself."""
     _same_device(q, scale, qweight, wscale, bias, residual, out)
-    _code_rows("q", q)
-    _code_rows("qweight", qweight)
-    m, k = q.shape
-    n = qweight.shape[0]
-    if qweight.shape[1] != k or k == 0 or n == 0:
+    m, k, lda = _code_rows("q", q)
+    n, kw, ldw = _code_rows("qweight", qweight)
+    if kw != k or k == 0 or n == 0:
         raise ValueError("linear input/weight shapes do not match")
     kb = _blocks(k)
-    sa, sw = _scales("scale", scale, m, kb), _scales("wscale", wscale, _blocks(n), kb)
+    sa, ld_sa = _scales("scale", scale, m, kb)
+    sw, ld_sw = _scales("wscale", wscale, _blocks(n), kb)
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.bfloat16
     if out_dtype not in _DT16:
@@ -255,9 +252,10 @@ def linear_blocks(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w
                 residual is not None and out is not residual and _overlap(out, residual)):
             raise ValueError("out may be residual itself, but not overlap an input otherwise")
     if m:
-        _call(L.lib.npl_fp8_linear, q.device, q.data_ptr(), _ld16(q), sa.data_ptr(), _ld(sa), qweight.data_ptr(),
-              _ld16(qweight), sw.data_ptr(), _ld(sw), L.ptr(bias), m, n, k, L.ptr(res),
-              0 if res is None else _ld(res), out.data_ptr(), _ld(out), _DT16[out_dtype])
+        _call(L.lib.npl_fp8_linear, q.device, q.data_ptr(), lda, sa.data_ptr(), ld_sa, qweight.data_ptr(), ldw,
+              sw.data_ptr(), ld_sw, L.ptr(bias), m, n, k, L.ptr(res),
+              0 if res is None else res.stride(0) if m > 1 else n, out.data_ptr(), out.stride(0) if m > 1 else n,
+              _DT16[out_dtype])
     return out
 
 

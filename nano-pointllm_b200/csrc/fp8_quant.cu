@@ -58,7 +58,7 @@ __device__ __forceinline__ void ld32(const void* p, uint32_t* r) {  // one 256-b
 
 // 16 consecutive elements at any p: the aligned 16-byte words around them,
 // shifted into place. [lo, hi) bounds what may be read; false where the words
-// do not lie in it. Element by element 1000 x 5003 fp16 took X us, so Y.
+// do not lie in it. (Tokens 1000 x 5003 fp16: 4.5 us; element by element 7.7.)
 template <typename T>
 __device__ __forceinline__ bool load_shifted(const T* p, const T* lo, const T* hi, Raw<T>& r) {
   constexpr int W = Raw<T>::kWords;
@@ -322,7 +322,10 @@ constexpr int kNormThreads = 512;
 
 // A warp takes 4 U consecutive blocks of a row, each of its four 8-lane groups
 // every fourth, all loads before the first store, which the compiler would not
-// move them across.
+// move them across. Bound by instructions and memory alike: 16000 x 4096 fp16
+// takes 36.9 us (5.4 TB/s), SiLU * up of 16000 x 11008 197 us (4.5 TB/s). With 8
+// columns a thread, which doubles the work per block, they took 48 and 281;
+// warps that stay and load their next span first, 53 and 281.
 template <typename Source, int U, bool kVecQ>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(typename Source::Loaded) > 32 ? 4 : 5)
     fp8_quant_kernel(const Source src, const CodeSink out, int rows, int cols, unsigned spans) {
@@ -428,47 +431,56 @@ __global__ void __launch_bounds__(kMaxThreads ? kMaxThreads : kNormThreads, kMax
   }
 }
 
-// One 128 x 128 weight block per CTA: 8 threads across, 32 rows at a time, the
-// block held in registers between its maximum and its codes.
+// 128 x 128 weight blocks, one after the other in each of kWeightCtas CTAs an
+// SM: 8 threads across, 32 rows at a time, the block held in registers between
+// its maximum and its codes. Bound by the way of a block through a CTA (load,
+// join, store): 32003 x 4096 fp16 takes 88.7 us, 4.4 TB/s; fp32, twice the
+// bytes, 105. A CTA for every block, each with the fence at its end, took 102
+// us; loading the next block first, for which half of the warps' registers
+// go, 86 at best and 118 in fp32.
 constexpr int kWeightThreads = 256;
+constexpr int kWeightCtas = 3;
 constexpr int kWeightRows = kWeightThreads / kGroup;
 
 template <typename T, int kAccess, bool kVecQ>
-__global__ void __launch_bounds__(kWeightThreads, 3) fp8_quant_weight_kernel(const T* __restrict__ w, long long ldw,
-                                                                          int rows, int cols, int k_blocks,
-                                                                          const CodeSink out) {
-  __shared__ uint32_t red[kWeightThreads / 32];
+__global__ void __launch_bounds__(kWeightThreads, kWeightCtas)
+    fp8_quant_weight_kernel(const T* __restrict__ w, long long ldw, int rows, int cols, int k_blocks, unsigned blocks,
+                            const CodeSink out) {
+  __shared__ uint32_t red[2][kWeightThreads / 32];
   pdl_wait();
   constexpr int kSteps = kBlock / kWeightRows;
-  const int nb = (int)(blockIdx.x / (unsigned)k_blocks), kb = (int)(blockIdx.x - (unsigned)nb * (unsigned)k_blocks);
-  const int col = kb * kBlock + (int)(threadIdx.x % kGroup) * kCols;
-  const int row0 = nb * kBlock + (int)threadIdx.x / kGroup;
-  Raw<T> raw[kSteps];
+  const T* end = w + (long long)(rows - 1) * ldw + cols;
+  int turn = 0;
+  for (unsigned block = blockIdx.x; block < blocks; block += gridDim.x, turn ^= 1) {
+    const int nb = (int)(block / (unsigned)k_blocks), kb = (int)(block - (unsigned)nb * (unsigned)k_blocks);
+    const int col = kb * kBlock + (int)(threadIdx.x % kGroup) * kCols;
+    const int row0 = nb * kBlock + (int)threadIdx.x / kGroup;
+    Raw<T> raw[kSteps];
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int row = row0 + i * kWeightRows;
-    const bool in = row < rows && col < cols;
-    raw[i] = load16<kAccess>(w + (in ? (long long)row * ldw + col : 0), in ? cols - col : 0, w,
-                             w + (long long)(rows - 1) * ldw + cols);
+    for (int i = 0; i < kSteps; ++i) {
+      const int row = row0 + i * kWeightRows;
+      const bool in = row < rows && col < cols;
+      raw[i] = load16<kAccess>(w + (in ? (long long)row * ldw + col : 0), in ? cols - col : 0, w, end);
+    }
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) a = max(a, key_of(raw[i]));
+    a = __reduce_max_sync(0xffffffffu, a);
+    if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = a;
+    __syncthreads();  // the other turn's maxima have been read, too
+    a = __reduce_max_sync(0xffffffffu, red[turn][threadIdx.x & (kWeightThreads / 32 - 1)]);
+    const float s = block_scale(key_value<T>(a));
+    const float inv = __frcp_rn(s);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int row = row0 + i * kWeightRows;
+      float v[kCols];
+      widen(raw[i], v);
+      if (row < rows && col < cols)
+        store_codes<kVecQ>(out.q + (long long)row * out.ldq + col, codes16(v, inv), cols - col);
+    }
+    if (threadIdx.x == 0) out.scale[(long long)nb * out.ld_scale + kb] = s;
   }
-  uint32_t a = 0;
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) a = max(a, key_of(raw[i]));
-  a = __reduce_max_sync(0xffffffffu, a);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
-  __syncthreads();
-  a = __reduce_max_sync(0xffffffffu, red[threadIdx.x & (kWeightThreads / 32 - 1)]);
-  const float s = block_scale(key_value<T>(a));
-  const float inv = __frcp_rn(s);
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int row = row0 + i * kWeightRows;
-    float v[kCols];
-    widen(raw[i], v);
-    if (row < rows && col < cols)
-      store_codes<kVecQ>(out.q + (long long)row * out.ldq + col, codes16(v, inv), cols - col);
-  }
-  if (threadIdx.x == 0) out.scale[(long long)nb * out.ld_scale + kb] = s;
   pdl_trigger_after_writes();
 }
 
@@ -538,7 +550,8 @@ int launch_quant_spans(const char* what, const Source& src, const CodeSink& out,
 
 // Two blocks a thread where a thread's loads are 32 bytes, except where the
 // rows are short (half of the warps' lanes or more would idle) or so few that
-// one block a thread fits on the SMs at once (8 x 4096: X us against Y).
+// one block a thread fits on the SMs at once. For SiLU, whose values take 16
+// registers a block, one (16000 x 4096: 71 us, with two 114).
 template <typename Source>
 int launch_quant(const char* what, const Source& src, const CodeSink& out, int rows, int cols, cudaStream_t st) {
   constexpr int U = sizeof(typename Source::Loaded) > 32 ? 1 : 2;
@@ -658,9 +671,9 @@ extern "C" int npl_fp8_quant_weight(const void* w, int w_dtype, int64_t rows, in
     using T = decltype(t);
     return by_access(row_access(w, rows, ldw, w_dtype), [&](auto a) {
       auto kern = vecq ? fp8_quant_weight_kernel<T, a.value, true> : fp8_quant_weight_kernel<T, a.value, false>;
-      return launch_pdl(what, kern, dim3((unsigned)(nb * kb)), dim3(kWeightThreads), 0,
-                        static_cast<cudaStream_t>(stream), static_cast<const T*>(w), ldw, (int)rows, (int)cols, (int)kb,
-                        out);
+      return launch_pdl(what, kern, dim3((unsigned)std::min(nb * kb, (long long)kWeightCtas * num_sms())),
+                        dim3(kWeightThreads), 0, static_cast<cudaStream_t>(stream), static_cast<const T*>(w), ldw,
+                        (int)rows, (int)cols, (int)kb, (unsigned)(nb * kb), out);
     });
   });
 }

@@ -449,8 +449,8 @@ int npl_fp8_silu_mul_quant(const void* gate, int64_t ld_gate, const void* up, in
  * NPL_BF16, which is residual's type too. qa e4m3 [M, K], qw e4m3 [N, K]: rows
  * on 16-byte boundaries (lda, ldw multiples of 16); K itself is arbitrary.
  * sa fp32 [M, ceil(K / 128)], sw fp32 [ceil(N / 128), ceil(K / 128)]; bias
- * fp32 [N]. out may be residual itself (same row stride). Equal inputs give
- * equal bits. The kernel runs on any stream, in any number at once.
+ * fp32 [N]. out may be residual itself (same row stride). Equal calls give
+ * equal bits; how a sum is split, and so its last bits, goes by M, N and K.
  */
 int npl_fp8_linear(const uint8_t* qa, int64_t lda, const float* sa, int64_t ld_sa, const uint8_t* qw, int64_t ldw,
                    const float* sw, int64_t ld_sw, const float* bias_or_null, int64_t M, int64_t N, int64_t K,

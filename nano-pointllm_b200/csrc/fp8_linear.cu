@@ -9,7 +9,7 @@
 // epilogue warps add it, scaled, to fp32 sums in registers. The output is rounded
 // to T once, after bias and residual.
 //
-// Decode tiles (M <= 64): the weight tile is the MMA's A operand and the tokens
+// Decode tiles (M <= 64, some M <= 128): the weight tile is the MMA's A operand and the tokens
 // are its N dimension (D[n, m], 128 weight rows x NT tokens), so a decode
 // batch fills an MMA with NT = 16..64. Prefill tiles: see below.
 //
@@ -26,7 +26,7 @@
 // Each leaves its fp32 sums in its own shared memory; after a cluster barrier
 // CTA r adds those of ranks 0, 1, .. S - 1, in this order, for its share of
 // the tokens. No workspace and no atomics: two calls in flight share nothing,
-// and equal inputs give equal bits.
+// and equal calls give equal bits.
 //
 // All mbarrier waits are bounded (~1 s); on expiry the kernel records a code
 // in the device status word, drains its in-flight copies and MMAs, meets its
@@ -103,13 +103,13 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 
-// mbar_wait bounded by a count of polls (each takes 20 ns or more), without
-// the clock: fewer instructions where every block waits.
+// mbar_wait that looks at the clock only after many polls (of 20 ns or more):
+// where every block waits, reading it takes longer than most waits.
 __device__ __forceinline__ bool poll_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
-  for (int i = 0; i < (1 << 25); ++i)
+#pragma unroll 1
+  for (int i = 0; i < 1024; ++i)
     if (mbar_try_wait(bar, parity)) return true;
-  if (status) atomicExch(status, code);
-  return false;
+  return mbar_wait(bar, parity, status, code);
 }
 
 // Instruction descriptor of kind::f8f6f4: fp32 accumulator (c_format [4,6) =
@@ -125,6 +125,13 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) {
 // 16000 x 22016 x 4096.)
 __device__ __forceinline__ void fma_after_ld(float& acc, uint32_t d, float s) {
   asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(__uint_as_float(d)), "f"(s));
+}
+
+__device__ __forceinline__ void tma_prefetch_l2(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1)
+               : "memory");
 }
 
 __device__ __forceinline__ void lds128(const float* p, float* v) {
@@ -147,7 +154,7 @@ __device__ __forceinline__ void narrow(float v, __nv_bfloat16& o) { o = __float2
 
 // T: element type of residual and out; NT: tokens per tile.
 template <typename T, int NT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     fp8_linear_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                              const Fp8LinearArgs p) {
   extern __shared__ unsigned char smem_raw[];
@@ -205,28 +212,23 @@ __global__ void __launch_bounds__(kThreads)
     const bool issuer = elect_one();
     const uint64_t pol_w = policy_evict_first();
     const uint64_t pol_x = policy_evict_last();
-    auto load_w = [&](int kb, int stage) {
-      if (issuer) {
-        mbar_arrive_expect_tx(&c.full[stage], kStageW + kStageX);
-        tma_load_2d(ring_w + (size_t)stage * kStageW, &tmap_w, kb * kBlockK, n_tile * kTileN, &c.full[stage], pol_w);
-      }
-    };
-    // Weights do not depend on the kernels before this one on its stream
-    // (npl_fp8_quant_weight lets this one start only when its codes are
-    // visible), so the ring is filled with them before the wait.
+    // Before the kernels ahead of this one on its stream are done nothing may
+    // be read, not even weights, which one of them may have written. But their
+    // first tiles may be brought into L2, where such a write would meet them.
     const int ahead = min(p.stages, kb1 - kb0);
-    for (int i = 0; i < ahead; ++i) load_w(kb0 + i, i);
+    for (int i = 0; i < ahead; ++i)
+      if (issuer) tma_prefetch_l2(&tmap_w, (kb0 + i) * kBlockK, n_tile * kTileN);
     pdl_wait();
     int stage = 0, loads = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (loads >= ahead) {
-        if (!poll_wait(&c.empty[stage], phase ^ 1, p.status, NPL_DEV_TIMEOUT_TMA)) break;
-        load_w(kb, stage);
-      }
-      if (issuer)
+      if (!poll_wait(&c.empty[stage], phase ^ 1, p.status, NPL_DEV_TIMEOUT_TMA)) break;
+      if (issuer) {
+        mbar_arrive_expect_tx(&c.full[stage], kStageW + kStageX);
+        tma_load_2d(ring_w + (size_t)stage * kStageW, &tmap_w, kb * kBlockK, n_tile * kTileN, &c.full[stage], pol_w);
         tma_load_2d(ring_x + (size_t)stage * kStageX, &tmap_x, kb * kBlockK, m_tile * NT, &c.full[stage], pol_x);
-      ++loads;
+      }
+      loads = min(loads + 1, p.stages);
       if (++stage == p.stages) {
         stage = 0;
         phase ^= 1;
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     // every issued load lands before the ring is used again or released: stage
     // i was last loaded with the parity of that load
-    for (int i = 0; i < min(loads, p.stages); ++i)
+    for (int i = 0; i < loads; ++i)
       poll_wait(&c.full[i], i < stage ? phase : phase ^ 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
     __syncwarp();
   } else if (warp == 1) {
@@ -867,12 +869,12 @@ struct Operands {
   int out_dtype;
 };
 
-// Shared memory of a decode CTA. More than a third of an SM's, so that at
-// most two CTAs share an SM: their TMEM (at most 2 x 256 columns) then always
-// fits, and no CTA of a cluster waits for TMEM that a CTA of another cluster
-// holds.
-constexpr int kDecodeSmemMin = 78 * 1024;
-constexpr int kDecodeSmemMax = 110 * 1024;
+// Shared memory of a decode CTA: more than a third of an SM's, so that at most
+// two such CTAs share an SM. Their TMEM (2 x 256 columns) then always fits, and
+// no CTA of a cluster waits for TMEM that a CTA of another cluster holds (a
+// prefill CTA, with 512 columns, fills an SM's shared memory alone).
+constexpr int kDecodeSmem = 110 * 1024;
+constexpr int kThirdOfSm = 76 * 1024;
 
 // CTAs that share a decode tile: as many as keep 1.75 CTAs an SM (beyond it not
 // all clusters run at once: 96 tiles of 32 blocks take 12.0 us unsplit, 13.9
@@ -890,15 +892,17 @@ int launch_decode(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
   if (int rc = code_map(&tw, o.qw, p.N, o.K, o.ldw, kTileN)) return rc;
   if (int rc = code_map(&tx, o.qa, p.M, o.K, o.lda, NT)) return rc;
   constexpr int stage = (kTileN + NT) * kBlockK;
-  p.stages = std::min(kMaxStages, (kDecodeSmemMax - 1024) / stage);
-  const int smem = std::max(p.stages * stage + 1024, kDecodeSmemMin);
+  constexpr int stages = std::min(kMaxStages, (kDecodeSmem - 1024) / stage);
+  constexpr int smem = stages * stage + 1024;
+  static_assert(smem > kThirdOfSm && kPSmem + smem > 3 * kThirdOfSm);
+  p.stages = stages;
   const long long m_tiles = (p.M + NT - 1) / NT;
   const long long tiles = m_tiles * p.n_tiles;
   p.split = decode_split(tiles, p.k_blocks);
   if (tiles * p.split > 2147483647ll)
     return fail(NPL_ERR_UNSUPPORTED, "npl_fp8_linear: M=%d N=%d has too many tiles", p.M, p.N);
   auto kern = fp8_linear_decode_kernel<T, NT>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecodeSmemMax) != cudaSuccess)
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status("npl_fp8_linear: smem attribute");
   return launch_pdl_cluster("npl_fp8_linear", kern, dim3((unsigned)(tiles * p.split)), dim3(kThreads), (size_t)smem,
                             st, (unsigned)p.split, tw, tx, p);

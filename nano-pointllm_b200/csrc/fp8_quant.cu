@@ -448,6 +448,7 @@ __global__ void __launch_bounds__(kWeightThreads, kWeightCtas)
                             const CodeSink out) {
   __shared__ uint32_t red[2][kWeightThreads / 32];
   pdl_wait();
+  pdl_trigger();
   constexpr int kSteps = kBlock / kWeightRows;
   const T* end = w + (long long)(rows - 1) * ldw + cols;
   int turn = 0;
@@ -481,7 +482,6 @@ __global__ void __launch_bounds__(kWeightThreads, kWeightCtas)
     }
     if (threadIdx.x == 0) out.scale[(long long)nb * out.ld_scale + kb] = s;
   }
-  pdl_trigger_after_writes();
 }
 
 // ------------------------------------------------------------------ host

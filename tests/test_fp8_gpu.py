@@ -425,3 +425,73 @@ def test_weight_written_just_before(F, cuda_device):
     got = [F.linear_blocks(qa, sa, *F.quantize_weight_blocks(w)) for w in ws]
     for g, e in zip(got, want):
         assert torch.equal(g, e)
+
+
+def test_calls_at_once_on_streams(F, cuda_device):
+    """Decode and prefill tiles, split and whole, quantisers and the int8
+    linear on four streams at once: nothing is shared between calls."""
+    from nanopointllm_b200 import w8a8 as W
+    x = rand((300, 2048), F16, 1).to(cuda_device)
+    q, s = F.quantize_token_blocks(x)
+    weights = [F.quantize_weight_blocks(rand((n, 2048), F16, n, 0.02).to(cuda_device)) for n in (1000, 4096)]
+    i8 = W.dynamic_per_token_quant(x[:40])
+    i8w = W.per_output_weight_quant(rand((1024, 2048), F16, 5, 0.02).to(cuda_device))
+    work = [
+        lambda: F.linear_blocks(q[:8], s[:8], *weights[0]),     # decode tiles, split
+        lambda: F.linear_blocks(q[:64], s[:64], *weights[1]),   # 64-token tiles, split
+        lambda: F.linear_blocks(q, s, *weights[0]),             # prefill tiles, two pairs each
+        lambda: F.quantize_token_blocks(x)[1],
+        lambda: F.linear_blocks(q, s, *weights[1], out_dtype=F16),
+        lambda: W.linear_q(i8[0], i8[1].reshape(-1), *i8w),
+    ]
+    want = [f().clone() for f in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for turn in range(25):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                # the int8 linear has one workspace, so one stream
+                j = (turn + i) % 5 if i else (5 if turn % 2 else 0)
+                got.append((j, work[j]()))
+    torch.cuda.synchronize()
+    for j, g in got:
+        assert torch.equal(g, want[j]), j
+
+
+def test_far_rows(F, cuda_device):
+    """Offsets past 2^31 elements: the last rows of large operands. The linear
+    is held to the 64-bit sums and not to the bits of a call on these rows
+    alone: 200 rows make two tiles, whose 64 blocks two pairs of CTAs share, so
+    s0 + .. + s63 is there (s0 + .. + s31) + (s32 + .. + s63), another order of
+    fp32 additions than that of 270000 rows."""
+    m, k = 270000, 8192
+    x = torch.zeros(m, k, dtype=F16, device=cuda_device)
+    x[-200:] = rand((200, k), F16, 1).to(cuda_device)
+    q, s = F.quantize_token_blocks(x)
+    q1, s1 = F.quantize_token_blocks(x[-200:].clone())
+    assert torch.equal(q[-200:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[-200:], s1)
+    w = F.quantize_weight_blocks(rand((136, k), F16, 2, 0.02).to(cuda_device))
+    for out in (F.linear_blocks(q, s, *w)[-200:], F.linear_blocks(q1, s1, *w)):
+        want, mag = O.linear(cpu(q1), cpu(s1), cpu(w[0]), cpu(w[1]))
+        tol = (128 + 64 + 12) * 2.0 ** -23 * mag
+        assert (np.abs(cpu(out) - want) <= tol + torch.finfo(BF16).eps / 2 * (np.abs(want) + tol)).all()
+    nw = torch.ones(k, dtype=F16, device=cuda_device)
+    assert torch.equal(F.rmsnorm_quant_blocks(x, nw, 1e-6)[1][-200:], F.rmsnorm_quant_blocks(x[-200:], nw, 1e-6)[1])
+    del x, q
+    n = 32776
+    q, s = F.quantize_token_blocks(rand((66000, 128), F16, 3).to(cuda_device))
+    w = F.quantize_weight_blocks(rand((n, 128), F16, 4, 0.02).to(cuda_device))
+    out = F.linear_blocks(q, s, *w)
+    assert torch.equal(out[-300:], F.linear_blocks(q[-300:], s[-300:], *w))
+
+
+@pytest.mark.parametrize("m", [1, 100, 300])
+def test_operands_of_two_devices_are_refused(F, cuda_device, m):
+    x = rand((m, 256), F16, 1).to(cuda_device)
+    w = F.quantize_weight_blocks(rand((64, 256), F16, 2).to(cuda_device))
+    q, s = F.quantize_token_blocks(x)
+    with pytest.raises(ValueError, match="device"):
+        F.linear_blocks(q, s.cpu(), *w)
+    with pytest.raises(ValueError, match="device"):
+        F.rmsnorm_quant_blocks(x, torch.ones(256, dtype=F16), 1e-6)

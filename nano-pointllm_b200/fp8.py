@@ -41,6 +41,10 @@ _E4M3 = torch.float8_e4m3fn
 _DT16 = {torch.float16: L.NPL_F16, torch.bfloat16: L.NPL_BF16}
 _DT = {torch.float32: L.NPL_F32, **_DT16}
 
+_quant_rows, _quant_weight = L.lib.npl_fp8_quant_rows, L.lib.npl_fp8_quant_weight
+_rmsnorm_quant, _silu_mul_quant = L.lib.npl_fp8_rmsnorm_quant, L.lib.npl_fp8_silu_mul_quant
+_linear = L.lib.npl_fp8_linear
+
 
 def _blocks(n: int) -> int:
     return -(-n // BLOCK)
@@ -55,16 +59,21 @@ def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
             raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
 
 
+# Raw queries and bound names below: a call on a few rows is bound by the host
+# (torch.cuda.current_stream alone takes as long as the kernel).
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_empty = torch.empty_strided
+
+
 def _call(fn, device: torch.device, *args) -> None:
-    """fn(*args, stream) with ``device`` current, on its current stream. (The
-    raw queries: a call on a few rows is bound by the host, and
-    torch.cuda.current_stream alone takes as long as the kernel.)"""
+    """fn(*args, stream) with ``device`` current, on its current stream."""
     i = device.index
-    if i == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if i == _current_device():
+        rc = fn(*args, _current_stream(i))
     else:
         with torch.cuda.device(i):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+            rc = fn(*args, _current_stream(i))
     if rc:
         L.check(rc)
 
@@ -83,19 +92,23 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _new_codes(rows: int, k: int, device: torch.device) -> torch.Tensor:
     """e4m3 [rows, K] whose rows start on 16-byte boundaries, as the linear reads them."""
-    return torch.empty_strided((rows, k), (-(-k // 16) * 16, 1), dtype=_E4M3, device=device)
+    return _empty((rows, k), (-(-k // 16) * 16, 1), dtype=_E4M3, device=device)
 
 
-def _new_scales(rows: int, blocks: int, device: torch.device) -> torch.Tensor:
-    return torch.empty_strided((rows, blocks), (blocks, 1), dtype=torch.float32, device=device)
+def _outputs(rows: int, k: int, device: torch.device, scale_rows: int) -> tuple[torch.Tensor, torch.Tensor, int, int]:
+    """New (codes [rows, K], scales [scale_rows, ceil(K / 128)]) and their row strides."""
+    ld, kb = (k + 15) & ~15, (k + 127) // BLOCK
+    return (_empty((rows, k), (ld, 1), dtype=_E4M3, device=device),
+            _empty((scale_rows, kb), (kb, 1), dtype=torch.float32, device=device), ld, kb)
 
 
 def _activation(name: str, t: torch.Tensor, types: dict) -> int:
+    dt = types.get(t.dtype)
+    if dt is None:
+        raise ValueError(f"{name} must be one of {', '.join(str(d).replace('torch.', '') for d in types)}")
     if t.dim() == 0 or t.shape[-1] == 0:
         raise ValueError(f"{name} needs at least one column")
-    if t.dtype not in types:
-        raise ValueError(f"{name} must be one of {', '.join(str(d).replace('torch.', '') for d in types)}")
-    return types[t.dtype]
+    return dt
 
 
 def quantize_token_blocks(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -105,10 +118,10 @@ def quantize_token_blocks(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     dt = _activation("x", x, _DT)
     v = _rows(x)
     m, k = v.shape
-    dev, kb = x.device, _blocks(k)
-    q, s = _new_codes(m, k, dev), _new_scales(m, kb, dev)
+    dev = x.device
+    q, s, ldq, kb = _outputs(m, k, dev, m)
     if m:
-        _call(L.lib.npl_fp8_quant_rows, dev, v.data_ptr(), dt, m, k, v.stride(0), q.data_ptr(), q.stride(0), s.data_ptr(), kb)
+        _call(_quant_rows, dev, v.data_ptr(), dt, m, k, v.stride(0), q.data_ptr(), ldq, s.data_ptr(), kb)
     return (q, s) if x.dim() == 2 else (q.reshape(x.shape), s.reshape(*x.shape[:-1], kb))
 
 
@@ -121,9 +134,9 @@ def quantize_weight_blocks(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Te
     dt = _activation("weight", weight, _DT)
     w = _rows(weight.detach())
     n, k = w.shape
-    dev, kb = w.device, _blocks(k)
-    q, s = _new_codes(n, k, dev), _new_scales(_blocks(n), kb, dev)
-    _call(L.lib.npl_fp8_quant_weight, dev, w.data_ptr(), dt, n, k, w.stride(0), q.data_ptr(), q.stride(0), s.data_ptr(), kb)
+    dev = w.device
+    q, s, ldq, kb = _outputs(n, k, dev, _blocks(n))
+    _call(_quant_weight, dev, w.data_ptr(), dt, n, k, w.stride(0), q.data_ptr(), ldq, s.data_ptr(), kb)
     return q, s
 
 
@@ -136,34 +149,37 @@ def rmsnorm_quant_blocks(x: torch.Tensor, weight: torch.Tensor, eps: float, resi
     residual itself), else in new rows that start 32 bytes aligned; None
     without a residual. The norm stays in fp32 up to the codes."""
     _same_device(x, weight, residual, sum_out)
-    dt = _activation("x", x, _DT16)
-    if x.dim() != 2 or weight.shape != x.shape[1:] or weight.dtype != x.dtype:
+    dt, shape = _activation("x", x, _DT16), x.shape
+    if len(shape) != 2 or weight.shape != shape[1:] or weight.dtype is not x.dtype:
         raise ValueError("x must be [M, K] and weight [K], of one type")
-    if residual is None:
-        if sum_out is not None:
-            raise ValueError("sum_out needs a residual")
-    else:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError("residual must have the shape and type of x")
-        if sum_out is None:
-            k = x.shape[1]
-            sum_out = torch.empty_strided(x.shape, (-(-k // 16) * 16, 1), dtype=x.dtype, device=x.device)
-        elif sum_out.shape != x.shape or sum_out.dtype != x.dtype:
-            raise ValueError("sum_out must have the shape and type of x")
-        elif sum_out is not x and sum_out is not residual and _overlap(sum_out, x, residual):
-            raise ValueError("sum_out may be x or residual itself, but not overlap them otherwise")
-        if _rows(sum_out) is not sum_out:
-            raise ValueError("sum_out needs contiguous columns and rows that do not overlap")
+    m, k = shape
+    dev = x.device
     v = _rows(x)
-    r = None if residual is None else _rows(residual)
     w = weight if weight.is_contiguous() else weight.contiguous()
-    m, k = v.shape
-    dev, kb = x.device, _blocks(k)
-    q, s = _new_codes(m, k, dev), _new_scales(m, kb, dev)
+    res = total = None
+    ld_res = ld_sum = 0
+    if residual is not None:
+        if residual.shape != shape or residual.dtype is not x.dtype:
+            raise ValueError("residual must have the shape and type of x")
+        r = _rows(residual)
+        if sum_out is None:
+            ld_sum = (k + 15) & ~15
+            sum_out = _empty(shape, (ld_sum, 1), dtype=x.dtype, device=dev)
+        else:
+            if sum_out.shape != shape or sum_out.dtype is not x.dtype:
+                raise ValueError("sum_out must have the shape and type of x")
+            if _rows(sum_out) is not sum_out:
+                raise ValueError("sum_out needs contiguous columns and rows that do not overlap")
+            if sum_out is not x and sum_out is not residual and _overlap(sum_out, x, residual):
+                raise ValueError("sum_out may be x or residual itself, but not overlap them otherwise")
+            ld_sum = sum_out.stride(0)
+        res, ld_res, total = r.data_ptr(), r.stride(0), sum_out.data_ptr()
+    elif sum_out is not None:
+        raise ValueError("sum_out needs a residual")
+    q, s, ldq, kb = _outputs(m, k, dev, m)
     if m:
-        _call(L.lib.npl_fp8_rmsnorm_quant, dev, v.data_ptr(), v.stride(0), L.ptr(r), 0 if r is None else r.stride(0),
-              w.data_ptr(), dt, float(eps), m, k, L.ptr(sum_out), 0 if r is None else sum_out.stride(0), q.data_ptr(),
-              q.stride(0), s.data_ptr(), kb)
+        _call(_rmsnorm_quant, dev, v.data_ptr(), v.stride(0), res, ld_res, w.data_ptr(), dt, eps, m, k, total, ld_sum,
+              q.data_ptr(), ldq, s.data_ptr(), kb)
     return q, s, sum_out
 
 
@@ -172,26 +188,39 @@ def silu_mul_quant_blocks(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.T
     projection: its two column halves), in fp32 up to the codes. Returns
     (codes [M, K], scales [M, ceil(K / 128)])."""
     _same_device(gate, up)
-    dt = _activation("gate", gate, _DT16)
-    if gate.dim() != 2 or up.shape != gate.shape or up.dtype != gate.dtype:
+    dt, shape = _activation("gate", gate, _DT16), gate.shape
+    if len(shape) != 2 or up.shape != shape or up.dtype is not gate.dtype:
         raise ValueError("gate and up must be [M, K] of one shape and type")
     g, u = _rows(gate), _rows(up)
-    m, k = g.shape
-    dev, kb = g.device, _blocks(k)
-    q, s = _new_codes(m, k, dev), _new_scales(m, kb, dev)
+    m, k = shape
+    dev = g.device
+    q, s, ldq, kb = _outputs(m, k, dev, m)
     if m:
-        _call(L.lib.npl_fp8_silu_mul_quant, dev, g.data_ptr(), g.stride(0), u.data_ptr(), u.stride(0), dt, m, k, q.data_ptr(),
-              q.stride(0), s.data_ptr(), kb)
+        _call(_silu_mul_quant, dev, g.data_ptr(), g.stride(0), u.data_ptr(), u.stride(0), dt, m, k, q.data_ptr(), ldq,
+              s.data_ptr(), kb)
     return q, s
 
 
-def _overlap(out: torch.Tensor, *others: torch.Tensor) -> bool:
-    """Whether the memory spans of ``out`` and another tensor meet."""
+def _overlap(out: torch.Tensor, *others: torch.Tensor | None) -> bool:
+    """Whether the memory of ``out`` and another tensor may meet: their spans
+    do, and they are not different columns of one buffer's rows."""
     def span(t):
         n = sum((d - 1) * abs(st) for d, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
         return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+    def columns(a, b):
+        ld, size = a.stride(0), a.element_size()
+        at, off = divmod(b.data_ptr() - a.data_ptr(), size)
+        return (a.dim() == b.dim() == 2 and a.stride() == b.stride() and a.stride(1) == 1 and size == b.element_size()
+                and off == 0 and ld > 0 and at % ld >= a.shape[1] and at % ld + b.shape[1] <= ld)
+
     a0, a1 = span(out)
-    return any(a0 < b1 and b0 < a1 for b0, b1 in map(span, others))
+    for t in others:
+        if t is not None:
+            b0, b1 = span(t)
+            if a0 < b1 and b0 < a1 and not columns(out, t):
+                return True
+    return False
 
 
 def _code_rows(name: str, q: torch.Tensor) -> tuple[int, int, int]:
@@ -227,35 +256,40 @@ def linear_blocks(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w
     n, kw, ldw = _code_rows("qweight", qweight)
     if kw != k or k == 0 or n == 0:
         raise ValueError("linear input/weight shapes do not match")
-    kb = _blocks(k)
+    kb = (k + 127) // BLOCK
     sa, ld_sa = _scales("scale", scale, m, kb)
-    sw, ld_sw = _scales("wscale", wscale, _blocks(n), kb)
+    sw, ld_sw = _scales("wscale", wscale, (n + 127) // BLOCK, kb)
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.bfloat16
-    if out_dtype not in _DT16:
+    dt = _DT16.get(out_dtype)
+    if dt is None:
         raise ValueError("out_dtype must be float16 or bfloat16")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
-        raise ValueError("bias must be contiguous float32 [N]")
-    res = None
+    add = res = None
+    ld_res, ld_out = 0, n
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.shape != (n,) or not bias.is_contiguous():
+            raise ValueError("bias must be contiguous float32 [N]")
+        add = bias.data_ptr()
     if residual is not None:
-        if residual.shape != (m, n) or residual.dtype != out_dtype:
+        if residual.shape != (m, n) or residual.dtype is not out_dtype:
             raise ValueError("residual must be [M, N] of out_dtype")
-        res = _rows(residual)
+        r = _rows(residual)
+        res, ld_res = r.data_ptr(), r.stride(0) if m > 1 else n
+    dev = q.device
     if out is None:
-        out = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=q.device)
+        out = _empty((m, n), (n, 1), dtype=out_dtype, device=dev)
     else:
-        if out.shape != (m, n) or out.dtype != out_dtype:
+        if out.shape != (m, n) or out.dtype is not out_dtype:
             raise ValueError("out must be [M, N] of out_dtype")
         if _rows(out) is not out:
             raise ValueError("out needs contiguous columns and rows that do not overlap")
-        if _overlap(out, q, scale, qweight, wscale, *(t for t in (bias,) if t is not None)) or (
-                residual is not None and out is not residual and _overlap(out, residual)):
+        if _overlap(out, q, scale, qweight, wscale, bias, None if out is residual else residual):
             raise ValueError("out may be residual itself, but not overlap an input otherwise")
+        if m > 1:
+            ld_out = out.stride(0)
     if m:
-        _call(L.lib.npl_fp8_linear, q.device, q.data_ptr(), lda, sa.data_ptr(), ld_sa, qweight.data_ptr(), ldw,
-              sw.data_ptr(), ld_sw, L.ptr(bias), m, n, k, L.ptr(res),
-              0 if res is None else res.stride(0) if m > 1 else n, out.data_ptr(), out.stride(0) if m > 1 else n,
-              _DT16[out_dtype])
+        _call(_linear, dev, q.data_ptr(), lda, sa.data_ptr(), ld_sa, qweight.data_ptr(), ldw, sw.data_ptr(), ld_sw, add,
+              m, n, k, res, ld_res, out.data_ptr(), ld_out, dt)
     return out
 
 

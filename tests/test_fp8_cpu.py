@@ -169,6 +169,10 @@ def test_refusals_of_the_python_calls(F):
     wide = torch.zeros(4, 128, dtype=torch.bfloat16)
     assert f.linear_blocks(qa, sa, qw, sw, out=wide[:, :100]).dtype == torch.bfloat16
     assert calls[-1][1][-2] == 128
+    halves = torch.zeros(4, 200, dtype=h)  # two columns of one buffer's rows do not overlap
+    assert f.linear_blocks(qa, sa, qw, sw, residual=halves[:, 100:], out=halves[:, :100]).shape == (4, 100)
+    pair = torch.zeros(4, 512, dtype=h)
+    assert f.rmsnorm_quant_blocks(pair[:, :256], w, 1e-6, x, sum_out=pair[:, 256:])[2].shape == (4, 256)
     odd = f._new_codes(1, 77, torch.device("cpu"))
     f.linear_blocks(odd, torch.ones(1, 1), f._new_codes(9, 77, torch.device("cpu")), torch.ones(1, 1))
     assert calls[-1][1][1] == 80 and calls[-1][1][5] == 80 and calls[-1][1][9:12] == (1, 9, 77)

@@ -152,6 +152,14 @@ def test_rmsnorm(F, cuda_device, m, k, residual, dtype, how):
     check_codes(q, s, O.rmsnorm(cpu(t), cpu(w), 1e-6))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("k", [5120, 5121, 6656, 6657, 8191, 8192, 8193, 11264, 11265, 16385])
+def test_rmsnorm_row_lengths(F, cuda_device, k, residual, dtype):
+    """Both sides of each length at which the kernel's registers a thread change."""
+    test_rmsnorm(F, cuda_device, 2, k, residual, dtype, "strided")
+
+
 @pytest.mark.parametrize("k", [256, 4096, 20000])
 def test_rmsnorm_in_place(F, cuda_device, k):
     """The sum in place of x or of the residual, rows past the batch untouched."""

@@ -567,11 +567,15 @@ int launch_rmsnorm(const T* x, long long ldx, const T* res, long long ld_res, co
   const int lanes = (cols + kCols - 1) / kCols;
   const int threads = lanes <= 1024 ? (lanes + 31) / 32 * 32 : kNormThreads;
   // The instance of 704 threads has 40 registers a thread, so that an SM holds three
-  // rows of 8192 columns; that of 512 (48 for bf16, 56 for fp16) two. bf16: 1000 x
-  // 6144 with residual 10.2 us with 48 and 9.1 with 40, 4000 x 8192 50.0 and 42.3, but
-  // 560 x 4096 4.4 and 4.9. fp16 spills 60 bytes at 40: 4000 x 8192 31.5 us and 27.5,
-  // 1000 x 5120 5.9 and 5.6, but with a residual 1000 x 8192 13.5 and 14.7.
-  const int few = !std::is_same<T, __half>::value ? 320 : res ? 512 : 416;
+  // rows of 8192 columns; that of 512 (48 for bf16, 56 for fp16) two. bf16 takes it
+  // for long rows (1000 x 6144 with residual 10.2 us with 48, 9.1 with 40; 4000 x 8192
+  // 50.0 and 42.6) and for more rows than the SMs hold at once, 1280 threads each
+  // (16000 x 4096 83.3 and 80.6, 4000 x 3584 21.2 and 19.8, 1200 x 2560 5.9 and 5.4;
+  // 4000 x 1024 6.8 and 7.1), not where they hold all (560 x 4096 4.4 and 4.9). fp16
+  // spills 60 bytes at 40: 4000 x 8192 31.5 us and 27.5, 1000 x 5120 5.9 and 5.6, but
+  // with a residual 1000 x 8192 13.5 and 14.7.
+  const bool fills = (long long)rows * threads > 1280ll * num_sms();
+  const int few = !std::is_same<T, __half>::value ? (fills ? 0 : 320) : res ? 512 : 416;
   auto kern = lanes <= few    ? fp8_rmsnorm_kernel<T, 512, kAccess, kVecQ>
               : lanes <= 704  ? fp8_rmsnorm_kernel<T, 704, kAccess, kVecQ>
               : lanes <= 1024 ? fp8_rmsnorm_kernel<T, 1024, kAccess, kVecQ>

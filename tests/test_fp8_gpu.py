@@ -160,6 +160,13 @@ def test_rmsnorm_row_lengths(F, cuda_device, k, residual, dtype):
     test_rmsnorm(F, cuda_device, 2, k, residual, dtype, "strided")
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m,k", [(1300, 2111), (6100, 520)])
+def test_rmsnorm_many_rows(F, cuda_device, m, k, dtype):
+    """More rows than the SMs hold at once."""
+    test_rmsnorm(F, cuda_device, m, k, True, dtype, "contiguous")
+
+
 @pytest.mark.parametrize("k", [256, 4096, 20000])
 def test_rmsnorm_in_place(F, cuda_device, k):
     """The sum in place of x or of the residual, rows past the batch untouched."""

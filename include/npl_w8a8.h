@@ -408,7 +408,7 @@ int npl_tp_allreduce_dequant(const npl_tp_peers* peers, const int32_t* acc, int 
  * elements only (32-byte aligned rows are fastest). Nothing outside the given
  * rows and columns is written, and nothing before the first or after the last
  * element read (unaligned rows are read with what lies between them). rows == 0
- * launches nothing.
+ * launches nothing. At most 2^31 - 257 rows and 2^31 - 8193 columns.
  * q: e4m3 codes [rows, cols], stride ldq. scale: fp32 [rows, ceil(cols /
  * 128)], stride ld_scale. dtype: NPL_F16 or NPL_BF16, and NPL_F32 where said.
  * No workspace: calls on different streams share nothing.

@@ -486,6 +486,7 @@ __global__ void __launch_bounds__(kWeightThreads, kWeightCtas)
 
 // ------------------------------------------------------------------ host
 constexpr long long kMaxInt = 2147483647ll;
+constexpr long long kMaxCols = kMaxInt - kNormThreads * kCols;  // a step past the last column is an int, too
 
 int elem_size(int dtype) { return dtype == NPL_F32 ? 4 : 2; }
 
@@ -505,7 +506,7 @@ int by_access(int access, Fn&& fn) {
 
 int check_codes(const char* what, long long rows, long long cols, const void* q, long long ldq, const void* scale,
                 long long ld_scale) {
-  if (rows < 0 || cols <= 0 || rows > kMaxInt - kBlock || cols > kMaxInt - kBlock)
+  if (rows < 0 || cols <= 0 || rows > kMaxInt - kBlock || cols > kMaxCols)
     return fail(NPL_ERR_ARG, "%s: bad shape rows=%lld cols=%lld", what, rows, cols);
   const long long kb = (cols + kBlock - 1) / kBlock;
   if (ldq < cols || ld_scale < kb)
@@ -562,7 +563,7 @@ int launch_quant(const char* what, const Source& src, const CodeSink& out, int r
 }
 
 template <typename T, int kAccess, bool kVecQ>
-int launch_rmsnorm(const T* x, long long ldx, const T* res, long long ld_res, const T* w, float eps, int rows,
+int launch_rmsnorm(const T* x, long long ldx, const T* res, long long ld_res, const T* __restrict__ w, float eps, int rows,
                    int cols, T* sum_out, long long ld_sum, bool sum_by16, const CodeSink& out, cudaStream_t st) {
   const int lanes = (cols + kCols - 1) / kCols;
   const int threads = lanes <= 1024 ? (lanes + 31) / 32 * 32 : kNormThreads;

@@ -119,6 +119,18 @@ def test_quantiser_layouts(F):
     assert a[1] == a[3] == 400 and a[2] - a[0] == 400 and a[5:7] == (5, 200)
 
 
+def test_c_entries_refuse_rows_past_int_columns(L):
+    """The kernels' column counters are 32-bit and go one step past the row."""
+    keep, p = _buf()
+    for cols in ((1 << 31) - 129, (1 << 31) - 1000, (1 << 31) - 8192):
+        ld, kb = 1 << 31, 1 << 24
+        rc = [L.lib.npl_fp8_quant_rows(p, 1, 1, cols, ld, p, ld, p, kb, None),
+              L.lib.npl_fp8_quant_weight(p, 1, 1, cols, ld, p, ld, p, kb, None),
+              L.lib.npl_fp8_rmsnorm_quant(p, ld, None, 0, p, 1, 1e-6, 1, cols, None, 0, p, ld, p, kb, None),
+              L.lib.npl_fp8_silu_mul_quant(p, ld, p, ld, 1, 1, cols, p, ld, p, kb, None)]
+        assert rc == [L.NPL_ERR_ARG] * 4, (cols, rc)
+
+
 def test_refusals_of_the_python_calls(F):
     f, calls = F
     h = torch.float16

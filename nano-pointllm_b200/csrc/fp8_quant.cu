@@ -16,6 +16,8 @@
 //
 // Every kernel is one pass over its input: the block stays in registers
 // between the maximum and the codes, 16 columns a thread, 8 threads a block.
+// No input is __restrict__: a load that may take memory for constant could be
+// moved ahead of the wait for the kernel that writes it.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(typename Source::Loaded)
 // read again for the second half.
 template <typename T, int kMaxThreads, int kAccess, bool kVecQ>
 __global__ void __launch_bounds__(kMaxThreads ? kMaxThreads : kNormThreads, kMaxThreads == 704 ? 2 : 1)
-    fp8_rmsnorm_kernel(const T* x, long long ldx, const T* res, long long ld_res, const T* __restrict__ w, float eps,
+    fp8_rmsnorm_kernel(const T* x, long long ldx, const T* res, long long ld_res, const T* w, float eps,
                        int cols, T* sum_out, long long ld_sum, bool sum_by16, const CodeSink out) {  // sum_out may be x or res
   constexpr bool kInRegs = kMaxThreads > 0;
   __shared__ float red[32];
@@ -444,7 +446,7 @@ constexpr int kWeightRows = kWeightThreads / kGroup;
 
 template <typename T, int kAccess, bool kVecQ>
 __global__ void __launch_bounds__(kWeightThreads, kWeightCtas)
-    fp8_quant_weight_kernel(const T* __restrict__ w, long long ldw, int rows, int cols, int k_blocks, unsigned blocks,
+    fp8_quant_weight_kernel(const T* w, long long ldw, int rows, int cols, int k_blocks, unsigned blocks,
                             const CodeSink out) {
   __shared__ uint32_t red[2][kWeightThreads / 32];
   pdl_wait();
@@ -563,7 +565,7 @@ int launch_quant(const char* what, const Source& src, const CodeSink& out, int r
 }
 
 template <typename T, int kAccess, bool kVecQ>
-int launch_rmsnorm(const T* x, long long ldx, const T* res, long long ld_res, const T* __restrict__ w, float eps, int rows,
+int launch_rmsnorm(const T* x, long long ldx, const T* res, long long ld_res, const T* w, float eps, int rows,
                    int cols, T* sum_out, long long ld_sum, bool sum_by16, const CodeSink& out, cudaStream_t st) {
   const int lanes = (cols + kCols - 1) / kCols;
   const int threads = lanes <= 1024 ? (lanes + 31) / 32 * 32 : kNormThreads;

@@ -170,8 +170,8 @@ def rmsnorm_quant_blocks(x: torch.Tensor, weight: torch.Tensor, eps: float, resi
                 raise ValueError("sum_out must have the shape and type of x")
             if _rows(sum_out) is not sum_out:
                 raise ValueError("sum_out needs contiguous columns and rows that do not overlap")
-            if sum_out is not x and sum_out is not residual and _overlap(sum_out, x, residual):
-                raise ValueError("sum_out may be x or residual itself, but not overlap them otherwise")
+            if _overlap(sum_out, x, residual, itself=True) or _overlap(sum_out, weight):
+                raise ValueError("sum_out may be x or residual itself, but not overlap an input otherwise")
             ld_sum = sum_out.stride(0)
         res, ld_res, total = r.data_ptr(), r.stride(0), sum_out.data_ptr()
     elif sum_out is not None:
@@ -201,11 +201,15 @@ def silu_mul_quant_blocks(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.T
     return q, s
 
 
-def _overlap(out: torch.Tensor, *others: torch.Tensor | None) -> bool:
+def _overlap(out: torch.Tensor, *others: torch.Tensor | None, itself: bool = False) -> bool:
     """Whether the memory of ``out`` and another tensor may meet: their spans
-    do, and they are not different columns of one buffer's rows."""
+    do, and they are not different columns of one buffer's rows. With
+    ``itself`` the same elements of the same memory do not count."""
     def span(t):
-        n = sum((d - 1) * abs(st) for d, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        if t.is_contiguous():
+            n = t.numel()
+        else:
+            n = sum((d - 1) * abs(st) for d, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
         return t.data_ptr(), t.data_ptr() + n * t.element_size()
 
     def columns(a, b):
@@ -216,10 +220,12 @@ def _overlap(out: torch.Tensor, *others: torch.Tensor | None) -> bool:
 
     a0, a1 = span(out)
     for t in others:
-        if t is not None:
-            b0, b1 = span(t)
-            if a0 < b1 and b0 < a1 and not columns(out, t):
-                return True
+        if t is None or (itself and t is out):
+            continue
+        b0, b1 = span(t)
+        if a0 < b1 and b0 < a1 and not columns(out, t) and not (
+                itself and a0 == b0 and t.shape == out.shape and t.stride() == out.stride()):
+            return True
     return False
 
 
@@ -283,7 +289,7 @@ def linear_blocks(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w
             raise ValueError("out must be [M, N] of out_dtype")
         if _rows(out) is not out:
             raise ValueError("out needs contiguous columns and rows that do not overlap")
-        if _overlap(out, q, scale, qweight, wscale, bias, None if out is residual else residual):
+        if _overlap(out, residual, itself=True) or _overlap(out, q, scale, qweight, wscale, bias):
             raise ValueError("out may be residual itself, but not overlap an input otherwise")
         if m > 1:
             ld_out = out.stride(0)

@@ -131,6 +131,27 @@ def test_c_entries_refuse_rows_past_int_columns(L):
         assert rc == [L.NPL_ERR_ARG] * 4, (cols, rc)
 
 
+def test_outputs_that_are_an_input_by_another_name(F):
+    """A view of the same rows is the input itself; an output that is one input
+    must not overlap the other."""
+    f, calls = F
+    h = torch.float16
+    flat, w, other = torch.zeros(4096, dtype=h), torch.ones(256, dtype=h), torch.zeros(4, 256, dtype=h)
+    x, shifted = flat[:1024].view(4, 256), flat[256:1280].view(4, 256)
+    for call in (lambda: f.rmsnorm_quant_blocks(x, w, 1e-6, shifted, sum_out=x),
+                 lambda: f.rmsnorm_quant_blocks(shifted, w, 1e-6, x, sum_out=x),
+                 lambda: f.rmsnorm_quant_blocks(other, flat[:256], 1e-6, shifted, sum_out=x)):
+        with pytest.raises(ValueError):
+            call()
+    assert not calls
+    f.rmsnorm_quant_blocks(x, w, 1e-6, other, sum_out=flat[:1024].view(4, 256))
+    f.rmsnorm_quant_blocks(other, w, 1e-6, x, sum_out=flat[:1024].view(4, 256))
+    f.rmsnorm_quant_blocks(x, w, 1e-6, x, sum_out=x)
+    qa, qw = torch.zeros(4, 256).to(E4M3), torch.zeros(256, 256).to(E4M3)
+    f.linear_blocks(qa, torch.ones(4, 2), qw, torch.ones(2, 2), residual=x, out=flat[:1024].view(4, 256))
+    assert len(calls) == 4
+
+
 def test_refusals_of_the_python_calls(F):
     f, calls = F
     h = torch.float16

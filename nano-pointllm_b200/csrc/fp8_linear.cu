@@ -387,14 +387,15 @@ __global__ void __launch_bounds__(kThreads, 2)
 //
 // Two CTAs of a cluster share a tile of 256 tokens x 256 weight rows
 // (cta_group::2): each loads 128 rows of both, CTA 0 issues the MMAs for both,
-// and each holds the accumulator of its 128 tokens. An SM takes in about 58
+// and each holds the accumulator of its 128 tokens. (Or x 192 weight rows; see
+// launch_prefill.) An SM takes in about 58
 // bytes a cycle from L2 (measured), and a block's MMAs run 512 cycles; a CTA
 // of its own with a 128 x 256 tile needs 48 KB for a block and waits for them,
 // one of a pair 32 KB.
 //
 // Per CTA (384 threads, one CTA per SM, persistent): warp 0 TMA, warp 1 MMA,
-// warps 2-3 the scales, two warpgroups the epilogue of 128 columns each, with
-// all of its sums in registers (128 a thread; the first warpgroup hands most
+// warps 2-3 the scales, two warpgroups the epilogue of half the columns each, with
+// all of its sums in registers (128 a thread, or 96; the first warpgroup hands most
 // of its registers to the other two). Two 256-column accumulators fill TMEM:
 // the MMAs of a block run while the epilogue adds up the one before, so the
 // block's whole round (MMAs, hand-over, TMEM loads, hand-back) has to fit into
@@ -404,21 +405,28 @@ __global__ void __launch_bounds__(kThreads, 2)
 // the threads that use them, every load would touch 32 rows, and these loads
 // alone took as long as the MMAs.
 constexpr int kPM = 128;   // tokens per CTA
-constexpr int kPN = 256;   // weight rows per tile
-constexpr int kPGroups = 2;                           // epilogue warpgroups
-constexpr int kPGroupCols = kPN / kPGroups;           // 128: one weight scale
+constexpr int kPGroups = 2;  // epilogue warpgroups
 constexpr int kPThreads = 128 + 128 * kPGroups;
 // 168 a thread at launch (65536 / 384); 56 + 2 * 224 = 3 * 168
 constexpr int kPRegsFew = 56, kPRegsMany = 224;
-constexpr int kPStages = 5;
-constexpr uint32_t kPStageX = kPM * kBlockK, kPStageW = kPN / 2 * kBlockK;
-constexpr uint32_t kPStage = kPStageX + kPStageW;
-constexpr int kPOutCols = 64;                         // columns staged at a time by a warpgroup
-constexpr uint32_t kPOut = kPM * kPOutCols * 2;       // 16 KB
-constexpr int kPScaleBlocks = 8;                     // blocks of scales loaded at a time
-constexpr int kPScaleLd = kPM + 4;                    // a warp's 8 blocks x 4 tokens hit 32 banks
-constexpr int kPSmem = kPStages * (int)kPStage + kPGroups * (int)kPOut + 1024;
+constexpr uint32_t kPStageX = kPM * kBlockK;
+constexpr uint32_t kPAccCols = 256;  // TMEM columns from one accumulator to the other
+constexpr int kPScaleBlocks = 8;     // blocks of scales loaded at a time
+constexpr int kPScaleLd = kPM + 4;   // a warp's 8 blocks x 4 tokens hit 32 banks
 
+// What follows from a tile's weight rows, 256 or 192.
+template <int kPN>
+struct PrefillTile {
+  static constexpr int kGroupCols = kPN / kPGroups;
+  static constexpr int kStages = kPN == 256 ? 5 : 6;
+  static constexpr uint32_t kStageW = kPN / 2 * kBlockK;
+  static constexpr uint32_t kStage = kPStageX + kStageW;
+  static constexpr int kOutCols = kPN == 256 ? 64 : 32;     // columns staged at a time by a warpgroup
+  static constexpr uint32_t kOut = kPM * kOutCols * 2;
+  static constexpr int kSmem = kStages * (int)kStage + kPGroups * (int)kOut + 1024;
+};
+
+template <int kPStages>
 struct PrefillCtl {
   uint64_t full[kPStages];   // CTA 0's: both CTAs' loads of a stage
   uint64_t empty[kPStages];
@@ -428,7 +436,7 @@ struct PrefillCtl {
   uint64_t sempty[2];
   uint64_t teardown;
   uint32_t tmem_base;
-  __align__(16) float scale[2][kPGroups][kPScaleBlocks][kPScaleLd];
+  __align__(16) float scale[2][2][kPScaleBlocks][kPScaleLd];  // with each of the tile's two weight scales
 };
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* smem, int c0, int c1) {
@@ -483,9 +491,13 @@ __device__ __forceinline__ void mbar_arrive_pair(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
-// Byte offset of 16-byte chunk `ch` of row `row` in a staged box of 128-byte
-// rows: the 128-byte swizzle of the output's tensor map.
-__device__ __forceinline__ int staged(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
+// Byte offset of 16-byte chunk `ch` of row `row` in a staged box of 128- or
+// 64-byte rows: the swizzle of the output's tensor map.
+template <int kOutCols>
+__device__ __forceinline__ int staged(int row, int ch) {
+  if constexpr (kOutCols == 64) return row * 128 + ((ch ^ (row & 7)) << 4);
+  return row * 64 + ((ch ^ ((row >> 1) & 3)) << 4);
+}
 
 // Tile t -> (token tile, weight tile): groups of raster_g token tiles, the
 // token tile running fastest, so that the tiles in flight at one time share
@@ -509,18 +521,21 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
   return u;
 }
 
-// kSplit: pairs per tile, which share its blocks (1 or 2).
-template <typename T, int kSplit>
+// kSplit: pairs per tile, which share its blocks (1 or 2). kPN: weight rows per tile.
+template <typename T, int kSplit, int kPN>
 __global__ void __launch_bounds__(kPThreads, 1)
     fp8_linear_prefill_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                               const __grid_constant__ CUtensorMap tmap_out, const Fp8LinearArgs p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                          ~uintptr_t(1023));
+  using Tile = PrefillTile<kPN>;
+  constexpr int kPStages = Tile::kStages, kPGroupCols = Tile::kGroupCols, kPOutCols = Tile::kOutCols;
+  constexpr uint32_t kPStage = Tile::kStage, kPOut = Tile::kOut;
   unsigned char* staging = ring + kPStages * kPStage;
-  __shared__ PrefillCtl c;
+  __shared__ PrefillCtl<kPStages> c;
   constexpr uint32_t kIdesc = idesc_e4m3(2 * kPM, kPN);
-  constexpr uint32_t kTmemCols = 2 * kPN;
+  constexpr uint32_t kTmemCols = 2 * kPAccCols;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = p.m_tiles * p.n_tiles;
   constexpr int cluster_size = 2 * kSplit;
@@ -619,7 +634,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
           }
           tc_fence_after();
           const uint64_t a = desc0 + (uint32_t)stage * (kPStage >> 4), b = a + (kPStageX >> 4);
-          const uint32_t d = tmem_base + buf * kPN;
+          const uint32_t d = tmem_base + buf * kPAccCols;
           if (issuer) {
             mma_e4m3_pair<false>(d, a, b, kIdesc);
 #pragma unroll
@@ -650,8 +665,9 @@ __global__ void __launch_bounds__(kPThreads, 1)
         int m_tile, n_tile;
         prefill_tile(p, t, m_tile, n_tile);
         const int m0 = (2 * m_tile + rank) * kPM;
-        const float* sw0 = p.sw + (long long)(2 * n_tile) * p.ld_sw;
-        const bool two = (2 * n_tile + 1) * kTileN < p.N;  // the tile's second half has weight rows
+        const int nb = n_tile * kPN / kTileN;  // the tile's first block of weight rows
+        const float* sw0 = p.sw + (long long)nb * p.ld_sw;
+        const bool two = (nb + 1) * kTileN < p.N;  // it has a second one
         for (int kb = kb0 + kk; kb - kk < kb1; kb += kPScaleBlocks, ++chunk) {
           const uint32_t buf = chunk & 1;
           const bool in = kb < kb1;
@@ -695,6 +711,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
       prefill_tile(p, t, m_tile, n_tile);
       const int m_base = (2 * m_tile + rank) * kPM, m = m_base + row;
       const int n0 = n_tile * kPN + group * kPGroupCols;
+      const int second = (n_tile * kPN / kTileN + 1) * kTileN - n0;  // the group's first column of the second block
       float acc[kPGroupCols];
 #pragma unroll
       for (int j = 0; j < kPGroupCols; ++j) acc[j] = 0.f;
@@ -702,29 +719,32 @@ __global__ void __launch_bounds__(kPThreads, 1)
         const uint32_t sbuf = chunk & 1;
         ok = poll_wait(&c.sfull[sbuf], (chunk >> 1) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
         const int kn = min(kPScaleBlocks, kb1 - kb);
-        const float* scale = &c.scale[sbuf][group][0][row];
+        const float* scale = &c.scale[sbuf][kPN == 256 ? group : 0][0][row];
         for (int kk = 0; ok && kk < kn; ++kk, ++it, scale += kPScaleLd) {
           const uint32_t buf = it & 1;
           const float s = *scale;
+          const float s2 = kPN == 256 ? s : scale[kPScaleBlocks * kPScaleLd];
           if (!poll_wait(&c.tfull[buf], (it >> 1) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t taddr = taddr0 + buf * kPN;
-          uint32_t d[2][32];
+          const uint32_t taddr = taddr0 + buf * kPAccCols;
+          constexpr int kRead = kPN == 256 ? 64 : 96;  // columns at a time
+          uint32_t d[kRead / 32][32];
 #pragma unroll
-          for (int q = 0; q < kPGroupCols; q += 64) {
-            tmem_ld_x32(taddr + q, d[0]);
-            tmem_ld_x32(taddr + q + 32, d[1]);
+          for (int q = 0; q < kPGroupCols; q += kRead) {
+#pragma unroll
+            for (int i = 0; i < kRead / 32; ++i) tmem_ld_x32(taddr + q + 32 * i, d[i]);
             tmem_wait_ld();
-            if (q + 64 == kPGroupCols) {  // the accumulator is read: its next MMAs may start
+            if (q + kRead == kPGroupCols) {  // the accumulator is read: its next MMAs may start
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive_pair(buf ? tempty1 : tempty0);
             }
 #pragma unroll
-            for (int j = 0; j < 64; ++j) fma_after_ld(acc[q + j], d[j >> 5][j & 31], s);
+            for (int j = 0; j < kRead; ++j)
+              fma_after_ld(acc[q + j], d[j >> 5][j & 31], kPN == 256 || q + (j & ~31) < second ? s : s2);
           }
         }
         __syncwarp();
@@ -797,7 +817,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
           o.y = narrow2<T>(v[2], v[3]);
           o.z = narrow2<T>(v[4], v[5]);
           o.w = narrow2<T>(v[6], v[7]);
-          *reinterpret_cast<uint4*>(stg + staged(row, ch)) = o;
+          *reinterpret_cast<uint4*>(stg + staged<kPOutCols>(row, ch)) = o;
         }
         if (p.tma_out) {
           fence_proxy_async_smem();
@@ -812,7 +832,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
             for (int e = lane; e < kPOutCols; e += 32)
               if (nh + e < p.N)
                 out[mr * p.ld_out + nh + e] =
-                    *reinterpret_cast<const T*>(stg + staged(r, e >> 3) + (e & 7) * 2);
+                    *reinterpret_cast<const T*>(stg + staged<kPOutCols>(r, e >> 3) + (e & 7) * 2);
           }
         }
       }
@@ -894,7 +914,7 @@ int launch_decode(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
   constexpr int stage = (kTileN + NT) * kBlockK;
   constexpr int stages = std::min(kMaxStages, (kDecodeSmem - 1024) / stage);
   constexpr int smem = stages * stage + 1024;
-  static_assert(smem > kThirdOfSm && kPSmem + smem > 3 * kThirdOfSm);
+  static_assert(smem > kThirdOfSm && PrefillTile<192>::kSmem + smem > 3 * kThirdOfSm);
   p.stages = stages;
   const long long m_tiles = (p.M + NT - 1) / NT;
   const long long tiles = m_tiles * p.n_tiles;
@@ -908,23 +928,25 @@ int launch_decode(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
                             st, (unsigned)p.split, tw, tx, p);
 }
 
-// Row-major [rows, cols] of a 16-bit type with row stride ld, in boxes of 128 rows x 64 columns.
-int out_map(CUtensorMap* map, void* base, int dtype, long long rows, long long cols, long long ld) {
+// Row-major [rows, cols] of a 16-bit type with row stride ld, in boxes of 128 rows x 64 or 32 columns.
+int out_map(CUtensorMap* map, void* base, int dtype, long long rows, long long cols, long long ld, int box_cols) {
   auto fn = tensor_map_encoder();
   if (!fn) return fail(NPL_ERR_LAUNCH, "npl_fp8_linear: cuTensorMapEncodeTiled unavailable");
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {(cuuint32_t)kPOutCols, (cuuint32_t)kPM};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)kPM};
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r = fn(map, dtype == NPL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                        base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                         CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(NPL_ERR_ARG, "npl_fp8_linear: cuTensorMapEncodeTiled failed (%d)", (int)r);
   return NPL_OK;
 }
 
-template <typename T>
-int launch_prefill(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
+template <typename T, int kSplit, int kPN>
+int launch_prefill_tiles(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
+  using Tile = PrefillTile<kPN>;
   CUtensorMap tx, tw, to;
   if (int rc = code_map(&tx, o.qa, p.M, o.K, o.lda, kPM)) return rc;
   if (int rc = code_map(&tw, o.qw, p.N, o.K, o.ldw, kPN / 2)) return rc;
@@ -932,25 +954,45 @@ int launch_prefill(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
   p.vec_res = aligned16(p.residual) && p.ld_res % 8 == 0;
   to = tx;
   if (p.tma_out)
-    if (int rc = out_map(&to, p.out, o.out_dtype, p.M, p.N, p.ld_out)) return rc;
+    if (int rc = out_map(&to, p.out, o.out_dtype, p.M, p.N, p.ld_out, Tile::kOutCols)) return rc;
   p.m_tiles = (p.M + 2 * kPM - 1) / (2 * kPM);
   p.n_tiles = (p.N + kPN - 1) / kPN;
   const long long tiles = (long long)p.m_tiles * p.n_tiles;
   if (tiles > 1ll << 30)
     return fail(NPL_ERR_UNSUPPORTED, "npl_fp8_linear: M=%d N=%d has too many tiles", p.M, p.N);
   p.raster_g = std::min(8, p.m_tiles);
-  // Few tiles: two pairs share one where all run at once and have 8 blocks
-  // each or more (512 x 4096 x 11008: 30.4 us against 45.2; 256 x 4096 x 1024,
-  // with 4 blocks each, 10.2 against 9.4). Four pairs, clusters of 8 CTAs with an
-  // SM each, take 29 us where two take 16 (256 x 4096 x 4096).
-  const int pairs = num_sms() / 2;
-  const bool split = 2 * tiles <= pairs && p.k_blocks >= 16;
-  auto kern = split ? fp8_linear_prefill_kernel<T, 2> : fp8_linear_prefill_kernel<T, 1>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPSmem) != cudaSuccess)
+  auto kern = fp8_linear_prefill_kernel<T, kSplit, kPN>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem) != cudaSuccess)
     return launch_status("npl_fp8_linear: smem attribute");
-  const unsigned clusters = (unsigned)std::min<long long>(tiles, pairs), size = split ? 4 : 2;
-  return launch_pdl_cluster("npl_fp8_linear", kern, dim3(clusters * size), dim3(kPThreads), (size_t)kPSmem, st, size, tx,
-                            tw, to, p);
+  const unsigned clusters = (unsigned)std::min<long long>(tiles, num_sms() / 2);
+  return launch_pdl_cluster("npl_fp8_linear", kern, dim3(clusters * 2 * kSplit), dim3(kPThreads), (size_t)Tile::kSmem, st,
+                            2u * kSplit, tx, tw, to, p);
+}
+
+// Few tiles of 256 weight rows: two pairs share one where all clusters run at
+// once (33 of them do; with 34 256 x 8704 x 4096 takes 32.3 us, unsplit 18.3) and
+// have 12 blocks a pair or more (512 x 4096 x 11008: 27.2 us, unsplit 37.6; 256 x
+// 4096 x 3584 14.4 and 15.6; 512 x 4096 x 2560 14.2 and 13.9). Four pairs, clusters
+// of 8 CTAs with an SM each, take 29 us where two take 16 (256 x 4096 x 4096).
+// Otherwise tiles of 192 weight rows, whose blocks take seven eighths of the time,
+// where the pairs have them done in as many rounds as those of 256 (560 x 4096 x
+// 11008, 66 tiles or 48: 40.1 us against 45.3; 1024 x 5120 x 5120, 108 or 80: 36.6
+// against 40.7), but not for one round more (560 x 12288 x 4096, 192 or 144: 47.6
+// against 37.9; 560 x 32003 x 4096, 501 or 378: 145 against 130).
+template <typename T>
+int launch_prefill(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
+  const long long pairs = num_sms() / 2, m_tiles = ((long long)p.M + 2 * kPM - 1) / (2 * kPM);
+  const long long wide = m_tiles * ((p.N + 255ll) / 256), narrow = m_tiles * ((p.N + 191ll) / 192);
+  if (2 * wide <= pairs && p.k_blocks >= 24) {
+    auto* kern = fp8_linear_prefill_kernel<T, 2, 256>;
+    constexpr int smem = PrefillTile<256>::kSmem;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return launch_status("npl_fp8_linear: smem attribute");
+    if (wide <= max_active_clusters(reinterpret_cast<const void*>(kern), smem, 4, kPThreads))
+      return launch_prefill_tiles<T, 2, 256>(o, p, st);
+  }
+  if ((narrow + pairs - 1) / pairs <= (wide + pairs - 1) / pairs) return launch_prefill_tiles<T, 1, 192>(o, p, st);
+  return launch_prefill_tiles<T, 1, 256>(o, p, st);
 }
 
 // Decode tiles up to 64 tokens. Two rows of them, up to 128 tokens, as long as

@@ -51,8 +51,6 @@
 #include <algorithm>
 #include <atomic>
 #include <initializer_list>
-#include <mutex>
-#include <vector>
 
 #include "npl_common.cuh"
 
@@ -1190,41 +1188,6 @@ size_t ws_bytes(int M) {
 }
 
 constexpr uint32_t align1k(size_t x) { return (uint32_t)((x + 1023) & ~size_t(1023)); }
-
-// Clusters of `split` CTAs of `kern` with `smem` bytes that fit on the
-// device at once (cached per device, kernel, shared memory and size).
-int max_active_clusters(const void* kern, int smem, int split, int block) {
-  struct Entry {
-    int dev;
-    const void* kern;
-    int smem, split, n;
-  };
-  static std::mutex mu;
-  static std::vector<Entry> cache;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  std::lock_guard<std::mutex> lock(mu);
-  for (const Entry& e : cache)
-    if (e.dev == dev && e.kern == kern && e.smem == smem && e.split == split) return e.n;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)split);
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
-    (void)cudaGetLastError();
-    n = 0;
-  }
-  cache.push_back({dev, kern, smem, split, n});
-  return n;
-}
 
 // Shared memory that leaves room for one CTA per SM only: the cluster
 // capacity at this size is the number of clusters that fit with every CTA on

@@ -24,6 +24,7 @@ void set_error(const char* fmt, ...);
 int fail(int code, const char* fmt, ...);
 int launch_status(const char* what);   // maps cudaGetLastError to NPL_ERR_LAUNCH
 int num_sms();                         // cached per current device
+int max_active_clusters(const void* kern, int smem, int split, int block);
 int* device_status_ptr();              // address of the per-device error word
 int check_device();                    // NPL_OK on an sm_100 device
 

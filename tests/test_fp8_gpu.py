@@ -295,6 +295,18 @@ def test_linear_random(F, cuda_device, m, n, k, dtype):
     assert (np.abs(out - want) <= tol + half * (np.abs(want) + tol)).all()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m,n,k", [
+    (150, 190, 200), (300, 193, 300), (260, 385, 130), (257, 4000, 260), (800, 4093, 300), (800, 4096, 300),
+    (1025, 3900, 140), (140, 200, 3071), (300, 700, 2944), (300, 700, 2945), (129, 8448, 3200), (129, 8449, 3200),
+    (200, 9472, 3200)])
+def test_linear_tile_choices(F, cuda_device, m, n, k, dtype):
+    """Tiles of 192 and 256 weight rows in one round or two, ragged or not, and
+    tiles shared by two pairs of CTAs, up to more than fit on the device at
+    once. The sums are exact (K <= 2^13, as test_linear_exact_sums)."""
+    test_linear_exact_sums(F, cuda_device, m, n, k, dtype)
+
+
 def test_linear_layouts(F, cuda_device):
     """Strided scales, residual and output; the residual in place; columns and
     rows around the output untouched; odd output strides."""

@@ -825,14 +825,20 @@ __global__ void __launch_bounds__(kPThreads, 1)
           if (elected && nh < p.N && m_base < p.M) tma_store_2d(&tmap_out, stg, nh, m_base);
         } else {  // rows that TMA cannot store: element by element, 32 columns a warp
           group_bar();
-          for (int r = (warp & 3); r < kPM; r += 4) {
-            const long long mr = (long long)m_base + r;
-            if (mr >= p.M) break;
+          constexpr int kAtOnce = 8;  // rows read before the first store (8000 x 513 x 1024: 22.6 us, one by one 28.3)
+          for (int r0 = (warp & 3); r0 < kPM && m_base + r0 < p.M; r0 += 4 * kAtOnce) {
 #pragma unroll
-            for (int e = lane; e < kPOutCols; e += 32)
-              if (nh + e < p.N)
-                out[mr * p.ld_out + nh + e] =
-                    *reinterpret_cast<const T*>(stg + staged<kPOutCols>(r, e >> 3) + (e & 7) * 2);
+            for (int e = lane; e < kPOutCols; e += 32) {
+              T v[kAtOnce];
+#pragma unroll
+              for (int i = 0; i < kAtOnce; ++i)
+                v[i] = *reinterpret_cast<const T*>(stg + staged<kPOutCols>(r0 + 4 * i, e >> 3) + (e & 7) * 2);
+#pragma unroll
+              for (int i = 0; i < kAtOnce; ++i) {
+                const long long mr = (long long)m_base + r0 + 4 * i;
+                if (mr < p.M && nh + e < p.N) out[mr * p.ld_out + nh + e] = v[i];
+              }
+            }
           }
         }
       }

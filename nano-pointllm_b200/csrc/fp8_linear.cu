@@ -1002,14 +1002,16 @@ int launch_prefill(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
 }
 
 // Decode tiles up to 64 tokens. Two rows of them, up to 128 tokens, as long as
-// they still split three ways (128 x 4096 x 4096: 12.1 us against 15.3 with
-// prefill tiles; 128 x 12288 x 4096, which does not split: 21.0 against 20.1;
-// four rows, 200 x 4096 x 4096: 20.0 against 15.5).
+// they still split three ways (100 x 4096 x 4096: 12.6 us against 15.1 with
+// prefill tiles; 100 x 5504 x 4096 15.0 and 16.3; 100 x 6144 x 4096, which does not
+// split, 20.1 and 16.4) and the rows are not short (128 x 4096 x 1024: 9.5 and 7.5;
+// x 2048 10.6 and 10.2). Four rows: 200 x 4096 x 4096 20.0 and 15.5.
 template <typename T>
 int launch(const Operands& o, Fp8LinearArgs& p, cudaStream_t st) {
   if (p.M <= 16) return launch_decode<T, 16>(o, p, st);
   if (p.M <= 32) return launch_decode<T, 32>(o, p, st);
-  if (p.M <= 64 || (p.M <= 128 && decode_split(2ll * p.n_tiles, p.k_blocks) >= 3)) return launch_decode<T, 64>(o, p, st);
+  const bool two_rows = p.M <= 128 && p.k_blocks >= 20 && decode_split(2ll * p.n_tiles, p.k_blocks) >= 3;
+  if (p.M <= 64 || two_rows) return launch_decode<T, 64>(o, p, st);
   return launch_prefill<T>(o, p, st);
 }
 

@@ -299,11 +299,11 @@ def test_linear_random(F, cuda_device, m, n, k, dtype):
 @pytest.mark.parametrize("m,n,k", [
     (150, 190, 200), (300, 193, 300), (260, 385, 130), (257, 4000, 260), (800, 4093, 300), (800, 4096, 300),
     (1025, 3900, 140), (140, 200, 3071), (300, 700, 2944), (300, 700, 2945), (129, 8448, 3200), (129, 8449, 3200),
-    (200, 9472, 3200)])
+    (200, 9472, 3200), (100, 300, 2432), (100, 300, 2433), (128, 5504, 2500), (65, 5505, 2500)])
 def test_linear_tile_choices(F, cuda_device, m, n, k, dtype):
     """Tiles of 192 and 256 weight rows in one round or two, ragged or not, and
     tiles shared by two pairs of CTAs, up to more than fit on the device at
-    once. The sums are exact (K <= 2^13, as test_linear_exact_sums)."""
+    once; 65 to 128 tokens in decode tiles or not. The sums are exact (K <= 2^13, as test_linear_exact_sums)."""
     test_linear_exact_sums(F, cuda_device, m, n, k, dtype)
 
 

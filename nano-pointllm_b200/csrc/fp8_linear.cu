@@ -36,6 +36,7 @@
 
 #include <algorithm>
 
+#include "fp8_epilogue.cuh"
 #include "npl_common.cuh"
 
 namespace npl {
@@ -103,13 +104,41 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 
-// mbar_wait that looks at the clock only after many polls (of 20 ns or more):
-// where every block waits, reading it takes longer than most waits.
+// mbar_wait of a whole warp, the same in all lanes. It looks at the clock only
+// after many polls (of 20 ns or more): where every block waits, reading it
+// takes longer than most waits. kVote: the lanes vote on every poll, which is
+// faster in the decode kernel (32 x 12288 x 4096: 15.5 us, without 16.4) and slower
+// in the prefill kernel (16000 x 22016 x 4096: 1568 us, without 1530).
+template <bool kVote>
 __device__ __forceinline__ bool poll_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
-#pragma unroll 1
-  for (int i = 0; i < 1024; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, status, code);
+  uint64_t t0 = 0;
+  auto try_once = [&] { return mbar_try_wait(bar, parity); };
+  auto late = [&] {
+    const uint64_t t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    return t - t0 > kWaitLimitNs;
+  };
+  bool done;
+  if constexpr (kVote)
+    done = wait_voting(1024, try_once, [](bool v) { return __all_sync(0xffffffffu, v) != 0; }, late);
+  else
+    done = wait_as_one(1024, try_once, [](bool v) { return __any_sync(__activemask(), v) != 0; }, late);
+  if (!done && status) atomicExch(status, code);
+  return done;
+}
+
+// Whether ok holds in all 128 threads of a warpgroup, which meet at barrier `id`.
+__device__ __forceinline__ bool warpgroup_agrees(int id, bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(id), "r"((uint32_t)ok)
+      : "memory");
+  return all != 0;
 }
 
 // Instruction descriptor of kind::f8f6f4: fp32 accumulator (c_format [4,6) =
@@ -222,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     int stage = 0, loads = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!poll_wait(&c.empty[stage], phase ^ 1, p.status, NPL_DEV_TIMEOUT_TMA)) break;
+      if (!poll_wait<true>(&c.empty[stage], phase ^ 1, p.status, NPL_DEV_TIMEOUT_TMA)) break;
       if (issuer) {
         mbar_arrive_expect_tx(&c.full[stage], kStageW + kStageX);
         tma_load_2d(ring_w + (size_t)stage * kStageW, &tmap_w, kb * kBlockK, n_tile * kTileN, &c.full[stage], pol_w);
@@ -237,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     // every issued load lands before the ring is used again or released: stage
     // i was last loaded with the parity of that load
     for (int i = 0; i < loads; ++i)
-      poll_wait(&c.full[i], i < stage ? phase : phase ^ 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+      poll_wait<true>(&c.full[i], i < stage ? phase : phase ^ 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
     __syncwarp();
   } else if (warp == 1) {
     // The whole warp runs this loop and one lane issues, so that descriptors
@@ -248,8 +277,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
       const int i = kb - kb0, unit = i / U, buf = unit % kUnits, u = i % U;
-      if (!poll_wait(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA)) break;
-      if (u == 0 && !poll_wait(&c.tempty[buf], ((unit / kUnits) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA)) break;
+      if (!poll_wait<true>(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA)) break;
+      if (u == 0 && !poll_wait<true>(&c.tempty[buf], ((unit / kUnits) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA)) break;
       tc_fence_after();
       const uint64_t a = desc_w + (uint32_t)stage * (kStageW >> 4), b = desc_x + (uint32_t)stage * (kStageX >> 4);
       const uint32_t d = tmem_base + (uint32_t)(buf * kUnitCols + u * NT);
@@ -268,63 +297,57 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     // all MMAs issued complete before the ring and TMEM are given up
     if (issuer) tc_commit(&c.teardown);
-    poll_wait(&c.teardown, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+    poll_wait<true>(&c.teardown, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
     __syncwarp();
   } else {
     pdl_wait();
-    bool ok = true;
-    int unit = 0;
-    for (int kc = kb0; ok && kc < kb1; kc += kScaleBlocks) {
-      // The scales of the next kScaleBlocks blocks: a warp reads a token's with
-      // one load, all loads of a thread at once.
-      {
-        const int b = kc + lane;
-        const float w = b < kb1 ? p.sw[(long long)n_tile * p.ld_sw + b] : 0.f;
-        float a[NT / 4];
+    // The scales of the next kScaleBlocks blocks: a warp reads a token's with
+    // one load, all loads of a thread at once.
+    auto scales = [&](int kc) {
+      const int b = kc + lane;
+      const float w = b < kb1 ? p.sw[(long long)n_tile * p.ld_sw + b] : 0.f;
+      float a[NT / 4];
 #pragma unroll
-        for (int i = 0; i < NT / 4; ++i) {
-          const int m = m_tile * NT + 4 * i + quarter;
-          a[i] = b < kb1 && m < p.M ? p.sa[(long long)m * p.ld_sa + b] : 0.f;
-        }
-        if (kc > kb0) asm volatile("bar.sync 1, 128;" ::: "memory");  // the scales before are read
-#pragma unroll
-        for (int i = 0; i < NT / 4; ++i) s_scale[lane][4 * i + quarter] = __fmul_rn(a[i], w);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int i = 0; i < NT / 4; ++i) {
+        const int m = m_tile * NT + 4 * i + quarter;
+        a[i] = b < kb1 && m < p.M ? p.sa[(long long)m * p.ld_sa + b] : 0.f;
       }
-      const int kn = min(kScaleBlocks, kb1 - kc);
-      for (int k = 0; k < kn; k += U, ++unit) {
-        const int buf = unit % kUnits;
-        if (!poll_wait(&c.tfull[buf], (unit / kUnits) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
-          ok = false;
-          break;
+      if (kc > kb0) asm volatile("bar.sync 1, 128;" ::: "memory");  // the scales before are read
+#pragma unroll
+      for (int i = 0; i < NT / 4; ++i) s_scale[lane][4 * i + quarter] = __fmul_rn(a[i], w);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    };
+    auto add_unit = [&](int unit, int, int k, int kn) {
+      const int buf = unit % kUnits;
+      if (!poll_wait<true>(&c.tfull[buf], (unit / kUnits) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) return false;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * kUnitCols);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float sc[32];  // loaded ahead of their uses
+#pragma unroll
+        for (int q = 0; q < 32; q += 4) {
+          const int at = 32 * h + q;
+          lds128(&s_scale[k + at / NT][at % NT], sc + q);
         }
-        tc_fence_after();
-        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * kUnitCols);
+        uint32_t d[32];
+        tmem_ld_x32(taddr + 32 * h, d);
+        tmem_wait_ld();
+        if (h == 1) {  // the unit is read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&c.tempty[buf]);
+        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float sc[32];  // loaded ahead of their uses
-#pragma unroll
-          for (int q = 0; q < 32; q += 4) {
-            const int at = 32 * h + q;
-            lds128(&s_scale[k + at / NT][at % NT], sc + q);
-          }
-          uint32_t d[32];
-          tmem_ld_x32(taddr + 32 * h, d);
-          tmem_wait_ld();
-          if (h == 1) {  // the unit is read
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&c.tempty[buf]);
-          }
-#pragma unroll
-          for (int q = 0; q < 32; ++q) {
-            const int at = 32 * h + q;  // block at / NT, which a last unit may lack: what TMEM holds there is not used
-            if (at % NT == 0 && k + at / NT >= kn) break;
-            fma_after_ld(acc[at % NT], d[q], sc[q]);
-          }
+        for (int q = 0; q < 32; ++q) {
+          const int at = 32 * h + q;  // block at / NT, which a last unit may lack: what TMEM holds there is not used
+          if (at % NT == 0 && k + at / NT >= kn) break;
+          fma_after_ld(acc[at % NT], d[q], sc[q]);
         }
       }
-    }
+      return true;
+    };
+    decode_epilogue(kb0, kb1, kScaleBlocks, U, scales, add_unit);
   }
 
   tc_fence_before();
@@ -627,8 +650,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
       for (int t = cluster; ok && t < tiles; t += clusters) {
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const uint32_t buf = it & 1;
-          if (!poll_wait(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA) ||
-              !poll_wait(&c.tempty[buf], ((it >> 1) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA)) {
+          if (!poll_wait<false>(&c.full[stage], phase, p.status, NPL_DEV_TIMEOUT_MMA) ||
+              !poll_wait<false>(&c.tempty[buf], ((it >> 1) & 1) ^ 1, p.status, NPL_DEV_TIMEOUT_MMA)) {
             ok = false;
             break;
           }
@@ -651,7 +674,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
       }
       // all MMAs complete, in both CTAs' view, before TMEM is freed
       if (rank == 0 && issuer) tc_commit_pair(&c.teardown, both);
-      poll_wait(&c.teardown, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+      poll_wait<false>(&c.teardown, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
       __syncwarp();
     } else if (warp >= 2) {
       // A load of a warp reads kPScaleBlocks blocks of 32 / kPScaleBlocks tokens;
@@ -705,26 +728,29 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const uint32_t tempty0 = cluster_map(&c.tempty[0], leader), tempty1 = cluster_map(&c.tempty[1], leader);
     const uint32_t taddr0 = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + group * kPGroupCols;
     uint32_t it = 0, chunk = 0;
-    bool ok = true;
-    for (int t = cluster; ok && t < tiles; t += clusters) {
+    float acc[kPGroupCols];
+    int m_base = 0, n_out = 0;  // the first token and column that this warpgroup writes, in `boxes` boxes
+    constexpr int boxes = kSplit > 1 ? 1 : kPGroupCols / kPOutCols;
+    auto sums_of = [&](int t) {
       int m_tile, n_tile;
       prefill_tile(p, t, m_tile, n_tile);
-      const int m_base = (2 * m_tile + rank) * kPM, m = m_base + row;
+      m_base = (2 * m_tile + rank) * kPM;
       const int n0 = n_tile * kPN + group * kPGroupCols;
       const int second = (n_tile * kPN / kTileN + 1) * kTileN - n0;  // the group's first column of the second block
-      float acc[kPGroupCols];
+      bool ok = true;
+      n_out = n0;
 #pragma unroll
       for (int j = 0; j < kPGroupCols; ++j) acc[j] = 0.f;
       for (int kb = kb0; ok && kb < kb1; kb += kPScaleBlocks, ++chunk) {
         const uint32_t sbuf = chunk & 1;
-        ok = poll_wait(&c.sfull[sbuf], (chunk >> 1) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
+        ok = poll_wait<false>(&c.sfull[sbuf], (chunk >> 1) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
         const int kn = min(kPScaleBlocks, kb1 - kb);
         const float* scale = &c.scale[sbuf][kPN == 256 ? group : 0][0][row];
         for (int kk = 0; ok && kk < kn; ++kk, ++it, scale += kPScaleLd) {
           const uint32_t buf = it & 1;
           const float s = *scale;
           const float s2 = kPN == 256 ? s : scale[kPScaleBlocks * kPScaleLd];
-          if (!poll_wait(&c.tfull[buf], (it >> 1) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
+          if (!poll_wait<false>(&c.tfull[buf], (it >> 1) & 1, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
             ok = false;
             break;
           }
@@ -750,7 +776,6 @@ __global__ void __launch_bounds__(kPThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&c.sempty[sbuf]);  // the chunk of scales is read
       }
-      int boxes = kPGroupCols / kPOutCols, n_out = n0;
       if constexpr (kSplit > 1) {
         // The sums of this CTA's blocks go to its ring, which its last MMAs are
         // done with, [column][token]; after the barrier the CTAs of one rank add
@@ -764,7 +789,6 @@ __global__ void __launch_bounds__(kPThreads, 1)
         cluster_arrive_release();
         cluster_wait_acquire();
         const int col = (part * kPGroups + group) * kPOutCols;
-        boxes = 1;
         n_out = n_tile * kPN + col;
         if (ok) {
           uint32_t from[kSplit];
@@ -779,11 +803,13 @@ __global__ void __launch_bounds__(kPThreads, 1)
           }
         }
       }
-      if (!ok) break;
-      // bias, residual, rounding; 64 columns at a time through shared memory
+      return ok;
+    };
+    auto write = [&](int) {
+      const int m = m_base + row;
+      // bias, residual, rounding; kPOutCols columns at a time through shared memory
 #pragma unroll
-      for (int h = 0; h < kPGroupCols / kPOutCols; ++h) {
-        if (h >= boxes) break;
+      for (int h = 0; h < boxes; ++h) {
         const int nh = n_out + h * kPOutCols;
         if (elected) tma_store_wait_read();
         group_bar();  // the staging buffer is free
@@ -842,7 +868,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
           }
         }
       }
-    }
+    };
+    prefill_epilogue(cluster, clusters, tiles, sums_of, [&](bool ok) { return warpgroup_agrees(1 + group, ok); }, write);
     if (elected) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   if (kSplit > 1 && warp < 4) {  // the epilogue warps' barrier over the sums

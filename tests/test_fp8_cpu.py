@@ -217,3 +217,134 @@ def test_block_linear_lays_out_checkpoint_rows():
     lin = fp8.Fp8BlockLinear(codes, torch.ones(1, 1))
     assert lin.qweight.stride(0) == 80 and torch.equal(lin.qweight.float(), codes.float())
     assert (lin.in_features, lin.out_features) == (77, 10)
+
+
+_EPILOGUE = r"""
+// Threads as lanes or warps on the loops of fp8_epilogue.cuh; a meeting that one of them
+// misses is seen after a second and ends the program.
+#include <chrono>
+#include <condition_variable>
+#include <cstdio>
+#include <cstdlib>
+#include <functional>
+#include <mutex>
+#include <thread>
+#include <vector>
+#include "fp8_epilogue.cuh"
+
+struct Meeting {  // n threads; and of what they bring
+  std::mutex m;
+  std::condition_variable cv;
+  int n, here = 0, turn = 0;
+  bool all = true, result[2];
+  explicit Meeting(int k) : n(k) {}
+  void leave() {
+    std::unique_lock<std::mutex> l(m);
+    if (here == --n && n > 0) done();
+  }
+  void done() {
+    result[turn & 1] = all, all = true, here = 0, ++turn;
+    cv.notify_all();
+  }
+  bool meet(bool v, const char* what) {
+    std::unique_lock<std::mutex> l(m);
+    const int t = turn;
+    all = all && v;
+    if (++here == n) {
+      done();
+    } else if (!cv.wait_for(l, std::chrono::seconds(1), [&] { return turn != t; })) {
+      std::printf("left alone in %s\n", what);
+      std::fflush(stdout);
+      std::_Exit(1);
+    }
+    return result[t & 1];
+  }
+};
+
+void run(int n, const std::function<void(int)>& f) {
+  std::vector<std::thread> ts;
+  for (int i = 0; i < n; ++i) ts.emplace_back(f, i);
+  for (auto& t : ts) t.join();
+}
+
+void expect(bool v, const char* what) {
+  if (v) return;
+  std::printf("%s\n", what);
+  std::fflush(stdout);
+  std::_Exit(1);
+}
+
+int main() {
+  // one warp gives up at a unit, or none does (fail = -1)
+  for (int fail : {-1, 0, 7, 8, 9, 35, 36}) {
+    Meeting m(4);
+    std::vector<int> units(4, 0), chunks(4, 0);
+    run(4, [&](int w) {
+      npl::decode_epilogue(3, 76, 32, 2, [&](int kc) { ++chunks[w], m.meet(true, "the scales"); },
+                           [&](int i, int kc, int k, int kn) {
+                             expect(i == units[w] && i == (kc - 3 + k) / 2 && kn == (kc == 67 ? 9 : 32), "wrong unit");
+                             if (w == 2 && i == fail) return false;
+                             ++units[w];
+                             return true;
+                           });
+      expect(chunks[w] == 3 && units[w] == (w == 2 && fail >= 0 ? fail : 37), "wrong count");
+    });
+  }
+  // one warp has no sums of a tile: none writes it or goes on
+  for (int fail : {-1, 0, 2, 4}) {
+    Meeting m(4);
+    std::vector<int> wrote(4, 0);
+    run(4, [&](int w) {
+      npl::prefill_epilogue(5, 3, 19, [&](int t) { return !(w == 1 && t == 5 + 3 * fail); },
+                            [&](bool ok) { return m.meet(ok, "the agreement"); },
+                            [&](int t) {
+                              expect(t == 5 + 3 * wrote[w], "wrong tile");
+                              for (int box = 0; box < 4; ++box) m.meet(true, "the boxes");
+                              ++wrote[w];
+                            });
+      expect(wrote[w] == (fail < 0 ? 5 : fail), "wrote a tile that a warp has no sums of");
+    });
+  }
+  // One lane's deadline passes after three tries, all others' never. The phase is complete for lanes 6
+  // and 7 in try arrival / 2, for the others one try later where the arrival is odd.
+  for (int arrival : {0, 3, 5, 6, 7, 8, 9, 1000})
+    for (bool voting : {false, true}) {
+      Meeting vote(8), after(8);
+      std::vector<int> got(8, -1);
+      run(8, [&](int lane) {
+        int tries = 0;
+        auto try_once = [&] { return 2 * tries++ + (lane > 5) >= arrival; };
+        auto late = [&] { return lane == 3; };
+        got[lane] = voting ? npl::wait_voting(3, try_once, [&](bool x) { return vote.meet(x, "a vote"); }, late)
+                           : npl::wait_as_one(3, try_once, [&](bool x) { return !vote.meet(!x, "the vote"); }, late);
+        vote.leave();
+        after.meet(true, "a warp-wide instruction");
+      });
+      for (int lane = 0; lane < 8; ++lane) expect(got[lane] == (arrival < (voting ? 5 : 8)), "lanes differ");
+    }
+  std::printf("ok\n");
+}
+"""
+
+
+def test_epilogue_meets_in_full_when_a_wait_runs_out(tmp_path):
+    """The epilogue's own loops, compiled for the host: whichever warp (or lane)
+    gives up a wait, all of them meet as often as each other."""
+    import pathlib
+    import shutil
+    import subprocess
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no C++ compiler")
+    src = tmp_path / "epilogue.cpp"
+    src.write_text(_EPILOGUE)
+    csrc = pathlib.Path(__file__).resolve().parent.parent / "nano-pointllm_b200" / "csrc"
+    subprocess.run([cxx, "-std=c++17", "-O1", "-pthread", f"-I{csrc}", str(src), "-o", str(tmp_path / "epilogue")],
+                   check=True)
+    out = subprocess.run([str(tmp_path / "epilogue")], capture_output=True, text=True, timeout=60)
+    assert out.returncode == 0 and out.stdout == "ok\n", out.stdout
+    # the kernels run these loops, and meet at a named barrier nowhere else
+    kernel = (csrc / "fp8_linear.cu").read_text()
+    for loop in ("wait_as_one(", "wait_voting(", "decode_epilogue(kb0", "prefill_epilogue(cluster"):
+        assert kernel.count(loop) == 1, loop
+    assert kernel.count("bar.sync") == 3 and kernel.count("barrier.cta") == 1

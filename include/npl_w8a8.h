@@ -435,8 +435,10 @@ int npl_fp8_rmsnorm_quant(const void* x, int64_t ldx, const void* residual_or_nu
                           int dtype, float eps, int64_t rows, int64_t cols, void* sum_out_or_null, int64_t ld_sum,
                           uint8_t* q, int64_t ldq, float* scale, int64_t ld_scale, void* stream);
 
-/* v = gate / (1 + exp(-gate)) * up (fp32), then npl_fp8_quant_rows of v. gate
- * and up may be the two halves of one packed projection's rows. */
+/* v = gate / (1 + exp(-gate)) * up, then npl_fp8_quant_rows of v. In fp32 steps
+ * that keep v within 2^-18 also where exp(-gate) leaves fp32's range; a gate of
+ * -inf gives NaN. gate and up may be the two halves of one packed projection's
+ * rows. */
 int npl_fp8_silu_mul_quant(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int dtype, int64_t rows,
                            int64_t cols, uint8_t* q, int64_t ldq, float* scale, int64_t ld_scale, void* stream);
 

@@ -256,7 +256,8 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, uint4 q, int n) {
 }
 
 // Where the quantised values come from: what a thread loads for its columns,
-// what it keeps of them, their key and the fp32 values.
+// what it keeps of them, what is worked out anew of it (from the same columns,
+// loaded again, for a warp that holds rare values), their key and the fp32 values.
 template <typename T, int kAccess>
 struct RowSource {  // the row itself
   using Elem = T;
@@ -269,12 +270,22 @@ struct RowSource {  // the row itself
     return load16<kAccess>(x + row * ldx + col, n, x, end);
   }
   __device__ __forceinline__ static Kept keep(const Loaded& r) { return r; }
+  __device__ __forceinline__ void rework(int, int, int, Kept&) const {}
   __device__ __forceinline__ static uint32_t key(const Kept& k) { return key_of(k); }
   __device__ __forceinline__ static void values(const Kept& k, float (&v)[kCols]) { widen(k, v); }
 };
 
-// silu(g) up = g / (1 + e^-g) up in fp32, within a few ulps. For g below
-// -87.3, where it is under 1e-36, the approximate reciprocal gives 0.
+// silu(g) up = g / (1 + e^-g) up in fp32, within a few ulps. Below -87.3 the
+// approximate reciprocal flushes to 0, and from -88.7 on e^-g overflows, although
+// a large up makes such a product any size. For these far gates, where 1 + e^g is
+// 1 in fp32, it is (g p) (p up) with p = e^(g / 2). Below -174 p is subnormal, off
+// by 2^-150 at most, and the product by 2^-149 |g| p up: at scales of 2^-126 or
+// more under 2^-13 in units of a code, whose smallest is 2^-9. A warp that holds
+// one loads its columns again for it: 16000 x 11008 takes 206 us (bf16 209), 199
+// without the question, 229 (239) with this formula for all gates, which needs
+// no question, and 217 (232) with the columns kept until it is answered.
+constexpr float kFarGate = -86.0f;
+
 template <typename T, int kAccess>
 struct SiluSource {
   using Elem = float;
@@ -283,7 +294,10 @@ struct SiluSource {
   };
   struct Kept {
     float v[kCols];
+    bool far;
   };
+  // Patterns above kFarGate's: numbers below it, and NaNs with a sign.
+  static constexpr uint32_t kFarBits = std::is_same_v<T, __half> ? 0xd560u : 0xc2acu;
   const T* gate;
   const T* up;
   long long ld_gate, ld_up;
@@ -294,6 +308,12 @@ struct SiluSource {
   }
   __device__ __forceinline__ static Kept keep(const Loaded& r) {
     Kept k;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r.g);
+    uint32_t top = __vimax3_u16x2(w[0], w[1], w[2]);
+    top = __vimax3_u16x2(top, w[3], w[4]);
+    top = __vimax3_u16x2(top, w[5], w[6]);
+    top = __vmaxu2(top, w[7]);
+    k.far = max(top & 0xffffu, top >> 16) > kFarBits;
     float up[kCols];
     widen(r.g, k.v);
     widen(r.u, up);
@@ -304,6 +324,18 @@ struct SiluSource {
       k.v[i] = __fmul_rn(__fmul_rn(k.v[i], sig), up[i]);
     }
     return k;
+  }
+  __device__ __forceinline__ void rework(int row, int col, int n, Kept& k) const {
+    if (!__any_sync(0xffffffffu, k.far)) return;
+    const Loaded r = load(row, col, n);
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) {
+      const float g = (float)r.g.e[i];
+      if (g < kFarGate) {
+        const float p = expf(__fmul_rn(0.5f, g));
+        k.v[i] = __fmul_rn(__fmul_rn(g, p), __fmul_rn(p, (float)r.u.e[i]));
+      }
+    }
   }
   __device__ __forceinline__ static uint32_t key(const Kept& k) { return key_of(k.v); }
   __device__ __forceinline__ static void values(const Kept& k, float (&v)[kCols]) {
@@ -325,9 +357,9 @@ constexpr int kNormThreads = 512;
 // A warp takes 4 U consecutive blocks of a row, each of its four 8-lane groups
 // every fourth, all loads before the first store, which the compiler would not
 // move them across. Bound by instructions and memory alike: 16000 x 4096 fp16
-// takes 36.9 us (5.4 TB/s), SiLU * up of 16000 x 11008 197 us (4.5 TB/s). With 8
-// columns a thread, which doubles the work per block, they took 48 and 281;
-// warps that stay and load their next span first, 53 and 281.
+// takes 37.8 us (5.3 TB/s), SiLU * up of 16000 x 11008 206 us (4.3 TB/s). With 8
+// columns a thread, which doubles the work per block, they took 48 and 281
+// (when SiLU took 197); warps that stay and load their next span first, 53 and 281.
 template <typename Source, int U, bool kVecQ>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(typename Source::Loaded) > 32 ? 4 : 5)
     fp8_quant_kernel(const Source src, const CodeSink out, int rows, int cols, unsigned spans) {
@@ -349,7 +381,9 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(typename Source::Loaded)
   uint32_t key[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
+    const int col = col0 + u * (4 * kBlock);
     kept[u] = Source::keep(raw[u]);
+    src.rework(row, col < cols ? col : 0, cols - col, kept[u]);
     key[u] = Source::key(kept[u]);
   }
   const float s = block_scale(key_value<typename Source::Elem>(block_key<U>(key, lane)));
@@ -554,7 +588,7 @@ int launch_quant_spans(const char* what, const Source& src, const CodeSink& out,
 // Two blocks a thread where a thread's loads are 32 bytes, except where the
 // rows are short (half of the warps' lanes or more would idle) or so few that
 // one block a thread fits on the SMs at once. For SiLU, whose values take 16
-// registers a block, one (16000 x 4096: 71 us, with two 114).
+// registers a block, one (16000 x 4096: 71 us when this was chosen, with two 114).
 template <typename Source>
 int launch_quant(const char* what, const Source& src, const CodeSink& out, int rows, int cols, cudaStream_t st) {
   constexpr int U = sizeof(typename Source::Loaded) > 32 ? 1 : 2;

@@ -522,3 +522,50 @@ def test_operands_of_two_devices_are_refused(F, cuda_device, m):
         F.linear_blocks(q, s.cpu(), *w)
     with pytest.raises(ValueError, match="device"):
         F.rmsnorm_quant_blocks(x, torch.ones(256, dtype=F16), 1e-6)
+
+
+# ------------------------------------------------------------- far SiLU gates
+@pytest.mark.parametrize("how", ["contiguous", "unaligned"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lo,hi", [(-88.5, -87.4), (-89.0, -85.0), (-104.0, -88.8), (-170.0, -110.0), (-210.0, -165.0)])
+def test_silu_blocks_of_far_gates(F, cuda_device, lo, hi, dtype, how):
+    """Blocks whose gates are all far below 0, so that e^-g leaves fp32's
+    normal range, under ups of any size. VAL, and 2^-13 in units of a code for
+    p = e^(g / 2) once it is subnormal: 2^-149 |g| p up / scale with |g| < 2^8, p < 2^-126,
+    up < 2^128 and scale >= 2^-126."""
+    m, k = 6, 300
+    gen = torch.Generator().manual_seed(int(-lo * 8))
+    g = (lo + (hi - lo) * torch.rand(m, k, generator=gen)).to(dtype)
+    u = torch.rand(m, k, generator=gen) * 0.5 + 0.25
+    big = float(torch.finfo(dtype).max)
+    u = (u * torch.tensor([big, big / 1e3, 3e4, 1.0, -big, 1e-3]).double()[:, None]).to(dtype)
+    q, s = F.silu_mul_quant_blocks(laid_out(g, how, cuda_device), laid_out(u, how, cuda_device))
+    v = O.silu_mul(cpu(g), cpu(u))
+    es = O.block_scales(v, 1)
+    np.testing.assert_allclose(cpu(s), es, rtol=VAL + 2.0 ** -23, atol=0)
+    want = v / O.spread(es, 1, v.shape)
+    off = np.abs(cpu(q) - want)
+    assert (off <= O.half_step_e4m3(want) + 2 * VAL * np.abs(want) + 2.0 ** -13).all()
+
+
+def test_silu_far_gates_beside_others(F, cuda_device):
+    """A far gate changes no other value of its block, and an infinite or NaN
+    one makes its block NaN."""
+    u = rand((3, 256), BF16, 3)
+    g = rand((3, 256), BF16, 4)
+    plain = [cpu(t) for t in F.silu_mul_quant_blocks(g.to(cuda_device), u.to(cuda_device))]
+    g[:, 5], g[:, 133] = -100.0, -300.0
+    q, s = (cpu(t) for t in F.silu_mul_quant_blocks(g.to(cuda_device), u.to(cuda_device)))
+    keep = np.ones(256, bool)
+    keep[[5, 133]] = False
+    old = np.abs(O.silu_mul(cpu(g), cpu(u))).reshape(3, 2, 128).argmax(2)
+    assert not (old == 5).any()
+    np.testing.assert_array_equal(s, plain[1])
+    np.testing.assert_array_equal(q[:, keep], plain[0][:, keep])
+    assert (q[:, ~keep] == 0).all()
+    g[0, 6], g[1, 140] = float("-inf"), float("nan")
+    q, s = (cpu(t) for t in F.silu_mul_quant_blocks(g.to(cuda_device), u.to(cuda_device)))
+    vals = q * O.spread(s, 1, q.shape)
+    bad = np.zeros((3, 256), bool)
+    bad[0, :128] = bad[1, 128:] = True
+    assert np.isnan(vals[bad]).all() and np.isfinite(vals[~bad]).all()

@@ -448,7 +448,11 @@ int npl_fp8_silu_mul_quant(const void* gate, int64_t ld_gate, const void* up, in
  *   out[m, n] = T(v + bias[n] + residual[m, n])
  * with fp32 sums (the inner one on the tensor cores, the outer one in
  * registers, block after block) and one rounding to T = out_dtype, NPL_F16 or
- * NPL_BF16, which is residual's type too. qa e4m3 [M, K], qw e4m3 [N, K]: rows
+ * NPL_BF16, which is residual's type too. sa * sw is formed first, in fp32: where it
+ * falls below 2^-126 it keeps fewer bits, which moves an output by up to
+ * 2^-125 a block, and where it passes fp32's largest number the outputs of that
+ * token and those 128 weight rows are infinite or NaN, whatever the sum is.
+ * qa e4m3 [M, K], qw e4m3 [N, K]: rows
  * on 16-byte boundaries (lda, ldw multiples of 16); K itself is arbitrary.
  * sa fp32 [M, ceil(K / 128)], sw fp32 [ceil(N / 128), ceil(K / 128)]; bias
  * fp32 [N]. out may be residual itself (same row stride). Equal calls give

@@ -256,7 +256,10 @@ def linear_blocks(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w
     with scales [ceil(N / 128), ceil(K / 128)] -> [M, N] (+ bias fp32 [N])
     (+ residual [M, N]), rounded once to ``out_dtype``: fp16 or bf16, by default
     the type of ``out`` or ``residual``, else bf16. ``out`` may be ``residual``
-    itself."""
+    itself. The product of two scales is formed first, in fp32: below 2^-126 it
+    loses bits (2^-125 of an output for each such block), above fp32's largest
+    number it makes the outputs of that token and those weight rows infinite or
+    NaN."""
     _same_device(q, scale, qweight, wscale, bias, residual, out)
     m, k, lda = _code_rows("q", q)
     n, kw, ldw = _code_rows("qweight", qweight)

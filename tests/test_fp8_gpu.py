@@ -569,3 +569,48 @@ def test_silu_far_gates_beside_others(F, cuda_device):
     bad = np.zeros((3, 256), bool)
     bad[0, :128] = bad[1, 128:] = True
     assert np.isnan(vals[bad]).all() and np.isfinite(vals[~bad]).all()
+
+
+# ------------------------------------------------- products of far apart scales
+@pytest.mark.parametrize("m", [5, 40, 100, 300])
+def test_linear_products_of_tiny_scales(F, cuda_device, m):
+    """Scales whose product is subnormal: it is off by 2^-150 at most, and a
+    block's sum here at most 128 * 4 * 4 = 2^11 (128 * 448^2 < 2^25 in general),
+    which is 2^-139 a block, beside the linear's own bound and half a step of bf16 (2^-134
+    below its smallest normal number)."""
+    n, k = 300, 640
+    kb, nb = -(-k // 128), -(-n // 128)
+    gen = torch.Generator().manual_seed(m)
+    qa, qw = codes(m, k, 1, cuda_device), codes(n, k, 2, cuda_device)
+    sa = (2.0 ** -70 * (1 + torch.rand(m, kb, generator=gen))).to(cuda_device)
+    sw = (2.0 ** -66 * (1 + torch.rand(nb, kb, generator=gen))).to(cuda_device)
+    sa[1], sw[1] = 2.0 ** -126, 2.0 ** -126  # blocks of zeros would have these; their product is 0
+    out = cpu(F.linear_blocks(qa, sa, qw, sw, out_dtype=BF16))
+    want, mag = O.linear(cpu(qa), cpu(sa), cpu(qw), cpu(sw))
+    tol = (128 + kb + 12) * 2.0 ** -23 * mag + kb * 2.0 ** -139
+    half = np.maximum(torch.finfo(BF16).eps / 2 * (np.abs(want) + tol), 2.0 ** -134)
+    assert np.abs(want).max() > 2.0 ** -130 and (np.abs(out - want) <= tol + half).all()
+
+
+@pytest.mark.parametrize("m", [5, 40, 100, 300])
+def test_linear_products_of_huge_scales(F, cuda_device, m):
+    """Scales whose product overflows make their token infinite or NaN in those
+    128 columns, and nothing else."""
+    n, k = 300, 640
+    qa, qw = codes(m, k, 1, cuda_device), codes(n, k, 2, cuda_device)
+    sa, sw = powers(m, 5, 3, cuda_device), powers(3, 5, 4, cuda_device)
+    plain = F.linear_blocks(qa, sa, qw, sw)
+    sa2, sw2 = sa.clone(), sw.clone()
+    sa2[2, 1], sw2[1, 1] = 2.0 ** 70, 2.0 ** 70
+    with_far = F.linear_blocks(qa, sa2, qw, sw2)
+    assert not with_far[2, 128:256].isfinite().any()
+    # the other tokens and columns by the oracle, whose terms stay finite
+    want, mag = O.linear(cpu(qa), cpu(sa2), cpu(qw), cpu(sw2))
+    tol = (128 + 5 + 12) * 2.0 ** -23 * mag
+    ok = np.ones((m, n), bool)
+    ok[2, 128:256] = False
+    got = cpu(with_far)
+    assert (np.abs(got - want) <= tol + torch.finfo(BF16).eps / 2 * (np.abs(want) + tol))[ok].all()
+    rest = torch.ones(m, n, dtype=torch.bool)
+    rest[2], rest[:, 128:256] = False, False
+    assert torch.equal(with_far.cpu()[rest], plain.cpu()[rest])

@@ -60,9 +60,11 @@ def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
 
 
 # Raw queries and bound names below: a call on a few rows is bound by the host
-# (torch.cuda.current_stream alone takes as long as the kernel).
-_current_device = getattr(torch._C, "_cuda_getDevice", None)
-_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# (torch.cuda.current_stream alone takes as long as the kernel). A torch build
+# without the raw ones has the public ones.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 _empty = torch.empty_strided
 
 

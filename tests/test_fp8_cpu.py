@@ -219,6 +219,25 @@ def test_block_linear_lays_out_checkpoint_rows():
     assert (lin.in_features, lin.out_features) == (77, 10)
 
 
+
+def test_torch_without_the_raw_queries(monkeypatch):
+    """A torch build that lacks the private queries falls back to the public
+    ones, also while the module is loaded."""
+    import importlib.util
+    import types
+    from nanopointllm_b200 import fp8
+    for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+        monkeypatch.delattr(torch._C, name, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda i: types.SimpleNamespace(cuda_stream=100 + i))
+    spec = importlib.util.spec_from_file_location("nanopointllm_b200.fp8_without_raw", fp8.__file__)
+    again = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(again)
+    seen = []
+    again._call(lambda *args: seen.append(args) or 0, torch.device("cuda", 3), 7)
+    assert seen == [(7, 103)]
+
+
 _EPILOGUE = r"""
 // Threads as lanes or warps on the loops of fp8_epilogue.cuh; a meeting that one of them
 // misses is seen after a second and ends the program.

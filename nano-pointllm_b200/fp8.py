@@ -220,13 +220,15 @@ def _overlap(out: torch.Tensor, *others: torch.Tensor | None, itself: bool = Fal
         return (a.dim() == b.dim() == 2 and a.stride() == b.stride() and a.stride(1) == 1 and size == b.element_size()
                 and off == 0 and ld > 0 and at % ld >= a.shape[1] and at % ld + b.shape[1] <= ld)
 
+    def same(a, b):  # the stride of a single row or column does not count
+        return a.shape == b.shape and all(n == 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
+
     a0, a1 = span(out)
     for t in others:
         if t is None or (itself and t is out):
             continue
         b0, b1 = span(t)
-        if a0 < b1 and b0 < a1 and not columns(out, t) and not (
-                itself and a0 == b0 and t.shape == out.shape and t.stride() == out.stride()):
+        if a0 < b1 and b0 < a1 and not columns(out, t) and not (itself and a0 == b0 and same(t, out)):
             return True
     return False
 

@@ -238,6 +238,31 @@ def test_torch_without_the_raw_queries(monkeypatch):
     assert seen == [(7, 103)]
 
 
+
+def test_a_single_row_by_another_stride_is_the_input_itself(F):
+    """One row of a wide buffer, seen with the buffer's row stride or its own."""
+    f, calls = F
+    h = torch.float16
+    wide, w, other = torch.zeros(3, 512, dtype=h), torch.ones(256, dtype=h), torch.zeros(1, 256, dtype=h)
+    x, same = wide[:1, :256], wide[0, :256].unsqueeze(0)
+    assert x.stride() != same.stride()
+    assert f.rmsnorm_quant_blocks(x, w, 1e-6, other, sum_out=same)[2] is same
+    assert f.rmsnorm_quant_blocks(other, w, 1e-6, same, sum_out=x)[2] is x
+    qa, qw = torch.zeros(1, 256).to(E4M3), torch.zeros(256, 256).to(E4M3)
+    assert f.linear_blocks(qa, torch.ones(1, 2), qw, torch.ones(2, 2), residual=x, out=same) is same
+    column = torch.zeros(4, 8, dtype=h)[:, :1]
+    f.linear_blocks(torch.zeros(4, 256).to(E4M3), torch.ones(4, 2), torch.zeros(1, 256).to(E4M3), torch.ones(1, 2),
+                    residual=column.as_strided((4, 1), (8, 5)), out=column)
+    assert len(calls) == 4
+    with pytest.raises(ValueError):  # one element on, and two rows that only start alike
+        f.rmsnorm_quant_blocks(x, w, 1e-6, other, sum_out=wide[0, 1:257].unsqueeze(0))
+    flat = torch.zeros(1024, dtype=h)
+    with pytest.raises(ValueError):
+        f.rmsnorm_quant_blocks(flat[:512].view(2, 256), w, 1e-6, torch.zeros(2, 256, dtype=h),
+                               sum_out=flat.as_strided((2, 256), (512, 1)))
+    assert len(calls) == 4
+
+
 _EPILOGUE = r"""
 // Threads as lanes or warps on the loops of fp8_epilogue.cuh; a meeting that one of them
 // misses is seen after a second and ends the program.

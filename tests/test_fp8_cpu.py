@@ -263,6 +263,39 @@ def test_a_single_row_by_another_stride_is_the_input_itself(F):
     assert len(calls) == 4
 
 
+
+def linear_path(m, n, k, sms=148, clusters_of_4=33):
+    """Which tiles npl_fp8_linear takes on a B200: its host code's rules once
+    more (launch, launch_prefill and decode_split of csrc/fp8_linear.cu)."""
+    up = lambda a, b: -(-a // b)  # noqa: E731
+    kb, n_tiles, pairs, m_tiles = up(k, 128), up(n, 128), sms // 2, up(m, 256)
+
+    def split(tiles):
+        s = min(8, 7 * sms // (4 * tiles), kb // 2)
+        return 1 if s <= 2 else s
+
+    if m <= 64 or (m <= 128 and kb >= 20 and split(2 * n_tiles) >= 3):
+        tokens = 16 if m <= 16 else 32 if m <= 32 else 64
+        s = split(up(m, tokens) * n_tiles)
+        return "decode", tokens, s, up(kb, s), 1
+    wide, narrow = m_tiles * up(n, 256), m_tiles * up(n, 192)
+    if 2 * wide <= pairs and kb >= 24 and wide <= clusters_of_4:
+        return "prefill", 256, 2, up(kb, 2), 1
+    rows, tiles = (192, narrow) if up(narrow, pairs) <= up(wide, pairs) else (256, wide)
+    return "prefill", rows, 1, kb, up(tiles, pairs)
+
+
+def test_cases_reach_the_paths_that_they_name():
+    from test_fp8_gpu import LINEAR_PATHS
+    for shape, path in LINEAR_PATHS.items():
+        assert linear_path(*shape) == path, (shape, linear_path(*shape))
+    # a 7B layer's own sizes go by paths that have a case above
+    named = {path[:3] for path in LINEAR_PATHS.values()}
+    for m, n, k in ((8, 12288, 4096), (8, 22016, 4096), (64, 32003, 4096), (560, 4096, 11008), (560, 12288, 4096),
+                    (16000, 22016, 4096), (16000, 4096, 11008)):
+        assert linear_path(m, n, k)[:3] in named, (m, n, k)
+
+
 _EPILOGUE = r"""
 // Threads as lanes or warps on the loops of fp8_epilogue.cuh; a meeting that one of them
 // misses is seen after a second and ends the program.

@@ -614,3 +614,88 @@ def test_linear_products_of_huge_scales(F, cuda_device, m):
     rest = torch.ones(m, n, dtype=torch.bool)
     rest[2], rest[:, 128:256] = False, False
     assert torch.equal(with_far.cpu()[rest], plain.cpu()[rest])
+
+
+# ------------------------------------ the paths that layers of real sizes take
+# (M, N, K) -> (kernel, tokens or weight rows of a tile, CTAs or pairs that share one, blocks of each
+# at most, tiles of a cluster at most); test_fp8_cpu.py holds these to the rules of the host code.
+LINEAR_PATHS = {
+    (8, 12288, 5000): ("decode", 16, 1, 40, 1),
+    (24, 12291, 5000): ("decode", 32, 1, 40, 1),
+    (50, 12288, 5000): ("decode", 64, 1, 40, 1),
+    (3, 11137, 8300): ("decode", 16, 1, 65, 1),
+    (8, 1000, 33000): ("decode", 16, 8, 33, 1),
+    (100, 1003, 33000): ("decode", 64, 8, 33, 1),
+    (800, 4096, 2300): ("prefill", 256, 1, 18, 1),
+    (300, 14400, 2300): ("prefill", 256, 1, 18, 2),
+    (150, 28501, 1300): ("prefill", 256, 1, 11, 2),
+    (2100, 2100, 2300): ("prefill", 192, 1, 18, 2),
+    (4200, 2101, 1300): ("prefill", 192, 1, 11, 3),
+    (200, 1000, 8000): ("prefill", 256, 2, 32, 1),
+}
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m,n,k", LINEAR_PATHS)
+def test_linear_long_sums(F, cuda_device, m, n, k, dtype):
+    """More blocks than a CTA holds scales or ring stages for, and several tiles
+    a cluster. Sums are exact: multiples of 2^-4 up to 16 K < 2^20."""
+    test_linear_exact_sums(F, cuda_device, m, n, k, dtype)
+
+
+def compare_with_bad_blocks(F, x, rows, call, dev, how):
+    """Codes and scales bit for bit, a NaN and an infinite block apart, which read back as NaN."""
+    q, s = (cpu(t) for t in call(laid_out(x, how, dev)))
+    with np.errstate(all="ignore"):
+        oq, os = O.quant_fp32(cpu(x), rows)
+        vals = q * O.spread(s, rows, q.shape)
+    bad_scale = ~np.isfinite(os)
+    assert bad_scale.sum() == 2
+    bad = O.spread(bad_scale.astype(np.float64), rows, q.shape) > 0
+    assert np.isnan(vals[bad]).all()
+    np.testing.assert_array_equal(s[~bad_scale], os[~bad_scale])
+    np.testing.assert_array_equal(q[~bad], oq[~bad])
+
+
+@pytest.mark.parametrize("how", ["contiguous", "unaligned"])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("n,k", [(4000, 2100), (8200, 1100), (20000, 1099)])
+def test_weight_of_many_blocks(F, cuda_device, n, k, dtype, how):
+    """More blocks than CTAs: each takes several, one after the other."""
+    w = rand((n, k), dtype, n + k, 0.02)
+    w[700, 300], w[n - 1, k - 1] = float("nan"), float("inf")
+    compare_with_bad_blocks(F, w, 128, F.quantize_weight_blocks, cuda_device, how)
+
+
+@pytest.mark.parametrize("how", ["contiguous", "strided", "unaligned"])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("m,k", [(3000, 1000), (1200, 2111), (2400, 1024), (4000, 513)])
+def test_tokens_two_blocks_a_thread(F, cuda_device, m, k, dtype, how):
+    """More than 128 blocks an SM: a thread takes two blocks of a row, four apart."""
+    assert m * -(-k // 128) > 128 * 148
+    x = rand((m, k), dtype, m + k)
+    x[1] = 0
+    x[7, 130], x[m - 1, k - 1] = float("nan"), float("-inf")
+    compare_with_bad_blocks(F, x, 1, F.quantize_token_blocks, cuda_device, how)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("m,k", [(3, 40001), (2, 200000)])
+def test_rmsnorm_of_long_rows(F, cuda_device, m, k, residual, dtype):
+    """Rows that are read twice. A thread adds 16 squares in each of ceil(K /
+    8192) steps and the sums are joined in 10 more: so many roundings of 2^-24,
+    halved by the square root, and five more."""
+    x, r = rand((m, k), dtype, m + k), rand((m, k), dtype, m + k + 1)
+    w = (1 + 0.1 * rand((1, k), F32, k)[0]).to(dtype)
+    q, s, total = F.rmsnorm_quant_blocks(x.to(cuda_device), w.to(cuda_device), 1e-6,
+                                         r.to(cuda_device) if residual else None)
+    t = (x.float() + r.float()).to(dtype) if residual else x
+    if residual:
+        assert torch.equal(total.cpu(), t)
+    off = ((16 * -(-k // 8192) + 10) / 2 + 5) * 2.0 ** -24
+    v = O.rmsnorm(cpu(t), cpu(w), 1e-6)
+    es = O.block_scales(v, 1)
+    np.testing.assert_allclose(cpu(s), es, rtol=off + 2.0 ** -23, atol=0)
+    want = v / O.spread(es, 1, v.shape)
+    assert (np.abs(cpu(q) - want) <= O.half_step_e4m3(want) + 2 * off * np.abs(want)).all()

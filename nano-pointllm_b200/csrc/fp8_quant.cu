@@ -256,8 +256,9 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, uint4 q, int n) {
 }
 
 // Where the quantised values come from: what a thread loads for its columns,
-// what it keeps of them, what is worked out anew of it (from the same columns,
-// loaded again, for a warp that holds rare values), their key and the fp32 values.
+// what it keeps of them, their key and the fp32 values. rework() works them out
+// anew from the same columns, loaded again, for a warp that holds rare values;
+// whether it did so is the same in all lanes.
 template <typename T, int kAccess>
 struct RowSource {  // the row itself
   using Elem = T;
@@ -270,7 +271,7 @@ struct RowSource {  // the row itself
     return load16<kAccess>(x + row * ldx + col, n, x, end);
   }
   __device__ __forceinline__ static Kept keep(const Loaded& r) { return r; }
-  __device__ __forceinline__ void rework(int, int, int, Kept&) const {}
+  __device__ __forceinline__ bool rework(int, int, int, Kept&) const { return false; }
   __device__ __forceinline__ static uint32_t key(const Kept& k) { return key_of(k); }
   __device__ __forceinline__ static void values(const Kept& k, float (&v)[kCols]) { widen(k, v); }
 };
@@ -281,7 +282,7 @@ struct RowSource {  // the row itself
 // 1 in fp32, it is (g p) (p up) with p = e^(g / 2). Below -174 p is subnormal, off
 // by 2^-150 at most, and the product by 2^-149 |g| p up: at scales of 2^-126 or
 // more under 2^-13 in units of a code, whose smallest is 2^-9. A warp that holds
-// one loads its columns again for it: 16000 x 11008 takes 206 us (bf16 209), 199
+// one loads its columns again for it: 16000 x 11008 takes 205 us (bf16 210), 201
 // without the question, 229 (239) with this formula for all gates, which needs
 // no question, and 217 (232) with the columns kept until it is answered.
 constexpr float kFarGate = -86.0f;
@@ -296,8 +297,8 @@ struct SiluSource {
     float v[kCols];
     bool far;
   };
-  // Patterns above kFarGate's: numbers below it, and NaNs with a sign.
-  static constexpr uint32_t kFarBits = std::is_same_v<T, __half> ? 0xd560u : 0xc2acu;
+  // Two of kFarGate. Patterns above it are those of numbers below it, and of NaNs with a sign.
+  static constexpr uint32_t kFarBits = std::is_same_v<T, __half> ? 0xd560d560u : 0xc2acc2acu;
   const T* gate;
   const T* up;
   long long ld_gate, ld_up;
@@ -312,8 +313,7 @@ struct SiluSource {
     uint32_t top = __vimax3_u16x2(w[0], w[1], w[2]);
     top = __vimax3_u16x2(top, w[3], w[4]);
     top = __vimax3_u16x2(top, w[5], w[6]);
-    top = __vmaxu2(top, w[7]);
-    k.far = max(top & 0xffffu, top >> 16) > kFarBits;
+    k.far = __vimax3_u16x2(top, w[7], kFarBits) != kFarBits;
     float up[kCols];
     widen(r.g, k.v);
     widen(r.u, up);
@@ -325,8 +325,8 @@ struct SiluSource {
     }
     return k;
   }
-  __device__ __forceinline__ void rework(int row, int col, int n, Kept& k) const {
-    if (!__any_sync(0xffffffffu, k.far)) return;
+  __device__ __forceinline__ bool rework(int row, int col, int n, Kept& k) const {
+    if (!__any_sync(0xffffffffu, k.far)) return false;
     const Loaded r = load(row, col, n);
 #pragma unroll
     for (int i = 0; i < kCols; ++i) {
@@ -336,6 +336,7 @@ struct SiluSource {
         k.v[i] = __fmul_rn(__fmul_rn(g, p), __fmul_rn(p, (float)r.u.e[i]));
       }
     }
+    return true;
   }
   __device__ __forceinline__ static uint32_t key(const Kept& k) { return key_of(k.v); }
   __device__ __forceinline__ static void values(const Kept& k, float (&v)[kCols]) {
@@ -357,7 +358,7 @@ constexpr int kNormThreads = 512;
 // A warp takes 4 U consecutive blocks of a row, each of its four 8-lane groups
 // every fourth, all loads before the first store, which the compiler would not
 // move them across. Bound by instructions and memory alike: 16000 x 4096 fp16
-// takes 37.8 us (5.3 TB/s), SiLU * up of 16000 x 11008 206 us (4.3 TB/s). With 8
+// takes 37.8 us (5.3 TB/s), SiLU * up of 16000 x 11008 205 us (4.3 TB/s). With 8
 // columns a thread, which doubles the work per block, they took 48 and 281
 // (when SiLU took 197); warps that stay and load their next span first, 53 and 281.
 template <typename Source, int U, bool kVecQ>
@@ -381,10 +382,13 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(typename Source::Loaded)
   uint32_t key[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int col = col0 + u * (4 * kBlock);
     kept[u] = Source::keep(raw[u]);
-    src.rework(row, col < cols ? col : 0, cols - col, kept[u]);
     key[u] = Source::key(kept[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int col = col0 + u * (4 * kBlock);
+    if (src.rework(row, col < cols ? col : 0, cols - col, kept[u])) key[u] = Source::key(kept[u]);
   }
   const float s = block_scale(key_value<typename Source::Elem>(block_key<U>(key, lane)));
   const float inv = __frcp_rn(s);

@@ -429,7 +429,8 @@ int npl_fp8_quant_weight(const void* w, int w_dtype, int64_t rows, int64_t cols,
  *   v = s * (1 / sqrt(mean(s^2) + eps)) * weight     (fp32, not rounded to T)
  *   q, scale = npl_fp8_quant_rows of v
  * residual and sum_out are given together or not at all; sum_out may be x or
- * residual itself (same row stride). The mean is an fp32 sum.
+ * residual itself (same row stride). The mean is an fp32 sum: a row whose sum of
+ * squares reaches 2^128 reads back as zeros.
  */
 int npl_fp8_rmsnorm_quant(const void* x, int64_t ldx, const void* residual_or_null, int64_t ld_res, const void* weight,
                           int dtype, float eps, int64_t rows, int64_t cols, void* sum_out_or_null, int64_t ld_sum,

@@ -30,7 +30,8 @@
 //
 // All mbarrier waits are bounded (~1 s); on expiry the kernel records a code
 // in the device status word, drains its in-flight copies and MMAs, meets its
-// cluster, frees TMEM and returns.
+// cluster, frees TMEM and returns. Warps that meet at named barriers do so
+// whether or not their waits ran out (fp8_epilogue.cuh).
 #include <cuda_bf16.h>
 #include <cudaTypedefs.h>
 
@@ -406,7 +407,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 //
 // Tokens are the MMA's A rows and weights its N columns here: a thread of the
 // epilogue holds one token, so a block's scale is one value per thread and 128
-// columns (one weight scale), and the update is one packed FMA for two sums.
+// columns (one weight scale; two where they straddle blocks of a 192-row tile),
+// and the update is one FMA a sum.
 //
 // Two CTAs of a cluster share a tile of 256 tokens x 256 weight rows
 // (cta_group::2): each loads 128 rows of both, CTA 0 issues the MMAs for both,
@@ -718,7 +720,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPRegsMany));
-    const int group = (warp - 4) >> 2;  // columns [128 group, 128 group + 128) of the tile
+    const int group = (warp - 4) >> 2;  // columns [kPGroupCols group, kPGroupCols (group + 1)) of the tile
     const int row = (warp & 3) * 32 + lane;
     const bool elected = (threadIdx.x & 127) == 0;
     unsigned char* stg = staging + group * kPOut;
@@ -930,10 +932,11 @@ constexpr int kDecodeSmem = 110 * 1024;
 constexpr int kThirdOfSm = 76 * 1024;
 
 // CTAs that share a decode tile: as many as keep 1.75 CTAs an SM (beyond it not
-// all clusters run at once: 96 tiles of 32 blocks take 12.0 us unsplit, 13.9
-// two-way, 17.9 three-way; 76 tiles 12.4, 13.0, 10.8, 15.3 four-way) and two
-// blocks a CTA. Two CTAs cost more to join than they save at any size tried (8 x
-// 5120..16384 x 4096).
+// all clusters run at once: 96 tiles of 32 blocks take 12.6 us unsplit, 13.6
+// two-way, 17.9 three-way; 76 tiles 12.6, 13.0, 10.7, 14.3 four-way) and two
+// blocks a CTA. Where that gives two, from 87 to 129 tiles, joining costs more
+// than two CTAs save (96 tiles above; 128 tiles 13.4 us unsplit, 15.0 two-way), so
+// such tiles stay whole, and 96 of them leave 52 SMs without one.
 int decode_split(long long tiles, int k_blocks) {
   const long long s = std::min({(long long)kMaxSplit, 7ll * num_sms() / (4 * tiles), (long long)k_blocks / 2});
   return s <= 2 ? 1 : (int)s;

@@ -450,7 +450,10 @@ __global__ void __launch_bounds__(kMaxThreads ? kMaxThreads : kNormThreads, kMax
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
   __syncthreads();
   ss = warp_sum((threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0.f);
-  const float r = rsqrtf(__fadd_rn(__fdividef(ss, (float)cols), eps));  // both within 2 ulps
+  // Both within 2 ulps of the IEEE steps, which every thread of the row would
+  // pay; the tests count them. cols < 2^31 is far below 2^126, from where on
+  // __fdividef gives 0. (A row whose squares overflow fp32 has r = 0.)
+  const float r = rsqrtf(__fadd_rn(__fdividef(ss, (float)cols), eps));
   for (int base = 0; base < cols; base += step) {
     const int col = base + col0;
     if (!kInRegs) {  // the stored sum, where there is one: it may have replaced x or the residual

@@ -685,7 +685,8 @@ def test_tokens_two_blocks_a_thread(F, cuda_device, m, k, dtype, how):
 def test_rmsnorm_of_long_rows(F, cuda_device, m, k, residual, dtype):
     """Rows that are read twice. A thread adds 16 squares in each of ceil(K /
     8192) steps and the sums are joined in 10 more: so many roundings of 2^-24,
-    halved by the square root, and five more."""
+    halved by the square root. The quotient and rsqrtf are within 2 ulps, 4
+    roundings each, the former halved too; with eps and two products 8.5 more."""
     x, r = rand((m, k), dtype, m + k), rand((m, k), dtype, m + k + 1)
     w = (1 + 0.1 * rand((1, k), F32, k)[0]).to(dtype)
     q, s, total = F.rmsnorm_quant_blocks(x.to(cuda_device), w.to(cuda_device), 1e-6,
@@ -693,9 +694,22 @@ def test_rmsnorm_of_long_rows(F, cuda_device, m, k, residual, dtype):
     t = (x.float() + r.float()).to(dtype) if residual else x
     if residual:
         assert torch.equal(total.cpu(), t)
-    off = ((16 * -(-k // 8192) + 10) / 2 + 5) * 2.0 ** -24
+    off = ((16 * -(-k // 8192) + 10) / 2 + 8.5) * 2.0 ** -24
     v = O.rmsnorm(cpu(t), cpu(w), 1e-6)
     es = O.block_scales(v, 1)
     np.testing.assert_allclose(cpu(s), es, rtol=off + 2.0 ** -23, atol=0)
     want = v / O.spread(es, 1, v.shape)
     assert (np.abs(cpu(q) - want) <= O.half_step_e4m3(want) + 2 * off * np.abs(want)).all()
+
+
+def test_rmsnorm_of_squares_that_overflow(F, cuda_device):
+    """Rows whose sum of squares is past fp32 read back as zeros, rows just
+    below it as their norm."""
+    x = rand((4, 512), BF16, 1)
+    x[1] = (x[1].float() * 2.0 ** 70).to(BF16)
+    x[2] = (x[2].float().clamp(-4, 4) * 2.0 ** 50).to(BF16)
+    w = torch.ones(512, dtype=BF16)
+    q, s, _ = F.rmsnorm_quant_blocks(x.to(cuda_device), w.to(cuda_device), 1e-6)
+    assert (cpu(q)[1] == 0).all() and (cpu(s)[1] == 2.0 ** -126).all()
+    keep = [0, 2, 3]
+    check_codes(q[keep], s[keep], O.rmsnorm(cpu(x)[keep], cpu(w), 1e-6))

@@ -39,7 +39,7 @@ extern "C" {
 /* element types */
 #define NPL_F32 0
 #define NPL_F16 1
-#define NPL_BF16 2 /* the npl_fp8_* entries only */
+#define NPL_BF16 2 /* the npl_fp8_*, tree / window attention and log probability entries */
 
 /* fused epilogues of npl_w8a8_linear / npl_w8a8_linear_ex */
 #define NPL_EPI_NONE 0     /* out = dequant(acc)                                  */
@@ -463,6 +463,65 @@ int npl_fp8_linear(const uint8_t* qa, int64_t lda, const float* sa, int64_t ld_s
                    const float* sw, int64_t ld_sw, const float* bias_or_null, int64_t M, int64_t N, int64_t K,
                    const void* residual_or_null, int64_t ld_res, void* out, int64_t ld_out, int out_dtype,
                    void* stream);
+
+/*
+ * Attention of a tree of drafted tokens over the paged pool (no counterpart in
+ * the reference). q [total_q, H, D] (token stride ld_q elements, heads
+ * contiguous), caches [num_blocks, block_size, Hkv, D] and out are all of one
+ * type, NPL_F16 or NPL_BF16. Sequence b owns rows [q_offsets[b], q_offsets[b] +
+ * q_lens[b]) of q, its drafts, whose keys and values are the last q_lens[b] of
+ * the first context_lens[b] slots of its block table. Draft i sees every key
+ * before the drafts, and draft j where tree_mask[row of i, j] is not 0
+ * (tree_mask uint8 [total_q, mask_cols], row stride ld_mask); a row that sees
+ * nothing gives zeros. Scores are fp32 dot products times `scale`, the softmax
+ * runs in fp32, probabilities are rounded to the type of the caches for the
+ * P.V product (fp32 accumulation), and out is rounded once. What a masked slot
+ * holds, infinities and NaN included, never reaches a row that does not see it.
+ * Rows of no sequence are not written; context_lens[b] == 0 gives zeros.
+ * max_q_len >= every q_lens[b] sizes the launch. D is 64 or 128, block_size a
+ * multiple of 8, H / Hkv at most 128. Bad table entries (read as zeros),
+ * offsets and lengths (skipped) set NPL_DEV code 5 (npl_device_status). No
+ * workspace; graph-capturable.
+ */
+int npl_paged_tree_attention(const void* q, int dtype, int64_t ld_q, int total_q, int H, int Hkv, int D,
+                             const void* k_cache, const void* v_cache, int num_blocks, int block_size,
+                             const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                             const int32_t* context_lens, const int32_t* q_lens, const int32_t* q_offsets, int B,
+                             int max_q_len, const uint8_t* tree_mask, int64_t ld_mask, int mask_cols, float scale,
+                             void* out, int64_t ld_out, void* stream);
+
+/*
+ * Causal attention with a sliding window and sinks over the paged pool (no
+ * counterpart in the reference): as npl_paged_tree_attention, with query j of
+ * sequence b at position p = context_lens[b] - q_lens[b] + j, which sees key i
+ * where i <= p and (i > p - window or i < sinks). window >= 1, sinks >= 0.
+ * Table entries of pages that no query sees are not read: they may have been
+ * freed. q_lens and q_offsets null: row b of q is the one new token of
+ * sequence b (total_q == B; max_q_len is not read).
+ */
+int npl_paged_window_attention(const void* q, int dtype, int64_t ld_q, int total_q, int H, int Hkv, int D,
+                               const void* k_cache, const void* v_cache, int num_blocks, int block_size,
+                               const int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                               const int32_t* context_lens, const int32_t* q_lens_or_null,
+                               const int32_t* q_offsets_or_null, int B, int max_q_len, int window, int sinks,
+                               float scale, void* out, int64_t ld_out, void* stream);
+
+/*
+ * Log probabilities of given tokens from rows of logits [rows, vocab] (NPL_F32,
+ * NPL_F16 or NPL_BF16; row stride ld, any alignment of the elements' size). In
+ * fp32, with p = softmax of a row:
+ *   logprobs[r] = ln p[token_ids[r]],  entropy[r] = -sum p ln p (0 for p = 0)
+ *   top_ids, top_logprobs [rows, top_k]: the largest logits, of equal ones the
+ *   first, and their log probabilities
+ * token_ids[r] = -1 (a padding row) gives 0 for logprobs[r]; any other id
+ * outside the row gives NaN and sets NPL_DEV code 5. Logits of minus infinity
+ * have probability 0; a row of nothing else, or with a NaN or plus infinity,
+ * gives NaN. NaN logits come first among the top ones. top_k is 0 to 32 and at
+ * most vocab. No workspace; graph-capturable.
+ */
+int npl_token_logprobs(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab,
+                       const int64_t* token_ids, int top_k, float* logprobs, float* entropy, int64_t* top_ids,
+                       float* top_logprobs, void* stream);
 
 #ifdef __cplusplus
 }

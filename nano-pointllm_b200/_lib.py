@@ -99,6 +99,11 @@ SIGNATURES = {
     "npl_fp8_rmsnorm_quant": (_I, [_P, _Q, _P, _Q, _P, _I, _F, _Q, _Q, _P, _Q, _P, _Q, _P, _Q, _P]),
     "npl_fp8_silu_mul_quant": (_I, [_P, _Q, _P, _Q, _I, _Q, _Q, _P, _Q, _P, _Q, _P]),
     "npl_fp8_linear": (_I, [_P, _Q, _P, _Q, _P, _Q, _P, _Q, _P, _Q, _Q, _Q, _P, _Q, _P, _Q, _I, _P]),
+    "npl_paged_tree_attention": (_I, [_P, _I, _Q, _I, _I, _I, _I, _P, _P, _I, _I, _P, _Q, _I, _P, _P, _P, _I, _I, _P,
+                                      _Q, _I, _F, _P, _Q, _P]),
+    "npl_paged_window_attention": (_I, [_P, _I, _Q, _I, _I, _I, _I, _P, _P, _I, _I, _P, _Q, _I, _P, _P, _P, _I, _I,
+                                        _I, _I, _F, _P, _Q, _P]),
+    "npl_token_logprobs": (_I, [_P, _I, _Q, _Q, _Q, _P, _I, _P, _P, _P, _P, _P]),
     "npl_paged_prefill_attention": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _I, _I, _F,
                                          _P, _I, _P]),
 }

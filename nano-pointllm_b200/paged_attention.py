@@ -7,6 +7,15 @@
 * ``rope_store_kvcache``     - paged_attention.py:1284-1294 (rotary_fn on q/k of
                                the packed QKV projection, then store_kvcache)
 
+Beside them, without a counterpart in the reference, on fp16 or bf16 tensors:
+
+* ``paged_tree_attention``   - every draft of a tree of drafted tokens sees the
+                               cache and the drafts that it follows
+* ``tree_mask_from_parents`` - that tree's mask from each draft's parent
+* ``paged_window_attention`` - causal attention with a sliding window and a few
+                               first tokens that stay visible (sinks), for
+                               prompts and single tokens
+
 KV pool layout per layer (kv_pool.py:9-24): fp16 [num_blocks, block_size,
 Hkv, D]; ``slot_mapping`` int32 (-1 = padding, skipped); ``block_tables`` int32
 [B, max_blocks]; ``context_lens`` int32 [B]. CUDA tensors only.
@@ -16,6 +25,16 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
+from .fp8 import _call, _overlap
+
+
+def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    d = first.get_device()
+    if d < 0:
+        raise ValueError("the paged path runs on CUDA tensors only")
+    for t in others:
+        if t is not None and t.get_device() != d:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
 
 
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
@@ -142,3 +161,156 @@ def paged_varlen_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         out.stride(0), L.stream_ptr(q.device)))
     return out
 
+
+
+_DT16 = {torch.float16: L.NPL_F16, torch.bfloat16: L.NPL_BF16}
+_tree_attention, _window_attention = L.lib.npl_paged_tree_attention, L.lib.npl_paged_window_attention
+
+
+def _masked_arguments(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                      context_lens: torch.Tensor, q_lens: torch.Tensor | None, q_offsets: torch.Tensor | None,
+                      num_kv_groups: int, max_q_len: int | None, out: torch.Tensor | None,
+                      mask: torch.Tensor | None = None):
+    """Checks what tree and window attention share. Returns (q, block_tables,
+    context_lens, q_lens, q_offsets, max_q_len, out) as the C entries read them."""
+    _same_device(q, k_cache, v_cache, block_tables, context_lens, q_lens, q_offsets, mask, out)
+    dt = q.dtype
+    if dt not in _DT16:
+        raise ValueError("q must be float16 or bfloat16")
+    if k_cache.dtype is not dt or v_cache.dtype is not dt:
+        raise ValueError("KV caches must have the type of q")
+    if k_cache.shape != v_cache.shape or k_cache.dim() != 4:
+        raise ValueError("KV caches must be [num_blocks, block_size, Hkv, D]")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("KV caches must be contiguous")
+    if q.dim() != 3:
+        raise ValueError("q must be [total_q, H, D]")
+    total_q, h, d = q.shape
+    if k_cache.shape[3] != d or k_cache.shape[2] * num_kv_groups != h:
+        raise ValueError("q / KV cache head geometry mismatch")
+    if block_tables.dtype is not torch.int32 or block_tables.dim() != 2:
+        raise ValueError("block_tables must be int32 [B, max_blocks]")
+    b = block_tables.shape[0]
+    for name, t in (("context_lens", context_lens), ("q_lens", q_lens), ("q_offsets", q_offsets)):
+        if t is not None and (t.dtype is not torch.int32 or t.shape != (b,)):
+            raise ValueError(f"{name} must be int32 [B]")
+    if (q_lens is None) != (q_offsets is None):
+        raise ValueError("q_lens and q_offsets go together")
+    if q_lens is None and total_q != b:
+        raise ValueError("without q_lens every sequence has one token: q must be [B, H, D]")
+    if q.stride(2) != 1 or q.stride(1) != d or q.stride(0) % 8 or q.stride(0) < h * d or q.data_ptr() % 16:
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+    if block_tables.stride(1) != 1 or block_tables.stride(0) < block_tables.shape[1]:
+        block_tables = block_tables.contiguous()
+    context_lens = context_lens.contiguous()
+    if q_lens is None:
+        max_q_len = 1
+    else:
+        q_lens, q_offsets = q_lens.contiguous(), q_offsets.contiguous()
+        if max_q_len is None:
+            max_q_len = int(q_lens.max().item()) if b else 0
+    if out is None:
+        out = torch.empty((total_q, h, d), dtype=dt, device=q.device)
+    else:
+        if out.shape != (total_q, h, d) or out.dtype is not dt:
+            raise ValueError("out must have the shape and type of q")
+        if out.numel() and (out.stride(2) != 1 or out.stride(1) != d or out.stride(0) % 8 or out.stride(0) < h * d
+                            or out.data_ptr() % 16):
+            raise ValueError("out needs contiguous heads and tokens on 16-byte boundaries that do not overlap")
+        if _overlap(out, q, k_cache, v_cache):
+            raise ValueError("out may not overlap q or the caches")
+    return q, block_tables, context_lens, q_lens, q_offsets, int(max_q_len), out
+
+
+def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                         context_lens: torch.Tensor, q_lens: torch.Tensor, q_offsets: torch.Tensor, scale: float,
+                         num_kv_groups: int, tree_mask: torch.Tensor, *, max_q_len: int | None = None,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a tree of drafted tokens: q fp16 or bf16 [total_q, H, D] ->
+    [total_q, H, D]; the arguments of ``paged_varlen_attention`` and the mask.
+
+    The rows of sequence b, q[q_offsets[b] : q_offsets[b] + q_lens[b]], are its
+    drafts, and their keys and values the last q_lens[b] of the context_lens[b]
+    that its block table holds. Every draft sees all keys before the drafts,
+    and draft j of its sequence where ``tree_mask`` [total_q, >= max_q_len]
+    (bool or uint8) says so: itself and those that it follows
+    (``tree_mask_from_parents``). A draft that sees nothing gets zeros. What a
+    masked slot holds, infinities and NaN included, never reaches a row that
+    does not see it. Probabilities are rounded to the type of the caches.
+    ``max_q_len`` (>= every q_lens) avoids reading q_lens back to the host."""
+    if tree_mask.dtype not in (torch.bool, torch.uint8):
+        raise ValueError("tree_mask must be bool or uint8")
+    if q_lens is None or q_offsets is None:
+        raise ValueError("tree attention needs q_lens and q_offsets")
+    q, block_tables, context_lens, q_lens, q_offsets, most, out = _masked_arguments(
+        q, k_cache, v_cache, block_tables, context_lens, q_lens, q_offsets, num_kv_groups, max_q_len, out, tree_mask)
+    total_q, h, d = q.shape
+    if tree_mask.dim() != 2 or tree_mask.shape[0] != total_q or tree_mask.shape[1] < most:
+        raise ValueError("tree_mask must be [total_q, at least max_q_len]")
+    if tree_mask.stride(1) != 1 or tree_mask.stride(0) < tree_mask.shape[1]:
+        tree_mask = tree_mask.contiguous()
+    if total_q == 0 or most == 0 or block_tables.shape[0] == 0:
+        return out
+    nb, bs, hkv, _ = k_cache.shape
+    _call(_tree_attention, q.device, q.data_ptr(), _DT16[q.dtype], q.stride(0), total_q, h, hkv, d,
+          k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, block_tables.data_ptr(), block_tables.stride(0),
+          block_tables.shape[1], context_lens.data_ptr(), q_lens.data_ptr(), q_offsets.data_ptr(),
+          block_tables.shape[0], most, tree_mask.data_ptr(), tree_mask.stride(0), tree_mask.shape[1], float(scale),
+          out.data_ptr(), out.stride(0))
+    return out
+
+
+def tree_mask_from_parents(parents: torch.Tensor, q_offsets: torch.Tensor, max_q_len: int) -> torch.Tensor:
+    """bool [total_q, max_q_len] for ``paged_tree_attention``: each draft sees
+    itself and the drafts that it follows. ``parents`` [total_q] holds the
+    place of each draft's parent within its sequence (0 to max_q_len - 1), -1
+    where it follows the last token of the cache; parents come before their
+    children. Rows of no sequence come out as if they belonged to the one
+    before. Elementary torch operations, on any device: built once per tree."""
+    total = parents.shape[0]
+    if parents.dim() != 1 or parents.is_floating_point() or q_offsets.dim() != 1 or max_q_len < 1:
+        raise ValueError("parents must be whole numbers [total_q], q_offsets [B], max_q_len at least 1")
+    row = torch.arange(total, device=parents.device)
+    order = torch.sort(q_offsets.long()).values
+    first = order[(torch.searchsorted(order, row, right=True) - 1).clamp_min(0)]  # each draft's first row
+    place = (row - first).clamp_(0, max_q_len - 1)
+    mask = torch.zeros((total, max_q_len + 1), dtype=torch.bool, device=parents.device)
+    at = place
+    for _ in range(max_q_len):
+        # a finished path stays at -1, in the spare last column
+        mask[row, torch.where(at < 0, torch.full_like(at, max_q_len), at)] = True
+        at = torch.where(at < 0, at, parents.long()[(first + at).clamp(0, total - 1)])
+    return mask[:, :max_q_len]
+
+
+def paged_window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                           context_lens: torch.Tensor, q_lens: torch.Tensor | None, q_offsets: torch.Tensor | None,
+                           scale: float, num_kv_groups: int, window: int, sinks: int = 0, *,
+                           max_q_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention with a sliding window and sinks: q fp16 or bf16
+    [total_q, H, D] -> [total_q, H, D]; the arguments of
+    ``paged_varlen_attention``, and ``window`` >= 1 and ``sinks`` >= 0.
+
+    Query j of sequence b stands at position p = context_lens[b] - q_lens[b] + j
+    and sees key i where i <= p and (i > p - window or i < sinks). ``q_lens`` and
+    ``q_offsets`` None: q [B, H, D] holds the one new token of each sequence, as
+    in ``paged_decode_attention``. Table entries of pages that no query sees are
+    not read, so those pages may have been freed. What a masked slot holds,
+    infinities and NaN included, never reaches a row that does not see it.
+    Probabilities are rounded to the type of the caches. ``max_q_len`` (>= every
+    q_lens) avoids reading q_lens back to the host."""
+    if not 1 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31:
+        raise ValueError("window must be at least 1 and sinks at least 0, below 2^31")
+    q, block_tables, context_lens, q_lens, q_offsets, most, out = _masked_arguments(
+        q, k_cache, v_cache, block_tables, context_lens, q_lens, q_offsets, num_kv_groups, max_q_len, out)
+    total_q, h, d = q.shape
+    if total_q == 0 or most == 0 or block_tables.shape[0] == 0:
+        return out
+    nb, bs, hkv, _ = k_cache.shape
+    _call(_window_attention, q.device, q.data_ptr(), _DT16[q.dtype], q.stride(0), total_q, h, hkv, d,
+          k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, block_tables.data_ptr(), block_tables.stride(0),
+          block_tables.shape[1], context_lens.data_ptr(), L.ptr(q_lens), L.ptr(q_offsets), block_tables.shape[0],
+          most, int(window), int(sinks), float(scale), out.data_ptr(), out.stride(0))
+    return out

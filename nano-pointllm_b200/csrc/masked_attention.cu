@@ -1,15 +1,59 @@
 // Attention over the paged KV pool under masks other than the causal one: a
 // tree of drafted tokens, and a sliding window with sinks.
+//
+// npl_paged_tree_attention, npl_paged_window_attention (no counterpart in the
+// reference, whose kernels are causal).
+//
+// For a query row with the keys S that it sees:
+//   s_i = scale * q . k_i,  out = sum_{i in S} e^(s_i - m) v_i / sum_{i in S} e^(s_i - m)
+// in one pass over the keys. m is a running reference of the row, not its
+// maximum: it moves only when a tile's maximum is more than 2^8 above it (in
+// the exponentials), so that the sums in tensor memory are rarely rescaled.
+// p = 2^(s log2(e) + 6 - m): at most 2^14, and an fp16 p keeps 2^-30 of the
+// largest. p is rounded to the type of the caches because it is an operand of
+// the P.V product; the normaliser sums the unrounded p.
+//
+// On the tensor cores (tcgen05 kind::f16, fp32 sums in TMEM): the rows of a
+// tile are (token, query head of one kv head), so grouped heads share the keys
+// they read. A CTA works on two streams, each with its own 128 rows, its own
+// warpgroup (one thread a row) and its own TMEM, so that one stream's softmax
+// runs while the tensor core works for the other:
+//   shared (more rows than one tile): two neighbouring row tiles of one kv head
+//     read the same K and V tiles;
+//   not shared (decode, small trees): the same rows of two kv heads.
+// 384 threads: warps 0-3 and 4-7 softmax of the streams, warp 8 TMA, warp 9 MMA
+// (one thread). S_j = Q K_j^T goes to TMEM, a thread reads its row of 128
+// scores, writes p over them in TMEM, and O += P V_j reads it there. The order
+// S0, S1, then O0 S0 O1 S1 ... makes every S of a stream arrive after the O
+// before it, so no further barrier guards a rescale.
+//
+// Keys come in pieces of gcd(block_size, 32): the visible ones of a CTA's rows
+// only (the sinks' pieces, then the window's), four or more pieces to a tile.
+// A long axis with few rows is split over a cluster of CTAs, whose partial sums
+// are joined through distributed shared memory.
+//
+// What a masked slot holds must not reach a row that does not see it, and
+// 0 * infinity would: in tiles that some row sees in part, the V rows that no
+// row sees are zeroed, and V elements that are not finite are replaced by 0 and
+// added at the end to the rows that do see them.
 #include <algorithm>
-#include <cfloat>
 #include <initializer_list>
 
 #include <cuda_bf16.h>
+#include <cudaTypedefs.h>
 
 #include "npl_common.cuh"
 
 namespace npl {
 namespace {
+
+constexpr int kMaThreads = 384;
+constexpr int kMaTile = 128;
+constexpr uint32_t kMaTmemCols = 512;  // S of the streams at 0 and 128 (P over it), O at 256 and 384
+constexpr int kMaBad = 32;             // keys with V elements that are not finite, remembered for an item
+constexpr int kMaPiece = 32;           // keys of a piece at most
+constexpr float kMaShift = 6.f;        // p = 2^(x - m + 6)
+constexpr float kMaSlack = 8.f;        // m moves when a score is more than this above it
 
 struct MaArgs {
   const void* q;
@@ -27,76 +71,824 @@ struct MaArgs {
   int mask_cols;
   int window, sinks;
   int B, H, Hkv, G, num_blocks, block_size, max_blocks, total_q, max_q_len;
-  float scale;
+  int tokens;   // of a row tile: 128 / G
+  int piece;    // keys of a piece
+  int levels;   // items of a sequence and kv head (or pair of them)
+  int n_items;  // levels * B * (kv heads, or pairs of them)
+  int split;    // CTAs of a cluster, which share an item's keys
+  float c2;     // scale * log2(e)
   int* status;
 };
 
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_float(__half* p, float x) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void from_float(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+template <int D>
+struct MaSmem {
+  static constexpr uint32_t kHalf = kMaTile * 128;  // 128 rows x 64 elements (one swizzle span)
+  static constexpr uint32_t kTileBytes = kMaTile * D * 2;
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  alignas(1024) uint8_t q[2][kTileBytes];
+  alignas(1024) uint8_t kv[kStages][kTileBytes];  // K and V tiles in the order of their use; partial sums at the end
+  uint64_t full[kStages], empty[kStages];
+  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], mma_done;
+  uint32_t tmem_base;
+  int abort;
+  int n_bad[3][2];        // [item % 3][stream whose threads clean its V tiles]
+  int bad[3][2][kMaBad];  // keys whose V rows held elements that are not finite
+};
 
-// One warp for each (sequence, token, head): keys one after the other, the
-// head dimension over the lanes.
-template <typename T, int D, bool kTree>
-__global__ void __launch_bounds__(128) masked_attn_simple(const MaArgs p) {
-  const int b = blockIdx.y, h = blockIdx.z * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (h >= p.H) return;
-  const int n = p.q_lens ? p.q_lens[b] : 1, start = p.q_offsets ? p.q_offsets[b] : b, ctx = p.ctx_lens[b];
-  if (n <= 0) return;
-  if (start < 0 || start > p.total_q - n || n > p.max_q_len) {
-    atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
-    return;
+static_assert(sizeof(MaSmem<128>) + 1024 <= 232448 && sizeof(MaSmem<64>) + 1024 <= 232448, "shared memory of an SM");
+
+template <typename T>
+struct MaType;
+template <>
+struct MaType<__half> {
+  static constexpr uint32_t kIdesc = 0;  // a_format, b_format: F16
+  static constexpr uint32_t kExp = 0x7c007c00u, kOne = 0x04000400u;
+  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  __device__ static uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-  const int prefix = ctx - n, kvh = h / p.G;
-  for (int j = blockIdx.x; j < n; j += gridDim.x) {
-    constexpr int E = D / 32;
-    float q[E], acc[E], m = -INFINITY, l = 0.f;
-    const T* qp = static_cast<const T*>(p.q) + (start + j) * p.ld_q + (long long)h * D + lane * E;
-    for (int e = 0; e < E; ++e) q[e] = to_float(qp[e]) * p.scale, acc[e] = 0.f;
-    const int pos = prefix + j, end = kTree ? ctx : min(ctx, pos + 1);
-    if (prefix < 0 && ctx != 0) atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
-    for (int i = 0; i < (prefix < 0 ? 0 : end); ++i) {
-      if (kTree) {
-        const int c = i - prefix;
-        if (c >= 0 && (c >= p.mask_cols || !p.mask[(start + j) * p.ld_mask + c])) continue;
-      } else if (i <= pos - p.window && i >= p.sinks) {
-        i = pos - p.window;
-        continue;
-      }
-      const int page = i / p.block_size;
-      const int blk = page < p.max_blocks ? p.bt[b * p.bt_stride + page] : -1;
-      float s = 0.f, x[E];
-      const bool ok = blk >= 0 && blk < p.num_blocks;
-      const long long row = ok ? (((long long)blk * p.block_size + i % p.block_size) * p.Hkv + kvh) * D + lane * E : 0;
-      if (!ok) atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
-      for (int e = 0; e < E; ++e) s += ok ? q[e] * to_float(static_cast<const T*>(p.k)[row + e]) : 0.f;
-      for (int e = 0; e < E; ++e) x[e] = ok ? to_float(static_cast<const T*>(p.v)[row + e]) : 0.f;
-      s = warp_sum(s);
-      const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-      const float a = expf(m - base), w = expf(s - base);
-      m = mn;
-      l = l * a + w;
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * a + w * x[e];
+  __device__ static float get(const void* p, size_t i) { return __half2float(static_cast<const __half*>(p)[i]); }
+  __device__ static void add(__half* p, float x) { *p = __float2half_rn(__half2float(*p) + x); }
+};
+template <>
+struct MaType<__nv_bfloat16> {
+  static constexpr uint32_t kIdesc = (1u << 7) | (1u << 10);
+  static constexpr uint32_t kExp = 0x7f807f80u, kOne = 0x00800080u;
+  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  __device__ static uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static float get(const void* p, size_t i) {
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  }
+  __device__ static void add(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(__bfloat162float(*p) + x); }
+};
+
+// 2^x (ex2.approx.ftz: a result below 2^-126 is 0, which adds less than that to sums of 2^6 and more).
+__device__ __forceinline__ float ma_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Bounded wait that also gives up once another role of the CTA gave up.
+__device__ __forceinline__ bool ma_wait(uint64_t* bar, uint32_t parity, int* abort, int* status, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*reinterpret_cast<volatile int*>(abort)) return false;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      *reinterpret_cast<volatile int*>(abort) = 1;
+      if (status) atomicCAS(status, 0, code);
+      return false;
     }
-    T* op = static_cast<T*>(p.out) + (start + j) * p.ld_out + (long long)h * D + lane * E;
-    for (int e = 0; e < E; ++e) from_float(op + e, l == 0.f ? 0.f : acc[e] / l);
   }
 }
 
+// The same for a warp: its lanes go on, or give up, together.
+__device__ __forceinline__ bool ma_wait_warp(uint64_t* bar, uint32_t parity, int* abort, int* status, int code) {
+  return __all_sync(0xffffffffu, ma_wait(bar, parity, abort, status, code));
+}
+
+// D[tmem] (+)= A[tmem] * B[smem], 16-bit floats, fp32 sums (kind::f16); A packed two K elements a column.
+__device__ __forceinline__ void ma_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 lanes x 16 columns from registers (thread i of the warp: lane i).
+__device__ __forceinline__ void ma_tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// Loads from TMEM have arrived; the registers go through it, so that no use of them moves ahead of it.
+__device__ __forceinline__ void ma_tmem_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]));
+  asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ void ma_tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float4 ma_ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ma_ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// One item: 128 rows (or twice 128, shared) of one sequence and kv head (or
+// the same rows of two). Every role decodes the same items from the same
+// read-only metadata. The keys that some row of the item sees are numbered by
+// x = 0, 1, ...: key(x) = x below first * piece (the sinks' pieces), x + shift
+// from there on. This CTA takes x0 <= x < x1.
+struct MaItem {
+  int b, kvh, tok0, n, ctx, start, prefix;
+  int lo, hi;  // keys that some row of the item sees: lo <= key < hi, and the sinks
+  int sink_x, shift, x0, x1, nt;
+  bool skip, second;  // no such rows; the second stream has rows
+};
+
+template <bool kTree, bool kShared>
+__device__ __forceinline__ MaItem ma_item(const MaArgs& p, int i, int rank) {
+  MaItem it;
+  const int units = kShared ? p.Hkv : (p.Hkv + 1) / 2;
+  const int level = i % p.levels, rem = i / p.levels;
+  it.b = rem / units;
+  it.kvh = (rem - it.b * units) * (kShared ? 1 : 2);
+  it.tok0 = level * p.tokens * (kShared ? 2 : 1);
+  it.n = p.q_lens ? p.q_lens[it.b] : 1;
+  it.start = p.q_offsets ? p.q_offsets[it.b] : it.b;
+  it.ctx = p.ctx_lens[it.b];
+  it.prefix = it.ctx - it.n;
+  it.skip = it.tok0 >= it.n || it.n > p.max_q_len || it.start < 0 || it.start > p.total_q - it.n;
+  it.second = kShared ? it.tok0 + p.tokens < it.n : it.kvh + 1 < p.Hkv;
+  const int last = min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1));  // one past the item's last token
+  int pieces = 0;
+  it.lo = it.sink_x = it.shift = 0;
+  it.hi = kTree ? it.ctx : it.prefix + last;
+  if (it.prefix < 0) it.hi = 0;
+  if (it.hi > 0) {
+    const int to = (it.hi - 1) / p.piece + 1;
+    pieces = to;
+    if (!kTree) {
+      it.lo = max(0, it.prefix + it.tok0 - p.window + 1);
+      const int sp = (min(p.sinks, it.lo) + p.piece - 1) / p.piece, lp = it.lo / p.piece;
+      if (sp < lp) {
+        pieces = sp + to - lp;
+        it.sink_x = sp * p.piece;
+        it.shift = (lp - sp) * p.piece;
+      }
+    }
+  }
+  it.x0 = (int)((long long)pieces * rank / p.split) * p.piece;
+  it.x1 = (int)((long long)pieces * (rank + 1) / p.split) * p.piece;
+  it.nt = (it.x1 - it.x0 + kMaTile - 1) / kMaTile;
+  if (it.skip) it.nt = 0;
+  return it;
+}
+
+// The n lowest bits of word w of a 128-bit mask of columns.
+__device__ __forceinline__ uint32_t ma_low(int n, int w) {
+  n -= w * 32;
+  return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+}
+
+// Whether the row of a token sees a key (the same as the bits below, for one key).
+template <bool kTree>
+__device__ __forceinline__ bool ma_sees(const MaArgs& p, const MaItem& it, int token, int key) {
+  if (kTree) return key < it.prefix || p.mask[(it.start + token) * p.ld_mask + (key - it.prefix)] != 0;
+  const int pos = it.prefix + token;
+  return key <= pos && (key > pos - p.window || key < p.sinks);
+}
+
+// V row of a tile (in shared memory) made safe to multiply by 0. Returns
+// whether it held elements that are not finite, which are now 0.
+template <typename T, int D>
+__device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int hf = 0; hf < D / 64; ++hf) {
+    uint4* line = reinterpret_cast<uint4*>(tile + hf * MaSmem<D>::kHalf + row * 128);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      if (!seen) {
+        line[c] = make_uint4(0, 0, 0, 0);
+      } else {
+        const uint4 x = line[c];
+        any |= ((x.x & MaType<T>::kExp) + MaType<T>::kOne) | ((x.y & MaType<T>::kExp) + MaType<T>::kOne) |
+               ((x.z & MaType<T>::kExp) + MaType<T>::kOne) | ((x.w & MaType<T>::kExp) + MaType<T>::kOne);
+      }
+    }
+  }
+  if (!(any & 0x80008000u)) return false;
+  for (int hf = 0; hf < D / 64; ++hf) {
+    uint32_t* line = reinterpret_cast<uint32_t*>(tile + hf * MaSmem<D>::kHalf + row * 128);
+    for (int c = 0; c < 32; ++c) {
+      const uint32_t t = ((line[c] & MaType<T>::kExp) + MaType<T>::kOne) & 0x80008000u;
+      line[c] &= ~((t >> 15) * 0xffffu);
+    }
+  }
+  return true;
+}
+
+// Sum of the V elements of column col that are not finite, that ma_clean_row
+// took out, and whose keys the row of a token sees (a rare path).
 template <typename T, int D, bool kTree>
-int launch(const char* what, const MaArgs& p, cudaStream_t st) {
-  masked_attn_simple<T, D, kTree><<<dim3(std::min(p.max_q_len, 65535), p.B, (p.H + 3) / 4), 128, 0, st>>>(p);
-  return launch_status(what);
+__device__ __forceinline__ float ma_bad_sum(const MaArgs* args, const int* keys, int n_keys, int item, int rank,
+                                         bool shared, int token, int kvh, int col) {
+  const MaArgs& p = *args;
+  const MaItem it = shared ? ma_item<kTree, true>(p, item, rank) : ma_item<kTree, false>(p, item, rank);
+  const bool all = n_keys > kMaBad;  // more than were remembered: look at every key of this CTA
+  const int n = all ? it.x1 - it.x0 : n_keys;
+  float sum = 0.f;
+  for (int j = 0; j < n; ++j) {
+    const int x = it.x0 + j;
+    const int key = !all ? keys[j] : x < it.sink_x ? x : x + it.shift;
+    if (key >= it.hi || !ma_sees<kTree>(p, it, token, key)) continue;
+    const int page = key / p.block_size;
+    const int blk = page < p.max_blocks ? p.bt[it.b * p.bt_stride + page] : -1;
+    if (blk < 0 || blk >= p.num_blocks) continue;
+    const size_t at = (((size_t)blk * p.block_size + key % p.block_size) * p.Hkv + kvh) * D + col;
+    const float v = MaType<T>::get(p.v, at);
+    if (!isfinite(v)) sum += v;
+  }
+  return sum;
+}
+
+template <typename T, int D, bool kTree, bool kShared>
+__global__ void __launch_bounds__(kMaThreads, 1)
+    masked_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ MaArgs p) {
+  using S = MaSmem<D>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  S& s = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // a cluster of `split` CTAs works on one item; without a split a CTA takes items with the grid's stride
+  const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
+  const int first = p.split > 1 ? blockIdx.x / p.split : blockIdx.x;
+  const int stride = p.split > 1 ? p.n_items : gridDim.x;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    mbar_init(&s.q_full, 1);
+    mbar_init(&s.q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], 4);  // one arrival a warp
+      mbar_init(&s.o_full[i], 1);
+    }
+    mbar_init(&s.mma_done, 1);
+    s.abort = 0;
+    for (int i = 0; i < 6; ++i) s.n_bad[i >> 1][i & 1] = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&s.tmem_base, kMaTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  pdl_wait();  // q, the pool and the metadata come from earlier work on the stream
+  pdl_trigger();
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ TMA
+    // Lane i looks up and loads piece i of a tile.
+    if (lane == 0) {
+      prefetch_tensormap(&tmap_q);
+      prefetch_tensormap(&tmap_k);
+      prefetch_tensormap(&tmap_v);
+    }
+    const uint64_t pol_q = policy_evict_first();
+    const uint64_t pol_kv = policy_evict_normal();
+    const int oob = p.num_blocks * p.block_size;
+    const int per_tile = kMaTile / p.piece;
+    int nq = 0, ring = 0;  // Q loads and K / V tiles issued
+    bool ok = true;
+    for (int i = first; ok && i < p.n_items; i += stride) {
+      const MaItem it = ma_item<kTree, kShared>(p, i, rank);
+      if (it.skip) {
+        if (lane == 0 && it.tok0 < it.n) atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
+        continue;
+      }
+      if (lane == 0 && (it.ctx < 0 || (it.prefix < 0 && it.ctx != 0) ||
+                        (long long)it.ctx > (long long)p.max_blocks * p.block_size))
+        atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
+      if (it.nt == 0) continue;
+      const int32_t* table = p.bt + it.b * p.bt_stride;
+      // the pool row of this lane's piece of tile t (zeros where its page is none of the pool)
+      auto lookup = [&](int t) -> int {
+        const int x = it.x0 + t * kMaTile + lane * p.piece;
+        if (lane >= per_tile || x >= it.x1) return oob;
+        const int key = x < it.sink_x ? x : x + it.shift;
+        const int page = key / p.block_size;
+        const int blk = page < p.max_blocks ? table[page] : -1;
+        if (blk < 0 || blk >= p.num_blocks) {
+          atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
+          return oob;
+        }
+        return blk * p.block_size + (key - page * p.block_size);
+      };
+      auto load = [&](const CUtensorMap* map, int t, int row, int kvh) -> bool {
+        const int st = ring % kStages;
+        bool go = true;
+        const int n = min(per_tile, (it.x1 - it.x0 - t * kMaTile) / p.piece);
+        if (lane == 0) {
+          go = ma_wait(&s.empty[st], ((ring / kStages) & 1) ^ 1, &s.abort, p.status, NPL_DEV_TIMEOUT_TMA);
+          if (go) mbar_arrive_expect_tx(&s.full[st], n * p.piece * D * 2);
+        }
+        go = __shfl_sync(0xffffffffu, (int)go, 0);
+        if (!go) return false;
+        if (lane < n) {
+#pragma unroll
+          for (int hf = 0; hf < D / 64; ++hf)
+            tma_load_3d(s.kv[st] + hf * S::kHalf + lane * p.piece * 128, map, hf * 64, kvh, row, &s.full[st], pol_kv);
+        }
+        ++ring;
+        return true;
+      };
+      if (lane == 0) {
+        ok = nq == 0 || ma_wait(&s.q_empty, (nq - 1) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_TMA);
+        if (ok) {
+          mbar_arrive_expect_tx(&s.q_full, (it.second ? 2 : 1) * p.tokens * p.G * D * 2);
+          for (int q = 0; q < (it.second ? 2 : 1); ++q)
+#pragma unroll
+            for (int hf = 0; hf < D / 64; ++hf)
+              tma_load_3d(s.q[q] + hf * S::kHalf, &tmap_q, hf * 64, (it.kvh + (kShared ? 0 : q)) * p.G,
+                          it.start + it.tok0 + (kShared ? q * p.tokens : 0), &s.q_full, pol_q);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+      if (!ok) break;
+      ++nq;
+      int row = lookup(0);
+      ok = load(&tmap_k, 0, row, it.kvh);
+      if (!kShared && it.second) ok = ok && load(&tmap_k, 0, row, it.kvh + 1);
+      for (int t = 0; ok && t < it.nt; ++t) {
+        const bool more = t + 1 < it.nt;
+        const int next = more ? lookup(t + 1) : oob;
+        ok = load(&tmap_v, t, row, it.kvh);
+        if (more) ok = ok && load(&tmap_k, t + 1, next, it.kvh);
+        if (!kShared && it.second) {
+          ok = ok && load(&tmap_v, t, row, it.kvh + 1);
+          if (more) ok = ok && load(&tmap_k, t + 1, next, it.kvh + 1);
+        }
+        row = next;
+      }
+    }
+    // Every load issued here has landed before the CTA may exit.
+    if (lane == 0) {
+      if (nq > 0) mbar_wait(&s.q_full, (nq - 1) & 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+      for (int j = max(0, ring - kStages); j < ring; ++j)
+        mbar_wait(&s.full[j % kStages], (j / kStages) & 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA
+    if (lane == 0) {
+      constexpr uint32_t kIdQK = idesc_f16(kMaTile, kMaTile, false) | MaType<T>::kIdesc;
+      constexpr uint32_t kIdPV = idesc_f16(kMaTile, D, true) | MaType<T>::kIdesc;
+      int ring = 0, nq = 0;
+      uint32_t p_phase[2] = {0, 0};
+      auto full = [&](int r) -> bool {
+        return ma_wait(&s.full[r % kStages], (r / kStages) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
+      };
+      auto issue_s = [&](int st, int r) {  // S of stream st from the K tile at ring position r
+        const uint32_t qa = smem_u32(s.q[st]), ka = smem_u32(s.kv[r % kStages]);
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * S::kHalf + (kk & 3) * 32;
+          mma_f16(tmem + st * 128, sdesc_k_sw128(qa + off), sdesc_k_sw128(ka + off), kIdQK, kk > 0 ? 1u : 0u);
+        }
+        tc_commit(&s.s_full[st]);
+      };
+      auto issue_o = [&](int st, int r, int t, bool last) -> bool {  // O of stream st (+)= P V
+        if (!ma_wait(&s.p_full[st], p_phase[st], &s.abort, p.status, NPL_DEV_TIMEOUT_MMA) || !full(r)) return false;
+        p_phase[st] ^= 1;
+        tc_fence_after();
+        const uint32_t va = smem_u32(s.kv[r % kStages]);
+#pragma unroll
+        for (int kk = 0; kk < kMaTile / 16; ++kk)
+          ma_mma_ts(tmem + 256 + st * 128, tmem + st * 128 + kk * 8, sdesc_mn_sw128(va + kk * 16 * 128, S::kHalf, 1024),
+                    kIdPV, (t > 0 || kk > 0) ? 1u : 0u);
+        if (last) tc_commit(&s.o_full[st]);
+        return true;
+      };
+      bool ok = true;
+      for (int i = first; ok && i < p.n_items; i += stride) {
+        const MaItem it = ma_item<kTree, kShared>(p, i, rank);
+        if (it.nt == 0) continue;
+        ok = ma_wait(&s.q_full, nq & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
+        ++nq;
+        const int streams = it.second ? 2 : 1;
+        if (kShared) {
+          if (!ok || !(ok = full(ring))) break;
+          for (int st = 0; st < streams; ++st) issue_s(st, ring);
+          tc_commit(&s.empty[ring % kStages]);
+          if (it.nt == 1) tc_commit(&s.q_empty);
+          for (int t = 0; ok && t < it.nt; ++t) {
+            const int rv = ring + 1 + 2 * t, rk = rv + 1;
+            const bool more = t + 1 < it.nt;
+            for (int st = 0; ok && st < streams; ++st) {
+              ok = issue_o(st, rv, t, !more) && (!more || full(rk));
+              if (ok && st == streams - 1) tc_commit(&s.empty[rv % kStages]);
+              if (ok && more) issue_s(st, rk);
+            }
+            if (ok && more) {
+              tc_commit(&s.empty[rk % kStages]);
+              if (t + 2 == it.nt) tc_commit(&s.q_empty);
+            }
+          }
+          ring += 2 * it.nt;
+        } else {
+          for (int st = 0; ok && st < streams; ++st) {
+            if (!(ok = full(ring))) break;
+            issue_s(st, ring);
+            tc_commit(&s.empty[ring % kStages]);
+            ++ring;
+          }
+          if (ok && it.nt == 1) tc_commit(&s.q_empty);
+          for (int t = 0; ok && t < it.nt; ++t) {
+            const bool more = t + 1 < it.nt;
+            for (int st = 0; ok && st < streams; ++st) {
+              if (!(ok = issue_o(st, ring, t, !more))) break;
+              tc_commit(&s.empty[ring % kStages]);
+              ++ring;
+              if (!more) continue;
+              if (!(ok = full(ring))) break;
+              issue_s(st, ring);
+              tc_commit(&s.empty[ring % kStages]);
+              ++ring;
+            }
+            if (ok && t + 2 == it.nt) tc_commit(&s.q_empty);
+          }
+        }
+      }
+      tc_commit(&s.mma_done);  // arrives once every MMA issued above has completed
+      mbar_wait(&s.mma_done, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    // -------------------------------------------------------- softmax
+    const int st = warp >> 2;            // stream
+    const int r = threadIdx.x & 127;     // row of the tile = TMEM lane
+    const int row_tok = r / p.G, row_head = r - row_tok * p.G;
+    const uint32_t lane_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_tm = lane_tm + st * 128, o_tm = lane_tm + 256 + st * 128;
+    const int owner = kShared ? 0 : st;  // the stream whose threads clean the V tiles that this one reads
+    uint32_t s_phase = 0, o_phase = 0;
+    int ring = 0, item_no = 0;
+    bool ok = true;
+    for (int i = first; ok && i < p.n_items; i += stride) {
+      const MaItem it = ma_item<kTree, kShared>(p, i, rank);
+      if (it.skip) continue;
+      const int base = ring;
+      ring += it.nt * (!kShared && it.second ? 4 : 2);
+      if (st == 1 && !it.second) {
+        if (it.nt > 0) ++item_no;
+        continue;
+      }
+      const int kvh = it.kvh + (kShared ? 0 : st);
+      const int tok0 = it.tok0 + (kShared ? st * p.tokens : 0);
+      const int n_rows = min(p.tokens, it.n - tok0) * p.G;
+      const bool row_ok = r < n_rows;
+      const bool warp_on = (warp & 3) * 32 < n_rows;
+      const int token = tok0 + row_tok, pos = it.prefix + token;
+      const int list = item_no % 3;
+      float m = -INFINITY, l = 0.f;  // m in units of log2
+      for (int t = 0; ok && t < it.nt; ++t) {
+        const int xt = it.x0 + t * kMaTile;
+        // which of the tile's columns this row sees
+        uint32_t seen[4];
+        bool part;  // some row of the CTA's item does not see some column
+        if (kTree) {
+          part = xt + kMaTile > min(it.prefix, it.x1);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) seen[w] = row_ok ? ma_low(min(it.prefix, it.x1) - xt, w) : 0u;
+          if (part && row_ok) {
+            const uint8_t* mask = p.mask + (it.start + token) * p.ld_mask;
+            const int j0 = xt - it.prefix, j1 = min(it.n, it.x1 - it.prefix);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              if (j0 + w * 32 + 32 <= 0 || j0 + w * 32 >= j1) continue;
+              uint32_t bits = 0;
+#pragma unroll
+              for (int c = 0; c < 32; ++c) {
+                const int j = j0 + w * 32 + c;
+                if (j >= 0 && j < j1 && mask[j]) bits |= 1u << c;
+              }
+              seen[w] |= bits;
+            }
+          }
+        } else {
+          const int a = min(it.sink_x ? p.sinks : min(p.sinks, pos + 1), it.x1) - xt;
+          const int b = max(0, pos - p.window + 1) - it.shift - xt;
+          const int e = min(pos + 1 - it.shift, it.x1) - xt;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) seen[w] = row_ok ? ma_low(a, w) | (ma_low(e, w) & ~ma_low(b, w)) : 0u;
+          // the columns that the item's first row and its last row both see, every row sees
+          const int pa = it.prefix + it.tok0, pb = it.prefix + min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1)) - 1;
+          const int a_all = min(it.sink_x ? p.sinks : min(p.sinks, pa + 1), it.x1) - xt;
+          part = !(a_all >= kMaTile || (min(pa + 1 - it.shift, it.x1) - xt >= kMaTile &&
+                                        max(0, pb - p.window + 1) - it.shift - xt <= max(0, a_all)));
+        }
+        if (!ma_wait_warp(&s.s_full[st], s_phase, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
+          ok = false;
+          break;
+        }
+        s_phase ^= 1;
+        tc_fence_after();
+        // The next item's list is emptied here. Its last readers were those of the item before the last one, which
+        // ended before the MMA warp could issue this S (it had waited for both streams' P of the last item), and
+        // its next writers wait for an S that follows this thread's next arrival.
+        if (t == 0 && st == owner && r == 0) s.n_bad[(item_no + 1) % 3][owner] = 0;
+        if (warp_on) {
+          // The row is read twice, 32 columns at a time: its maximum, then the exponentials. (Held in
+          // registers, its 128 scores spilled.)
+          const bool masked = __any_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu);
+          uint32_t v[2][32];
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          tmem_ld_x32(s_tm, v[0]);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            ma_tmem_wait_ld(v[h & 1]);
+            if (h < 3) tmem_ld_x32(s_tm + (h + 1) * 32, v[(h + 1) & 1]);
+            if (masked) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!(seen[h] & (1u << c))) v[h & 1][c] = 0xff800000u;  // minus infinity
+            }
+#pragma unroll
+            for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(v[h & 1][c]));
+          }
+          tmem_ld_x32(s_tm, v[0]);
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c2;
+          const bool move = t == 0 || top > m + kMaSlack;
+          const float m_new = move ? top : m;
+          if (t > 0 && __any_sync(0xffffffffu, move)) {
+            const float alpha = !move ? 1.f : m == -INFINITY ? 0.f : ma_exp2(m - m_new);
+            l *= alpha;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_x32(o_tm + c * 32, o);
+              ma_tmem_wait_ld(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              ma_tmem_st_x16(o_tm + c * 32, o);
+              ma_tmem_st_x16(o_tm + c * 32 + 16, o + 16);
+            }
+          }
+          m = m_new;
+          const float add = m == -INFINITY ? 0.f : kMaShift - m;
+          float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            uint32_t(&x)[32] = v[h & 1];
+            ma_tmem_wait_ld(x);
+            if (h < 3) tmem_ld_x32(s_tm + (h + 1) * 32, v[(h + 1) & 1]);
+            if (masked) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!(seen[h] & (1u << c))) x[c] = 0xff800000u;
+            }
+            uint32_t pk[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const float p0 = ma_exp2(fmaf(__uint_as_float(x[2 * c]), p.c2, add));
+              const float p1 = ma_exp2(fmaf(__uint_as_float(x[2 * c + 1]), p.c2, add));
+              ls[(2 * c) & 3] += p0;
+              ls[(2 * c + 1) & 3] += p1;
+              pk[c] = MaType<T>::pack(p0, p1);
+            }
+            // P goes over columns of S that have been read: 16 h + 16 <= 32 h + 32
+            ma_tmem_st_x16(s_tm + h * 16, pk);
+          }
+          l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+          ma_tmem_wait_st();
+        }
+        if (part && st == owner) {
+          const int rv = kShared || !it.second ? base + 1 + 2 * t : base + (st == 0 ? 2 : t + 1 < it.nt ? 4 : 3) + 4 * t;
+          if (!ma_wait_warp(&s.full[rv % kStages], (rv / kStages) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
+            ok = false;
+            break;
+          }
+          const int x = xt + r, key = x < it.sink_x ? x : x + it.shift;
+          const bool some = x < it.x1 && key < it.hi && (kTree || key >= it.lo || key < p.sinks);
+          if (ma_clean_row<T, D>(s.kv[rv % kStages], r, some)) {
+            const int at = atomicAdd(&s.n_bad[list][owner], 1);
+            if (at < kMaBad) s.bad[list][owner][at] = key;
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.p_full[st]);
+      }
+      // every MMA of the item has completed; before the partial sums go over the ring, those of the other stream too
+      if (ok && it.nt > 0) {
+        ok = ma_wait_warp(&s.o_full[st], o_phase, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
+        if (ok && p.split > 1 && it.second)
+          ok = ma_wait_warp(&s.o_full[st ^ 1], o_phase, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
+        o_phase ^= 1;
+        tc_fence_after();
+      }
+      if (!ok) break;
+      if (warp_on) {
+        const int n_bad = it.nt > 0 ? s.n_bad[list][owner] : 0;
+        const float inv = p.split > 1 ? 1.f : l == 0.f ? 0.f : __frcp_rn(l);
+        float* const stage = reinterpret_cast<float*>(s.kv) + (size_t)(st * kMaTile + r) * D;
+        T* const dst = static_cast<T*>(p.out) + (it.start + token) * p.ld_out +
+                       (long long)(kvh * p.G + row_head) * D;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (it.nt > 0) {
+            tmem_ld_x32(o_tm + c * 32, o);
+            ma_tmem_wait_ld(o);
+          }
+          float acc[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) acc[e] = l == 0.f ? 0.f : __uint_as_float(o[e]);
+          if (!row_ok) continue;
+          if (p.split > 1) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)  // 16-byte chunks exchanged within 8, so that 8 rows use all banks
+              *reinterpret_cast<float4*>(stage + (((c * 8 + e) ^ (r & 7)) << 2)) =
+                  make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint4 w;
+              w.x = MaType<T>::pack(acc[8 * e] * inv, acc[8 * e + 1] * inv);
+              w.y = MaType<T>::pack(acc[8 * e + 2] * inv, acc[8 * e + 3] * inv);
+              w.z = MaType<T>::pack(acc[8 * e + 4] * inv, acc[8 * e + 5] * inv);
+              w.w = MaType<T>::pack(acc[8 * e + 6] * inv, acc[8 * e + 7] * inv);
+              reinterpret_cast<uint4*>(dst)[c * 4 + e] = w;
+            }
+          }
+        }
+        if (n_bad > 0 && row_ok && l != 0.f) {
+          for (int d = 0; d < D; ++d) {
+            const float x = ma_bad_sum<T, D, kTree>(&p, s.bad[list][owner], n_bad, i, rank, kShared, token, kvh, d);
+            if (x == 0.f) continue;
+            if (p.split > 1)
+              stage[(((d >> 2) ^ (r & 7)) << 2) + (d & 3)] += x;
+            else
+              MaType<T>::add(dst + d, x);
+          }
+        }
+        if (p.split > 1 && row_ok)
+          reinterpret_cast<float2*>(reinterpret_cast<float*>(s.kv) + 2 * kMaTile * D)[st * kMaTile + r] =
+              make_float2(m, l);
+      }
+      if (it.nt > 0) ++item_no;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kMaTmemCols);
+  }
+  if (p.split > 1) {
+    // ------------------------------------------- join the partial sums
+    // A warp takes a row of the item: out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j over the cluster's CTAs.
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    const MaItem it = ma_item<kTree, kShared>(p, first, rank);
+    if (!it.skip) {
+      const int r0 = min(p.tokens, it.n - it.tok0) * p.G;
+      const int r1 = !it.second ? 0 : kShared ? min(p.tokens, it.n - it.tok0 - p.tokens) * p.G : r0;
+      constexpr int kLanes = D / 4;  // lanes of a row: 4 columns each
+      const int sub = lane / kLanes, col = lane % kLanes;
+      for (int w = (rank * (kMaThreads / 32) + warp) * (32 / kLanes); w < r0 + r1;
+           w += p.split * (kMaThreads / 32) * (32 / kLanes)) {
+        const int idx = w + sub;
+        const bool on = idx < r0 + r1;
+        const int st = on && idx >= r0 ? 1 : 0, r = on ? idx - (st ? r0 : 0) : 0;
+        const float* base = reinterpret_cast<const float*>(s.kv);
+        const float2* ml = reinterpret_cast<const float2*>(base + 2 * kMaTile * D) + st * kMaTile + r;
+        const float* o = base + (size_t)(st * kMaTile + r) * D + ((col ^ (r & 7)) << 2);
+        float top = -INFINITY;
+        for (int j = 0; j < p.split; ++j) {
+          const float2 x = ma_ld_cluster2(cluster_map(ml, j));
+          top = x.x > top || x.x != x.x ? x.x : top;
+        }
+        if (top == -INFINITY) top = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+        for (int j = 0; j < p.split; ++j) {
+          const float2 x = ma_ld_cluster2(cluster_map(ml, j));
+          const float4 v = ma_ld_cluster(cluster_map(o, j));
+          if (x.y == 0.f) continue;  // no key of this part is seen: its sums were not written
+          const float f = ma_exp2(x.x - top);
+          l = fmaf(x.y, f, l);
+          acc.x = fmaf(v.x, f, acc.x);
+          acc.y = fmaf(v.y, f, acc.y);
+          acc.z = fmaf(v.z, f, acc.z);
+          acc.w = fmaf(v.w, f, acc.w);
+        }
+        const float inv = l == 0.f ? 0.f : __frcp_rn(l);
+        if (on) {
+          const int tok = it.tok0 + (kShared ? st * p.tokens : 0) + r / p.G;
+          T* const dst = static_cast<T*>(p.out) + (it.start + tok) * p.ld_out +
+                         (long long)((it.kvh + (kShared ? 0 : st)) * p.G + r % p.G) * D;
+          reinterpret_cast<uint2*>(dst)[col] =
+              make_uint2(MaType<T>::pack(acc.x * inv, acc.y * inv), MaType<T>::pack(acc.z * inv, acc.w * inv));
+        }
+      }
+    }
+    cluster_arrive_release();  // no CTA leaves while another reads its shared memory
+    cluster_wait_acquire();
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 ma_encode_fn() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+// [rows][heads][D] (rows ld elements apart, heads contiguous) as a 3-D tensor
+// map with a (64, box_heads, box_rows) box and the 128-byte swizzle.
+int ma_map(const char* what, CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, int heads,
+           int D, long long ld, int box_heads, int box_rows) {
+  const PFN_cuTensorMapEncodeTiled_v12000 fn = ma_encode_fn();
+  if (!fn) return fail(NPL_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled unavailable", what);
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)ld * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult r = fn(map, type, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(NPL_ERR_ARG, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+  return NPL_OK;
+}
+
+template <typename T, int D, bool kTree, bool kShared>
+int launch(const char* what, MaArgs p, cudaStream_t st) {
+  CUtensorMap tq, tk, tv;
+  const long long slots = (long long)p.num_blocks * p.block_size;
+  if (int rc = ma_map(what, &tq, MaType<T>::kMap, p.q, p.total_q, p.H, D, p.ld_q, p.G, p.tokens)) return rc;
+  if (int rc = ma_map(what, &tk, MaType<T>::kMap, p.k, slots, p.Hkv, D, (long long)p.Hkv * D, 1, p.piece)) return rc;
+  if (int rc = ma_map(what, &tv, MaType<T>::kMap, p.v, slots, p.Hkv, D, (long long)p.Hkv * D, 1, p.piece)) return rc;
+  const auto kernel = masked_attn_kernel<T, D, kTree, kShared>;
+  const int smem = (int)sizeof(MaSmem<D>) + 1024;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launch_status(what);
+  const int sms = num_sms() > 0 ? num_sms() : 148;
+  const int grid = p.split > 1 ? p.n_items * p.split : std::min(p.n_items, sms);
+  return launch_pdl_cluster(what, kernel, dim3(grid), dim3(kMaThreads), (size_t)smem, st, (unsigned)p.split, tq, tk,
+                            tv, p);
 }
 
 template <bool kTree>
-int run(const char* what, const MaArgs& p, int dtype, int D, cudaStream_t st) {
-  if (dtype == NPL_F16) return D == 128 ? launch<__half, 128, kTree>(what, p, st) : launch<__half, 64, kTree>(what, p, st);
-  return D == 128 ? launch<__nv_bfloat16, 128, kTree>(what, p, st) : launch<__nv_bfloat16, 64, kTree>(what, p, st);
+int run(const char* what, MaArgs p, int dtype, int D, float scale, cudaStream_t st) {
+  p.c2 = scale * 1.4426950408889634f;
+  p.tokens = kMaTile / p.G;
+  p.piece = kMaPiece;
+  while (p.block_size % p.piece) p.piece /= 2;
+  const bool shared = p.max_q_len > p.tokens;
+  p.levels = shared ? (p.max_q_len + 2 * p.tokens - 1) / (2 * p.tokens) : 1;
+  const long long items = (long long)p.levels * p.B * (shared ? p.Hkv : (p.Hkv + 1) / 2);
+  if (items >= (1ll << 27)) return fail(NPL_ERR_UNSUPPORTED, "%s: too many row tiles", what);
+  p.n_items = (int)items;
+  const int sms = num_sms() > 0 ? num_sms() : 148;
+  long long keys = (long long)p.max_blocks * p.block_size;  // the most that a CTA's rows may see
+  if (!kTree) keys = std::min(keys, (long long)p.window + p.sinks + 2 * p.tokens);
+  p.split = 1;
+  while (p.split < 8 && items * p.split * 2 <= sms && keys >= p.split * 2 * kMaTile) p.split *= 2;
+  if (dtype == NPL_F16) {
+    if (D == 128)
+      return shared ? launch<__half, 128, kTree, true>(what, p, st) : launch<__half, 128, kTree, false>(what, p, st);
+    return shared ? launch<__half, 64, kTree, true>(what, p, st) : launch<__half, 64, kTree, false>(what, p, st);
+  }
+  if (D == 128)
+    return shared ? launch<__nv_bfloat16, 128, kTree, true>(what, p, st)
+                  : launch<__nv_bfloat16, 128, kTree, false>(what, p, st);
+  return shared ? launch<__nv_bfloat16, 64, kTree, true>(what, p, st)
+                : launch<__nv_bfloat16, 64, kTree, false>(what, p, st);
 }
 
-int check(const char* what, const MaArgs& p, int dtype, int D) {
+int check(const char* what, const MaArgs& p, int dtype, int D, float scale) {
   if (dtype != NPL_F16 && dtype != NPL_BF16)
     return fail(NPL_ERR_ARG, "%s: element type %d (NPL_F16 or NPL_BF16)", what, dtype);
   if (!p.q || !p.k || !p.v || !p.bt || !p.ctx_lens || !p.out) return fail(NPL_ERR_ARG, "%s: null pointer", what);
@@ -110,7 +902,7 @@ int check(const char* what, const MaArgs& p, int dtype, int D) {
   if (D != 128 && D != 64) return fail(NPL_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, D);
   if (p.ld_q < (long long)p.H * D || p.ld_out < (long long)p.H * D || p.ld_q % 8 || p.ld_out % 8)
     return fail(NPL_ERR_ARG, "%s: token strides must be multiples of 8 and hold all heads", what);
-  if (!(p.scale > 0.f) || !(p.scale < 3.0e38f))
+  if (!(scale > 0.f) || !(scale < 2.0e38f))
     return fail(NPL_ERR_ARG, "%s: scale must be positive and finite", what);
   if (p.block_size % 8) return fail(NPL_ERR_UNSUPPORTED, "%s: block_size %d (a multiple of 8)", what, p.block_size);
   if (p.G > 128) return fail(NPL_ERR_UNSUPPORTED, "%s: %d query heads for each kv head (at most 128)", what, p.G);
@@ -140,8 +932,8 @@ extern "C" int npl_paged_tree_attention(const void* q, int dtype, int64_t ld_q, 
   p.bt_stride = bt_stride, p.ctx_lens = context_lens, p.q_lens = q_lens, p.q_offsets = q_offsets;
   p.mask = tree_mask, p.ld_mask = ld_mask, p.mask_cols = mask_cols;
   p.B = B, p.H = H, p.Hkv = Hkv, p.G = Hkv > 0 ? H / Hkv : 0, p.num_blocks = num_blocks, p.block_size = block_size;
-  p.max_blocks = max_blocks, p.total_q = total_q, p.max_q_len = max_q_len, p.scale = scale;
-  if (int rc = check(what, p, dtype, D)) return rc;
+  p.max_blocks = max_blocks, p.total_q = total_q, p.max_q_len = max_q_len;
+  if (int rc = check(what, p, dtype, D, scale)) return rc;
   if (!tree_mask || !q_lens) return fail(NPL_ERR_ARG, "%s: null pointer", what);
   if (mask_cols < max_q_len || ld_mask < mask_cols)
     return fail(NPL_ERR_ARG, "%s: the mask has %d columns (stride %lld) for up to %d drafts", what, mask_cols,
@@ -149,7 +941,7 @@ extern "C" int npl_paged_tree_attention(const void* q, int dtype, int64_t ld_q, 
   if (int rc = check_device()) return rc;
   if (B == 0 || total_q == 0 || max_q_len == 0) return NPL_OK;
   p.status = device_status_ptr();
-  return run<true>(what, p, dtype, D, static_cast<cudaStream_t>(stream));
+  return run<true>(what, p, dtype, D, scale, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int npl_paged_window_attention(const void* q, int dtype, int64_t ld_q, int total_q, int H, int Hkv, int D,
@@ -164,12 +956,12 @@ extern "C" int npl_paged_window_attention(const void* q, int dtype, int64_t ld_q
   p.bt_stride = bt_stride, p.ctx_lens = context_lens, p.q_lens = q_lens, p.q_offsets = q_offsets;
   p.window = window, p.sinks = sinks;
   p.B = B, p.H = H, p.Hkv = Hkv, p.G = Hkv > 0 ? H / Hkv : 0, p.num_blocks = num_blocks, p.block_size = block_size;
-  p.max_blocks = max_blocks, p.total_q = total_q, p.max_q_len = q_lens ? max_q_len : 1, p.scale = scale;
-  if (int rc = check(what, p, dtype, D)) return rc;
+  p.max_blocks = max_blocks, p.total_q = total_q, p.max_q_len = q_lens ? max_q_len : 1;
+  if (int rc = check(what, p, dtype, D, scale)) return rc;
   if (window < 1 || sinks < 0)
     return fail(NPL_ERR_ARG, "%s: window %d (at least 1), sinks %d (at least 0)", what, window, sinks);
   if (int rc = check_device()) return rc;
   if (B == 0 || total_q == 0 || p.max_q_len == 0) return NPL_OK;
   p.status = device_status_ptr();
-  return run<false>(what, p, dtype, D, static_cast<cudaStream_t>(stream));
+  return run<false>(what, p, dtype, D, scale, static_cast<cudaStream_t>(stream));
 }

@@ -1,5 +1,24 @@
 // Log probabilities of given tokens, the entropy of their distributions and
 // the top alternatives, from rows of logits.
+//
+// npl_token_logprobs (no counterpart in the reference). With x a row, M its
+// maximum and d = x - M:
+//   S = sum e^d,  T = sum d e^d,  ln p = d - ln S,  entropy = ln S - T / S
+// in one read of the row: a thread keeps the maximum m of what it has read and
+// s, t relative to it; when m moves by delta = m - m' < 0,
+//   t' = e^delta (t + delta s),  s' = e^delta s
+// and the threads' sums are joined the same way.
+//
+// Top k: of the threads' maxima, the k-th largest is no larger than the k-th
+// largest logit, so only threads whose own maximum reaches it (k of them, and
+// those that tie) read their logits once more, from L2, for the logits that
+// reach it. Those few are ranked by counting: larger first, of equal ones the
+// lowest index.
+//
+// Bound by the read of the logits. One CTA takes a row; few rows are split over
+// a cluster of CTAs each, whose sums and best logits its first CTA joins.
+#include <algorithm>
+
 #include <cuda_bf16.h>
 
 #include "npl_common.cuh"
@@ -9,63 +28,399 @@ namespace {
 
 constexpr int kLpMaxTop = 32;
 constexpr int kLpThreads = 256;
-
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+constexpr int kLpUnroll = 4;      // 16-byte words that a thread has in flight
+constexpr int kLpCandidates = 1024;
+constexpr int kLpStep = 2048;     // logits that a CTA looks through at a time for equal ones
+constexpr int kLpMaxSplit = 8;    // CTAs of a cluster at most
+constexpr float kLpFar = -200.f;  // e^-200 is 0 in fp32: distances are cut here, so that 0 * infinity cannot arise
+constexpr float kLog2e = 1.4426950408889634f;
 
 // Whole numbers in the order of the values: equal ones for +0 and -0, the
-// largest for every NaN.
-__device__ __forceinline__ int order_key(float x) {
-  if (x != x) return 0x7fffffff;
+// largest for every NaN; 0 is left for "no value".
+__device__ __forceinline__ unsigned lp_key(float x) {
+  if (x != x) return 0xffffffffu;
   const int b = __float_as_int(x);
-  return b < 0 ? -(b & 0x7fffffff) : b;
+  return (unsigned)(b < 0 ? -(b & 0x7fffffff) : b) ^ 0x80000000u;
+}
+
+__device__ __forceinline__ float lp_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float lp_exp(float d) {  // e^d for d <= 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * kLog2e));
+  return y;
+}
+
+// 16 bytes of logits as floats, and their maximum (NaN if there is one).
+template <typename T>
+struct LpWord;
+template <>
+struct LpWord<float> {
+  static constexpr int kN = 4;
+  static constexpr uint32_t kNone = 0xff800000u;  // minus infinity
+  __device__ static float top(const uint4& w) {
+    return lp_max_nan(lp_max_nan(__uint_as_float(w.x), __uint_as_float(w.y)),
+                      lp_max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+  __device__ static void get(const uint4& w, float (&x)[4]) {
+    x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y);
+    x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+  }
+  __device__ static float one(float x) { return x; }
+};
+template <typename H2>
+__device__ __forceinline__ H2 lp_as(uint32_t w) {
+  return *reinterpret_cast<const H2*>(&w);
+}
+template <>
+struct LpWord<__half> {
+  static constexpr int kN = 8;
+  static constexpr uint32_t kNone = 0xfc00fc00u;
+  __device__ static float top(const uint4& w) {
+    const __half2 m = __hmax2_nan(__hmax2_nan(lp_as<__half2>(w.x), lp_as<__half2>(w.y)),
+                                  __hmax2_nan(lp_as<__half2>(w.z), lp_as<__half2>(w.w)));
+    return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+  }
+  __device__ static void get(const uint4& w, float (&x)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(lp_as<__half2>(u[i]));
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
+  __device__ static float one(__half x) { return __half2float(x); }
+};
+template <>
+struct LpWord<__nv_bfloat16> {
+  static constexpr int kN = 8;
+  static constexpr uint32_t kNone = 0xff80ff80u;
+  __device__ static float top(const uint4& w) {
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(lp_as<__nv_bfloat162>(w.x), lp_as<__nv_bfloat162>(w.y)),
+                                         __hmax2_nan(lp_as<__nv_bfloat162>(w.z), lp_as<__nv_bfloat162>(w.w)));
+    return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
+  }
+  __device__ static void get(const uint4& w, float (&x)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[2 * i] = __uint_as_float(u[i] << 16), x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  }
+  __device__ static float one(__nv_bfloat16 x) { return __bfloat162float(x); }
+};
+
+struct LpSum {  // of values seen so far: maximum, sum e^(x - m), sum (x - m) e^(x - m)
+  float m, s, t;
+};
+
+__device__ __forceinline__ void lp_move(LpSum& a, float m) {  // to a maximum m >= a.m (or NaN)
+  const float delta = fmaxf(a.m - m, kLpFar);  // a.m == m: 0; minus infinities and NaN: far, with s = t = 0 or no result
+  const float f = a.m == m ? 1.f : lp_exp(delta);
+  a.t = a.m == m ? a.t : f * fmaf(delta, a.s, a.t);
+  a.s *= f;
+  a.m = m;
+}
+
+__device__ __forceinline__ void lp_add(LpSum& a, float x) {  // x <= a.m
+  const float d = fmaxf(x - a.m, kLpFar), e = a.m == -INFINITY ? 0.f : lp_exp(d);
+  a.s += e;
+  a.t = fmaf(d, e, a.t);
+}
+
+struct LpSmem {
+  float red[3][kLpThreads / 32];
+  unsigned keys[kLpThreads];
+  unsigned threshold;
+  int n_candidates, n_greater;
+  unsigned long long candidate[kLpCandidates];  // key << 32 | ~index: larger is better
+  unsigned long long best[kLpMaxTop];           // of this CTA, best first
+  LpSum sum;                                    // of this CTA
+  unsigned scan[kLpThreads / 32];
+  unsigned long long round[kLpThreads / 32];
+};
+
+__device__ __forceinline__ unsigned long long lp_pack(unsigned key, int index) {
+  return ((unsigned long long)key << 32) | (unsigned)~index;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads)
-    logprobs_simple(const T* logits, long long ld, int V, const int64_t* ids, int top_k, float* lp, float* ent,
-                    int64_t* top_ids, float* top_lp, int* status) {
-  __shared__ float red[32];
-  __shared__ long long best[32];
-  const long long r = blockIdx.x;
-  const T* x = logits + r * ld;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < V; i += blockDim.x) m = fmaxf(m, to_float(x[i]));
-  m = block_max(m, red);
-  __syncthreads();
-  float s = 0.f, t = 0.f;
-  for (int i = threadIdx.x; i < V; i += blockDim.x) {
-    const float d = to_float(x[i]) - m, e = expf(d);
-    s += e;
-    t += d == -INFINITY ? 0.f : d * e;
+struct LpRow {  // this CTA's part of a row: words [w0, w1) of 16 bytes from `words`, and single logits around them
+  const T* x;
+  const uint4* words;
+  int head, w0, w1;  // logits before the first word; this CTA's words
+  int single;        // this thread's single logit, -1: none
+  bool first;        // the row's first part, to which the logits before the first word belong
+  int end;           // one past this part's last logit
+};
+
+template <typename T>
+__device__ __forceinline__ float lp_at(const T* x, int i) {
+  return LpWord<T>::one(x[i]);
+}
+
+template <typename T, typename F>
+__device__ __forceinline__ void lp_each(const LpRow<T>& r, F&& f) {  // this thread's logits: f(value, index)
+  constexpr int N = LpWord<T>::kN;
+  if (r.single >= 0) f(lp_at(r.x, r.single), r.single);
+  for (int w = r.w0 + (int)threadIdx.x; w < r.w1; w += kLpThreads) {
+    float v[N];
+    LpWord<T>::get(r.words[w], v);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f(v[e], r.head + w * N + e);
   }
-  s = block_sum(s, red);
+}
+
+// The k best of this CTA's logits into s.best (empty places are 0).
+template <typename T>
+__device__ void lp_top(LpSmem& s, const LpRow<T>& r, float own_max, bool any, int k) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const unsigned own = any ? lp_key(own_max) : 0u;
+  s.keys[tid] = own;
+  if (tid == 0) s.n_candidates = s.n_greater = 0;
+  if (tid < kLpMaxTop) s.best[tid] = 0;
   __syncthreads();
-  t = block_sum(t, red);
-  const float ls = logf(s);
-  if (threadIdx.x == 0) {
-    const long long id = ids[r];
-    if (id < -1 || id >= V) atomicCAS(status, 0, NPL_DEV_BAD_INDEX);
-    lp[r] = id == -1 ? 0.f : id < 0 || id >= V ? NAN : to_float(x[id]) - m - ls;
-    ent[r] = ls - t / s;
+  if (warp == 0) {
+    // the largest threshold, of 20 leading bits, that k of the maxima reach (0 where fewer threads have any)
+    unsigned key[kLpThreads / 32], lo = 0;
+#pragma unroll
+    for (int i = 0; i < kLpThreads / 32; ++i) key[i] = s.keys[lane + i * 32];
+    for (int bit = 31; bit >= 12; --bit) {
+      const unsigned c = lo | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kLpThreads / 32; ++i) n += key[i] >= c;
+      if (__reduce_add_sync(0xffffffffu, n) >= k) lo = c;
+    }
+    if (lane == 0) s.threshold = lo;
   }
-  long long prev = 0x7fffffffffffffffll;  // (key, places from the end) of the last one taken
-  for (int k = 0; k < top_k; ++k) {
-    long long c = -0x7fffffffffffffffll;
-    for (int i = threadIdx.x; i < V; i += blockDim.x) {
-      const long long y = ((long long)order_key(to_float(x[i])) << 32) | (unsigned)(0x7fffffff - i);
-      if (y < prev && y > c) c = y;
+  __syncthreads();
+  const unsigned least = max(s.threshold, 1u);
+  if (own >= least) {
+    lp_each(r, [&](float x, int i) {
+      const unsigned key = lp_key(x);
+      if (key < least) return;
+      const int at = atomicAdd(&s.n_candidates, 1);
+      if (at < kLpCandidates) s.candidate[at] = lp_pack(key, i);
+    });
+  }
+  __syncthreads();
+  int n = s.n_candidates;
+  if (n > kLpCandidates) {
+    // Many equal logits (the zeros of a padding row, say), or many large ones with one thread. A pass finds the best
+    // logit after the last one taken; then those equal to it are taken in the order of their places, a few at a time.
+    const int from = r.first ? 0 : r.head + r.w0 * LpWord<T>::kN;
+    unsigned long long last = ~0ull;
+    for (int j = 0; j < k;) {
+      unsigned long long c = 0;
+      lp_each(r, [&](float x, int i) {
+        const unsigned long long y = lp_pack(lp_key(x), i);
+        if (y < last && y > c) c = y;
+      });
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) c = max(c, __shfl_xor_sync(0xffffffffu, c, o));
+      if (lane == 0) s.round[warp] = c;
+      __syncthreads();
+      c = 0;
+#pragma unroll
+      for (int i = 0; i < kLpThreads / 32; ++i) c = max(c, s.round[i]);
+      if (c == 0) break;  // this part holds no more logits
+      const unsigned key = (unsigned)(c >> 32);
+      int place = (int)~(unsigned)c;
+      if (tid == 0) s.best[j] = c;
+      ++j;
+      for (int base = from + (place - from) / kLpStep * kLpStep; j < k && base < r.end;) {
+        unsigned next = 0x7fffffffu;
+        for (int e = kLpStep / kLpThreads - 1; e >= 0; --e) {
+          const int i = base + tid * (kLpStep / kLpThreads) + e;
+          if (i > place && i < r.end && lp_key(lp_at(r.x, i)) == key) next = i;
+        }
+        next = __reduce_min_sync(0xffffffffu, next);
+        __syncthreads();
+        if (lane == 0) s.scan[warp] = next;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kLpThreads / 32; ++i) next = min(next, s.scan[i]);
+        if (next == 0x7fffffffu) {
+          base += kLpStep;
+        } else {
+          place = (int)next;
+          if (tid == 0) s.best[j] = lp_pack(key, place);
+          ++j;
+        }
+      }
+      last = (unsigned long long)key << 32;  // where places are left, all that are equal have been taken
+      __syncthreads();
     }
     __syncthreads();
-    c = block_max(c, best);
-    prev = c;
-    if (threadIdx.x == 0) {
-      const int id = 0x7fffffff - (int)(unsigned)c;
-      top_ids[r * top_k + k] = id;
-      top_lp[r * top_k + k] = to_float(x[id]) - m - ls;
+    return;
+  }
+  for (int i = tid; i < n; i += kLpThreads) {
+    const unsigned long long mine = s.candidate[i];
+    int better = 0;
+    for (int j = 0; j < n && better < k; ++j) better += s.candidate[j] > mine;
+    if (better < k) s.best[better] = mine;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ LpSum lp_ld_sum(const LpSum* p, int rank) {
+  const uint32_t a = cluster_map(p, rank);
+  LpSum r;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.m) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.s) : "r"(a + 4) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.t) : "r"(a + 8) : "memory");
+  return r;
+}
+
+struct LpArgs {
+  const void* logits;
+  long long ld;
+  int vocab, top_k, split;
+  const int64_t* ids;
+  float* lp;
+  float* entropy;
+  int64_t* top_ids;
+  float* top_lp;
+  int* status;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs p) {
+  __shared__ LpSmem s;
+  constexpr int N = LpWord<T>::kN;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
+  const long long row = p.split > 1 ? blockIdx.x / p.split : blockIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  LpRow<T> r;
+  r.x = static_cast<const T*>(p.logits) + row * p.ld;
+  r.head = min(p.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(r.x) & 15)) & 15) / (int)sizeof(T));
+  r.words = reinterpret_cast<const uint4*>(r.x + r.head);
+  const int words = (p.vocab - r.head) / N;
+  r.w0 = (int)((long long)words * rank / p.split);
+  r.w1 = (int)((long long)words * (rank + 1) / p.split);
+  const int tail = r.head + words * N;  // the first logit behind the words
+  r.first = rank == 0;
+  r.end = rank == p.split - 1 ? p.vocab : r.head + r.w1 * N;
+  r.single = -1;
+  if (rank == 0 && tid < r.head) r.single = tid;
+  if (rank == p.split - 1 && tid >= 32 && tid - 32 < p.vocab - tail) r.single = tail + tid - 32;
+
+  LpSum a = {-INFINITY, 0.f, 0.f};
+  if (r.single >= 0) a = {lp_at(r.x, r.single), 1.f, 0.f};
+  if (a.m == -INFINITY) a.s = 0.f;
+  for (int w = r.w0 + tid; w < r.w1; w += kLpThreads * kLpUnroll) {
+    uint4 v[kLpUnroll];
+#pragma unroll
+    for (int u = 0; u < kLpUnroll; ++u)
+      v[u] = w + u * kLpThreads < r.w1 ? r.words[w + u * kLpThreads]
+                                       : make_uint4(LpWord<T>::kNone, LpWord<T>::kNone, LpWord<T>::kNone,
+                                                    LpWord<T>::kNone);
+    float m = a.m;
+#pragma unroll
+    for (int u = 0; u < kLpUnroll; ++u) m = lp_max_nan(m, LpWord<T>::top(v[u]));
+    lp_move(a, m);
+#pragma unroll
+    for (int u = 0; u < kLpUnroll; ++u) {
+      float x[N];
+      LpWord<T>::get(v[u], x);
+#pragma unroll
+      for (int e = 0; e < N; ++e) lp_add(a, x[e]);
     }
   }
+
+  // the CTA's maximum and sums
+  const float own_max = a.m;
+  float m = a.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = lp_max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) s.red[0][warp] = m;
+  __syncthreads();
+  m = s.red[0][0];
+#pragma unroll
+  for (int i = 1; i < kLpThreads / 32; ++i) m = lp_max_nan(m, s.red[0][i]);
+  lp_move(a, m);
+  a.s = warp_sum(a.s);
+  a.t = warp_sum(a.t);
+  if (lane == 0) s.red[1][warp] = a.s, s.red[2][warp] = a.t;
+  __syncthreads();
+  a.s = a.t = 0.f;
+#pragma unroll
+  for (int i = 0; i < kLpThreads / 32; ++i) a.s += s.red[1][i], a.t += s.red[2][i];
+
+  if (p.top_k) lp_top(s, r, own_max, r.single >= 0 || r.w0 + tid < r.w1, p.top_k);
+
+  if (p.split > 1) {
+    if (tid == 0) s.sum = a;
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    if (rank == 0) {
+      LpSum part[kLpMaxSplit];
+      m = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kLpMaxSplit; ++j) {
+        if (j >= p.split) break;
+        part[j] = lp_ld_sum(&s.sum, j);
+        m = lp_max_nan(m, part[j].m);
+      }
+      a = {m, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < kLpMaxSplit; ++j) {
+        if (j >= p.split) break;
+        lp_move(part[j], m);
+        a.s += part[j].s, a.t += part[j].t;
+      }
+      const int n = p.split * p.top_k;  // at most kLpThreads
+      unsigned long long mine = 0;
+      if (tid < n) {
+        const uint32_t at = cluster_map(&s.best[tid % p.top_k], tid / p.top_k);
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(mine) : "r"(at) : "memory");
+        s.candidate[tid] = mine;
+      }
+      __syncthreads();
+      if (mine) {
+        int better = 0;
+        for (int j = 0; j < n; ++j) better += s.candidate[j] > mine;
+        if (better < p.top_k) s.candidate[kLpThreads + better] = mine;
+      }
+      __syncthreads();
+      if (tid < p.top_k) s.best[tid] = s.candidate[kLpThreads + tid];
+    }
+    cluster_arrive_release();  // no CTA leaves while the first reads its shared memory
+    cluster_wait_acquire();
+    if (rank != 0) return;
+  }
+
+  const bool bad = !(fabsf(a.m) < INFINITY);  // NaN, plus infinity, or nothing but minus infinity
+  const float ls = bad ? NAN : logf(a.s);
+  if (tid < p.top_k) {
+    const int i = (int)~(unsigned)s.best[tid];
+    p.top_ids[row * p.top_k + tid] = i;
+    p.top_lp[row * p.top_k + tid] = lp_at(r.x, i) - a.m - ls;
+  }
+  if (tid == kLpThreads - 1) {
+    const long long id = p.ids[row];
+    const bool in = id >= 0 && id < p.vocab;
+    if (!in && id != -1) atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
+    p.lp[row] = in ? lp_at(r.x, (int)id) - a.m - ls : id == -1 ? 0.f : NAN;
+    p.entropy[row] = ls - a.t / a.s;
+  }
+}
+
+template <typename T>
+int launch(const char* what, LpArgs p, long long rows, cudaStream_t st) {
+  const int sms = num_sms() > 0 ? num_sms() : 148;
+  p.split = 1;
+  while (p.split < kLpMaxSplit && rows * p.split * 2 <= 4ll * sms &&
+         p.vocab >= p.split * 2 * kLpThreads * LpWord<T>::kN)
+    p.split *= 2;
+  return launch_pdl_cluster(what, logprobs_kernel<T>, dim3((unsigned)(rows * p.split)), dim3(kLpThreads), 0, st,
+                            (unsigned)p.split, p);
 }
 
 }  // namespace
@@ -95,19 +450,11 @@ extern "C" int npl_token_logprobs(const void* logits, int dtype, int64_t ld, int
     return fail(NPL_ERR_ARG, "%s: ids or outputs are not aligned to their elements", what);
   if (int rc = check_device()) return rc;
   if (rows == 0) return NPL_OK;
-  int* status = device_status_ptr();
+  LpArgs p{};
+  p.logits = logits, p.ld = ld, p.vocab = (int)vocab, p.top_k = top_k, p.ids = token_ids;
+  p.lp = logprobs, p.entropy = entropy, p.top_ids = top_ids, p.top_lp = top_logprobs;
+  p.status = device_status_ptr();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == NPL_F32)
-    logprobs_simple<<<(unsigned)rows, kLpThreads, 0, st>>>(static_cast<const float*>(logits), ld, (int)vocab,
-                                                          token_ids, top_k, logprobs, entropy, top_ids,
-                                                          top_logprobs, status);
-  else if (dtype == NPL_F16)
-    logprobs_simple<<<(unsigned)rows, kLpThreads, 0, st>>>(static_cast<const __half*>(logits), ld, (int)vocab,
-                                                          token_ids, top_k, logprobs, entropy, top_ids,
-                                                          top_logprobs, status);
-  else
-    logprobs_simple<<<(unsigned)rows, kLpThreads, 0, st>>>(static_cast<const __nv_bfloat16*>(logits), ld, (int)vocab,
-                                                          token_ids, top_k, logprobs, entropy, top_ids,
-                                                          top_logprobs, status);
-  return launch_status(what);
+  if (dtype == NPL_F32) return launch<float>(what, p, rows, st);
+  return dtype == NPL_F16 ? launch<__half>(what, p, rows, st) : launch<__nv_bfloat16>(what, p, rows, st);
 }

@@ -190,3 +190,20 @@ def test_written_just_before(P):
         x.copy_(keep)
         for a, b in zip(P.token_logprobs(x, ids, 5), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [3, 330])
+def test_large_logits_that_share_their_places(P, n, kind):
+    """Rows whose largest logits stand where one thread reads them all, more
+    than any list of candidates holds; few of them, many equal ones, and equal
+    ones that end within the row."""
+    v = 70000
+    x = torch.zeros(n, v)
+    for i in range(n):
+        lo = 2048 * (1 + i % 5) + 16 * (i % 3)
+        at = torch.cat([torch.arange(lo + 2048 * j, lo + 2048 * j + 64) for j in range(28)])
+        x[i, at] = 50.0 + (torch.arange(at.numel()) % (3, 40, 1000)[i % 3]).float() / 16
+    x = x.to(TYPES[kind]).cuda()
+    ids = torch.arange(n).cuda()
+    check(P.token_logprobs(x, ids, 32), x, ids, 32)

@@ -50,8 +50,10 @@ namespace {
 constexpr int kMaThreads = 384;
 constexpr int kMaTile = 128;
 constexpr uint32_t kMaTmemCols = 512;  // S of the streams at 0 and 128 (P over it), O at 256 and 384
+constexpr int kMaFixed = 4;             // what a CTA costs beside its tiles, in tiles
 constexpr int kMaBad = 32;             // keys with V elements that are not finite, remembered for an item
-constexpr int kMaPiece = 32;           // keys of a piece at most
+constexpr int kMaPieceLog = 5;         // 32 keys of a piece at most
+constexpr int kMaMaxSplit = 8;          // CTAs of a cluster at most
 constexpr float kMaShift = 6.f;        // p = 2^(x - m + 6)
 constexpr float kMaSlack = 8.f;        // m moves when a score is more than this above it
 
@@ -72,10 +74,10 @@ struct MaArgs {
   int window, sinks;
   int B, H, Hkv, G, num_blocks, block_size, max_blocks, total_q, max_q_len;
   int tokens;   // of a row tile: 128 / G
-  int piece;    // keys of a piece
+  int piece, piece_log;  // keys of a piece, a power of two
   int levels;   // items of a sequence and kv head (or pair of them)
   int n_items;  // levels * B * (kv heads, or pairs of them)
-  int split;    // CTAs of a cluster, which share an item's keys
+  int split, split_log;  // CTAs of a cluster, which share an item's keys, a power of two
   float c2;     // scale * log2(e)
   int* status;
 };
@@ -133,9 +135,10 @@ __device__ __forceinline__ float ma_exp2(float x) {
   return y;
 }
 
-// Bounded wait that also gives up once another role of the CTA gave up.
-__device__ __forceinline__ bool ma_wait(uint64_t* bar, uint32_t parity, int* abort, int* status, int code) {
-  if (mbar_try_wait(bar, parity)) return true;
+// Bounded wait that also gives up once another role of the CTA gave up. (Its
+// loop is a call: a CTA of few tiles runs most of its code once, and fetching
+// that code is what it waits for.)
+__device__ __noinline__ bool ma_wait_long(uint64_t* bar, uint32_t parity, int* abort, int* status, int code) {
   const uint64_t t0 = globaltimer_ns();
   while (true) {
     for (int i = 0; i < 32; ++i)
@@ -147,6 +150,9 @@ __device__ __forceinline__ bool ma_wait(uint64_t* bar, uint32_t parity, int* abo
       return false;
     }
   }
+}
+__device__ __forceinline__ bool ma_wait(uint64_t* bar, uint32_t parity, int* abort, int* status, int code) {
+  return mbar_try_wait(bar, parity) || ma_wait_long(bar, parity, abort, status, code);
 }
 
 // The same for a warp: its lanes go on, or give up, together.
@@ -198,6 +204,27 @@ __device__ __forceinline__ float2 ma_ld_cluster2(uint32_t addr) {
   return v;
 }
 
+// Scores of columns that are not seen become minus infinity.
+__device__ __forceinline__ void ma_hide(uint32_t (&v)[32], uint32_t seen) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c)
+    if (!(seen & (1u << c))) v[c] = 0xff800000u;
+}
+
+// p = 2^(score c2 + add) of 32 columns, packed; their sums go to ls.
+template <typename T>
+__device__ __forceinline__ void ma_exp_pack(const uint32_t (&v)[32], float c2, float add, float (&ls)[4],
+                                            uint32_t (&pk)[16]) {
+#pragma unroll
+  for (int c = 0; c < 16; ++c) {
+    const float p0 = ma_exp2(fmaf(__uint_as_float(v[2 * c]), c2, add));
+    const float p1 = ma_exp2(fmaf(__uint_as_float(v[2 * c + 1]), c2, add));
+    ls[(2 * c) & 3] += p0;
+    ls[(2 * c + 1) & 3] += p1;
+    pk[c] = MaType<T>::pack(p0, p1);
+  }
+}
+
 // One item: 128 rows (or twice 128, shared) of one sequence and kv head (or
 // the same rows of two). Every role decodes the same items from the same
 // read-only metadata. The keys that some row of the item sees are numbered by
@@ -230,11 +257,11 @@ __device__ __forceinline__ MaItem ma_item(const MaArgs& p, int i, int rank) {
   it.hi = kTree ? it.ctx : it.prefix + last;
   if (it.prefix < 0) it.hi = 0;
   if (it.hi > 0) {
-    const int to = (it.hi - 1) / p.piece + 1;
+    const int to = ((it.hi - 1) >> p.piece_log) + 1;
     pieces = to;
     if (!kTree) {
       it.lo = max(0, it.prefix + it.tok0 - p.window + 1);
-      const int sp = (min(p.sinks, it.lo) + p.piece - 1) / p.piece, lp = it.lo / p.piece;
+      const int sp = (min(p.sinks, it.lo) + p.piece - 1) >> p.piece_log, lp = it.lo >> p.piece_log;
       if (sp < lp) {
         pieces = sp + to - lp;
         it.sink_x = sp * p.piece;
@@ -242,8 +269,8 @@ __device__ __forceinline__ MaItem ma_item(const MaArgs& p, int i, int rank) {
       }
     }
   }
-  it.x0 = (int)((long long)pieces * rank / p.split) * p.piece;
-  it.x1 = (int)((long long)pieces * (rank + 1) / p.split) * p.piece;
+  it.x0 = (int)(((long long)pieces * rank) >> p.split_log) << p.piece_log;
+  it.x1 = (int)(((long long)pieces * (rank + 1)) >> p.split_log) << p.piece_log;
   it.nt = (it.x1 - it.x0 + kMaTile - 1) / kMaTile;
   if (it.skip) it.nt = 0;
   return it;
@@ -268,14 +295,15 @@ __device__ __forceinline__ bool ma_sees(const MaArgs& p, const MaItem& it, int t
 template <typename T, int D>
 __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) {
   uint32_t any = 0;
-#pragma unroll
+#pragma unroll 1
   for (int hf = 0; hf < D / 64; ++hf) {
     uint4* line = reinterpret_cast<uint4*>(tile + hf * MaSmem<D>::kHalf + row * 128);
+    if (!seen) {
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      if (!seen) {
-        line[c] = make_uint4(0, 0, 0, 0);
-      } else {
+      for (int c = 0; c < 8; ++c) line[c] = make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
         const uint4 x = line[c];
         any |= ((x.x & MaType<T>::kExp) + MaType<T>::kOne) | ((x.y & MaType<T>::kExp) + MaType<T>::kOne) |
                ((x.z & MaType<T>::kExp) + MaType<T>::kOne) | ((x.w & MaType<T>::kExp) + MaType<T>::kOne);
@@ -283,26 +311,26 @@ __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) 
     }
   }
   if (!(any & 0x80008000u)) return false;
-  for (int hf = 0; hf < D / 64; ++hf) {
-    uint32_t* line = reinterpret_cast<uint32_t*>(tile + hf * MaSmem<D>::kHalf + row * 128);
-    for (int c = 0; c < 32; ++c) {
-      const uint32_t t = ((line[c] & MaType<T>::kExp) + MaType<T>::kOne) & 0x80008000u;
-      line[c] &= ~((t >> 15) * 0xffffu);
-    }
+#pragma unroll 1
+  for (int c = 0; c < D / 2; ++c) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(tile + (c >> 5) * MaSmem<D>::kHalf + row * 128) + (c & 31);
+    const uint32_t t = ((*w & MaType<T>::kExp) + MaType<T>::kOne) & 0x80008000u;
+    *w &= ~((t >> 15) * 0xffffu);
   }
   return true;
 }
 
 // Sum of the V elements of column col that are not finite, that ma_clean_row
 // took out, and whose keys the row of a token sees (a rare path).
-template <typename T, int D, bool kTree>
-__device__ __forceinline__ float ma_bad_sum(const MaArgs* args, const int* keys, int n_keys, int item, int rank,
-                                         bool shared, int token, int kvh, int col) {
+template <typename T, int D, bool kTree, bool kShared>
+__device__ __noinline__ float ma_bad_sum(const MaArgs* args, const int* keys, int n_keys, int item, int rank, int token,
+                                         int kvh, int col) {
   const MaArgs& p = *args;
-  const MaItem it = shared ? ma_item<kTree, true>(p, item, rank) : ma_item<kTree, false>(p, item, rank);
+  const MaItem it = ma_item<kTree, kShared>(p, item, rank);
   const bool all = n_keys > kMaBad;  // more than were remembered: look at every key of this CTA
   const int n = all ? it.x1 - it.x0 : n_keys;
   float sum = 0.f;
+#pragma unroll 1
   for (int j = 0; j < n; ++j) {
     const int x = it.x0 + j;
     const int key = !all ? keys[j] : x < it.sink_x ? x : x + it.shift;
@@ -327,8 +355,8 @@ __global__ void __launch_bounds__(kMaThreads, 1)
   S& s = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // a cluster of `split` CTAs works on one item; without a split a CTA takes items with the grid's stride
-  const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
-  const int first = p.split > 1 ? blockIdx.x / p.split : blockIdx.x;
+  const int rank = blockIdx.x & (p.split - 1);
+  const int first = blockIdx.x >> p.split_log;
   const int stride = p.split > 1 ? p.n_items : gridDim.x;
 
   if (threadIdx.x == 0) {
@@ -429,19 +457,20 @@ __global__ void __launch_bounds__(kMaThreads, 1)
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
       if (!ok) break;
       ++nq;
-      int row = lookup(0);
-      ok = load(&tmap_k, 0, row, it.kvh);
-      if (!kShared && it.second) ok = ok && load(&tmap_k, 0, row, it.kvh + 1);
-      for (int t = 0; ok && t < it.nt; ++t) {
-        const bool more = t + 1 < it.nt;
-        const int next = more ? lookup(t + 1) : oob;
-        ok = load(&tmap_v, t, row, it.kvh);
-        if (more) ok = ok && load(&tmap_k, t + 1, next, it.kvh);
-        if (!kShared && it.second) {
-          ok = ok && load(&tmap_v, t, row, it.kvh + 1);
-          if (more) ok = ok && load(&tmap_k, t + 1, next, it.kvh + 1);
+      // K of the first tile, then V of tile t and K of the next one, for each stream of its own tiles
+      int row = oob, next = lookup(0);
+      const int streams = !kShared && it.second ? 2 : 1;
+#pragma unroll 1
+      for (int t = -1; ok && t < it.nt; ++t) {
+        const int after = t + 2 < it.nt ? lookup(t + 2) : oob;  // ahead of the wait for a free stage
+#pragma unroll 1
+        for (int n = t < 0 ? 1 : 0; ok && n < 2 * streams; ++n) {
+          const bool k = n & 1;
+          if (t < 0 && !k) continue;
+          if (!k || t + 1 < it.nt) ok = load(k ? &tmap_k : &tmap_v, k ? t + 1 : t, k ? next : row, it.kvh + (n >> 1));
         }
         row = next;
+        next = after;
       }
     }
     // Every load issued here has landed before the CTA may exit.
@@ -490,47 +519,26 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         ok = ma_wait(&s.q_full, nq & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
         ++nq;
         const int streams = it.second ? 2 : 1;
-        if (kShared) {
-          if (!ok || !(ok = full(ring))) break;
-          for (int st = 0; st < streams; ++st) issue_s(st, ring);
-          tc_commit(&s.empty[ring % kStages]);
-          if (it.nt == 1) tc_commit(&s.q_empty);
-          for (int t = 0; ok && t < it.nt; ++t) {
-            const int rv = ring + 1 + 2 * t, rk = rv + 1;
-            const bool more = t + 1 < it.nt;
-            for (int st = 0; ok && st < streams; ++st) {
-              ok = issue_o(st, rv, t, !more) && (!more || full(rk));
-              if (ok && st == streams - 1) tc_commit(&s.empty[rv % kStages]);
-              if (ok && more) issue_s(st, rk);
-            }
-            if (ok && more) {
-              tc_commit(&s.empty[rk % kStages]);
-              if (t + 2 == it.nt) tc_commit(&s.q_empty);
-            }
-          }
-          ring += 2 * it.nt;
-        } else {
+        // S of the first tile, then O of tile t and S of the next one, for each stream
+#pragma unroll 1
+        for (int t = -1; ok && t < it.nt; ++t) {
+          const bool more = t + 1 < it.nt;
+#pragma unroll 1
           for (int st = 0; ok && st < streams; ++st) {
-            if (!(ok = full(ring))) break;
-            issue_s(st, ring);
-            tc_commit(&s.empty[ring % kStages]);
-            ++ring;
-          }
-          if (ok && it.nt == 1) tc_commit(&s.q_empty);
-          for (int t = 0; ok && t < it.nt; ++t) {
-            const bool more = t + 1 < it.nt;
-            for (int st = 0; ok && st < streams; ++st) {
-              if (!(ok = issue_o(st, ring, t, !more))) break;
-              tc_commit(&s.empty[ring % kStages]);
-              ++ring;
-              if (!more) continue;
-              if (!(ok = full(ring))) break;
-              issue_s(st, ring);
-              tc_commit(&s.empty[ring % kStages]);
-              ++ring;
+            const bool last = !kShared || st == streams - 1;  // of those that read these tiles
+            const int rv = ring, rk = t >= 0 ? ring + 1 : ring;
+            if (t >= 0) {
+              if (!(ok = issue_o(st, rv, t, !more))) break;
+              if (last) tc_commit(&s.empty[rv % kStages]);
             }
-            if (ok && t + 2 == it.nt) tc_commit(&s.q_empty);
+            if (more) {
+              if (!(ok = full(rk))) break;
+              issue_s(st, rk);
+              if (last) tc_commit(&s.empty[rk % kStages]);
+            }
+            if (last) ring += (t >= 0) + more;
           }
+          if (ok && t + 2 == it.nt) tc_commit(&s.q_empty);  // the last S of the item has been issued
         }
       }
       tc_commit(&s.mma_done);  // arrives once every MMA issued above has completed
@@ -576,17 +584,19 @@ __global__ void __launch_bounds__(kMaThreads, 1)
           for (int w = 0; w < 4; ++w) seen[w] = row_ok ? ma_low(min(it.prefix, it.x1) - xt, w) : 0u;
           if (part && row_ok) {
             const uint8_t* mask = p.mask + (it.start + token) * p.ld_mask;
-            const int j0 = xt - it.prefix, j1 = min(it.n, it.x1 - it.prefix);
-#pragma unroll
+            const int j1 = min(it.n, it.x1 - it.prefix);
+#pragma unroll 1
             for (int w = 0; w < 4; ++w) {
-              if (j0 + w * 32 + 32 <= 0 || j0 + w * 32 >= j1) continue;
+              const int j0 = xt - it.prefix + w * 32;
+              if (j0 + 32 <= 0 || j0 >= j1) continue;
               uint32_t bits = 0;
 #pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                const int j = j0 + w * 32 + c;
-                if (j >= 0 && j < j1 && mask[j]) bits |= 1u << c;
-              }
-              seen[w] |= bits;
+              for (int c = 0; c < 32; ++c)
+                if (j0 + c >= 0 && j0 + c < j1 && mask[j0 + c]) bits |= 1u << c;
+              seen[0] |= w == 0 ? bits : 0u;
+              seen[1] |= w == 1 ? bits : 0u;
+              seen[2] |= w == 2 ? bits : 0u;
+              seen[3] |= w == 3 ? bits : 0u;
             }
           }
         } else {
@@ -612,32 +622,33 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         // its next writers wait for an S that follows this thread's next arrival.
         if (t == 0 && st == owner && r == 0) s.n_bad[(item_no + 1) % 3][owner] = 0;
         if (warp_on) {
-          // The row is read twice, 32 columns at a time: its maximum, then the exponentials. (Held in
-          // registers, its 128 scores spilled.)
+          // The row is read twice, 32 columns at a time and the next ones ahead: its maximum, then the exponentials.
+          // (Held in registers, its 128 scores spilled; and the loops stay rolled for the sake of short calls.)
           const bool masked = __any_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu);
-          uint32_t v[2][32];
+          uint32_t va[32], vb[32];
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          tmem_ld_x32(s_tm, v[0]);
+          tmem_ld_x32(s_tm, va);
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            ma_tmem_wait_ld(va);
+            tmem_ld_x32(s_tm + h * 64 + 32, vb);
+            if (masked) ma_hide(va, h ? seen[2] : seen[0]);
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            ma_tmem_wait_ld(v[h & 1]);
-            if (h < 3) tmem_ld_x32(s_tm + (h + 1) * 32, v[(h + 1) & 1]);
-            if (masked) {
+            for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(va[c]));
+            ma_tmem_wait_ld(vb);
+            tmem_ld_x32(s_tm + (h ? 0 : 64), va);  // at the end: the first columns again
+            if (masked) ma_hide(vb, h ? seen[3] : seen[1]);
 #pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (!(seen[h] & (1u << c))) v[h & 1][c] = 0xff800000u;  // minus infinity
-            }
-#pragma unroll
-            for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(v[h & 1][c]));
+            for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(vb[c]));
           }
-          tmem_ld_x32(s_tm, v[0]);
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c2;
           const bool move = t == 0 || top > m + kMaSlack;
           const float m_new = move ? top : m;
           if (t > 0 && __any_sync(0xffffffffu, move)) {
             const float alpha = !move ? 1.f : m == -INFINITY ? 0.f : ma_exp2(m - m_new);
             l *= alpha;
-#pragma unroll
+            ma_tmem_wait_ld(va);
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
               tmem_ld_x32(o_tm + c * 32, o);
@@ -651,27 +662,20 @@ __global__ void __launch_bounds__(kMaThreads, 1)
           m = m_new;
           const float add = m == -INFINITY ? 0.f : kMaShift - m;
           float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            uint32_t(&x)[32] = v[h & 1];
-            ma_tmem_wait_ld(x);
-            if (h < 3) tmem_ld_x32(s_tm + (h + 1) * 32, v[(h + 1) & 1]);
-            if (masked) {
-#pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (!(seen[h] & (1u << c))) x[c] = 0xff800000u;
-            }
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            // P goes over columns of S that have been read
             uint32_t pk[16];
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const float p0 = ma_exp2(fmaf(__uint_as_float(x[2 * c]), p.c2, add));
-              const float p1 = ma_exp2(fmaf(__uint_as_float(x[2 * c + 1]), p.c2, add));
-              ls[(2 * c) & 3] += p0;
-              ls[(2 * c + 1) & 3] += p1;
-              pk[c] = MaType<T>::pack(p0, p1);
-            }
-            // P goes over columns of S that have been read: 16 h + 16 <= 32 h + 32
-            ma_tmem_st_x16(s_tm + h * 16, pk);
+            ma_tmem_wait_ld(va);
+            tmem_ld_x32(s_tm + h * 64 + 32, vb);
+            if (masked) ma_hide(va, h ? seen[2] : seen[0]);
+            ma_exp_pack<T>(va, p.c2, add, ls, pk);
+            ma_tmem_st_x16(s_tm + h * 32, pk);
+            ma_tmem_wait_ld(vb);
+            if (h == 0) tmem_ld_x32(s_tm + 64, va);
+            if (masked) ma_hide(vb, h ? seen[3] : seen[1]);
+            ma_exp_pack<T>(vb, p.c2, add, ls, pk);
+            ma_tmem_st_x16(s_tm + h * 32 + 16, pk);
           }
           l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
           ma_tmem_wait_st();
@@ -709,7 +713,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         float* const stage = reinterpret_cast<float*>(s.kv) + (size_t)(st * kMaTile + r) * D;
         T* const dst = static_cast<T*>(p.out) + (it.start + token) * p.ld_out +
                        (long long)(kvh * p.G + row_head) * D;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           if (it.nt > 0) {
@@ -738,8 +742,9 @@ __global__ void __launch_bounds__(kMaThreads, 1)
           }
         }
         if (n_bad > 0 && row_ok && l != 0.f) {
+#pragma unroll 1
           for (int d = 0; d < D; ++d) {
-            const float x = ma_bad_sum<T, D, kTree>(&p, s.bad[list][owner], n_bad, i, rank, kShared, token, kvh, d);
+            const float x = ma_bad_sum<T, D, kTree, kShared>(&p, s.bad[list][owner], n_bad, i, rank, token, kvh, d);
             if (x == 0.f) continue;
             if (p.split > 1)
               stage[(((d >> 2) ^ (r & 7)) << 2) + (d & 3)] += x;
@@ -780,24 +785,28 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         const float* base = reinterpret_cast<const float*>(s.kv);
         const float2* ml = reinterpret_cast<const float2*>(base + 2 * kMaTile * D) + st * kMaTile + r;
         const float* o = base + (size_t)(st * kMaTile + r) * D + ((col ^ (r & 7)) << 2);
-        float top = -INFINITY;
-        for (int j = 0; j < p.split; ++j) {
-          const float2 x = ma_ld_cluster2(cluster_map(ml, j));
-          top = x.x > top || x.x != x.x ? x.x : top;
+        float2 part[kMaMaxSplit];
+        float4 v[kMaMaxSplit];
+#pragma unroll
+        for (int j = 0; j < kMaMaxSplit; ++j) {  // all on their way at once; the last CTA's again where there are fewer
+          part[j] = ma_ld_cluster2(cluster_map(ml, min(j, p.split - 1)));
+          v[j] = ma_ld_cluster(cluster_map(o, min(j, p.split - 1)));
         }
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kMaMaxSplit; ++j) top = part[j].x > top || part[j].x != part[j].x ? part[j].x : top;
         if (top == -INFINITY) top = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float l = 0.f;
-        for (int j = 0; j < p.split; ++j) {
-          const float2 x = ma_ld_cluster2(cluster_map(ml, j));
-          const float4 v = ma_ld_cluster(cluster_map(o, j));
-          if (x.y == 0.f) continue;  // no key of this part is seen: its sums were not written
-          const float f = ma_exp2(x.x - top);
-          l = fmaf(x.y, f, l);
-          acc.x = fmaf(v.x, f, acc.x);
-          acc.y = fmaf(v.y, f, acc.y);
-          acc.z = fmaf(v.z, f, acc.z);
-          acc.w = fmaf(v.w, f, acc.w);
+#pragma unroll
+        for (int j = 0; j < kMaMaxSplit; ++j) {
+          if (j >= p.split || part[j].y == 0.f) continue;  // y 0: no key of this part is seen, its sums were not written
+          const float f = ma_exp2(part[j].x - top);
+          l = fmaf(part[j].y, f, l);
+          acc.x = fmaf(v[j].x, f, acc.x);
+          acc.y = fmaf(v[j].y, f, acc.y);
+          acc.z = fmaf(v[j].z, f, acc.z);
+          acc.w = fmaf(v[j].w, f, acc.w);
         }
         const float inv = l == 0.f ? 0.f : __frcp_rn(l);
         if (on) {
@@ -854,7 +863,20 @@ int launch(const char* what, MaArgs p, cudaStream_t st) {
   const int smem = (int)sizeof(MaSmem<D>) + 1024;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status(what);
+  // Clusters of the size with the least rounds of (tiles of a CTA + kMaFixed for a CTA's start and the join).
+  long long keys = (long long)p.max_blocks * p.block_size;  // the most that an item's rows may see
+  if (!kTree) keys = std::min(keys, (long long)p.window + p.sinks + 2 * p.tokens);
   const int sms = num_sms() > 0 ? num_sms() : 148;
+  p.split_log = 0;
+  long long least = 0;
+  for (int lg = 0; (1 << lg) <= kMaMaxSplit && (lg == 0 || p.n_items << (lg - 1) < sms); ++lg) {
+    const int fit = lg == 0 ? sms : max_active_clusters(reinterpret_cast<const void*>(kernel), smem, 1 << lg, kMaThreads);
+    if (fit <= 0) break;
+    const long long tiles = ((keys >> lg) + kMaTile - 1) / kMaTile;
+    const long long cost = (p.n_items + fit - 1) / fit * (tiles + kMaFixed);
+    if (lg == 0 || cost < least) least = cost, p.split_log = lg;
+  }
+  p.split = 1 << p.split_log;
   const int grid = p.split > 1 ? p.n_items * p.split : std::min(p.n_items, sms);
   return launch_pdl_cluster(what, kernel, dim3(grid), dim3(kMaThreads), (size_t)smem, st, (unsigned)p.split, tq, tk,
                             tv, p);
@@ -864,18 +886,14 @@ template <bool kTree>
 int run(const char* what, MaArgs p, int dtype, int D, float scale, cudaStream_t st) {
   p.c2 = scale * 1.4426950408889634f;
   p.tokens = kMaTile / p.G;
-  p.piece = kMaPiece;
-  while (p.block_size % p.piece) p.piece /= 2;
+  p.piece_log = kMaPieceLog;
+  while (p.block_size & ((1 << p.piece_log) - 1)) --p.piece_log;
+  p.piece = 1 << p.piece_log;
   const bool shared = p.max_q_len > p.tokens;
   p.levels = shared ? (p.max_q_len + 2 * p.tokens - 1) / (2 * p.tokens) : 1;
   const long long items = (long long)p.levels * p.B * (shared ? p.Hkv : (p.Hkv + 1) / 2);
   if (items >= (1ll << 27)) return fail(NPL_ERR_UNSUPPORTED, "%s: too many row tiles", what);
   p.n_items = (int)items;
-  const int sms = num_sms() > 0 ? num_sms() : 148;
-  long long keys = (long long)p.max_blocks * p.block_size;  // the most that a CTA's rows may see
-  if (!kTree) keys = std::min(keys, (long long)p.window + p.sinks + 2 * p.tokens);
-  p.split = 1;
-  while (p.split < 8 && items * p.split * 2 <= sms && keys >= p.split * 2 * kMaTile) p.split *= 2;
   if (dtype == NPL_F16) {
     if (D == 128)
       return shared ? launch<__half, 128, kTree, true>(what, p, st) : launch<__half, 128, kTree, false>(what, p, st);

@@ -22,6 +22,7 @@ from .fp8 import _call
 MAX_TOP = 32
 
 _DT = {torch.float32: L.NPL_F32, torch.float16: L.NPL_F16, torch.bfloat16: L.NPL_BF16}
+_empty = torch.empty_strided
 _token_logprobs = L.lib.npl_token_logprobs
 
 
@@ -55,23 +56,29 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0
     dt = _DT.get(logits.dtype)
     if dt is None:
         raise ValueError("logits must be one of float32, float16, bfloat16")
-    if logits.dim() == 0 or logits.shape[-1] == 0:
+    if logits.dim() == 0 or logits.size(-1) == 0:
         raise ValueError("logits need at least one column")
-    lead, v = logits.shape[:-1], logits.shape[-1]
+    shape = logits.shape
+    lead, v = shape[:-1], shape[-1]
     if token_ids.dtype is not torch.int64 or token_ids.shape != lead:
         raise ValueError("token_ids must be int64 with the shape of the logits without their last dimension")
     if not 0 <= top_k <= min(MAX_TOP, v):
         raise ValueError(f"top_k must be 0 to {MAX_TOP}, and no more than the vocabulary")
-    x = logits if logits.dim() == 2 else logits.reshape(-1, v)
-    n = x.shape[0]
-    if (v > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < v):
-        x = x.contiguous()
+    x = logits if len(shape) == 2 else logits.reshape(-1, v)
+    n, ld = (shape if len(shape) == 2 else x.shape)[0], v
+    if not x.is_contiguous():
+        ld, one = x.stride()
+        if (v > 1 and one != 1) or (n > 1 and ld < v):
+            x, ld = x.contiguous(), v
     ids = token_ids.contiguous()
     dev = logits.device
-    lp, entropy = torch.empty((2, *lead), dtype=torch.float32, device=dev).unbind(0)
-    top_ids = torch.empty((*lead, top_k), dtype=torch.int64, device=dev)
-    top_lp = torch.empty((*lead, top_k), dtype=torch.float32, device=dev)
+    lp, entropy = _empty((n,), (1,), dtype=torch.float32, device=dev), _empty((n,), (1,), dtype=torch.float32, device=dev)
+    top_ids = _empty((n, top_k), (top_k, 1), dtype=torch.int64, device=dev)
+    top_lp = _empty((n, top_k), (top_k, 1), dtype=torch.float32, device=dev)
     if n:
-        _call(_token_logprobs, dev, x.data_ptr(), dt, x.stride(0), n, v, ids.data_ptr(), top_k, lp.data_ptr(),
+        _call(_token_logprobs, dev, x.data_ptr(), dt, ld, n, v, ids.data_ptr(), top_k, lp.data_ptr(),
               entropy.data_ptr(), top_ids.data_ptr(), top_lp.data_ptr())
+    if len(shape) != 2:
+        lp, entropy = lp.view(lead), entropy.view(lead)
+        top_ids, top_lp = top_ids.view(*lead, top_k), top_lp.view(*lead, top_k)
     return TokenLogprobs(lp, entropy, top_ids, top_lp)

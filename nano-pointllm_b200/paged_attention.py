@@ -171,57 +171,74 @@ def _masked_arguments(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
                       context_lens: torch.Tensor, q_lens: torch.Tensor | None, q_offsets: torch.Tensor | None,
                       num_kv_groups: int, max_q_len: int | None, out: torch.Tensor | None,
                       mask: torch.Tensor | None = None):
-    """Checks what tree and window attention share. Returns (q, block_tables,
-    context_lens, q_lens, q_offsets, max_q_len, out) as the C entries read them."""
+    """Checks what tree and window attention share. Returns (the C entries'
+    leading arguments up to max_q_len, out and its stride, the tensors that
+    they point to). Few steps: a call on single tokens is bound by the host."""
     _same_device(q, k_cache, v_cache, block_tables, context_lens, q_lens, q_offsets, mask, out)
     dt = q.dtype
-    if dt not in _DT16:
+    code = _DT16.get(dt)
+    if code is None:
         raise ValueError("q must be float16 or bfloat16")
     if k_cache.dtype is not dt or v_cache.dtype is not dt:
         raise ValueError("KV caches must have the type of q")
-    if k_cache.shape != v_cache.shape or k_cache.dim() != 4:
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("KV caches must be [num_blocks, block_size, Hkv, D]")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("KV caches must be contiguous")
     if q.dim() != 3:
         raise ValueError("q must be [total_q, H, D]")
     total_q, h, d = q.shape
-    if k_cache.shape[3] != d or k_cache.shape[2] * num_kv_groups != h:
+    nb, bs, hkv, dk = shape
+    if dk != d or hkv * num_kv_groups != h:
         raise ValueError("q / KV cache head geometry mismatch")
     if block_tables.dtype is not torch.int32 or block_tables.dim() != 2:
         raise ValueError("block_tables must be int32 [B, max_blocks]")
-    b = block_tables.shape[0]
-    for name, t in (("context_lens", context_lens), ("q_lens", q_lens), ("q_offsets", q_offsets)):
-        if t is not None and (t.dtype is not torch.int32 or t.shape != (b,)):
-            raise ValueError(f"{name} must be int32 [B]")
-    if (q_lens is None) != (q_offsets is None):
-        raise ValueError("q_lens and q_offsets go together")
-    if q_lens is None and total_q != b:
-        raise ValueError("without q_lens every sequence has one token: q must be [B, H, D]")
-    if q.stride(2) != 1 or q.stride(1) != d or q.stride(0) % 8 or q.stride(0) < h * d or q.data_ptr() % 16:
-        q = q.contiguous()
-        if q.data_ptr() % 16:
-            q = q.clone()
-    if block_tables.stride(1) != 1 or block_tables.stride(0) < block_tables.shape[1]:
-        block_tables = block_tables.contiguous()
-    context_lens = context_lens.contiguous()
+    b, width = block_tables.shape
+    if context_lens.dtype is not torch.int32 or context_lens.dim() != 1 or context_lens.numel() != b:
+        raise ValueError("context_lens must be int32 [B]")
     if q_lens is None:
-        max_q_len = 1
+        if q_offsets is not None:
+            raise ValueError("q_lens and q_offsets go together")
+        if total_q != b:
+            raise ValueError("without q_lens every sequence has one token: q must be [B, H, D]")
+        max_q_len, lens, offsets = 1, None, None
     else:
+        if q_offsets is None:
+            raise ValueError("q_lens and q_offsets go together")
+        for name, t in (("q_lens", q_lens), ("q_offsets", q_offsets)):
+            if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != b:
+                raise ValueError(f"{name} must be int32 [B]")
         q_lens, q_offsets = q_lens.contiguous(), q_offsets.contiguous()
         if max_q_len is None:
             max_q_len = int(q_lens.max().item()) if b else 0
+        lens, offsets = q_lens.data_ptr(), q_offsets.data_ptr()
+    if not q.is_contiguous():
+        ld, step, one = q.stride()
+        if one != 1 or step != d or ld % 8 or ld < h * d:
+            q = q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    if not block_tables.is_contiguous():
+        ld, one = block_tables.stride()
+        if one != 1 or ld < width:
+            block_tables = block_tables.contiguous()
+    context_lens = context_lens.contiguous()
     if out is None:
-        out = torch.empty((total_q, h, d), dtype=dt, device=q.device)
+        ld_out = h * d
+        out = torch.empty_strided((total_q, h, d), (ld_out, d, 1), dtype=dt, device=q.device)
     else:
         if out.shape != (total_q, h, d) or out.dtype is not dt:
             raise ValueError("out must have the shape and type of q")
-        if out.numel() and (out.stride(2) != 1 or out.stride(1) != d or out.stride(0) % 8 or out.stride(0) < h * d
-                            or out.data_ptr() % 16):
+        ld_out, step, one = out.stride()
+        if out.numel() and (one != 1 or step != d or ld_out % 8 or ld_out < h * d or out.data_ptr() % 16):
             raise ValueError("out needs contiguous heads and tokens on 16-byte boundaries that do not overlap")
         if _overlap(out, q, k_cache, v_cache):
             raise ValueError("out may not overlap q or the caches")
-    return q, block_tables, context_lens, q_lens, q_offsets, int(max_q_len), out
+    args = (q.data_ptr(), code, q.stride(0), total_q, h, hkv, d, k_cache.data_ptr(), v_cache.data_ptr(), nb, bs,
+            block_tables.data_ptr(), block_tables.stride(0), width, context_lens.data_ptr(), lens, offsets, b,
+            max_q_len)
+    return args, out, ld_out, (q, block_tables, context_lens, q_lens, q_offsets)
 
 
 def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -244,21 +261,17 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError("tree_mask must be bool or uint8")
     if q_lens is None or q_offsets is None:
         raise ValueError("tree attention needs q_lens and q_offsets")
-    q, block_tables, context_lens, q_lens, q_offsets, most, out = _masked_arguments(
-        q, k_cache, v_cache, block_tables, context_lens, q_lens, q_offsets, num_kv_groups, max_q_len, out, tree_mask)
-    total_q, h, d = q.shape
+    args, out, ld_out, _held = _masked_arguments(q, k_cache, v_cache, block_tables, context_lens, q_lens, q_offsets,
+                                                 num_kv_groups, max_q_len, out, tree_mask)
+    total_q, most = args[3], args[-1]
     if tree_mask.dim() != 2 or tree_mask.shape[0] != total_q or tree_mask.shape[1] < most:
         raise ValueError("tree_mask must be [total_q, at least max_q_len]")
-    if tree_mask.stride(1) != 1 or tree_mask.stride(0) < tree_mask.shape[1]:
+    cols = tree_mask.shape[1]
+    if tree_mask.stride(1) != 1 or tree_mask.stride(0) < cols:
         tree_mask = tree_mask.contiguous()
-    if total_q == 0 or most == 0 or block_tables.shape[0] == 0:
-        return out
-    nb, bs, hkv, _ = k_cache.shape
-    _call(_tree_attention, q.device, q.data_ptr(), _DT16[q.dtype], q.stride(0), total_q, h, hkv, d,
-          k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, block_tables.data_ptr(), block_tables.stride(0),
-          block_tables.shape[1], context_lens.data_ptr(), q_lens.data_ptr(), q_offsets.data_ptr(),
-          block_tables.shape[0], most, tree_mask.data_ptr(), tree_mask.stride(0), tree_mask.shape[1], float(scale),
-          out.data_ptr(), out.stride(0))
+    if total_q and most and args[-2]:
+        _call(_tree_attention, out.device, *args, tree_mask.data_ptr(), tree_mask.stride(0), cols, scale,
+              out.data_ptr(), ld_out)
     return out
 
 
@@ -303,14 +316,8 @@ def paged_window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     q_lens) avoids reading q_lens back to the host."""
     if not 1 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31:
         raise ValueError("window must be at least 1 and sinks at least 0, below 2^31")
-    q, block_tables, context_lens, q_lens, q_offsets, most, out = _masked_arguments(
-        q, k_cache, v_cache, block_tables, context_lens, q_lens, q_offsets, num_kv_groups, max_q_len, out)
-    total_q, h, d = q.shape
-    if total_q == 0 or most == 0 or block_tables.shape[0] == 0:
-        return out
-    nb, bs, hkv, _ = k_cache.shape
-    _call(_window_attention, q.device, q.data_ptr(), _DT16[q.dtype], q.stride(0), total_q, h, hkv, d,
-          k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, block_tables.data_ptr(), block_tables.stride(0),
-          block_tables.shape[1], context_lens.data_ptr(), L.ptr(q_lens), L.ptr(q_offsets), block_tables.shape[0],
-          most, int(window), int(sinks), float(scale), out.data_ptr(), out.stride(0))
+    args, out, ld_out, _held = _masked_arguments(q, k_cache, v_cache, block_tables, context_lens, q_lens, q_offsets,
+                                                 num_kv_groups, max_q_len, out)
+    if args[3] and args[-1] and args[-2]:
+        _call(_window_attention, out.device, *args, window, sinks, scale, out.data_ptr(), ld_out)
     return out

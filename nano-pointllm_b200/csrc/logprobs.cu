@@ -27,9 +27,11 @@ namespace npl {
 namespace {
 
 constexpr int kLpMaxTop = 32;
-constexpr int kLpThreads = 256;
-constexpr int kLpUnroll = 4;      // 16-byte words that a thread has in flight
-constexpr int kLpCandidates = 1024;
+constexpr int kLpThreads = 128;
+constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kLpUnroll = 8;      // 16-byte words that a thread has in flight
+constexpr int kLpCandidates = 512;  // at least kLpMaxTop * (kLpMaxSplit + 1)
+constexpr int kLpRounds = 6;
 constexpr int kLpStep = 2048;     // logits that a CTA looks through at a time for equal ones
 constexpr int kLpMaxSplit = 8;    // CTAs of a cluster at most
 constexpr float kLpFar = -200.f;  // e^-200 is 0 in fp32: distances are cut here, so that 0 * infinity cannot arise
@@ -71,10 +73,20 @@ struct LpWord<float> {
     x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
   }
   __device__ static float one(float x) { return x; }
+  // logits below kFloor taken as kFloor: where the maximum is above kSlow, e^(x - m) is 0 either way
+  static constexpr float kSlow = -1e29f;
+  __device__ static void cut(uint4& w) {
+    w.x = __float_as_uint(fmaxf(__uint_as_float(w.x), -1e30f)), w.y = __float_as_uint(fmaxf(__uint_as_float(w.y), -1e30f));
+    w.z = __float_as_uint(fmaxf(__uint_as_float(w.z), -1e30f)), w.w = __float_as_uint(fmaxf(__uint_as_float(w.w), -1e30f));
+  }
 };
 template <typename H2>
 __device__ __forceinline__ H2 lp_as(uint32_t w) {
   return *reinterpret_cast<const H2*>(&w);
+}
+template <typename H2>
+__device__ __forceinline__ uint32_t lp_bits(H2 h) {
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <>
 struct LpWord<__half> {
@@ -94,6 +106,12 @@ struct LpWord<__half> {
     }
   }
   __device__ static float one(__half x) { return __half2float(x); }
+  static constexpr float kSlow = -65000.f;
+  __device__ static void cut(uint4& w) {
+    const __half2 least = __half2half2(__ushort_as_half(0xfbff));  // -65504
+    w.x = lp_bits(__hmax2(lp_as<__half2>(w.x), least)), w.y = lp_bits(__hmax2(lp_as<__half2>(w.y), least));
+    w.z = lp_bits(__hmax2(lp_as<__half2>(w.z), least)), w.w = lp_bits(__hmax2(lp_as<__half2>(w.w), least));
+  }
 };
 template <>
 struct LpWord<__nv_bfloat16> {
@@ -111,6 +129,12 @@ struct LpWord<__nv_bfloat16> {
       x[2 * i] = __uint_as_float(u[i] << 16), x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
   }
   __device__ static float one(__nv_bfloat16 x) { return __bfloat162float(x); }
+  static constexpr float kSlow = -1e29f;
+  __device__ static void cut(uint4& w) {
+    const __nv_bfloat162 least = __float2bfloat162_rn(-1e30f);
+    w.x = lp_bits(__hmax2(lp_as<__nv_bfloat162>(w.x), least)), w.y = lp_bits(__hmax2(lp_as<__nv_bfloat162>(w.y), least));
+    w.z = lp_bits(__hmax2(lp_as<__nv_bfloat162>(w.z), least)), w.w = lp_bits(__hmax2(lp_as<__nv_bfloat162>(w.w), least));
+  }
 };
 
 struct LpSum {  // of values seen so far: maximum, sum e^(x - m), sum (x - m) e^(x - m)
@@ -131,16 +155,49 @@ __device__ __forceinline__ void lp_add(LpSum& a, float x) {  // x <= a.m
   a.t = fmaf(d, e, a.t);
 }
 
+// Two sums at a time (one instruction for two fp32 numbers).
+__device__ __forceinline__ uint64_t lp_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 lp_unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t lp_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t lp_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t lp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float lp_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct LpSmem {
-  float red[3][kLpThreads / 32];
-  unsigned keys[kLpThreads];
+  float red[3][kLpWarps];
+  alignas(16) unsigned keys[kLpThreads];
   unsigned threshold;
-  int n_candidates, n_greater;
+  int n_candidates, n_list;
+  int list[kLpThreads];  // threads whose maximum reaches the threshold
   unsigned long long candidate[kLpCandidates];  // key << 32 | ~index: larger is better
   unsigned long long best[kLpMaxTop];           // of this CTA, best first
   LpSum sum;                                    // of this CTA
-  unsigned scan[kLpThreads / 32];
-  unsigned long long round[kLpThreads / 32];
+  unsigned scan[kLpWarps];
+  unsigned long long round[kLpWarps];
 };
 
 __device__ __forceinline__ unsigned long long lp_pack(unsigned key, int index) {
@@ -152,9 +209,13 @@ struct LpRow {  // this CTA's part of a row: words [w0, w1) of 16 bytes from `wo
   const T* x;
   const uint4* words;
   int head, w0, w1;  // logits before the first word; this CTA's words
-  int single;        // this thread's single logit, -1: none
+  int tail, n_tail;  // logits behind the last word, and how many of them are this CTA's
   bool first;        // the row's first part, to which the logits before the first word belong
   int end;           // one past this part's last logit
+  __device__ int single(int thread) const {  // the single logit of a thread, -1: none
+    if (first && thread < head) return thread;
+    return thread >= 32 && thread - 32 < n_tail ? tail + thread - 32 : -1;
+  }
 };
 
 template <typename T>
@@ -165,7 +226,8 @@ __device__ __forceinline__ float lp_at(const T* x, int i) {
 template <typename T, typename F>
 __device__ __forceinline__ void lp_each(const LpRow<T>& r, F&& f) {  // this thread's logits: f(value, index)
   constexpr int N = LpWord<T>::kN;
-  if (r.single >= 0) f(lp_at(r.x, r.single), r.single);
+  const int single = r.single(threadIdx.x);
+  if (single >= 0) f(lp_at(r.x, single), single);
   for (int w = r.w0 + (int)threadIdx.x; w < r.w1; w += kLpThreads) {
     float v[N];
     LpWord<T>::get(r.words[w], v);
@@ -180,32 +242,64 @@ __device__ void lp_top(LpSmem& s, const LpRow<T>& r, float own_max, bool any, in
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const unsigned own = any ? lp_key(own_max) : 0u;
   s.keys[tid] = own;
-  if (tid == 0) s.n_candidates = s.n_greater = 0;
+  if (tid == 0) s.n_candidates = s.n_list = 0;
   if (tid < kLpMaxTop) s.best[tid] = 0;
   __syncthreads();
-  if (warp == 0) {
-    // the largest threshold, of 20 leading bits, that k of the maxima reach (0 where fewer threads have any)
-    unsigned key[kLpThreads / 32], lo = 0;
-#pragma unroll
-    for (int i = 0; i < kLpThreads / 32; ++i) key[i] = s.keys[lane + i * 32];
-    for (int bit = 31; bit >= 12; --bit) {
-      const unsigned c = lo | (1u << bit);
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < kLpThreads / 32; ++i) n += key[i] >= c;
-      if (__reduce_add_sync(0xffffffffu, n) >= k) lo = c;
+  // The k-th largest of the maxima (1, below every logit's key, where fewer threads have any): few of them one below
+  // the other by a warp, 130 cycles each; from kLpRounds on every thread counts those above its own, 500 in all.
+  if (k >= kLpRounds) {
+    int above[4] = {0, 0, 0, 0}, from[4] = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int i = 0; i < kLpThreads; i += 4) {
+      const uint4 y = *reinterpret_cast<const uint4*>(&s.keys[i]);
+      above[0] += y.x > own, above[1] += y.y > own, above[2] += y.z > own, above[3] += y.w > own;
+      from[0] += y.x >= own, from[1] += y.y >= own, from[2] += y.z >= own, from[3] += y.w >= own;
     }
-    if (lane == 0) s.threshold = lo;
+    if (above[0] + above[1] + above[2] + above[3] < k && from[0] + from[1] + from[2] + from[3] >= k) s.threshold = max(own, 1u);  // those that are equal write the same
+  } else if (warp == 0) {
+    unsigned key[kLpWarps], last = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < kLpWarps; ++i) key[i] = s.keys[lane + i * 32];
+    for (int have = 0; have < k && last;) {
+      unsigned c = 0;
+#pragma unroll
+      for (int i = 0; i < kLpWarps; ++i) c = max(c, key[i]);
+      last = __reduce_max_sync(0xffffffffu, c);
+      int equal = 0;
+#pragma unroll
+      for (int i = 0; i < kLpWarps; ++i) {
+        equal += key[i] == last;
+        if (key[i] == last) key[i] = 0;
+      }
+      have += __reduce_add_sync(0xffffffffu, equal);
+    }
+    if (lane == 0) s.threshold = max(last, 1u);
   }
   __syncthreads();
-  const unsigned least = max(s.threshold, 1u);
-  if (own >= least) {
-    lp_each(r, [&](float x, int i) {
+  const unsigned least = s.threshold;
+  if (own >= least) s.list[atomicAdd(&s.n_list, 1)] = tid;
+  __syncthreads();
+  // a warp takes threads that reach it, a lane one of a thread's words (of few words: several threads at a time)
+  int per_log = 5;
+  while (per_log > 0 && (kLpThreads << (per_log - 1)) >= r.w1 - r.w0) --per_log;
+  const int at_once = 32 >> per_log;
+  for (int q = warp * at_once + (lane >> per_log); q < s.n_list; q += kLpWarps * at_once) {
+    const int who = s.list[q], first = lane & ((1 << per_log) - 1);
+    auto take = [&](float x, int i) {
       const unsigned key = lp_key(x);
       if (key < least) return;
       const int at = atomicAdd(&s.n_candidates, 1);
       if (at < kLpCandidates) s.candidate[at] = lp_pack(key, i);
-    });
+    };
+    if (first == 0 && r.single(who) >= 0) take(lp_at(r.x, r.single(who)), r.single(who));
+    for (int w = r.w0 + who + first * kLpThreads; w < r.w1; w += kLpThreads << per_log) {
+      const uint4 word = r.words[w];
+      if (lp_key(LpWord<T>::top(word)) < least) continue;
+      float v[LpWord<T>::kN];
+      LpWord<T>::get(word, v);
+#pragma unroll
+      for (int e = 0; e < LpWord<T>::kN; ++e) take(v[e], r.head + w * LpWord<T>::kN + e);
+    }
   }
   __syncthreads();
   int n = s.n_candidates;
@@ -226,7 +320,7 @@ __device__ void lp_top(LpSmem& s, const LpRow<T>& r, float own_max, bool any, in
       __syncthreads();
       c = 0;
 #pragma unroll
-      for (int i = 0; i < kLpThreads / 32; ++i) c = max(c, s.round[i]);
+      for (int i = 0; i < kLpWarps; ++i) c = max(c, s.round[i]);
       if (c == 0) break;  // this part holds no more logits
       const unsigned key = (unsigned)(c >> 32);
       int place = (int)~(unsigned)c;
@@ -243,7 +337,7 @@ __device__ void lp_top(LpSmem& s, const LpRow<T>& r, float own_max, bool any, in
         if (lane == 0) s.scan[warp] = next;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kLpThreads / 32; ++i) next = min(next, s.scan[i]);
+        for (int i = 0; i < kLpWarps; ++i) next = min(next, s.scan[i]);
         if (next == 0x7fffffffu) {
           base += kLpStep;
         } else {
@@ -261,7 +355,8 @@ __device__ void lp_top(LpSmem& s, const LpRow<T>& r, float own_max, bool any, in
   for (int i = tid; i < n; i += kLpThreads) {
     const unsigned long long mine = s.candidate[i];
     int better = 0;
-    for (int j = 0; j < n && better < k; ++j) better += s.candidate[j] > mine;
+    #pragma unroll 4
+    for (int j = 0; j < n; ++j) better += s.candidate[j] > mine;
     if (better < k) s.best[better] = mine;
   }
   __syncthreads();
@@ -279,7 +374,7 @@ __device__ __forceinline__ LpSum lp_ld_sum(const LpSum* p, int rank) {
 struct LpArgs {
   const void* logits;
   long long ld;
-  int vocab, top_k, split;
+  int vocab, top_k, split, split_log;
   const int64_t* ids;
   float* lp;
   float* entropy;
@@ -293,8 +388,8 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs p) {
   __shared__ LpSmem s;
   constexpr int N = LpWord<T>::kN;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
-  const long long row = p.split > 1 ? blockIdx.x / p.split : blockIdx.x;
+  const int rank = blockIdx.x & (p.split - 1);
+  const long long row = blockIdx.x >> p.split_log;
   pdl_wait();
   pdl_trigger();
   LpRow<T> r;
@@ -302,17 +397,16 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs p) {
   r.head = min(p.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(r.x) & 15)) & 15) / (int)sizeof(T));
   r.words = reinterpret_cast<const uint4*>(r.x + r.head);
   const int words = (p.vocab - r.head) / N;
-  r.w0 = (int)((long long)words * rank / p.split);
-  r.w1 = (int)((long long)words * (rank + 1) / p.split);
-  const int tail = r.head + words * N;  // the first logit behind the words
+  r.w0 = (int)(((long long)words * rank) >> p.split_log);
+  r.w1 = (int)(((long long)words * (rank + 1)) >> p.split_log);
   r.first = rank == 0;
+  r.tail = r.head + words * N;
+  r.n_tail = rank == p.split - 1 ? p.vocab - r.tail : 0;
   r.end = rank == p.split - 1 ? p.vocab : r.head + r.w1 * N;
-  r.single = -1;
-  if (rank == 0 && tid < r.head) r.single = tid;
-  if (rank == p.split - 1 && tid >= 32 && tid - 32 < p.vocab - tail) r.single = tail + tid - 32;
+  const int single = r.single(tid);
 
   LpSum a = {-INFINITY, 0.f, 0.f};
-  if (r.single >= 0) a = {lp_at(r.x, r.single), 1.f, 0.f};
+  if (single >= 0) a = {lp_at(r.x, single), 1.f, 0.f};
   if (a.m == -INFINITY) a.s = 0.f;
   for (int w = r.w0 + tid; w < r.w1; w += kLpThreads * kLpUnroll) {
     uint4 v[kLpUnroll];
@@ -325,12 +419,35 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs p) {
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u) m = lp_max_nan(m, LpWord<T>::top(v[u]));
     lp_move(a, m);
+    if (m > LpWord<T>::kSlow) {
+      const uint64_t from = lp_pair(-m, -m), scale = lp_pair(kLog2e, kLog2e);
+      uint64_t s2 = lp_pair(0.f, 0.f), t2 = s2;
 #pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u) {
-      float x[N];
-      LpWord<T>::get(v[u], x);
+      for (int u = 0; u < kLpUnroll; ++u) {
+        float x[N];
+        LpWord<T>::cut(v[u]);
+        LpWord<T>::get(v[u], x);
 #pragma unroll
-      for (int e = 0; e < N; ++e) lp_add(a, x[e]);
+        for (int e = 0; e < N; e += 2) {
+          const uint64_t d = lp_add2(lp_pair(x[e], x[e + 1]), from);
+          const float2 y = lp_unpair(lp_mul2(d, scale));
+          const uint64_t ex = lp_pair(lp_exp2(y.x), lp_exp2(y.y));
+          s2 = lp_add2(s2, ex);
+          t2 = lp_fma2(d, ex, t2);
+        }
+      }
+      const float2 s1 = lp_unpair(s2), t1 = lp_unpair(t2);
+      a.s += s1.x + s1.y;
+      a.t += t1.x + t1.y;
+    } else if (m != -INFINITY) {  // nothing but logits near the type's lowest value so far (or a NaN)
+#pragma unroll 1
+      for (int u = 0; u < kLpUnroll; ++u) {
+        if (w + u * kLpThreads >= r.w1) break;
+        float x[N];
+        LpWord<T>::get(r.words[w + u * kLpThreads], x);
+#pragma unroll
+        for (int e = 0; e < N; ++e) lp_add(a, x[e]);
+      }
     }
   }
 
@@ -343,7 +460,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs p) {
   __syncthreads();
   m = s.red[0][0];
 #pragma unroll
-  for (int i = 1; i < kLpThreads / 32; ++i) m = lp_max_nan(m, s.red[0][i]);
+  for (int i = 1; i < kLpWarps; ++i) m = lp_max_nan(m, s.red[0][i]);
   lp_move(a, m);
   a.s = warp_sum(a.s);
   a.t = warp_sum(a.t);
@@ -351,9 +468,9 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs p) {
   __syncthreads();
   a.s = a.t = 0.f;
 #pragma unroll
-  for (int i = 0; i < kLpThreads / 32; ++i) a.s += s.red[1][i], a.t += s.red[2][i];
+  for (int i = 0; i < kLpWarps; ++i) a.s += s.red[1][i], a.t += s.red[2][i];
 
-  if (p.top_k) lp_top(s, r, own_max, r.single >= 0 || r.w0 + tid < r.w1, p.top_k);
+  if (p.top_k) lp_top(s, r, own_max, single >= 0 || r.w0 + tid < r.w1, p.top_k);
 
   if (p.split > 1) {
     if (tid == 0) s.sum = a;
@@ -363,33 +480,42 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs p) {
       LpSum part[kLpMaxSplit];
       m = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < kLpMaxSplit; ++j) {
-        if (j >= p.split) break;
-        part[j] = lp_ld_sum(&s.sum, j);
+      for (int j = 0; j < kLpMaxSplit; ++j) {  // where there are fewer, the first ones again
+        part[j] = lp_ld_sum(&s.sum, j & (p.split - 1));
         m = lp_max_nan(m, part[j].m);
       }
       a = {m, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < kLpMaxSplit; ++j) {
-        if (j >= p.split) break;
         lp_move(part[j], m);
-        a.s += part[j].s, a.t += part[j].t;
+        if (j < p.split) a.s += part[j].s, a.t += part[j].t;
       }
-      const int n = p.split * p.top_k;  // at most kLpThreads
-      unsigned long long mine = 0;
-      if (tid < n) {
-        const uint32_t at = cluster_map(&s.best[tid % p.top_k], tid / p.top_k);
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(mine) : "r"(at) : "memory");
-        s.candidate[tid] = mine;
+      const int n = p.top_k ? p.split * kLpMaxTop : 0;
+      for (int i = tid; i < n; i += kLpThreads) {
+        const uint32_t at = cluster_map(&s.best[i & (kLpMaxTop - 1)], i / kLpMaxTop);
+        unsigned long long y;
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(y) : "r"(at) : "memory");
+        s.candidate[i] = y;
       }
       __syncthreads();
-      if (mine) {
+      for (int i = tid; i < n; i += kLpThreads) {
+        const unsigned long long mine = s.candidate[i];
+        if (mine == 0) continue;
+        // those above it, in each CTA's list (best first, empty places 0) by halving
         int better = 0;
-        for (int j = 0; j < n; ++j) better += s.candidate[j] > mine;
-        if (better < p.top_k) s.candidate[kLpThreads + better] = mine;
+#pragma unroll
+        for (int j = 0; j < kLpMaxSplit; ++j) {
+          const unsigned long long* list = s.candidate + (j & (p.split - 1)) * kLpMaxTop;
+          int above = 0;
+#pragma unroll
+          for (int step = kLpMaxTop / 2; step > 0; step /= 2) above += list[above + step - 1] > mine ? step : 0;
+          above += list[above] > mine;
+          better += j < p.split ? above : 0;
+        }
+        if (better < p.top_k) s.candidate[n + better] = mine;
       }
       __syncthreads();
-      if (tid < p.top_k) s.best[tid] = s.candidate[kLpThreads + tid];
+      if (tid < p.top_k) s.best[tid] = s.candidate[n + tid];
     }
     cluster_arrive_release();  // no CTA leaves while the first reads its shared memory
     cluster_wait_acquire();
@@ -415,10 +541,11 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs p) {
 template <typename T>
 int launch(const char* what, LpArgs p, long long rows, cudaStream_t st) {
   const int sms = num_sms() > 0 ? num_sms() : 148;
-  p.split = 1;
-  while (p.split < kLpMaxSplit && rows * p.split * 2 <= 4ll * sms &&
-         p.vocab >= p.split * 2 * kLpThreads * LpWord<T>::kN)
-    p.split *= 2;
+  p.split_log = 0;
+  while ((1 << p.split_log) < kLpMaxSplit && (rows << p.split_log) * 2 <= 4ll * sms &&
+         p.vocab >> p.split_log >= 2 * kLpThreads * LpWord<T>::kN)
+    ++p.split_log;
+  p.split = 1 << p.split_log;
   return launch_pdl_cluster(what, logprobs_kernel<T>, dim3((unsigned)(rows * p.split)), dim3(kLpThreads), 0, st,
                             (unsigned)p.split, p);
 }

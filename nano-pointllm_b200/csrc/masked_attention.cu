@@ -49,7 +49,6 @@ namespace {
 
 constexpr int kMaThreads = 384;
 constexpr int kMaTile = 128;
-constexpr uint32_t kMaTmemCols = 512;  // S of the streams at 0 and 128 (P over it), O at 256 and 384
 constexpr int kMaFixed = 4;             // what a CTA costs beside its tiles, in tiles
 constexpr int kMaBad = 32;             // keys with V elements that are not finite, remembered for an item
 constexpr int kMaPieceLog = 5;         // 32 keys of a piece at most
@@ -82,14 +81,7 @@ struct MaArgs {
   int* status;
 };
 
-template <int D>
-struct MaSmem {
-  static constexpr uint32_t kHalf = kMaTile * 128;  // 128 rows x 64 elements (one swizzle span)
-  static constexpr uint32_t kTileBytes = kMaTile * D * 2;
-  static constexpr int kStages = D == 128 ? 5 : 8;
-  alignas(1024) uint8_t q[2][kTileBytes];
-  alignas(1024) uint8_t kv[kStages][kTileBytes];  // K and V tiles in the order of their use; partial sums at the end
-  uint64_t full[kStages], empty[kStages];
+struct MaBarriers {
   uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], mma_done;
   uint32_t tmem_base;
   int abort;
@@ -97,7 +89,45 @@ struct MaSmem {
   int bad[3][2][kMaBad];  // keys whose V rows held elements that are not finite
 };
 
-static_assert(sizeof(MaSmem<128>) + 1024 <= 232448 && sizeof(MaSmem<64>) + 1024 <= 232448, "shared memory of an SM");
+template <int D>
+struct MaSmem : MaBarriers {
+  static constexpr bool kFew = false;
+  static constexpr int kRows = kMaTile;
+  static constexpr uint32_t kHalf = kMaTile * 128;  // 128 rows x 64 elements (one swizzle span)
+  static constexpr uint32_t kQHalf = kHalf;
+  static constexpr uint32_t kTileBytes = kMaTile * D * 2;
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  static constexpr uint32_t kScoreCols = 128, kOutCols = 128, kTmemCols = 512;  // S of the streams (P over it), then O
+  uint64_t full[kStages], empty[kStages];
+  alignas(1024) uint8_t q[2][kTileBytes];
+  alignas(1024) uint8_t kv[kStages][kTileBytes];  // K and V tiles in the order of their use; partial sums at the end
+};
+
+// Few rows, as the N side of the products.
+template <int D, int kN>
+struct MaFewSmem : MaBarriers {
+  static constexpr bool kFew = true;
+  static constexpr int kRows = kN;
+  static constexpr uint32_t kHalf = kMaTile * 128;
+  static constexpr uint32_t kQHalf = kN * 128;
+  static constexpr uint32_t kTileBytes = kMaTile * D * 2;
+  static constexpr int kStages = D == 64 ? 10 : kN == 64 ? 4 : 5;
+  static constexpr uint32_t kScoreCols = kN, kOutCols = 2 * kN;  // S of the streams, then O and the normalisers
+  static constexpr uint32_t kTmemCols = 8 * kN;
+  uint64_t full[kStages], empty[kStages];
+  alignas(16) float add[2][kN];  // of a row: 6 - m
+  float alpha[2][kN];            // what its sums are scaled with
+  float top[2][4][kN];           // a warp's maxima
+  float2 ml[2][kN];              // m and the normaliser at the end
+  alignas(1024) uint8_t ones[1024];
+  alignas(1024) uint8_t q[2][kN * D * 2];
+  alignas(1024) uint8_t p[2][kMaTile * 128];  // P^T: a key's rows in one 128-byte line
+  alignas(1024) uint8_t kv[kStages][kTileBytes];
+};
+
+static_assert(sizeof(MaSmem<128>) + 1024 <= 232448 && sizeof(MaSmem<64>) + 1024 <= 232448 &&
+                  sizeof(MaFewSmem<128, 64>) + 1024 <= 232448 && sizeof(MaFewSmem<64, 64>) + 1024 <= 232448,
+              "shared memory of an SM");
 
 template <typename T>
 struct MaType;
@@ -111,6 +141,7 @@ struct MaType<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   __device__ static float get(const void* p, size_t i) { return __half2float(static_cast<const __half*>(p)[i]); }
+  __device__ static void put(__half* p, float x) { *p = __float2half_rn(x); }
   __device__ static void add(__half* p, float x) { *p = __float2half_rn(__half2float(*p) + x); }
 };
 template <>
@@ -125,6 +156,7 @@ struct MaType<__nv_bfloat16> {
   __device__ static float get(const void* p, size_t i) {
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
   }
+  __device__ static void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
   __device__ static void add(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(__bfloat162float(*p) + x); }
 };
 
@@ -297,7 +329,7 @@ __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) 
   uint32_t any = 0;
 #pragma unroll 1
   for (int hf = 0; hf < D / 64; ++hf) {
-    uint4* line = reinterpret_cast<uint4*>(tile + hf * MaSmem<D>::kHalf + row * 128);
+    uint4* line = reinterpret_cast<uint4*>(tile + hf * (kMaTile * 128) + row * 128);
     if (!seen) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) line[c] = make_uint4(0, 0, 0, 0);
@@ -313,7 +345,7 @@ __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) 
   if (!(any & 0x80008000u)) return false;
 #pragma unroll 1
   for (int c = 0; c < D / 2; ++c) {
-    uint32_t* w = reinterpret_cast<uint32_t*>(tile + (c >> 5) * MaSmem<D>::kHalf + row * 128) + (c & 31);
+    uint32_t* w = reinterpret_cast<uint32_t*>(tile + (c >> 5) * (kMaTile * 128) + row * 128) + (c & 31);
     const uint32_t t = ((*w & MaType<T>::kExp) + MaType<T>::kOne) & 0x80008000u;
     *w &= ~((t >> 15) * 0xffffu);
   }
@@ -345,20 +377,219 @@ __device__ __noinline__ float ma_bad_sum(const MaArgs* args, const int* keys, in
   return sum;
 }
 
-template <typename T, int D, bool kTree, bool kShared>
-__global__ void __launch_bounds__(kMaThreads, 1)
-    masked_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ MaArgs p) {
-  using S = MaSmem<D>;
-  constexpr int kStages = S::kStages;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  S& s = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // a cluster of `split` CTAs works on one item; without a split a CTA takes items with the grid's stride
-  const int rank = blockIdx.x & (p.split - 1);
-  const int first = blockIdx.x >> p.split_log;
-  const int stride = p.split > 1 ? p.n_items : gridDim.x;
+// Barriers among the 128 threads of a stream.
+__device__ __forceinline__ void ma_stream_sync(int st) {
+  if (st == 0)
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+  else
+    asm volatile("bar.sync 2, 128;" ::: "memory");
+}
+__device__ __forceinline__ bool ma_stream_any(int st, bool x) {
+  int r;
+  if (st == 0)
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\t"
+                 "selp.s32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((int)x) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, 2, 128, p;\n\t"
+                 "selp.s32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((int)x) : "memory");
+  return r != 0;
+}
 
+__device__ __forceinline__ float ma_warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// 16 columns of this lane from TMEM.
+__device__ __forceinline__ void ma_tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Warp 8: loads by TMA. Lane i looks up and loads piece i of a tile.
+template <typename S, int D, bool kTree, bool kShared>
+__device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtensorMap& tmap_q, const CUtensorMap& tmap_k,
+                                             const CUtensorMap& tmap_v, int first, int stride, int rank) {
+  constexpr int kStages = S::kStages;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) {
+    prefetch_tensormap(&tmap_q);
+    prefetch_tensormap(&tmap_k);
+    prefetch_tensormap(&tmap_v);
+  }
+  const uint64_t pol_q = policy_evict_first();
+  const uint64_t pol_kv = policy_evict_normal();
+  const int oob = p.num_blocks * p.block_size;
+  const int per_tile = kMaTile / p.piece;
+  int nq = 0, ring = 0;  // Q loads and K / V tiles issued
+  bool ok = true;
+  for (int i = first; ok && i < p.n_items; i += stride) {
+    const MaItem it = ma_item<kTree, kShared>(p, i, rank);
+    if (it.skip) {
+      if (lane == 0 && it.tok0 < it.n) atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
+      continue;
+    }
+    if (lane == 0 && (it.ctx < 0 || (it.prefix < 0 && it.ctx != 0) ||
+                      (long long)it.ctx > (long long)p.max_blocks * p.block_size))
+      atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
+    if (it.nt == 0) continue;
+    const int32_t* table = p.bt + it.b * p.bt_stride;
+    // the pool row of this lane's piece of tile t (zeros where its page is none of the pool)
+    auto lookup = [&](int t) -> int {
+      const int x = it.x0 + t * kMaTile + lane * p.piece;
+      if (lane >= per_tile || x >= it.x1) return oob;
+      const int key = x < it.sink_x ? x : x + it.shift;
+      const int page = key / p.block_size;
+      const int blk = page < p.max_blocks ? table[page] : -1;
+      if (blk < 0 || blk >= p.num_blocks) {
+        atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
+        return oob;
+      }
+      return blk * p.block_size + (key - page * p.block_size);
+    };
+    auto load = [&](const CUtensorMap* map, int t, int row, int kvh) -> bool {
+      const int st = ring % kStages;
+      bool go = true;
+      const int n = min(per_tile, (it.x1 - it.x0 - t * kMaTile) / p.piece);
+      if (lane == 0) {
+        go = ma_wait(&s.empty[st], ((ring / kStages) & 1) ^ 1, &s.abort, p.status, NPL_DEV_TIMEOUT_TMA);
+        if (go) mbar_arrive_expect_tx(&s.full[st], n * p.piece * D * 2);
+      }
+      go = __shfl_sync(0xffffffffu, (int)go, 0);
+      if (!go) return false;
+      if (lane < n) {
+#pragma unroll
+        for (int hf = 0; hf < D / 64; ++hf)
+          tma_load_3d(s.kv[st] + hf * S::kHalf + lane * p.piece * 128, map, hf * 64, kvh, row, &s.full[st], pol_kv);
+      }
+      ++ring;
+      return true;
+    };
+    if (lane == 0) {
+      ok = nq == 0 || ma_wait(&s.q_empty, (nq - 1) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_TMA);
+      if (ok) {
+        mbar_arrive_expect_tx(&s.q_full, (it.second ? 2 : 1) * p.tokens * p.G * D * 2);
+        for (int q = 0; q < (it.second ? 2 : 1); ++q)
+#pragma unroll
+          for (int hf = 0; hf < D / 64; ++hf)
+            tma_load_3d(s.q[q] + hf * S::kQHalf, &tmap_q, hf * 64, (it.kvh + (kShared ? 0 : q)) * p.G,
+                        it.start + it.tok0 + (kShared ? q * p.tokens : 0), &s.q_full, pol_q);
+      }
+    }
+    ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+    if (!ok) break;
+    ++nq;
+    // K of the first tile, then V of tile t and K of the next one, for each stream of its own tiles
+    int row = oob, next = lookup(0);
+    const int streams = !kShared && it.second ? 2 : 1;
+#pragma unroll 1
+    for (int t = -1; ok && t < it.nt; ++t) {
+      const int after = t + 2 < it.nt ? lookup(t + 2) : oob;  // ahead of the wait for a free stage
+#pragma unroll 1
+      for (int n = t < 0 ? 1 : 0; ok && n < 2 * streams; ++n) {
+        const bool k = n & 1;
+        if (t < 0 && !k) continue;
+        if (!k || t + 1 < it.nt) ok = load(k ? &tmap_k : &tmap_v, k ? t + 1 : t, k ? next : row, it.kvh + (n >> 1));
+      }
+      row = next;
+      next = after;
+    }
+  }
+  // Every load issued here has landed before the CTA may exit.
+  if (lane == 0) {
+    if (nq > 0) mbar_wait(&s.q_full, (nq - 1) & 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+    for (int j = max(0, ring - kStages); j < ring; ++j)
+      mbar_wait(&s.full[j % kStages], (j / kStages) & 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+  }
+  __syncwarp();
+}
+
+// Warp 9, one thread: matrix products.
+template <typename S, typename T, int D, bool kTree, bool kShared>
+__device__ __forceinline__ void ma_mma_role(S& s, const MaArgs& p, uint32_t tmem, int first, int stride, int rank) {
+  constexpr int kStages = S::kStages;
+  // rows as M: S = Q K^T, O = P V with P in TMEM; rows as N: S^T = K Q^T, O^T = V^T P^T with P^T in shared memory (for
+  // D = 64 the rows of O^T come twice, the second time to lanes that nobody reads)
+  constexpr uint32_t kIdQK = idesc_f16(kMaTile, S::kFew ? S::kRows : kMaTile, false) | MaType<T>::kIdesc;
+  constexpr uint32_t kIdPV =
+      idesc_f16(kMaTile, S::kFew ? S::kRows : D, true) | (S::kFew ? 1u << 15 : 0u) | MaType<T>::kIdesc;
+  int ring = 0, nq = 0;
+  uint32_t p_phase[2] = {0, 0};
+  auto full = [&](int r) -> bool {
+    return ma_wait(&s.full[r % kStages], (r / kStages) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
+  };
+  auto issue_s = [&](int st, int r) {  // S of stream st from the K tile at ring position r
+    const uint32_t qa = smem_u32(s.q[st]), ka = smem_u32(s.kv[r % kStages]);
+    tc_fence_after();
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const uint64_t qd = sdesc_k_sw128(qa + (kk >> 2) * S::kQHalf + (kk & 3) * 32);
+      const uint64_t kd = sdesc_k_sw128(ka + (kk >> 2) * S::kHalf + (kk & 3) * 32);
+      mma_f16(tmem + st * S::kScoreCols, S::kFew ? kd : qd, S::kFew ? qd : kd, kIdQK, kk > 0 ? 1u : 0u);
+    }
+    tc_commit(&s.s_full[st]);
+  };
+  auto issue_o = [&](int st, int r, int t, bool last) -> bool {  // O of stream st (+)= P V
+    if (!ma_wait(&s.p_full[st], p_phase[st], &s.abort, p.status, NPL_DEV_TIMEOUT_MMA) || !full(r)) return false;
+    p_phase[st] ^= 1;
+    tc_fence_after();
+    const uint32_t va = smem_u32(s.kv[r % kStages]);
+#pragma unroll
+    for (int kk = 0; kk < kMaTile / 16; ++kk) {
+      const uint64_t vd = sdesc_mn_sw128(va + kk * 16 * 128, S::kFew && D == 64 ? 0 : S::kHalf, 1024);
+      const uint32_t o = tmem + 2 * S::kScoreCols + st * S::kOutCols, on = (t > 0 || kk > 0) ? 1u : 0u;
+      if constexpr (S::kFew) {
+        const uint64_t pd = sdesc_mn_sw128(smem_u32(s.p[st]) + kk * 16 * 128, 0, 1024);
+        mma_f16(o, vd, pd, kIdPV, on);
+        mma_f16(o + S::kRows, sdesc_mn_sw128(smem_u32(s.ones), 0, 0), pd, kIdPV, on);  // each lane: the sums of P
+      } else
+        ma_mma_ts(o, tmem + st * S::kScoreCols + kk * 8, vd, kIdPV, on);
+    }
+    if (last) tc_commit(&s.o_full[st]);
+    return true;
+  };
+  bool ok = true;
+  for (int i = first; ok && i < p.n_items; i += stride) {
+    const MaItem it = ma_item<kTree, kShared>(p, i, rank);
+    if (it.nt == 0) continue;
+    ok = ma_wait(&s.q_full, nq & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
+    ++nq;
+    const int streams = it.second ? 2 : 1;
+    // S of the first tile, then O of tile t and S of the next one, for each stream
+#pragma unroll 1
+    for (int t = -1; ok && t < it.nt; ++t) {
+      const bool more = t + 1 < it.nt;
+#pragma unroll 1
+      for (int st = 0; ok && st < streams; ++st) {
+        const bool last = !kShared || st == streams - 1;  // of those that read these tiles
+        const int rv = ring, rk = t >= 0 ? ring + 1 : ring;
+        if (t >= 0) {
+          if (!(ok = issue_o(st, rv, t, !more))) break;
+          if (last) tc_commit(&s.empty[rv % kStages]);
+        }
+        if (more) {
+          if (!(ok = full(rk))) break;
+          issue_s(st, rk);
+          if (last) tc_commit(&s.empty[rk % kStages]);
+        }
+        if (last) ring += (t >= 0) + more;
+      }
+      if (ok && t + 2 == it.nt) tc_commit(&s.q_empty);  // the last S of the item has been issued
+    }
+  }
+  tc_commit(&s.mma_done);  // arrives once every MMA issued above has completed
+  mbar_wait(&s.mma_done, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+}
+
+// Barriers and tensor memory of a CTA.
+template <typename S>
+__device__ __forceinline__ void ma_start(S& s) {
+  constexpr int kStages = S::kStages;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.full[i], 1);
@@ -376,174 +607,91 @@ __global__ void __launch_bounds__(kMaThreads, 1)
     for (int i = 0; i < 6; ++i) s.n_bad[i >> 1][i & 1] = 0;
     fence_mbar_init();
   }
-  if (warp == 9) {
-    tmem_alloc(&s.tmem_base, kMaTmemCols);
+  if (threadIdx.x >> 5 == 9) {
+    tmem_alloc(&s.tmem_base, S::kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+}
+
+// Joins the partial sums of a cluster's CTAs. A warp takes a row of the item:
+// out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j. where(stream, row, chunk
+// of 4 columns) says where a CTA keeps its m and l, and its O.
+struct MaPart {
+  const float2* ml;
+  const float* o;
+};
+template <typename T, int D, typename Where, typename Head, typename Token>
+__device__ __forceinline__ void ma_join(const MaArgs& p, const MaItem& it, int rank, int r0, int r1, Where&& where,
+                                        Head&& head_of, Token&& token_of) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kLanes = D / 4;  // lanes of a row: 4 columns each
+  const int sub = lane / kLanes, col = lane % kLanes;
+#pragma unroll 1
+  for (int w = (rank * (kMaThreads / 32) + warp) * (32 / kLanes); w < r0 + r1;
+       w += p.split * (kMaThreads / 32) * (32 / kLanes)) {
+    const int idx = w + sub;
+    const bool on = idx < r0 + r1;
+    const int st = on && idx >= r0 ? 1 : 0, r = on ? idx - (st ? r0 : 0) : 0;
+    const MaPart at = where(st, r, col);
+    float2 part[kMaMaxSplit];
+    float4 v[kMaMaxSplit];
+#pragma unroll
+    for (int j = 0; j < kMaMaxSplit; ++j) {  // all on their way at once; the first ones again where there are fewer
+      part[j] = ma_ld_cluster2(cluster_map(at.ml, j & (p.split - 1)));
+      v[j] = ma_ld_cluster(cluster_map(at.o, j & (p.split - 1)));
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kMaMaxSplit; ++j) top = part[j].x > top || part[j].x != part[j].x ? part[j].x : top;
+    if (top == -INFINITY) top = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll
+    for (int j = 0; j < kMaMaxSplit; ++j) {
+      if (j >= p.split || part[j].y == 0.f) continue;  // y 0: no key of this part is seen
+      const float f = ma_exp2(part[j].x - top);
+      l = fmaf(part[j].y, f, l);
+      acc.x = fmaf(v[j].x, f, acc.x);
+      acc.y = fmaf(v[j].y, f, acc.y);
+      acc.z = fmaf(v[j].z, f, acc.z);
+      acc.w = fmaf(v[j].w, f, acc.w);
+    }
+    const float inv = l == 0.f ? 0.f : __frcp_rn(l);
+    if (on) {
+      T* const dst = static_cast<T*>(p.out) + (it.start + it.tok0 + token_of(st) + r / p.G) * p.ld_out +
+                     (long long)((it.kvh + head_of(st)) * p.G + r % p.G) * D;
+      reinterpret_cast<uint2*>(dst)[col] =
+          make_uint2(MaType<T>::pack(acc.x * inv, acc.y * inv), MaType<T>::pack(acc.z * inv, acc.w * inv));
+    }
+  }
+}
+
+template <typename T, int D, bool kTree, bool kShared>
+__global__ void __launch_bounds__(kMaThreads, 1)
+    masked_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ MaArgs p) {
+  using S = MaSmem<D>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  S& s = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // a cluster of `split` CTAs works on one item; without a split a CTA takes items with the grid's stride
+  const int rank = blockIdx.x & (p.split - 1);
+  const int first = blockIdx.x >> p.split_log;
+  const int stride = p.split > 1 ? p.n_items : gridDim.x;
+
+  ma_start(s);
   const uint32_t tmem = s.tmem_base;
   pdl_wait();  // q, the pool and the metadata come from earlier work on the stream
   pdl_trigger();
 
   if (warp == 8) {
-    // ------------------------------------------------------------ TMA
-    // Lane i looks up and loads piece i of a tile.
-    if (lane == 0) {
-      prefetch_tensormap(&tmap_q);
-      prefetch_tensormap(&tmap_k);
-      prefetch_tensormap(&tmap_v);
-    }
-    const uint64_t pol_q = policy_evict_first();
-    const uint64_t pol_kv = policy_evict_normal();
-    const int oob = p.num_blocks * p.block_size;
-    const int per_tile = kMaTile / p.piece;
-    int nq = 0, ring = 0;  // Q loads and K / V tiles issued
-    bool ok = true;
-    for (int i = first; ok && i < p.n_items; i += stride) {
-      const MaItem it = ma_item<kTree, kShared>(p, i, rank);
-      if (it.skip) {
-        if (lane == 0 && it.tok0 < it.n) atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
-        continue;
-      }
-      if (lane == 0 && (it.ctx < 0 || (it.prefix < 0 && it.ctx != 0) ||
-                        (long long)it.ctx > (long long)p.max_blocks * p.block_size))
-        atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
-      if (it.nt == 0) continue;
-      const int32_t* table = p.bt + it.b * p.bt_stride;
-      // the pool row of this lane's piece of tile t (zeros where its page is none of the pool)
-      auto lookup = [&](int t) -> int {
-        const int x = it.x0 + t * kMaTile + lane * p.piece;
-        if (lane >= per_tile || x >= it.x1) return oob;
-        const int key = x < it.sink_x ? x : x + it.shift;
-        const int page = key / p.block_size;
-        const int blk = page < p.max_blocks ? table[page] : -1;
-        if (blk < 0 || blk >= p.num_blocks) {
-          atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
-          return oob;
-        }
-        return blk * p.block_size + (key - page * p.block_size);
-      };
-      auto load = [&](const CUtensorMap* map, int t, int row, int kvh) -> bool {
-        const int st = ring % kStages;
-        bool go = true;
-        const int n = min(per_tile, (it.x1 - it.x0 - t * kMaTile) / p.piece);
-        if (lane == 0) {
-          go = ma_wait(&s.empty[st], ((ring / kStages) & 1) ^ 1, &s.abort, p.status, NPL_DEV_TIMEOUT_TMA);
-          if (go) mbar_arrive_expect_tx(&s.full[st], n * p.piece * D * 2);
-        }
-        go = __shfl_sync(0xffffffffu, (int)go, 0);
-        if (!go) return false;
-        if (lane < n) {
-#pragma unroll
-          for (int hf = 0; hf < D / 64; ++hf)
-            tma_load_3d(s.kv[st] + hf * S::kHalf + lane * p.piece * 128, map, hf * 64, kvh, row, &s.full[st], pol_kv);
-        }
-        ++ring;
-        return true;
-      };
-      if (lane == 0) {
-        ok = nq == 0 || ma_wait(&s.q_empty, (nq - 1) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_TMA);
-        if (ok) {
-          mbar_arrive_expect_tx(&s.q_full, (it.second ? 2 : 1) * p.tokens * p.G * D * 2);
-          for (int q = 0; q < (it.second ? 2 : 1); ++q)
-#pragma unroll
-            for (int hf = 0; hf < D / 64; ++hf)
-              tma_load_3d(s.q[q] + hf * S::kHalf, &tmap_q, hf * 64, (it.kvh + (kShared ? 0 : q)) * p.G,
-                          it.start + it.tok0 + (kShared ? q * p.tokens : 0), &s.q_full, pol_q);
-        }
-      }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-      if (!ok) break;
-      ++nq;
-      // K of the first tile, then V of tile t and K of the next one, for each stream of its own tiles
-      int row = oob, next = lookup(0);
-      const int streams = !kShared && it.second ? 2 : 1;
-#pragma unroll 1
-      for (int t = -1; ok && t < it.nt; ++t) {
-        const int after = t + 2 < it.nt ? lookup(t + 2) : oob;  // ahead of the wait for a free stage
-#pragma unroll 1
-        for (int n = t < 0 ? 1 : 0; ok && n < 2 * streams; ++n) {
-          const bool k = n & 1;
-          if (t < 0 && !k) continue;
-          if (!k || t + 1 < it.nt) ok = load(k ? &tmap_k : &tmap_v, k ? t + 1 : t, k ? next : row, it.kvh + (n >> 1));
-        }
-        row = next;
-        next = after;
-      }
-    }
-    // Every load issued here has landed before the CTA may exit.
-    if (lane == 0) {
-      if (nq > 0) mbar_wait(&s.q_full, (nq - 1) & 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
-      for (int j = max(0, ring - kStages); j < ring; ++j)
-        mbar_wait(&s.full[j % kStages], (j / kStages) & 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
-    }
-    __syncwarp();
+    ma_load_role<S, D, kTree, kShared>(s, p, tmap_q, tmap_k, tmap_v, first, stride, rank);
   } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA
-    if (lane == 0) {
-      constexpr uint32_t kIdQK = idesc_f16(kMaTile, kMaTile, false) | MaType<T>::kIdesc;
-      constexpr uint32_t kIdPV = idesc_f16(kMaTile, D, true) | MaType<T>::kIdesc;
-      int ring = 0, nq = 0;
-      uint32_t p_phase[2] = {0, 0};
-      auto full = [&](int r) -> bool {
-        return ma_wait(&s.full[r % kStages], (r / kStages) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
-      };
-      auto issue_s = [&](int st, int r) {  // S of stream st from the K tile at ring position r
-        const uint32_t qa = smem_u32(s.q[st]), ka = smem_u32(s.kv[r % kStages]);
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * S::kHalf + (kk & 3) * 32;
-          mma_f16(tmem + st * 128, sdesc_k_sw128(qa + off), sdesc_k_sw128(ka + off), kIdQK, kk > 0 ? 1u : 0u);
-        }
-        tc_commit(&s.s_full[st]);
-      };
-      auto issue_o = [&](int st, int r, int t, bool last) -> bool {  // O of stream st (+)= P V
-        if (!ma_wait(&s.p_full[st], p_phase[st], &s.abort, p.status, NPL_DEV_TIMEOUT_MMA) || !full(r)) return false;
-        p_phase[st] ^= 1;
-        tc_fence_after();
-        const uint32_t va = smem_u32(s.kv[r % kStages]);
-#pragma unroll
-        for (int kk = 0; kk < kMaTile / 16; ++kk)
-          ma_mma_ts(tmem + 256 + st * 128, tmem + st * 128 + kk * 8, sdesc_mn_sw128(va + kk * 16 * 128, S::kHalf, 1024),
-                    kIdPV, (t > 0 || kk > 0) ? 1u : 0u);
-        if (last) tc_commit(&s.o_full[st]);
-        return true;
-      };
-      bool ok = true;
-      for (int i = first; ok && i < p.n_items; i += stride) {
-        const MaItem it = ma_item<kTree, kShared>(p, i, rank);
-        if (it.nt == 0) continue;
-        ok = ma_wait(&s.q_full, nq & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
-        ++nq;
-        const int streams = it.second ? 2 : 1;
-        // S of the first tile, then O of tile t and S of the next one, for each stream
-#pragma unroll 1
-        for (int t = -1; ok && t < it.nt; ++t) {
-          const bool more = t + 1 < it.nt;
-#pragma unroll 1
-          for (int st = 0; ok && st < streams; ++st) {
-            const bool last = !kShared || st == streams - 1;  // of those that read these tiles
-            const int rv = ring, rk = t >= 0 ? ring + 1 : ring;
-            if (t >= 0) {
-              if (!(ok = issue_o(st, rv, t, !more))) break;
-              if (last) tc_commit(&s.empty[rv % kStages]);
-            }
-            if (more) {
-              if (!(ok = full(rk))) break;
-              issue_s(st, rk);
-              if (last) tc_commit(&s.empty[rk % kStages]);
-            }
-            if (last) ring += (t >= 0) + more;
-          }
-          if (ok && t + 2 == it.nt) tc_commit(&s.q_empty);  // the last S of the item has been issued
-        }
-      }
-      tc_commit(&s.mma_done);  // arrives once every MMA issued above has completed
-      mbar_wait(&s.mma_done, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
-    }
+    if (lane == 0) ma_mma_role<S, T, D, kTree, kShared>(s, p, tmem, first, stride, rank);
     __syncwarp();
   } else if (warp < 8) {
     // -------------------------------------------------------- softmax
@@ -764,59 +912,294 @@ __global__ void __launch_bounds__(kMaThreads, 1)
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, kMaTmemCols);
+    tmem_dealloc(tmem, S::kTmemCols);
   }
   if (p.split > 1) {
-    // ------------------------------------------- join the partial sums
-    // A warp takes a row of the item: out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j over the cluster's CTAs.
     cluster_arrive_release();
     cluster_wait_acquire();
     const MaItem it = ma_item<kTree, kShared>(p, first, rank);
     if (!it.skip) {
       const int r0 = min(p.tokens, it.n - it.tok0) * p.G;
       const int r1 = !it.second ? 0 : kShared ? min(p.tokens, it.n - it.tok0 - p.tokens) * p.G : r0;
-      constexpr int kLanes = D / 4;  // lanes of a row: 4 columns each
-      const int sub = lane / kLanes, col = lane % kLanes;
-      for (int w = (rank * (kMaThreads / 32) + warp) * (32 / kLanes); w < r0 + r1;
-           w += p.split * (kMaThreads / 32) * (32 / kLanes)) {
-        const int idx = w + sub;
-        const bool on = idx < r0 + r1;
-        const int st = on && idx >= r0 ? 1 : 0, r = on ? idx - (st ? r0 : 0) : 0;
-        const float* base = reinterpret_cast<const float*>(s.kv);
-        const float2* ml = reinterpret_cast<const float2*>(base + 2 * kMaTile * D) + st * kMaTile + r;
-        const float* o = base + (size_t)(st * kMaTile + r) * D + ((col ^ (r & 7)) << 2);
-        float2 part[kMaMaxSplit];
-        float4 v[kMaMaxSplit];
-#pragma unroll
-        for (int j = 0; j < kMaMaxSplit; ++j) {  // all on their way at once; the last CTA's again where there are fewer
-          part[j] = ma_ld_cluster2(cluster_map(ml, min(j, p.split - 1)));
-          v[j] = ma_ld_cluster(cluster_map(o, min(j, p.split - 1)));
+      const float* base = reinterpret_cast<const float*>(s.kv);
+      ma_join<T, D>(p, it, rank, r0, r1, [&](int st, int r, int chunk) {
+        return MaPart{reinterpret_cast<const float2*>(base + 2 * kMaTile * D) + st * kMaTile + r,
+                      base + (st * kMaTile + r) * D + ((chunk ^ (r & 7)) << 2)};
+      }, [&](int st) { return kShared ? 0 : st; }, [&](int st) { return kShared ? st * p.tokens : 0; });
+    }
+    cluster_arrive_release();  // no CTA leaves while another reads its shared memory
+    cluster_wait_acquire();
+  }
+}
+
+// Few rows (at most kN of a kv head: single tokens, small trees) as the N side:
+// S^T = K Q^T has a key a TMEM lane and a row a column, so that a thread takes
+// kN exponentials a tile and none is spent on rows that do not exist. O^T =
+// V^T P^T has a column of the head a lane; a product of P^T with ones gives
+// every lane the rows' normalisers, which here sum p as it is rounded. The
+// rows' references m are kept in shared memory and moved, by all threads of the
+// stream together, in the rare tile that exceeds one by more than 2^8. Columns
+// are taken 16 at a time in rolled loops: calls of few tiles wait for code.
+template <typename T, int D, bool kTree, int kN>
+__global__ void __launch_bounds__(kMaThreads, 1)
+    few_rows_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ MaArgs p) {
+  using S = MaFewSmem<D, kN>;
+  constexpr int kStages = S::kStages;
+  constexpr float kNone = 3e38f;  // 6 - m of a row that has seen no key yet
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  S& s = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & (p.split - 1);
+  const int first = blockIdx.x >> p.split_log;
+  const int stride = p.split > 1 ? p.n_items : gridDim.x;
+  if (threadIdx.x < 256) reinterpret_cast<uint32_t*>(s.ones)[threadIdx.x] = MaType<T>::pack(1.f, 1.f);
+  fence_proxy_async_smem();
+  ma_start(s);
+  const uint32_t tmem = s.tmem_base;
+  pdl_wait();  // q, the pool and the metadata come from earlier work on the stream
+  pdl_trigger();
+
+  if (warp == 8) {
+    ma_load_role<S, D, kTree, false>(s, p, tmap_q, tmap_k, tmap_v, first, stride, rank);
+  } else if (warp == 9) {
+    if (lane == 0) ma_mma_role<S, T, D, kTree, false>(s, p, tmem, first, stride, rank);
+    __syncwarp();
+  } else if (warp < 8) {
+    // -------------------------------------------------------- softmax
+    const int st = warp >> 2;         // stream
+    const int r = threadIdx.x & 127;  // key of the tile, and column of the output: TMEM lane
+    const uint32_t lane_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_tm = lane_tm + st * kN, o_tm = lane_tm + 2 * kN + st * 2 * kN;
+    uint32_t s_phase = 0, o_phase = 0;
+    int ring = 0, item_no = 0;
+    bool ok = true;  // the same for all threads of the stream at the top of a loop
+    for (int i = first; ok && i < p.n_items; i += stride) {
+      const MaItem it = ma_item<kTree, false>(p, i, rank);
+      if (it.skip) continue;
+      const int base = ring;
+      ring += it.nt * (it.second ? 4 : 2);
+      if (st == 1 && !it.second) {
+        if (it.nt > 0) ++item_no;
+        continue;
+      }
+      const int kvh = it.kvh + st;
+      const int n_rows = min(p.tokens, it.n - it.tok0) * p.G;
+      const int list = item_no % 3;
+      float m = -INFINITY;  // of row r, units of log2 (threads r < kN)
+      if (r < kN) s.add[st][r] = r < n_rows ? kNone : -INFINITY;  // p = 0 in rows that do not exist
+      ma_stream_sync(st);
+#pragma unroll 1
+      for (int t = 0; ok && t < it.nt; ++t) {
+        const int xt = it.x0 + t * kMaTile, x = xt + r, key = x < it.sink_x ? x : x + it.shift;
+        // which rows see this thread's key, and whether all rows see all of the tile's keys
+        bool part;
+        uint32_t seen[(kN + 31) / 32];
+        if (kTree) {
+          part = xt + kMaTile > min(it.prefix, it.x1);
+        } else {
+          const int pa = it.prefix + it.tok0, pb = it.prefix + it.n - 1;
+          const int a_all = min(it.sink_x ? p.sinks : min(p.sinks, pa + 1), it.x1) - xt;
+          part = !(a_all >= kMaTile || (min(pa + 1 - it.shift, it.x1) - xt >= kMaTile &&
+                                        max(0, pb - p.window + 1) - it.shift - xt <= max(0, a_all)));
         }
-        float top = -INFINITY;
+        const bool some = x < it.x1 && key < it.hi && (kTree || key >= it.lo || key < p.sinks);
+        if (part) {
+          int from = 0, to = some ? kN : 0;  // rows
+          if (!kTree && some) {
+            from = max(0, key - it.prefix - it.tok0) * p.G;
+            if (key >= p.sinks) to = (int)min((long long)kN, ((long long)key + p.window - it.prefix - it.tok0) * p.G);
+          }
+          if (kTree && some && key >= it.prefix) to = 0;
 #pragma unroll
-        for (int j = 0; j < kMaMaxSplit; ++j) top = part[j].x > top || part[j].x != part[j].x ? part[j].x : top;
-        if (top == -INFINITY) top = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
+          for (int w = 0; w < (kN + 31) / 32; ++w) seen[w] = ma_low(to, w) & ~ma_low(from, w);
+          if (kTree && some && key >= it.prefix) {
+            const uint8_t* mask = p.mask + (long long)it.start * p.ld_mask + (key - it.prefix);
+#pragma unroll 4
+            for (int tok = 0; tok < it.n; ++tok) {
+              if (!mask[tok * p.ld_mask]) continue;
 #pragma unroll
-        for (int j = 0; j < kMaMaxSplit; ++j) {
-          if (j >= p.split || part[j].y == 0.f) continue;  // y 0: no key of this part is seen, its sums were not written
-          const float f = ma_exp2(part[j].x - top);
-          l = fmaf(part[j].y, f, l);
-          acc.x = fmaf(v[j].x, f, acc.x);
-          acc.y = fmaf(v[j].y, f, acc.y);
-          acc.z = fmaf(v[j].z, f, acc.z);
-          acc.w = fmaf(v[j].w, f, acc.w);
+              for (int w = 0; w < (kN + 31) / 32; ++w)
+                seen[w] |= ma_low((tok + 1) * p.G, w) & ~ma_low(tok * p.G, w);
+            }
+          }
         }
-        const float inv = l == 0.f ? 0.f : __frcp_rn(l);
-        if (on) {
-          const int tok = it.tok0 + (kShared ? st * p.tokens : 0) + r / p.G;
-          T* const dst = static_cast<T*>(p.out) + (it.start + tok) * p.ld_out +
-                         (long long)((it.kvh + (kShared ? 0 : st)) * p.G + r % p.G) * D;
-          reinterpret_cast<uint2*>(dst)[col] =
-              make_uint2(MaType<T>::pack(acc.x * inv, acc.y * inv), MaType<T>::pack(acc.z * inv, acc.w * inv));
+        bool fine = ma_wait(&s.s_full[st], s_phase, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
+        s_phase ^= 1;
+        fine = __all_sync(0xffffffffu, fine);
+        tc_fence_after();
+        // As in the other kernel: the last readers of the next item's list ended before this S could be issued.
+        if (t == 0 && r == 0) s.n_bad[(item_no + 1) % 3][st] = 0;
+        auto hide = [&](uint32_t(&v)[16], int n) {  // scores of rows n .. n + 15 that do not see this key
+          const uint32_t bits = (n >> 5 ? seen[(kN - 1) >> 5] : seen[0]) >> (n & 31);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (!(bits & (1u << e))) v[e] = 0xff800000u;
+        };
+        uint32_t v[16];
+        bool above = false;
+        if (fine) {
+#pragma unroll 1
+          for (int n = 0; n < kN; n += 16) {
+            ma_tmem_ld_x16(s_tm + n, v);
+            if (part) hide(v, n);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const float4 add = *reinterpret_cast<const float4*>(&s.add[st][n + e]);
+              above |= fmaxf(fmaxf(fmaf(__uint_as_float(v[e]), p.c2, add.x), fmaf(__uint_as_float(v[e + 1]), p.c2, add.y)),
+                             fmaxf(fmaf(__uint_as_float(v[e + 2]), p.c2, add.z),
+                                   fmaf(__uint_as_float(v[e + 3]), p.c2, add.w))) > kMaShift + kMaSlack;
+            }
+          }
+        }
+        if (ma_stream_any(st, above || !fine)) {
+          if (ma_stream_any(st, !fine)) {
+            ok = false;
+            break;
+          }
+          // some row's reference moves to its maximum so far
+#pragma unroll 1
+          for (int n = 0; n < kN; n += 16) {
+            if (kN > 16) {
+              ma_tmem_ld_x16(s_tm + n, v);
+              if (part) hide(v, n);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float top = ma_warp_max(__uint_as_float(v[e]));
+              if (lane == 0) s.top[st][warp & 3][n + e] = top;
+            }
+          }
+          ma_stream_sync(st);
+          if (r < kN) {
+            const float top = fmaxf(fmaxf(s.top[st][0][r], s.top[st][1][r]),
+                                    fmaxf(s.top[st][2][r], s.top[st][3][r])) * p.c2;
+            const bool move = r < n_rows && (m == -INFINITY || top > m + kMaSlack);
+            const float m_new = move ? top : m;
+            s.alpha[st][r] = !move ? 1.f : m == -INFINITY ? 0.f : ma_exp2(m - m_new);
+            m = m_new;
+            if (r < n_rows) s.add[st][r] = m == -INFINITY ? kNone : kMaShift - m;
+          }
+          ma_stream_sync(st);
+          if (t > 0) {
+#pragma unroll 1
+            for (int n = 0; n < 2 * kN; n += 16) {  // sums and normalisers
+              uint32_t o[16];
+              ma_tmem_ld_x16(o_tm + n, o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * s.alpha[st][(n & (kN - 1)) + e]);
+              ma_tmem_st_x16(o_tm + n, o);
+            }
+            ma_tmem_wait_st();
+          }
+        }
+        // P^T of this key: 16-byte chunks exchanged with the key's place in its 8 (128-byte swizzle)
+        uint8_t* const line = s.p[st] + (r >> 3) * 1024 + (r & 7) * 128;
+#pragma unroll 1
+        for (int n = 0; n < kN; n += 16) {
+          if (kN > 16) {
+            ma_tmem_ld_x16(s_tm + n, v);
+            if (part) hide(v, n);
+          }
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const float4 add = *reinterpret_cast<const float4*>(&s.add[st][n + e]);
+            w[e / 2] = MaType<T>::pack(ma_exp2(fmaf(__uint_as_float(v[e]), p.c2, add.x)),
+                                       ma_exp2(fmaf(__uint_as_float(v[e + 1]), p.c2, add.y)));
+            w[e / 2 + 1] = MaType<T>::pack(ma_exp2(fmaf(__uint_as_float(v[e + 2]), p.c2, add.z)),
+                                           ma_exp2(fmaf(__uint_as_float(v[e + 3]), p.c2, add.w)));
+          }
+          *reinterpret_cast<uint4*>(line + (((n >> 3) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(line + (((n >> 3) + 1 ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+        if (part) {
+          const int rv = !it.second ? base + 1 + 2 * t : base + (st == 0 ? 2 : t + 1 < it.nt ? 4 : 3) + 4 * t;
+          fine = ma_wait_warp(&s.full[rv % kStages], (rv / kStages) & 1, &s.abort, p.status,
+                              NPL_DEV_TIMEOUT_EPILOGUE);
+          if (fine && ma_clean_row<T, D>(s.kv[rv % kStages], r, some)) {
+            const int at = atomicAdd(&s.n_bad[list][st], 1);
+            if (at < kMaBad) s.bad[list][st][at] = key;
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0 && fine) mbar_arrive(&s.p_full[st]);  // not fine: every role of the CTA gives up
+      }
+      // every MMA of the item has completed; before the partial sums go over the ring, those of the other stream too
+      if (it.nt > 0) {
+        bool fine = ok && ma_wait(&s.o_full[st], o_phase, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
+        if (fine && p.split > 1 && it.second)
+          fine = ma_wait(&s.o_full[st ^ 1], o_phase, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
+        o_phase ^= 1;
+        ok = !ma_stream_any(st, !fine);
+        tc_fence_after();
+      }
+      if (ok) {
+        float* const stage = reinterpret_cast<float*>(s.kv) + (size_t)st * kN * D + r;
+        T* const dst = static_cast<T*>(p.out) + (it.start + it.tok0) * p.ld_out + (long long)kvh * p.G * D + r;
+        int tok = 0, head = 0;
+#pragma unroll 1
+        for (int n = 0; n < n_rows; n += 16) {
+          uint32_t o[16], l[16];
+          if (it.nt > 0) {
+            ma_tmem_ld_x16(o_tm + n, o);
+            ma_tmem_ld_x16(o_tm + kN + n, l);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float sum = it.nt > 0 ? __uint_as_float(l[e]) : 0.f;
+            const float y = sum == 0.f ? 0.f : __uint_as_float(o[e]);
+            if (r == n + e) s.ml[st][n + e] = make_float2(m, sum);
+            if (n + e < n_rows && r < D) {
+              if (p.split > 1)
+                stage[(n + e) * D] = y;
+              else
+                MaType<T>::put(dst + tok * p.ld_out + head * D, sum == 0.f ? 0.f : y * __frcp_rn(sum));
+            }
+            if (++head == p.G) head = 0, ++tok;
+          }
+        }
+        const int n_bad = it.nt > 0 ? s.n_bad[list][st] : 0;
+        if (n_bad > 0) {
+          ma_stream_sync(st);
+#pragma unroll 1
+          for (int n = 0; n < n_rows; ++n) {
+            if (r >= D || s.ml[st][n].y == 0.f) continue;
+            const int of = n / p.G;
+            const float x = ma_bad_sum<T, D, kTree, false>(&p, s.bad[list][st], n_bad, i, rank, it.tok0 + of, kvh, r);
+            if (x == 0.f) continue;
+            if (p.split > 1)
+              stage[n * D] += x;
+            else
+              MaType<T>::add(dst + of * p.ld_out + (n - of * p.G) * D, x);
+          }
         }
       }
+      if (it.nt > 0) ++item_no;
+      tc_fence_before();  // O has been read before this thread's next arrival, which the next O waits for
+      ma_stream_sync(st);  // and the normalisers, before the next item's
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::kTmemCols);
+  }
+  if (p.split > 1) {
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    const MaItem it = ma_item<kTree, false>(p, first, rank);
+    if (!it.skip) {
+      const int rows = min(p.tokens, it.n - it.tok0) * p.G;
+      const float* base = reinterpret_cast<const float*>(s.kv);
+      ma_join<T, D>(p, it, rank, rows, it.second ? rows : 0, [&](int st, int r, int chunk) {
+        return MaPart{&s.ml[st][r], base + (st * kN + r) * D + chunk * 4};
+      }, [&](int st) { return st; }, [&](int) { return 0; });
     }
     cluster_arrive_release();  // no CTA leaves while another reads its shared memory
     cluster_wait_acquire();
@@ -852,15 +1235,29 @@ int ma_map(const char* what, CUtensorMap* map, CUtensorMapDataType type, const v
   return NPL_OK;
 }
 
-template <typename T, int D, bool kTree, bool kShared>
+// kRows: 0 for row tiles that share their keys, 128 for one row tile of two kv heads, else few rows.
+template <typename T, int D, bool kTree, int kRows>
 int launch(const char* what, MaArgs p, cudaStream_t st) {
+  constexpr bool kShared = kRows == 0, kFew = kRows > 0 && kRows < kMaTile;
+  p.tokens = (kFew ? kRows : kMaTile) / p.G;
+  p.levels = kShared ? (p.max_q_len + 2 * p.tokens - 1) / (2 * p.tokens) : 1;
+  const long long items = (long long)p.levels * p.B * (kShared ? p.Hkv : (p.Hkv + 1) / 2);
+  if (items >= (1ll << 27)) return fail(NPL_ERR_UNSUPPORTED, "%s: too many row tiles", what);
+  p.n_items = (int)items;
   CUtensorMap tq, tk, tv;
   const long long slots = (long long)p.num_blocks * p.block_size;
   if (int rc = ma_map(what, &tq, MaType<T>::kMap, p.q, p.total_q, p.H, D, p.ld_q, p.G, p.tokens)) return rc;
   if (int rc = ma_map(what, &tk, MaType<T>::kMap, p.k, slots, p.Hkv, D, (long long)p.Hkv * D, 1, p.piece)) return rc;
   if (int rc = ma_map(what, &tv, MaType<T>::kMap, p.v, slots, p.Hkv, D, (long long)p.Hkv * D, 1, p.piece)) return rc;
-  const auto kernel = masked_attn_kernel<T, D, kTree, kShared>;
-  const int smem = (int)sizeof(MaSmem<D>) + 1024;
+  void (*kernel)(CUtensorMap, CUtensorMap, CUtensorMap, MaArgs);
+  int smem;
+  if constexpr (kFew) {
+    kernel = few_rows_kernel<T, D, kTree, kRows>;
+    smem = (int)sizeof(MaFewSmem<D, kRows>) + 1024;
+  } else {
+    kernel = masked_attn_kernel<T, D, kTree, kShared>;
+    smem = (int)sizeof(MaSmem<D>) + 1024;
+  }
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status(what);
   // Clusters of the size with the least rounds of (tiles of a CTA + kMaFixed for a CTA's start and the join).
@@ -882,28 +1279,26 @@ int launch(const char* what, MaArgs p, cudaStream_t st) {
                             tv, p);
 }
 
+template <typename T, int D, bool kTree>
+int run_type(const char* what, const MaArgs& p, cudaStream_t st) {
+  const long long rows = (long long)p.max_q_len * p.G;
+  if (rows <= 16) return launch<T, D, kTree, 16>(what, p, st);
+  if (rows <= 32) return launch<T, D, kTree, 32>(what, p, st);
+  if (rows <= 64) return launch<T, D, kTree, 64>(what, p, st);
+  if (p.max_q_len <= kMaTile / p.G) return launch<T, D, kTree, 128>(what, p, st);
+  return launch<T, D, kTree, 0>(what, p, st);
+}
+
 template <bool kTree>
 int run(const char* what, MaArgs p, int dtype, int D, float scale, cudaStream_t st) {
   p.c2 = scale * 1.4426950408889634f;
-  p.tokens = kMaTile / p.G;
   p.piece_log = kMaPieceLog;
   while (p.block_size & ((1 << p.piece_log) - 1)) --p.piece_log;
   p.piece = 1 << p.piece_log;
-  const bool shared = p.max_q_len > p.tokens;
-  p.levels = shared ? (p.max_q_len + 2 * p.tokens - 1) / (2 * p.tokens) : 1;
-  const long long items = (long long)p.levels * p.B * (shared ? p.Hkv : (p.Hkv + 1) / 2);
-  if (items >= (1ll << 27)) return fail(NPL_ERR_UNSUPPORTED, "%s: too many row tiles", what);
-  p.n_items = (int)items;
-  if (dtype == NPL_F16) {
-    if (D == 128)
-      return shared ? launch<__half, 128, kTree, true>(what, p, st) : launch<__half, 128, kTree, false>(what, p, st);
-    return shared ? launch<__half, 64, kTree, true>(what, p, st) : launch<__half, 64, kTree, false>(what, p, st);
-  }
-  if (D == 128)
-    return shared ? launch<__nv_bfloat16, 128, kTree, true>(what, p, st)
-                  : launch<__nv_bfloat16, 128, kTree, false>(what, p, st);
-  return shared ? launch<__nv_bfloat16, 64, kTree, true>(what, p, st)
-                : launch<__nv_bfloat16, 64, kTree, false>(what, p, st);
+  if (dtype == NPL_F16)
+    return D == 128 ? run_type<__half, 128, kTree>(what, p, st) : run_type<__half, 64, kTree>(what, p, st);
+  return D == 128 ? run_type<__nv_bfloat16, 128, kTree>(what, p, st)
+                  : run_type<__nv_bfloat16, 64, kTree>(what, p, st);
 }
 
 int check(const char* what, const MaArgs& p, int dtype, int D, float scale) {

@@ -50,8 +50,10 @@ namespace {
 constexpr int kMaThreads = 384;
 constexpr int kMaTile = 128;
 constexpr int kMaFixed = 4;             // what a CTA costs beside its tiles, in tiles
-constexpr int kMaBad = 32;             // keys with V elements that are not finite, remembered for an item
+constexpr int kMaLists = 8;            // items whose lists of such keys are kept: more than the ring can be ahead
+constexpr int kMaBad = 12;             // keys with V elements that are not finite, remembered by a warp for an item
 constexpr int kMaPieceLog = 5;         // 32 keys of a piece at most
+constexpr int kMaBoxLog = 7;           // 128 keys of a load at most
 constexpr int kMaMaxSplit = 8;          // CTAs of a cluster at most
 constexpr float kMaShift = 6.f;        // p = 2^(x - m + 6)
 constexpr float kMaSlack = 8.f;        // m moves when a score is more than this above it
@@ -74,6 +76,7 @@ struct MaArgs {
   int B, H, Hkv, G, num_blocks, block_size, max_blocks, total_q, max_q_len;
   int tokens;   // of a row tile: 128 / G
   int piece, piece_log;  // keys of a piece, a power of two
+  int box_log;           // pieces of a large load, a power of two
   int levels;   // items of a sequence and kv head (or pair of them)
   int n_items;  // levels * B * (kv heads, or pairs of them)
   int split, split_log;  // CTAs of a cluster, which share an item's keys, a power of two
@@ -82,24 +85,26 @@ struct MaArgs {
 };
 
 struct MaBarriers {
-  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], mma_done;
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], mma_done;
   uint32_t tmem_base;
   int abort;
-  int n_bad[3][2];        // [item % 3][stream whose threads clean its V tiles]
-  int bad[3][2][kMaBad];  // keys whose V rows held elements that are not finite
+  // keys whose V rows held elements that are not finite: [item % kMaLists][stream whose V it is][warp 10 or 11]
+  int n_bad[kMaLists][2][2];
+  int bad[kMaLists][2][2][kMaBad];
 };
 
 template <int D>
 struct MaSmem : MaBarriers {
   static constexpr bool kFew = false;
   static constexpr int kRows = kMaTile;
-  static constexpr uint32_t kHalf = kMaTile * 128;  // 128 rows x 64 elements (one swizzle span)
-  static constexpr uint32_t kQHalf = kHalf;
+  static constexpr uint32_t kQHalf = kMaTile * 128;  // Q: 128 rows x 64 elements (one swizzle span), twice for D = 128
+  static constexpr uint32_t kGroup = 8 * D * 2;      // K, V: 8 rows x 64 elements, twice for D = 128, then 8 more rows
   static constexpr uint32_t kTileBytes = kMaTile * D * 2;
   static constexpr int kStages = D == 128 ? 5 : 8;
   static constexpr uint32_t kScoreCols = 128, kOutCols = 128, kTmemCols = 512;  // S of the streams (P over it), then O
-  uint64_t full[kStages], empty[kStages];
-  alignas(1024) uint8_t q[2][kTileBytes];
+  uint64_t full[kStages], empty[kStages], raw[kStages];
+  static constexpr int kQBufs = 1;
+  alignas(1024) uint8_t q[1][2][kTileBytes];
   alignas(1024) uint8_t kv[kStages][kTileBytes];  // K and V tiles in the order of their use; partial sums at the end
 };
 
@@ -108,19 +113,20 @@ template <int D, int kN>
 struct MaFewSmem : MaBarriers {
   static constexpr bool kFew = true;
   static constexpr int kRows = kN;
-  static constexpr uint32_t kHalf = kMaTile * 128;
   static constexpr uint32_t kQHalf = kN * 128;
+  static constexpr uint32_t kGroup = 8 * D * 2;
   static constexpr uint32_t kTileBytes = kMaTile * D * 2;
   static constexpr int kStages = D == 64 ? 10 : kN == 64 ? 4 : 5;
   static constexpr uint32_t kScoreCols = kN, kOutCols = 2 * kN;  // S of the streams, then O and the normalisers
   static constexpr uint32_t kTmemCols = 8 * kN;
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full[kStages], empty[kStages], raw[kStages];
   alignas(16) float add[2][kN];  // of a row: 6 - m
   float alpha[2][kN];            // what its sums are scaled with
   float top[2][4][kN];           // a warp's maxima
   float2 ml[2][kN];              // m and the normaliser at the end
   alignas(1024) uint8_t ones[1024];
-  alignas(1024) uint8_t q[2][kN * D * 2];
+  static constexpr int kQBufs = kN == 64 ? 1 : 2;  // Q of this item and of the next one
+  alignas(1024) uint8_t q[kQBufs][2][kN * D * 2];
   alignas(1024) uint8_t p[2][kMaTile * 128];  // P^T: a key's rows in one 128-byte line
   alignas(1024) uint8_t kv[kStages][kTileBytes];
 };
@@ -259,13 +265,14 @@ __device__ __forceinline__ void ma_exp_pack(const uint32_t (&v)[32], float c2, f
 
 // One item: 128 rows (or twice 128, shared) of one sequence and kv head (or
 // the same rows of two). Every role decodes the same items from the same
-// read-only metadata. The keys that some row of the item sees are numbered by
-// x = 0, 1, ...: key(x) = x below first * piece (the sinks' pieces), x + shift
-// from there on. This CTA takes x0 <= x < x1.
+// read-only metadata. Tiles are numbered through x: key(x) = x below sink_x
+// (the sinks' pieces), x + shift from hole_x on (the window's; shift is a
+// multiple of 128, so that a tile's keys lie in its pages as in its rows), and
+// nothing is loaded between. This CTA takes the tiles x0 <= x < x1.
 struct MaItem {
   int b, kvh, tok0, n, ctx, start, prefix;
   int lo, hi;  // keys that some row of the item sees: lo <= key < hi, and the sinks
-  int sink_x, shift, x0, x1, nt;
+  int sink_x, hole_x, shift, x0, x1, nt;
   bool skip, second;  // no such rows; the second stream has rows
 };
 
@@ -284,26 +291,29 @@ __device__ __forceinline__ MaItem ma_item(const MaArgs& p, int i, int rank) {
   it.skip = it.tok0 >= it.n || it.n > p.max_q_len || it.start < 0 || it.start > p.total_q - it.n;
   it.second = kShared ? it.tok0 + p.tokens < it.n : it.kvh + 1 < p.Hkv;
   const int last = min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1));  // one past the item's last token
-  int pieces = 0;
-  it.lo = it.sink_x = it.shift = 0;
+  int end = 0;
+  it.lo = it.sink_x = it.hole_x = it.shift = 0;
   it.hi = kTree ? it.ctx : it.prefix + last;
   if (it.prefix < 0) it.hi = 0;
   if (it.hi > 0) {
-    const int to = ((it.hi - 1) >> p.piece_log) + 1;
-    pieces = to;
+    end = (((it.hi - 1) >> p.piece_log) + 1) << p.piece_log;
     if (!kTree) {
       it.lo = max(0, it.prefix + it.tok0 - p.window + 1);
-      const int sp = (min(p.sinks, it.lo) + p.piece - 1) >> p.piece_log, lp = it.lo >> p.piece_log;
+      const int sp = (min(p.sinks, it.lo) + p.piece - 1) >> p.piece_log << p.piece_log;
+      const int lp = it.lo >> p.piece_log << p.piece_log;
       if (sp < lp) {
-        pieces = sp + to - lp;
-        it.sink_x = sp * p.piece;
-        it.shift = (lp - sp) * p.piece;
+        it.sink_x = sp;
+        it.hole_x = sp + ((lp - sp) & (kMaTile - 1));  // the first x from sp on with lp's place in a tile
+        it.shift = lp - it.hole_x;
+        end -= it.shift;
       }
     }
   }
-  it.x0 = (int)(((long long)pieces * rank) >> p.split_log) << p.piece_log;
-  it.x1 = (int)(((long long)pieces * (rank + 1)) >> p.split_log) << p.piece_log;
-  it.nt = (it.x1 - it.x0 + kMaTile - 1) / kMaTile;
+  const int tiles = (end + kMaTile - 1) / kMaTile;
+  const int t0 = (int)(((long long)tiles * rank) >> p.split_log);
+  it.nt = (int)(((long long)tiles * (rank + 1)) >> p.split_log) - t0;
+  it.x0 = t0 * kMaTile;
+  it.x1 = min(end, it.x0 + it.nt * kMaTile);
   if (it.skip) it.nt = 0;
   return it;
 }
@@ -312,6 +322,17 @@ __device__ __forceinline__ MaItem ma_item(const MaArgs& p, int i, int rank) {
 __device__ __forceinline__ uint32_t ma_low(int n, int w) {
   n -= w * 32;
   return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+}
+
+// Whether some row of a CTA's item does not see some of the tile's columns from xt on.
+template <bool kTree, bool kShared>
+__device__ __forceinline__ bool ma_part(const MaArgs& p, const MaItem& it, int xt) {
+  if (kTree) return xt + kMaTile > min(it.prefix, it.x1);
+  // the columns that the item's first row and its last row both see, every row sees
+  const int pa = it.prefix + it.tok0, pb = it.prefix + min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1)) - 1;
+  const int a = min(it.sink_x ? p.sinks : min(p.sinks, pa + 1), it.x1) - xt;
+  const int b = max(0, pb - p.window + 1) - it.shift - xt, e = min(pa + 1 - it.shift, it.x1) - xt;
+  return a < kMaTile && (e < kMaTile || b > max(0, a));
 }
 
 // Whether the row of a token sees a key (the same as the bits below, for one key).
@@ -329,7 +350,7 @@ __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) 
   uint32_t any = 0;
 #pragma unroll 1
   for (int hf = 0; hf < D / 64; ++hf) {
-    uint4* line = reinterpret_cast<uint4*>(tile + hf * (kMaTile * 128) + row * 128);
+    uint4* line = reinterpret_cast<uint4*>(tile + (row >> 3) * (8 * D * 2) + hf * 1024 + (row & 7) * 128);
     if (!seen) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) line[c] = make_uint4(0, 0, 0, 0);
@@ -345,7 +366,7 @@ __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) 
   if (!(any & 0x80008000u)) return false;
 #pragma unroll 1
   for (int c = 0; c < D / 2; ++c) {
-    uint32_t* w = reinterpret_cast<uint32_t*>(tile + (c >> 5) * (kMaTile * 128) + row * 128) + (c & 31);
+    uint32_t* w = reinterpret_cast<uint32_t*>(tile + (row >> 3) * (8 * D * 2) + (c >> 5) * 1024 + (row & 7) * 128) + (c & 31);
     const uint32_t t = ((*w & MaType<T>::kExp) + MaType<T>::kOne) & 0x80008000u;
     *w &= ~((t >> 15) * 0xffffu);
   }
@@ -355,17 +376,17 @@ __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) 
 // Sum of the V elements of column col that are not finite, that ma_clean_row
 // took out, and whose keys the row of a token sees (a rare path).
 template <typename T, int D, bool kTree, bool kShared>
-__device__ __noinline__ float ma_bad_sum(const MaArgs* args, const int* keys, int n_keys, int item, int rank, int token,
-                                         int kvh, int col) {
+__device__ __noinline__ float ma_bad_sum(const MaArgs* args, const int* counts, const int (*lists)[kMaBad], int item,
+                                         int rank, int token, int kvh, int col) {
   const MaArgs& p = *args;
   const MaItem it = ma_item<kTree, kShared>(p, item, rank);
-  const bool all = n_keys > kMaBad;  // more than were remembered: look at every key of this CTA
-  const int n = all ? it.x1 - it.x0 : n_keys;
+  const bool all = max(counts[0], counts[1]) > kMaBad;  // more than were remembered: look at every key of this CTA
+  const int n = all ? it.x1 - it.x0 : counts[0] + counts[1];
   float sum = 0.f;
 #pragma unroll 1
   for (int j = 0; j < n; ++j) {
     const int x = it.x0 + j;
-    const int key = !all ? keys[j] : x < it.sink_x ? x : x + it.shift;
+    const int key = all ? (x < it.sink_x ? x : x + it.shift) : j < counts[0] ? lists[0][j] : lists[1][j - counts[0]];
     if (key >= it.hi || !ma_sees<kTree>(p, it, token, key)) continue;
     const int page = key / p.block_size;
     const int blk = page < p.max_blocks ? p.bt[it.b * p.bt_stride + page] : -1;
@@ -411,22 +432,93 @@ __device__ __forceinline__ void ma_tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]
       : "r"(taddr)
       : "memory");
 }
+// Shared-memory descriptors of a K or V tile (128-byte swizzle, 8 rows of 64
+// elements in 1024 bytes, the rows' second halves in the next 1024): with the
+// head dimension as K (groups of 8 rows `group` bytes apart), and as M or N
+// (64-element halves `half` bytes apart).
+__device__ __forceinline__ uint64_t ma_desc_k(uint32_t addr, uint32_t group) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t ma_desc_mn(uint32_t addr, uint32_t half, uint32_t group) {
+  return sdesc_mn_sw128(addr, half, group);
+}
+
+// Rows of one kv head of the pool, 8 * row8 and following, by one load.
+__device__ __forceinline__ void ma_load_rows(void* dst, const CUtensorMap* map, int row8, int kvh, uint64_t* bar,
+                                             uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %2, %2, %3, %4}], [%5], %6;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row8), "r"(kvh), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
+// Warps 10 and 11: in tiles that some row sees in part, V rows are made safe to
+// multiply by 0 before the P.V product reads them. Such a tile's load arrives
+// at a barrier of its own, the tiles of the kind one after the other, and these
+// two warps arrive at the stage's in its place.
+template <typename S, typename T, int D, bool kTree, bool kShared>
+__device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, int stride, int rank) {
+  constexpr int kStages = S::kStages;
+  const int lane = threadIdx.x & 31, which = (threadIdx.x >> 5) - 10;
+  int ring = 0, n_raw = 0, item_no = 0;
+  bool ok = true;
+  for (int i = first; ok && i < p.n_items; i += stride) {
+    const MaItem it = ma_item<kTree, kShared>(p, i, rank);
+    if (it.nt == 0) continue;
+    const int streams = !kShared && it.second ? 2 : 1, list = item_no % kMaLists;
+    if (lane < 2) s.n_bad[list][lane][which] = 0;
+    __syncwarp();
+#pragma unroll 1
+    for (int t = 0; ok && t < it.nt; ++t) {
+      const int xt = it.x0 + t * kMaTile;
+      if (!ma_part<kTree, kShared>(p, it, xt)) continue;
+#pragma unroll 1
+      for (int st = 0; ok && st < streams; ++st) {
+        // V's place in the order of the loads
+        const int r = ring + (streams == 1 ? 1 + 2 * t : (st == 0 ? 2 : t + 1 < it.nt ? 4 : 3) + 4 * t);
+        ok = ma_wait_warp(&s.raw[n_raw % kStages], (n_raw / kStages) & 1, &s.abort, p.status,
+                          NPL_DEV_TIMEOUT_EPILOGUE);
+        if (!ok) break;
+        ++n_raw;
+#pragma unroll 1
+        for (int row = which * 64 + lane; row < which * 64 + 64; row += 32) {
+          const int x = xt + row, key = x < it.sink_x ? x : x + it.shift;
+          const bool some = x < it.x1 && key < it.hi && (kTree || key >= it.lo || key < p.sinks);
+          if (ma_clean_row<T, D>(s.kv[r % kStages], row, some)) {
+            const int at = atomicAdd(&s.n_bad[list][st][which], 1);
+            if (at < kMaBad) s.bad[list][st][which][at] = key;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.full[r % kStages]);
+      }
+    }
+    ring += 2 * it.nt * streams;
+    ++item_no;
+  }
+}
+
 // Warp 8: loads by TMA. Lane i looks up and loads piece i of a tile.
 template <typename S, int D, bool kTree, bool kShared>
 __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtensorMap& tmap_q, const CUtensorMap& tmap_k,
-                                             const CUtensorMap& tmap_v, int first, int stride, int rank) {
+                                             const CUtensorMap& tmap_v, const CUtensorMap& tmap_kb,
+                                             const CUtensorMap& tmap_vb, int first, int stride, int rank) {
   constexpr int kStages = S::kStages;
   const int lane = threadIdx.x & 31;
   if (lane == 0) {
     prefetch_tensormap(&tmap_q);
     prefetch_tensormap(&tmap_k);
     prefetch_tensormap(&tmap_v);
+    prefetch_tensormap(&tmap_kb);
+    prefetch_tensormap(&tmap_vb);
   }
   const uint64_t pol_q = policy_evict_first();
   const uint64_t pol_kv = policy_evict_normal();
   const int oob = p.num_blocks * p.block_size;
-  const int per_tile = kMaTile / p.piece;
-  int nq = 0, ring = 0;  // Q loads and K / V tiles issued
+  const int per_tile = kMaTile >> p.piece_log;
+  int nq = 0, ring = 0, n_raw = 0;  // Q loads, K and V tiles, and V tiles to be cleaned issued
   bool ok = true;
   for (int i = first; ok && i < p.n_items; i += stride) {
     const MaItem it = ma_item<kTree, kShared>(p, i, rank);
@@ -439,10 +531,10 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
       atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
     if (it.nt == 0) continue;
     const int32_t* table = p.bt + it.b * p.bt_stride;
-    // the pool row of this lane's piece of tile t (zeros where its page is none of the pool)
+    // the pool row of this lane's piece of tile t (zeros where its page is none of the pool), -1: not loaded
     auto lookup = [&](int t) -> int {
-      const int x = it.x0 + t * kMaTile + lane * p.piece;
-      if (lane >= per_tile || x >= it.x1) return oob;
+      const int x = it.x0 + t * kMaTile + (lane << p.piece_log);
+      if (lane >= per_tile || x >= it.x1 || (x >= it.sink_x && x < it.hole_x)) return -1;
       const int key = x < it.sink_x ? x : x + it.shift;
       const int page = key / p.block_size;
       const int blk = page < p.max_blocks ? table[page] : -1;
@@ -452,49 +544,61 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
       }
       return blk * p.block_size + (key - page * p.block_size);
     };
-    auto load = [&](const CUtensorMap* map, int t, int row, int kvh) -> bool {
+    auto load = [&](bool k, bool part, int t, int row, int kvh) -> bool {
       const int st = ring % kStages;
+      const uint32_t loaded = __ballot_sync(0xffffffffu, row >= 0);
       bool go = true;
-      const int n = min(per_tile, (it.x1 - it.x0 - t * kMaTile) / p.piece);
       if (lane == 0) {
         go = ma_wait(&s.empty[st], ((ring / kStages) & 1) ^ 1, &s.abort, p.status, NPL_DEV_TIMEOUT_TMA);
-        if (go) mbar_arrive_expect_tx(&s.full[st], n * p.piece * D * 2);
+        if (go) {
+          if (!part) mbar_arrive(&s.full[st]);  // the second of its two arrivals
+          mbar_arrive_expect_tx(part ? &s.raw[n_raw % kStages] : &s.full[st], (__popc(loaded) << p.piece_log) * D * 2);
+        }
       }
       go = __shfl_sync(0xffffffffu, (int)go, 0);
       if (!go) return false;
-      if (lane < n) {
-#pragma unroll
-        for (int hf = 0; hf < D / 64; ++hf)
-          tma_load_3d(s.kv[st] + hf * S::kHalf + lane * p.piece * 128, map, hf * 64, kvh, row, &s.full[st], pol_kv);
-      }
+      // pieces that lie together in the pool by one load, the ragged ends of a context or a window one by one
+      const int lead = lane >> p.box_log << p.box_log, lead_x = it.x0 + t * kMaTile + (lead << p.piece_log);
+      const uint32_t group = (1u << (1 << p.box_log)) - 1;  // at most 16 pieces of 8 keys
+      const bool big = ((loaded >> lead) & group) == group &&
+                       (lead_x >= it.hole_x || lead_x + (p.piece << p.box_log) <= it.sink_x);
+      if (row >= 0 && (!big || lane == lead))
+        ma_load_rows(s.kv[st] + (lane << p.piece_log) * D * 2, k ? (big ? &tmap_kb : &tmap_k) : (big ? &tmap_vb : &tmap_v),
+                     row >> 3, kvh, part ? &s.raw[n_raw % kStages] : &s.full[st], pol_kv);
       ++ring;
+      n_raw += part;
       return true;
     };
-    if (lane == 0) {
-      ok = nq == 0 || ma_wait(&s.q_empty, (nq - 1) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_TMA);
-      if (ok) {
-        mbar_arrive_expect_tx(&s.q_full, (it.second ? 2 : 1) * p.tokens * p.G * D * 2);
-        for (int q = 0; q < (it.second ? 2 : 1); ++q)
-#pragma unroll
-          for (int hf = 0; hf < D / 64; ++hf)
-            tma_load_3d(s.q[q] + hf * S::kQHalf, &tmap_q, hf * 64, (it.kvh + (kShared ? 0 : q)) * p.G,
-                        it.start + it.tok0 + (kShared ? q * p.tokens : 0), &s.q_full, pol_q);
-      }
-    }
-    ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-    if (!ok) break;
-    ++nq;
     // K of the first tile, then V of tile t and K of the next one, for each stream of its own tiles
-    int row = oob, next = lookup(0);
+    int row = -1, next = lookup(0);
     const int streams = !kShared && it.second ? 2 : 1;
 #pragma unroll 1
     for (int t = -1; ok && t < it.nt; ++t) {
-      const int after = t + 2 < it.nt ? lookup(t + 2) : oob;  // ahead of the wait for a free stage
+      const bool part = t >= 0 && ma_part<kTree, kShared>(p, it, it.x0 + t * kMaTile);
+      const int after = t + 2 < it.nt ? lookup(t + 2) : -1;  // ahead of the wait for a free stage
 #pragma unroll 1
       for (int n = t < 0 ? 1 : 0; ok && n < 2 * streams; ++n) {
         const bool k = n & 1;
         if (t < 0 && !k) continue;
-        if (!k || t + 1 < it.nt) ok = load(k ? &tmap_k : &tmap_v, k ? t + 1 : t, k ? next : row, it.kvh + (n >> 1));
+        if (!k || t + 1 < it.nt) ok = load(k, !k && part, k ? t + 1 : t, k ? next : row, it.kvh + (n >> 1));
+      }
+      if (t == (kShared ? 0 : -1) && ok) {  // three or two tiles ahead: less than the ring holds
+        // Q after the first tiles: those need not wait until the Q before has been read
+        if (lane == 0) {
+          const int buf = nq % S::kQBufs;
+          ok = ma_wait(&s.q_empty[buf], (nq / S::kQBufs & 1) ^ 1, &s.abort, p.status, NPL_DEV_TIMEOUT_TMA);
+          if (ok) {
+            mbar_arrive_expect_tx(&s.q_full[buf], (it.second ? 2 : 1) * p.tokens * p.G * D * 2);
+#pragma unroll 1
+            for (int q = 0; q < (it.second ? 2 : 1); ++q)
+#pragma unroll
+              for (int hf = 0; hf < D / 64; ++hf)
+                tma_load_3d(s.q[buf][q] + hf * S::kQHalf, &tmap_q, hf * 64, (it.kvh + (kShared ? 0 : q)) * p.G,
+                            it.start + it.tok0 + (kShared ? q * p.tokens : 0), &s.q_full[buf], pol_q);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+        if (ok) ++nq;
       }
       row = next;
       next = after;
@@ -502,7 +606,8 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
   }
   // Every load issued here has landed before the CTA may exit.
   if (lane == 0) {
-    if (nq > 0) mbar_wait(&s.q_full, (nq - 1) & 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+    for (int j = max(0, nq - S::kQBufs); j < nq; ++j)
+      mbar_wait(&s.q_full[j % S::kQBufs], (j / S::kQBufs) & 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
     for (int j = max(0, ring - kStages); j < ring; ++j)
       mbar_wait(&s.full[j % kStages], (j / kStages) & 1, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
   }
@@ -523,13 +628,13 @@ __device__ __forceinline__ void ma_mma_role(S& s, const MaArgs& p, uint32_t tmem
   auto full = [&](int r) -> bool {
     return ma_wait(&s.full[r % kStages], (r / kStages) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
   };
-  auto issue_s = [&](int st, int r) {  // S of stream st from the K tile at ring position r
-    const uint32_t qa = smem_u32(s.q[st]), ka = smem_u32(s.kv[r % kStages]);
+  auto issue_s = [&](int st, int r, int qb) {  // S of stream st from the K tile at ring position r
+    const uint32_t qa = smem_u32(s.q[qb][st]), ka = smem_u32(s.kv[r % kStages]);
     tc_fence_after();
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       const uint64_t qd = sdesc_k_sw128(qa + (kk >> 2) * S::kQHalf + (kk & 3) * 32);
-      const uint64_t kd = sdesc_k_sw128(ka + (kk >> 2) * S::kHalf + (kk & 3) * 32);
+      const uint64_t kd = ma_desc_k(ka + (kk >> 2) * 1024 + (kk & 3) * 32, S::kGroup);
       mma_f16(tmem + st * S::kScoreCols, S::kFew ? kd : qd, S::kFew ? qd : kd, kIdQK, kk > 0 ? 1u : 0u);
     }
     tc_commit(&s.s_full[st]);
@@ -541,7 +646,7 @@ __device__ __forceinline__ void ma_mma_role(S& s, const MaArgs& p, uint32_t tmem
     const uint32_t va = smem_u32(s.kv[r % kStages]);
 #pragma unroll
     for (int kk = 0; kk < kMaTile / 16; ++kk) {
-      const uint64_t vd = sdesc_mn_sw128(va + kk * 16 * 128, S::kFew && D == 64 ? 0 : S::kHalf, 1024);
+      const uint64_t vd = ma_desc_mn(va + kk * 2 * S::kGroup, S::kFew && D == 64 ? 0 : 1024, S::kGroup);
       const uint32_t o = tmem + 2 * S::kScoreCols + st * S::kOutCols, on = (t > 0 || kk > 0) ? 1u : 0u;
       if constexpr (S::kFew) {
         const uint64_t pd = sdesc_mn_sw128(smem_u32(s.p[st]) + kk * 16 * 128, 0, 1024);
@@ -557,7 +662,8 @@ __device__ __forceinline__ void ma_mma_role(S& s, const MaArgs& p, uint32_t tmem
   for (int i = first; ok && i < p.n_items; i += stride) {
     const MaItem it = ma_item<kTree, kShared>(p, i, rank);
     if (it.nt == 0) continue;
-    ok = ma_wait(&s.q_full, nq & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
+    const int qb = nq % S::kQBufs;
+    ok = ma_wait(&s.q_full[qb], (nq / S::kQBufs) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
     ++nq;
     const int streams = it.second ? 2 : 1;
     // S of the first tile, then O of tile t and S of the next one, for each stream
@@ -574,12 +680,12 @@ __device__ __forceinline__ void ma_mma_role(S& s, const MaArgs& p, uint32_t tmem
         }
         if (more) {
           if (!(ok = full(rk))) break;
-          issue_s(st, rk);
+          issue_s(st, rk, qb);
           if (last) tc_commit(&s.empty[rk % kStages]);
         }
         if (last) ring += (t >= 0) + more;
       }
-      if (ok && t + 2 == it.nt) tc_commit(&s.q_empty);  // the last S of the item has been issued
+      if (ok && t + 2 == it.nt) tc_commit(&s.q_empty[qb]);  // the last S of the item has been issued
     }
   }
   tc_commit(&s.mma_done);  // arrives once every MMA issued above has completed
@@ -592,19 +698,19 @@ __device__ __forceinline__ void ma_start(S& s) {
   constexpr int kStages = S::kStages;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&s.full[i], 1);
+      mbar_init(&s.full[i], 2);
       mbar_init(&s.empty[i], 1);
+      mbar_init(&s.raw[i], 1);
     }
-    mbar_init(&s.q_full, 1);
-    mbar_init(&s.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.q_full[i], 1);
+      mbar_init(&s.q_empty[i], 1);
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], 4);  // one arrival a warp
       mbar_init(&s.o_full[i], 1);
     }
     mbar_init(&s.mma_done, 1);
     s.abort = 0;
-    for (int i = 0; i < 6; ++i) s.n_bad[i >> 1][i & 1] = 0;
     fence_mbar_init();
   }
   if (threadIdx.x >> 5 == 9) {
@@ -672,7 +778,8 @@ __device__ __forceinline__ void ma_join(const MaArgs& p, const MaItem& it, int r
 template <typename T, int D, bool kTree, bool kShared>
 __global__ void __launch_bounds__(kMaThreads, 1)
     masked_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ MaArgs p) {
+                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_kb,
+                    const __grid_constant__ CUtensorMap tmap_vb, const __grid_constant__ MaArgs p) {
   using S = MaSmem<D>;
   constexpr int kStages = S::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -689,26 +796,26 @@ __global__ void __launch_bounds__(kMaThreads, 1)
   pdl_trigger();
 
   if (warp == 8) {
-    ma_load_role<S, D, kTree, kShared>(s, p, tmap_q, tmap_k, tmap_v, first, stride, rank);
+    ma_load_role<S, D, kTree, kShared>(s, p, tmap_q, tmap_k, tmap_v, tmap_kb, tmap_vb, first, stride, rank);
   } else if (warp == 9) {
     if (lane == 0) ma_mma_role<S, T, D, kTree, kShared>(s, p, tmem, first, stride, rank);
     __syncwarp();
-  } else if (warp < 8) {
+  } else if (warp >= 10) {
+    ma_clean_role<S, T, D, kTree, kShared>(s, p, first, stride, rank);
+  } else {
     // -------------------------------------------------------- softmax
     const int st = warp >> 2;            // stream
     const int r = threadIdx.x & 127;     // row of the tile = TMEM lane
     const int row_tok = r / p.G, row_head = r - row_tok * p.G;
     const uint32_t lane_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_tm = lane_tm + st * 128, o_tm = lane_tm + 256 + st * 128;
-    const int owner = kShared ? 0 : st;  // the stream whose threads clean the V tiles that this one reads
+    const int owner = kShared ? 0 : st;  // the stream whose V tiles this one reads
     uint32_t s_phase = 0, o_phase = 0;
-    int ring = 0, item_no = 0;
+    int item_no = 0;
     bool ok = true;
     for (int i = first; ok && i < p.n_items; i += stride) {
       const MaItem it = ma_item<kTree, kShared>(p, i, rank);
       if (it.skip) continue;
-      const int base = ring;
-      ring += it.nt * (!kShared && it.second ? 4 : 2);
       if (st == 1 && !it.second) {
         if (it.nt > 0) ++item_no;
         continue;
@@ -719,15 +826,16 @@ __global__ void __launch_bounds__(kMaThreads, 1)
       const bool row_ok = r < n_rows;
       const bool warp_on = (warp & 3) * 32 < n_rows;
       const int token = tok0 + row_tok, pos = it.prefix + token;
-      const int list = item_no % 3;
+      const int list = item_no % kMaLists;
+      bool any_part = false;
       float m = -INFINITY, l = 0.f;  // m in units of log2
       for (int t = 0; ok && t < it.nt; ++t) {
         const int xt = it.x0 + t * kMaTile;
         // which of the tile's columns this row sees
         uint32_t seen[4];
-        bool part;  // some row of the CTA's item does not see some column
+        const bool part = ma_part<kTree, kShared>(p, it, xt);
+        any_part |= part;
         if (kTree) {
-          part = xt + kMaTile > min(it.prefix, it.x1);
 #pragma unroll
           for (int w = 0; w < 4; ++w) seen[w] = row_ok ? ma_low(min(it.prefix, it.x1) - xt, w) : 0u;
           if (part && row_ok) {
@@ -753,11 +861,6 @@ __global__ void __launch_bounds__(kMaThreads, 1)
           const int e = min(pos + 1 - it.shift, it.x1) - xt;
 #pragma unroll
           for (int w = 0; w < 4; ++w) seen[w] = row_ok ? ma_low(a, w) | (ma_low(e, w) & ~ma_low(b, w)) : 0u;
-          // the columns that the item's first row and its last row both see, every row sees
-          const int pa = it.prefix + it.tok0, pb = it.prefix + min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1)) - 1;
-          const int a_all = min(it.sink_x ? p.sinks : min(p.sinks, pa + 1), it.x1) - xt;
-          part = !(a_all >= kMaTile || (min(pa + 1 - it.shift, it.x1) - xt >= kMaTile &&
-                                        max(0, pb - p.window + 1) - it.shift - xt <= max(0, a_all)));
         }
         if (!ma_wait_warp(&s.s_full[st], s_phase, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
           ok = false;
@@ -765,10 +868,6 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         }
         s_phase ^= 1;
         tc_fence_after();
-        // The next item's list is emptied here. Its last readers were those of the item before the last one, which
-        // ended before the MMA warp could issue this S (it had waited for both streams' P of the last item), and
-        // its next writers wait for an S that follows this thread's next arrival.
-        if (t == 0 && st == owner && r == 0) s.n_bad[(item_no + 1) % 3][owner] = 0;
         if (warp_on) {
           // The row is read twice, 32 columns at a time and the next ones ahead: its maximum, then the exponentials.
           // (Held in registers, its 128 scores spilled; and the loops stay rolled for the sake of short calls.)
@@ -828,20 +927,6 @@ __global__ void __launch_bounds__(kMaThreads, 1)
           l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
           ma_tmem_wait_st();
         }
-        if (part && st == owner) {
-          const int rv = kShared || !it.second ? base + 1 + 2 * t : base + (st == 0 ? 2 : t + 1 < it.nt ? 4 : 3) + 4 * t;
-          if (!ma_wait_warp(&s.full[rv % kStages], (rv / kStages) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
-            ok = false;
-            break;
-          }
-          const int x = xt + r, key = x < it.sink_x ? x : x + it.shift;
-          const bool some = x < it.x1 && key < it.hi && (kTree || key >= it.lo || key < p.sinks);
-          if (ma_clean_row<T, D>(s.kv[rv % kStages], r, some)) {
-            const int at = atomicAdd(&s.n_bad[list][owner], 1);
-            if (at < kMaBad) s.bad[list][owner][at] = key;
-          }
-          fence_proxy_async_smem();
-        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.p_full[st]);
@@ -856,7 +941,8 @@ __global__ void __launch_bounds__(kMaThreads, 1)
       }
       if (!ok) break;
       if (warp_on) {
-        const int n_bad = it.nt > 0 ? s.n_bad[list][owner] : 0;
+        const int* const n_bad = s.n_bad[list][owner];
+        const bool bad = any_part && n_bad[0] + n_bad[1] > 0;  // written before the P.V products of such tiles
         const float inv = p.split > 1 ? 1.f : l == 0.f ? 0.f : __frcp_rn(l);
         float* const stage = reinterpret_cast<float*>(s.kv) + (size_t)(st * kMaTile + r) * D;
         T* const dst = static_cast<T*>(p.out) + (it.start + token) * p.ld_out +
@@ -889,10 +975,10 @@ __global__ void __launch_bounds__(kMaThreads, 1)
             }
           }
         }
-        if (n_bad > 0 && row_ok && l != 0.f) {
+        if (bad && row_ok && l != 0.f) {
 #pragma unroll 1
           for (int d = 0; d < D; ++d) {
-            const float x = ma_bad_sum<T, D, kTree, kShared>(&p, s.bad[list][owner], n_bad, i, rank, token, kvh, d);
+            const float x = ma_bad_sum<T, D, kTree, kShared>(&p, n_bad, s.bad[list][owner], i, rank, token, kvh, d);
             if (x == 0.f) continue;
             if (p.split > 1)
               stage[(((d >> 2) ^ (r & 7)) << 2) + (d & 3)] += x;
@@ -943,7 +1029,8 @@ __global__ void __launch_bounds__(kMaThreads, 1)
 template <typename T, int D, bool kTree, int kN>
 __global__ void __launch_bounds__(kMaThreads, 1)
     few_rows_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ MaArgs p) {
+                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_kb,
+                    const __grid_constant__ CUtensorMap tmap_vb, const __grid_constant__ MaArgs p) {
   using S = MaFewSmem<D, kN>;
   constexpr int kStages = S::kStages;
   constexpr float kNone = 3e38f;  // 6 - m of a row that has seen no key yet
@@ -961,31 +1048,32 @@ __global__ void __launch_bounds__(kMaThreads, 1)
   pdl_trigger();
 
   if (warp == 8) {
-    ma_load_role<S, D, kTree, false>(s, p, tmap_q, tmap_k, tmap_v, first, stride, rank);
+    ma_load_role<S, D, kTree, false>(s, p, tmap_q, tmap_k, tmap_v, tmap_kb, tmap_vb, first, stride, rank);
   } else if (warp == 9) {
     if (lane == 0) ma_mma_role<S, T, D, kTree, false>(s, p, tmem, first, stride, rank);
     __syncwarp();
-  } else if (warp < 8) {
+  } else if (warp >= 10) {
+    ma_clean_role<S, T, D, kTree, false>(s, p, first, stride, rank);
+  } else {
     // -------------------------------------------------------- softmax
     const int st = warp >> 2;         // stream
     const int r = threadIdx.x & 127;  // key of the tile, and column of the output: TMEM lane
     const uint32_t lane_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_tm = lane_tm + st * kN, o_tm = lane_tm + 2 * kN + st * 2 * kN;
     uint32_t s_phase = 0, o_phase = 0;
-    int ring = 0, item_no = 0;
+    int item_no = 0;
     bool ok = true;  // the same for all threads of the stream at the top of a loop
     for (int i = first; ok && i < p.n_items; i += stride) {
       const MaItem it = ma_item<kTree, false>(p, i, rank);
       if (it.skip) continue;
-      const int base = ring;
-      ring += it.nt * (it.second ? 4 : 2);
       if (st == 1 && !it.second) {
         if (it.nt > 0) ++item_no;
         continue;
       }
       const int kvh = it.kvh + st;
       const int n_rows = min(p.tokens, it.n - it.tok0) * p.G;
-      const int list = item_no % 3;
+      const int list = item_no % kMaLists;
+      bool any_part = false;
       float m = -INFINITY;  // of row r, units of log2 (threads r < kN)
       if (r < kN) s.add[st][r] = r < n_rows ? kNone : -INFINITY;  // p = 0 in rows that do not exist
       ma_stream_sync(st);
@@ -993,16 +1081,9 @@ __global__ void __launch_bounds__(kMaThreads, 1)
       for (int t = 0; ok && t < it.nt; ++t) {
         const int xt = it.x0 + t * kMaTile, x = xt + r, key = x < it.sink_x ? x : x + it.shift;
         // which rows see this thread's key, and whether all rows see all of the tile's keys
-        bool part;
+        const bool part = ma_part<kTree, false>(p, it, xt);
+        any_part |= part;
         uint32_t seen[(kN + 31) / 32];
-        if (kTree) {
-          part = xt + kMaTile > min(it.prefix, it.x1);
-        } else {
-          const int pa = it.prefix + it.tok0, pb = it.prefix + it.n - 1;
-          const int a_all = min(it.sink_x ? p.sinks : min(p.sinks, pa + 1), it.x1) - xt;
-          part = !(a_all >= kMaTile || (min(pa + 1 - it.shift, it.x1) - xt >= kMaTile &&
-                                        max(0, pb - p.window + 1) - it.shift - xt <= max(0, a_all)));
-        }
         const bool some = x < it.x1 && key < it.hi && (kTree || key >= it.lo || key < p.sinks);
         if (part) {
           int from = 0, to = some ? kN : 0;  // rows
@@ -1028,8 +1109,6 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         s_phase ^= 1;
         fine = __all_sync(0xffffffffu, fine);
         tc_fence_after();
-        // As in the other kernel: the last readers of the next item's list ended before this S could be issued.
-        if (t == 0 && r == 0) s.n_bad[(item_no + 1) % 3][st] = 0;
         auto hide = [&](uint32_t(&v)[16], int n) {  // scores of rows n .. n + 15 that do not see this key
           const uint32_t bits = (n >> 5 ? seen[(kN - 1) >> 5] : seen[0]) >> (n & 31);
 #pragma unroll
@@ -1114,19 +1193,10 @@ __global__ void __launch_bounds__(kMaThreads, 1)
           *reinterpret_cast<uint4*>(line + (((n >> 3) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           *reinterpret_cast<uint4*>(line + (((n >> 3) + 1 ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
         }
-        if (part) {
-          const int rv = !it.second ? base + 1 + 2 * t : base + (st == 0 ? 2 : t + 1 < it.nt ? 4 : 3) + 4 * t;
-          fine = ma_wait_warp(&s.full[rv % kStages], (rv / kStages) & 1, &s.abort, p.status,
-                              NPL_DEV_TIMEOUT_EPILOGUE);
-          if (fine && ma_clean_row<T, D>(s.kv[rv % kStages], r, some)) {
-            const int at = atomicAdd(&s.n_bad[list][st], 1);
-            if (at < kMaBad) s.bad[list][st][at] = key;
-          }
-        }
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0 && fine) mbar_arrive(&s.p_full[st]);  // not fine: every role of the CTA gives up
+        if (lane == 0) mbar_arrive(&s.p_full[st]);
       }
       // every MMA of the item has completed; before the partial sums go over the ring, those of the other stream too
       if (it.nt > 0) {
@@ -1162,14 +1232,15 @@ __global__ void __launch_bounds__(kMaThreads, 1)
             if (++head == p.G) head = 0, ++tok;
           }
         }
-        const int n_bad = it.nt > 0 ? s.n_bad[list][st] : 0;
-        if (n_bad > 0) {
+        const int* const n_bad = s.n_bad[list][st];
+        if (any_part && n_bad[0] + n_bad[1] > 0) {  // written before the P.V products of such tiles
           ma_stream_sync(st);
 #pragma unroll 1
           for (int n = 0; n < n_rows; ++n) {
             if (r >= D || s.ml[st][n].y == 0.f) continue;
             const int of = n / p.G;
-            const float x = ma_bad_sum<T, D, kTree, false>(&p, s.bad[list][st], n_bad, i, rank, it.tok0 + of, kvh, r);
+            const float x = ma_bad_sum<T, D, kTree, false>(&p, n_bad, s.bad[list][st], i, rank, it.tok0 + of,
+                                                                     kvh, r);
             if (x == 0.f) continue;
             if (p.split > 1)
               stage[n * D] += x;
@@ -1218,6 +1289,25 @@ PFN_cuTensorMapEncodeTiled_v12000 ma_encode_fn() {
   return fn;
 }
 
+// K or V rows of the pool [rows][Hkv][D] as a 5-D tensor map whose box holds
+// `box` rows of one head: 8 rows of 64 elements (128-byte swizzle), their second
+// halves, the next 8 rows.
+int ma_pool_map(const char* what, CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, int Hkv,
+                int D, int box) {
+  const PFN_cuTensorMapEncodeTiled_v12000 fn = ma_encode_fn();
+  if (!fn) return fail(NPL_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled unavailable", what);
+  const cuuint64_t ld = (cuuint64_t)Hkv * D * 2;
+  const cuuint64_t dims[5] = {64, 8, (cuuint64_t)D / 64, (cuuint64_t)rows / 8, (cuuint64_t)Hkv};
+  const cuuint64_t strides[4] = {ld, 128, 8 * ld, (cuuint64_t)D * 2};
+  const cuuint32_t size[5] = {64, 8, (cuuint32_t)D / 64, (cuuint32_t)box / 8, 1};
+  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(map, type, 5, const_cast<void*>(base), dims, strides, size, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(NPL_ERR_ARG, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+  return NPL_OK;
+}
+
 // [rows][heads][D] (rows ld elements apart, heads contiguous) as a 3-D tensor
 // map with a (64, box_heads, box_rows) box and the 128-byte swizzle.
 int ma_map(const char* what, CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, int heads,
@@ -1244,12 +1334,15 @@ int launch(const char* what, MaArgs p, cudaStream_t st) {
   const long long items = (long long)p.levels * p.B * (kShared ? p.Hkv : (p.Hkv + 1) / 2);
   if (items >= (1ll << 27)) return fail(NPL_ERR_UNSUPPORTED, "%s: too many row tiles", what);
   p.n_items = (int)items;
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, tkb, tvb;
   const long long slots = (long long)p.num_blocks * p.block_size;
+  const int box = p.piece << p.box_log;
   if (int rc = ma_map(what, &tq, MaType<T>::kMap, p.q, p.total_q, p.H, D, p.ld_q, p.G, p.tokens)) return rc;
-  if (int rc = ma_map(what, &tk, MaType<T>::kMap, p.k, slots, p.Hkv, D, (long long)p.Hkv * D, 1, p.piece)) return rc;
-  if (int rc = ma_map(what, &tv, MaType<T>::kMap, p.v, slots, p.Hkv, D, (long long)p.Hkv * D, 1, p.piece)) return rc;
-  void (*kernel)(CUtensorMap, CUtensorMap, CUtensorMap, MaArgs);
+  if (int rc = ma_pool_map(what, &tk, MaType<T>::kMap, p.k, slots, p.Hkv, D, p.piece)) return rc;
+  if (int rc = ma_pool_map(what, &tv, MaType<T>::kMap, p.v, slots, p.Hkv, D, p.piece)) return rc;
+  if (int rc = ma_pool_map(what, &tkb, MaType<T>::kMap, p.k, slots, p.Hkv, D, box)) return rc;
+  if (int rc = ma_pool_map(what, &tvb, MaType<T>::kMap, p.v, slots, p.Hkv, D, box)) return rc;
+  void (*kernel)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, MaArgs);
   int smem;
   if constexpr (kFew) {
     kernel = few_rows_kernel<T, D, kTree, kRows>;
@@ -1276,7 +1369,7 @@ int launch(const char* what, MaArgs p, cudaStream_t st) {
   p.split = 1 << p.split_log;
   const int grid = p.split > 1 ? p.n_items * p.split : std::min(p.n_items, sms);
   return launch_pdl_cluster(what, kernel, dim3(grid), dim3(kMaThreads), (size_t)smem, st, (unsigned)p.split, tq, tk,
-                            tv, p);
+                            tv, tkb, tvb, p);
 }
 
 template <typename T, int D, bool kTree>
@@ -1295,6 +1388,8 @@ int run(const char* what, MaArgs p, int dtype, int D, float scale, cudaStream_t 
   p.piece_log = kMaPieceLog;
   while (p.block_size & ((1 << p.piece_log) - 1)) --p.piece_log;
   p.piece = 1 << p.piece_log;
+  p.box_log = kMaBoxLog - p.piece_log;
+  while (p.block_size & ((p.piece << p.box_log) - 1)) --p.box_log;
   if (dtype == NPL_F16)
     return D == 128 ? run_type<__half, 128, kTree>(what, p, st) : run_type<__half, 64, kTree>(what, p, st);
   return D == 128 ? run_type<__nv_bfloat16, 128, kTree>(what, p, st)

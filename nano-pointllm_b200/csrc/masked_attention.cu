@@ -117,14 +117,13 @@ struct MaFewSmem : MaBarriers {
   static constexpr uint32_t kGroup = 8 * D * 2;
   static constexpr uint32_t kTileBytes = kMaTile * D * 2;
   static constexpr int kStages = D == 64 ? 10 : kN == 64 ? 4 : 5;
-  static constexpr uint32_t kScoreCols = kN, kOutCols = 2 * kN;  // S of the streams, then O and the normalisers
-  static constexpr uint32_t kTmemCols = 8 * kN;
+  static constexpr uint32_t kScoreCols = kN, kOutCols = kN, kTmemCols = 4 * kN;  // S of the streams, then O
   uint64_t full[kStages], empty[kStages], raw[kStages];
   alignas(16) float add[2][kN];  // of a row: 6 - m
   float alpha[2][kN];            // what its sums are scaled with
-  float top[2][4][kN];           // a warp's maxima
+  float top[2][4][kN];           // a warp's maxima, at the end its sums
   float2 ml[2][kN];              // m and the normaliser at the end
-  alignas(1024) uint8_t ones[1024];
+  float inv[2][kN];              // and what a row of sums is multiplied with
   static constexpr int kQBufs = kN == 64 ? 1 : 2;  // Q of this item and of the next one
   alignas(1024) uint8_t q[kQBufs][2][kN * D * 2];
   alignas(1024) uint8_t p[2][kMaTile * 128];  // P^T: a key's rows in one 128-byte line
@@ -416,10 +415,19 @@ __device__ __forceinline__ bool ma_stream_any(int st, bool x) {
   return r != 0;
 }
 
-__device__ __forceinline__ float ma_warp_max(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
+// Reduces 16 values a lane over a warp: lane i is left with the result of value i % 16.
+template <typename Op>
+__device__ __forceinline__ void ma_warp_reduce(float (&v)[16], int lane, Op&& op) {
+#pragma unroll
+  for (int n = 8; n > 0; n /= 2) {
+#pragma unroll
+    for (int e = 0; e < n; ++e) {
+      const bool up = lane & n;
+      const float give = up ? v[e] : v[e + n], keep = up ? v[e + n] : v[e];
+      v[e] = op(keep, __shfl_xor_sync(0xffffffffu, give, n));
+    }
+  }
+  v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
 }
 
 // 16 columns of this lane from TMEM.
@@ -648,11 +656,9 @@ __device__ __forceinline__ void ma_mma_role(S& s, const MaArgs& p, uint32_t tmem
     for (int kk = 0; kk < kMaTile / 16; ++kk) {
       const uint64_t vd = ma_desc_mn(va + kk * 2 * S::kGroup, S::kFew && D == 64 ? 0 : 1024, S::kGroup);
       const uint32_t o = tmem + 2 * S::kScoreCols + st * S::kOutCols, on = (t > 0 || kk > 0) ? 1u : 0u;
-      if constexpr (S::kFew) {
-        const uint64_t pd = sdesc_mn_sw128(smem_u32(s.p[st]) + kk * 16 * 128, 0, 1024);
-        mma_f16(o, vd, pd, kIdPV, on);
-        mma_f16(o + S::kRows, sdesc_mn_sw128(smem_u32(s.ones), 0, 0), pd, kIdPV, on);  // each lane: the sums of P
-      } else
+      if constexpr (S::kFew)
+        mma_f16(o, vd, sdesc_mn_sw128(smem_u32(s.p[st]) + kk * 16 * 128, 0, 1024), kIdPV, on);
+      else
         ma_mma_ts(o, tmem + st * S::kScoreCols + kk * 8, vd, kIdPV, on);
     }
     if (last) tc_commit(&s.o_full[st]);
@@ -837,7 +843,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         any_part |= part;
         if (kTree) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) seen[w] = row_ok ? ma_low(min(it.prefix, it.x1) - xt, w) : 0u;
+          for (int w = 0; w < 4; ++w) seen[w] = !part ? 0xffffffffu : row_ok ? ma_low(min(it.prefix, it.x1) - xt, w) : 0u;
           if (part && row_ok) {
             const uint8_t* mask = p.mask + (it.start + token) * p.ld_mask;
             const int j1 = min(it.n, it.x1 - it.prefix);
@@ -856,11 +862,14 @@ __global__ void __launch_bounds__(kMaThreads, 1)
             }
           }
         } else {
-          const int a = min(it.sink_x ? p.sinks : min(p.sinks, pos + 1), it.x1) - xt;
-          const int b = max(0, pos - p.window + 1) - it.shift - xt;
-          const int e = min(pos + 1 - it.shift, it.x1) - xt;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) seen[w] = row_ok ? ma_low(a, w) | (ma_low(e, w) & ~ma_low(b, w)) : 0u;
+          for (int w = 0; w < 4; ++w) seen[w] = 0xffffffffu;
+          if (part) {
+            const int a = min(it.sink_x ? p.sinks : min(p.sinks, pos + 1), it.x1) - xt;
+            const int b = max(0, pos - p.window + 1) - it.shift - xt, e = min(pos + 1 - it.shift, it.x1) - xt;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) seen[w] = row_ok ? ma_low(a, w) | (ma_low(e, w) & ~ma_low(b, w)) : 0u;
+          }
         }
         if (!ma_wait_warp(&s.s_full[st], s_phase, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
           ok = false;
@@ -881,12 +890,14 @@ __global__ void __launch_bounds__(kMaThreads, 1)
             tmem_ld_x32(s_tm + h * 64 + 32, vb);
             if (masked) ma_hide(va, h ? seen[2] : seen[0]);
 #pragma unroll
-            for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(va[c]));
+            for (int c = 0; c < 32; c += 2)
+              mx[c >> 1 & 3] = fmaxf(mx[c >> 1 & 3], fmaxf(__uint_as_float(va[c]), __uint_as_float(va[c + 1])));
             ma_tmem_wait_ld(vb);
             tmem_ld_x32(s_tm + (h ? 0 : 64), va);  // at the end: the first columns again
             if (masked) ma_hide(vb, h ? seen[3] : seen[1]);
 #pragma unroll
-            for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(vb[c]));
+            for (int c = 0; c < 32; c += 2)
+              mx[c >> 1 & 3] = fmaxf(mx[c >> 1 & 3], fmaxf(__uint_as_float(vb[c]), __uint_as_float(vb[c + 1])));
           }
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c2;
           const bool move = t == 0 || top > m + kMaSlack;
@@ -1021,11 +1032,9 @@ __global__ void __launch_bounds__(kMaThreads, 1)
 // Few rows (at most kN of a kv head: single tokens, small trees) as the N side:
 // S^T = K Q^T has a key a TMEM lane and a row a column, so that a thread takes
 // kN exponentials a tile and none is spent on rows that do not exist. O^T =
-// V^T P^T has a column of the head a lane; a product of P^T with ones gives
-// every lane the rows' normalisers, which here sum p as it is rounded. The
-// rows' references m are kept in shared memory and moved, by all threads of the
-// stream together, in the rare tile that exceeds one by more than 2^8. Columns
-// are taken 16 at a time in rolled loops: calls of few tiles wait for code.
+// V^T P^T has a column of the head a lane. The rows' references m are kept in
+// shared memory and moved, by all threads of the stream together, in the rare
+// tile that exceeds one by more than 2^8. Columns are taken 16 at a time.
 template <typename T, int D, bool kTree, int kN>
 __global__ void __launch_bounds__(kMaThreads, 1)
     few_rows_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -1040,8 +1049,6 @@ __global__ void __launch_bounds__(kMaThreads, 1)
   const int rank = blockIdx.x & (p.split - 1);
   const int first = blockIdx.x >> p.split_log;
   const int stride = p.split > 1 ? p.n_items : gridDim.x;
-  if (threadIdx.x < 256) reinterpret_cast<uint32_t*>(s.ones)[threadIdx.x] = MaType<T>::pack(1.f, 1.f);
-  fence_proxy_async_smem();
   ma_start(s);
   const uint32_t tmem = s.tmem_base;
   pdl_wait();  // q, the pool and the metadata come from earlier work on the stream
@@ -1059,7 +1066,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
     const int st = warp >> 2;         // stream
     const int r = threadIdx.x & 127;  // key of the tile, and column of the output: TMEM lane
     const uint32_t lane_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t s_tm = lane_tm + st * kN, o_tm = lane_tm + 2 * kN + st * 2 * kN;
+    const uint32_t s_tm = lane_tm + st * kN, o_tm = lane_tm + 2 * kN + st * kN;
     uint32_t s_phase = 0, o_phase = 0;
     int item_no = 0;
     bool ok = true;  // the same for all threads of the stream at the top of a loop
@@ -1077,6 +1084,9 @@ __global__ void __launch_bounds__(kMaThreads, 1)
       float m = -INFINITY;  // of row r, units of log2 (threads r < kN)
       if (r < kN) s.add[st][r] = r < n_rows ? kNone : -INFINITY;  // p = 0 in rows that do not exist
       ma_stream_sync(st);
+      float l[kN];  // of this thread's keys
+#pragma unroll
+      for (int n = 0; n < kN; ++n) l[n] = 0.f;
 #pragma unroll 1
       for (int t = 0; ok && t < it.nt; ++t) {
         const int xt = it.x0 + t * kMaTile, x = xt + r, key = x < it.sink_x ? x : x + it.shift;
@@ -1143,11 +1153,11 @@ __global__ void __launch_bounds__(kMaThreads, 1)
               ma_tmem_ld_x16(s_tm + n, v);
               if (part) hide(v, n);
             }
+            float top[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float top = ma_warp_max(__uint_as_float(v[e]));
-              if (lane == 0) s.top[st][warp & 3][n + e] = top;
-            }
+            for (int e = 0; e < 16; ++e) top[e] = __uint_as_float(v[e]);
+            ma_warp_reduce(top, lane, [](float a, float b) { return fmaxf(a, b); });
+            if (lane < 16) s.top[st][warp & 3][n + lane] = top[0];
           }
           ma_stream_sync(st);
           if (r < kN) {
@@ -1160,14 +1170,16 @@ __global__ void __launch_bounds__(kMaThreads, 1)
             if (r < n_rows) s.add[st][r] = m == -INFINITY ? kNone : kMaShift - m;
           }
           ma_stream_sync(st);
+#pragma unroll
+          for (int n = 0; n < kN; ++n) l[n] *= s.alpha[st][n];
           if (t > 0) {
 #pragma unroll 1
-            for (int n = 0; n < 2 * kN; n += 16) {  // sums and normalisers
+            for (int n = 0; n < kN; n += 16) {
               uint32_t o[16];
               ma_tmem_ld_x16(o_tm + n, o);
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                o[e] = __float_as_uint(__uint_as_float(o[e]) * s.alpha[st][(n & (kN - 1)) + e]);
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * s.alpha[st][n + e]);
               ma_tmem_st_x16(o_tm + n, o);
             }
             ma_tmem_wait_st();
@@ -1175,7 +1187,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         }
         // P^T of this key: 16-byte chunks exchanged with the key's place in its 8 (128-byte swizzle)
         uint8_t* const line = s.p[st] + (r >> 3) * 1024 + (r & 7) * 128;
-#pragma unroll 1
+#pragma unroll
         for (int n = 0; n < kN; n += 16) {
           if (kN > 16) {
             ma_tmem_ld_x16(s_tm + n, v);
@@ -1185,10 +1197,16 @@ __global__ void __launch_bounds__(kMaThreads, 1)
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
             const float4 add = *reinterpret_cast<const float4*>(&s.add[st][n + e]);
-            w[e / 2] = MaType<T>::pack(ma_exp2(fmaf(__uint_as_float(v[e]), p.c2, add.x)),
-                                       ma_exp2(fmaf(__uint_as_float(v[e + 1]), p.c2, add.y)));
-            w[e / 2 + 1] = MaType<T>::pack(ma_exp2(fmaf(__uint_as_float(v[e + 2]), p.c2, add.z)),
-                                           ma_exp2(fmaf(__uint_as_float(v[e + 3]), p.c2, add.w)));
+            const float p0 = ma_exp2(fmaf(__uint_as_float(v[e]), p.c2, add.x));
+            const float p1 = ma_exp2(fmaf(__uint_as_float(v[e + 1]), p.c2, add.y));
+            const float p2 = ma_exp2(fmaf(__uint_as_float(v[e + 2]), p.c2, add.z));
+            const float p3 = ma_exp2(fmaf(__uint_as_float(v[e + 3]), p.c2, add.w));
+            l[n + e] += p0;
+            l[n + e + 1] += p1;
+            l[n + e + 2] += p2;
+            l[n + e + 3] += p3;
+            w[e / 2] = MaType<T>::pack(p0, p1);
+            w[e / 2 + 1] = MaType<T>::pack(p2, p3);
           }
           *reinterpret_cast<uint4*>(line + (((n >> 3) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           *reinterpret_cast<uint4*>(line + (((n >> 3) + 1 ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
@@ -1207,29 +1225,42 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         ok = !ma_stream_any(st, !fine);
         tc_fence_after();
       }
+      // the rows' normalisers: sums over the stream's keys
+#pragma unroll
+      for (int n = 0; n < kN; n += 16) {
+        float sum[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum[e] = l[n + e];
+        ma_warp_reduce(sum, lane, [](float a, float b) { return a + b; });
+        if (lane < 16) s.top[st][warp & 3][n + lane] = sum[0];
+      }
+      ma_stream_sync(st);
+      if (r < kN) {
+        const float sum = (s.top[st][0][r] + s.top[st][1][r]) + (s.top[st][2][r] + s.top[st][3][r]);
+        s.ml[st][r] = make_float2(m, sum);
+        s.inv[st][r] = sum == 0.f ? 0.f : p.split > 1 ? 1.f : __frcp_rn(sum);
+      }
+      ma_stream_sync(st);
       if (ok) {
         float* const stage = reinterpret_cast<float*>(s.kv) + (size_t)st * kN * D + r;
         T* const dst = static_cast<T*>(p.out) + (it.start + it.tok0) * p.ld_out + (long long)kvh * p.G * D + r;
-        int tok = 0, head = 0;
+        T* at = dst;
+        int head = 0;
 #pragma unroll 1
         for (int n = 0; n < n_rows; n += 16) {
-          uint32_t o[16], l[16];
-          if (it.nt > 0) {
-            ma_tmem_ld_x16(o_tm + n, o);
-            ma_tmem_ld_x16(o_tm + kN + n, l);
-          }
+          uint32_t o[16];
+          if (it.nt > 0) ma_tmem_ld_x16(o_tm + n, o);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float sum = it.nt > 0 ? __uint_as_float(l[e]) : 0.f;
-            const float y = sum == 0.f ? 0.f : __uint_as_float(o[e]);
-            if (r == n + e) s.ml[st][n + e] = make_float2(m, sum);
+            const float inv = s.inv[st][n + e], y = inv == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
             if (n + e < n_rows && r < D) {
               if (p.split > 1)
                 stage[(n + e) * D] = y;
               else
-                MaType<T>::put(dst + tok * p.ld_out + head * D, sum == 0.f ? 0.f : y * __frcp_rn(sum));
+                MaType<T>::put(at, y);
             }
-            if (++head == p.G) head = 0, ++tok;
+            at += D;
+            if (++head == p.G) head = 0, at += p.ld_out - p.G * D;
           }
         }
         const int* const n_bad = s.n_bad[list][st];

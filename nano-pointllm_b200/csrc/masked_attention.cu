@@ -197,6 +197,16 @@ __device__ __forceinline__ bool ma_wait_warp(uint64_t* bar, uint32_t parity, int
   return __all_sync(0xffffffffu, ma_wait(bar, parity, abort, status, code));
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 // D[tmem] (+)= A[tmem] * B[smem], 16-bit floats, fp32 sums (kind::f16); A packed two K elements a column.
 __device__ __forceinline__ void ma_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -356,7 +366,7 @@ __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) 
     } else {
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const uint4 x = line[c];
+        const uint4 x = line[c ^ (row & 7)];  // 8 rows use all banks
         any |= ((x.x & MaType<T>::kExp) + MaType<T>::kOne) | ((x.y & MaType<T>::kExp) + MaType<T>::kOne) |
                ((x.z & MaType<T>::kExp) + MaType<T>::kOne) | ((x.w & MaType<T>::kExp) + MaType<T>::kOne);
       }
@@ -622,80 +632,105 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
   __syncwarp();
 }
 
-// Warp 9, one thread: matrix products.
+// Warp 9: matrix products. All lanes go through it, one issues: addresses and
+// descriptors then stay in uniform registers, which tcgen05.mma reads, and the
+// votes tell the compiler that the branches are uniform too.
 template <typename S, typename T, int D, bool kTree, bool kShared>
 __device__ __forceinline__ void ma_mma_role(S& s, const MaArgs& p, uint32_t tmem, int first, int stride, int rank) {
   constexpr int kStages = S::kStages;
+  constexpr uint32_t kTile = S::kTileBytes >> 4;  // in units of a descriptor's address
   // rows as M: S = Q K^T, O = P V with P in TMEM; rows as N: S^T = K Q^T, O^T = V^T P^T with P^T in shared memory (for
   // D = 64 the rows of O^T come twice, the second time to lanes that nobody reads)
   constexpr uint32_t kIdQK = idesc_f16(kMaTile, S::kFew ? S::kRows : kMaTile, false) | MaType<T>::kIdesc;
   constexpr uint32_t kIdPV =
       idesc_f16(kMaTile, S::kFew ? S::kRows : D, true) | (S::kFew ? 1u << 15 : 0u) | MaType<T>::kIdesc;
-  int ring = 0, nq = 0;
-  uint32_t p_phase[2] = {0, 0};
-  auto full = [&](int r) -> bool {
-    return ma_wait(&s.full[r % kStages], (r / kStages) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
+  const bool issuer = elect_one();
+  const uint64_t q_desc = sdesc_k_sw128(smem_u32(s.q)), k_desc = ma_desc_k(smem_u32(s.kv), S::kGroup);
+  const uint64_t v_desc = ma_desc_mn(smem_u32(s.kv), S::kFew && D == 64 ? 0 : 1024, S::kGroup);
+  int stage = 0, nq = 0;
+  uint32_t phase = 0, p_phase[2] = {0, 0};
+  auto next = [&](int& st, uint32_t& ph) {
+    if (++st == kStages) st = 0, ph ^= 1;
   };
-  auto issue_s = [&](int st, int r, int qb) {  // S of stream st from the K tile at ring position r
-    const uint32_t qa = smem_u32(s.q[qb][st]), ka = smem_u32(s.kv[r % kStages]);
+  auto wait = [&](uint64_t* bar, uint32_t ph) -> bool {
+    const bool ok = ma_wait_warp(bar, ph, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
     tc_fence_after();
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      const uint64_t qd = sdesc_k_sw128(qa + (kk >> 2) * S::kQHalf + (kk & 3) * 32);
-      const uint64_t kd = ma_desc_k(ka + (kk >> 2) * 1024 + (kk & 3) * 32, S::kGroup);
-      mma_f16(tmem + st * S::kScoreCols, S::kFew ? kd : qd, S::kFew ? qd : kd, kIdQK, kk > 0 ? 1u : 0u);
-    }
-    tc_commit(&s.s_full[st]);
+    return ok;
   };
-  auto issue_o = [&](int st, int r, int t, bool last) -> bool {  // O of stream st (+)= P V
-    if (!ma_wait(&s.p_full[st], p_phase[st], &s.abort, p.status, NPL_DEV_TIMEOUT_MMA) || !full(r)) return false;
-    p_phase[st] ^= 1;
-    tc_fence_after();
-    const uint32_t va = smem_u32(s.kv[r % kStages]);
+  auto issue_s = [&](int st, int at, int qb) {  // S of stream st from the K tile in stage `at`
+    const uint64_t qd = q_desc + (uint32_t)(qb * 2 + st) * (sizeof(s.q[0][0]) >> 4), kd = k_desc + (uint32_t)at * kTile;
+    if (issuer) {
 #pragma unroll
-    for (int kk = 0; kk < kMaTile / 16; ++kk) {
-      const uint64_t vd = ma_desc_mn(va + kk * 2 * S::kGroup, S::kFew && D == 64 ? 0 : 1024, S::kGroup);
-      const uint32_t o = tmem + 2 * S::kScoreCols + st * S::kOutCols, on = (t > 0 || kk > 0) ? 1u : 0u;
-      if constexpr (S::kFew)
-        mma_f16(o, vd, sdesc_mn_sw128(smem_u32(s.p[st]) + kk * 16 * 128, 0, 1024), kIdPV, on);
-      else
-        ma_mma_ts(o, tmem + st * S::kScoreCols + kk * 8, vd, kIdPV, on);
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint64_t qk = qd + (((kk >> 2) * S::kQHalf + (kk & 3) * 32) >> 4), kk2 = kd + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
+        mma_f16(tmem + st * S::kScoreCols, S::kFew ? kk2 : qk, S::kFew ? qk : kk2, kIdQK, kk > 0 ? 1u : 0u);
+      }
+      tc_commit(&s.s_full[st]);
     }
-    if (last) tc_commit(&s.o_full[st]);
-    return true;
+  };
+  auto issue_o = [&](int st, int at, uint32_t add) {  // O of stream st (+)= P V
+    const uint64_t vd = v_desc + (uint32_t)at * kTile;
+    const uint32_t o = tmem + 2 * S::kScoreCols + st * S::kOutCols;
+    if (issuer) {
+#pragma unroll
+      for (int kk = 0; kk < kMaTile / 16; ++kk) {
+        const uint64_t vk = vd + (kk * 2 * S::kGroup >> 4);
+        if constexpr (S::kFew)
+          mma_f16(o, vk, sdesc_mn_sw128(smem_u32(s.p[st]), 0, 1024) + (kk * 16 * 128 >> 4), kIdPV, kk > 0 ? 1u : add);
+        else
+          ma_mma_ts(o, tmem + st * S::kScoreCols + kk * 8, vk, kIdPV, kk > 0 ? 1u : add);
+      }
+    }
   };
   bool ok = true;
   for (int i = first; ok && i < p.n_items; i += stride) {
     const MaItem it = ma_item<kTree, kShared>(p, i, rank);
-    if (it.nt == 0) continue;
+    if (__all_sync(0xffffffffu, it.nt == 0)) continue;
     const int qb = nq % S::kQBufs;
-    ok = ma_wait(&s.q_full[qb], (nq / S::kQBufs) & 1, &s.abort, p.status, NPL_DEV_TIMEOUT_MMA);
+    ok = wait(&s.q_full[qb], (nq / S::kQBufs) & 1);
     ++nq;
-    const int streams = it.second ? 2 : 1;
+    const bool two = __any_sync(0xffffffffu, it.second);
     // S of the first tile, then O of tile t and S of the next one, for each stream
 #pragma unroll 1
-    for (int t = -1; ok && t < it.nt; ++t) {
-      const bool more = t + 1 < it.nt;
-#pragma unroll 1
-      for (int st = 0; ok && st < streams; ++st) {
-        const bool last = !kShared || st == streams - 1;  // of those that read these tiles
-        const int rv = ring, rk = t >= 0 ? ring + 1 : ring;
-        if (t >= 0) {
-          if (!(ok = issue_o(st, rv, t, !more))) break;
-          if (last) tc_commit(&s.empty[rv % kStages]);
+    for (int t = -1; __all_sync(0xffffffffu, ok && t < it.nt); ++t) {
+      const bool more = __any_sync(0xffffffffu, t + 1 < it.nt), old = t >= 0;
+      int sv = stage, sk = stage;  // stages of the V and the K tile
+      uint32_t pv = phase, pk = phase;
+      if (old) next(sk, pk);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        if (st == 1 && !two) break;
+        const bool last = !kShared || st == 1 || !two;  // of those that read these tiles
+        if (old) {
+          ok = wait(&s.p_full[st], p_phase[st]) && wait(&s.full[sv], pv);
+          if (!ok) break;
+          p_phase[st] ^= 1;
+          issue_o(st, sv, t > 0 ? 1u : 0u);
+          if (issuer && last) tc_commit(&s.empty[sv]);
+          if (issuer && !more) tc_commit(&s.o_full[st]);
         }
         if (more) {
-          if (!(ok = full(rk))) break;
-          issue_s(st, rk, qb);
-          if (last) tc_commit(&s.empty[rk % kStages]);
+          ok = wait(&s.full[sk], pk);
+          if (!ok) break;
+          issue_s(st, sk, qb);
+          if (issuer && last) tc_commit(&s.empty[sk]);
         }
-        if (last) ring += (t >= 0) + more;
+        if (last) {
+          if (old) next(stage, phase);
+          if (more) next(stage, phase);
+          if (!kShared) {
+            sv = sk = stage;
+            pv = pk = phase;
+            if (old) next(sk, pk);
+          }
+        }
       }
-      if (ok && t + 2 == it.nt) tc_commit(&s.q_empty[qb]);  // the last S of the item has been issued
+      if (issuer && ok && t + 2 == it.nt) tc_commit(&s.q_empty[qb]);  // the last S of the item has been issued
     }
   }
-  tc_commit(&s.mma_done);  // arrives once every MMA issued above has completed
+  if (issuer) tc_commit(&s.mma_done);  // arrives once every MMA issued above has completed
   mbar_wait(&s.mma_done, 0, p.status, NPL_DEV_TIMEOUT_TEARDOWN);
+  __syncwarp();
 }
 
 // Barriers and tensor memory of a CTA.
@@ -787,7 +822,6 @@ __global__ void __launch_bounds__(kMaThreads, 1)
                        const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_kb,
                     const __grid_constant__ CUtensorMap tmap_vb, const __grid_constant__ MaArgs p) {
   using S = MaSmem<D>;
-  constexpr int kStages = S::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   S& s = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -804,8 +838,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
   if (warp == 8) {
     ma_load_role<S, D, kTree, kShared>(s, p, tmap_q, tmap_k, tmap_v, tmap_kb, tmap_vb, first, stride, rank);
   } else if (warp == 9) {
-    if (lane == 0) ma_mma_role<S, T, D, kTree, kShared>(s, p, tmem, first, stride, rank);
-    __syncwarp();
+    ma_mma_role<S, T, D, kTree, kShared>(s, p, tmem, first, stride, rank);
   } else if (warp >= 10) {
     ma_clean_role<S, T, D, kTree, kShared>(s, p, first, stride, rank);
   } else {
@@ -1041,7 +1074,6 @@ __global__ void __launch_bounds__(kMaThreads, 1)
                     const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_kb,
                     const __grid_constant__ CUtensorMap tmap_vb, const __grid_constant__ MaArgs p) {
   using S = MaFewSmem<D, kN>;
-  constexpr int kStages = S::kStages;
   constexpr float kNone = 3e38f;  // 6 - m of a row that has seen no key yet
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   S& s = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -1057,8 +1089,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
   if (warp == 8) {
     ma_load_role<S, D, kTree, false>(s, p, tmap_q, tmap_k, tmap_v, tmap_kb, tmap_vb, first, stride, rank);
   } else if (warp == 9) {
-    if (lane == 0) ma_mma_role<S, T, D, kTree, false>(s, p, tmem, first, stride, rank);
-    __syncwarp();
+    ma_mma_role<S, T, D, kTree, false>(s, p, tmem, first, stride, rank);
   } else if (warp >= 10) {
     ma_clean_role<S, T, D, kTree, false>(s, p, first, stride, rank);
   } else {

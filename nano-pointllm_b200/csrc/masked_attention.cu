@@ -49,7 +49,7 @@ namespace {
 
 constexpr int kMaThreads = 384;
 constexpr int kMaTile = 128;
-constexpr int kMaFixed = 4;             // what a CTA costs beside its tiles, in tiles
+constexpr int kMaFixed = 10;            // what a round of clusters costs beside its tiles, in tiles
 constexpr int kMaLists = 8;            // items whose lists of such keys are kept: more than the ring can be ahead
 constexpr int kMaBad = 12;             // keys with V elements that are not finite, remembered by a warp for an item
 constexpr int kMaPieceLog = 5;         // 32 keys of a piece at most
@@ -440,7 +440,14 @@ __device__ __forceinline__ void ma_warp_reduce(float (&v)[16], int lane, Op&& op
   v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
 }
 
-// 16 columns of this lane from TMEM.
+// 4 or 16 columns of this lane from TMEM.
+__device__ __forceinline__ void ma_tmem_ld_x4(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void ma_tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
@@ -485,6 +492,7 @@ __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, 
     const MaItem it = ma_item<kTree, kShared>(p, i, rank);
     if (it.nt == 0) continue;
     const int streams = !kShared && it.second ? 2 : 1, list = item_no % kMaLists;
+    const int pa = it.prefix + it.tok0, pb = it.prefix + min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1)) - 1;
     if (lane < 2) s.n_bad[list][lane][which] = 0;
     __syncwarp();
 #pragma unroll 1
@@ -503,6 +511,8 @@ __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, 
         for (int row = which * 64 + lane; row < which * 64 + 64; row += 32) {
           const int x = xt + row, key = x < it.sink_x ? x : x + it.shift;
           const bool some = x < it.x1 && key < it.hi && (kTree || key >= it.lo || key < p.sinks);
+          // a row that every row of the item sees is left as it is
+          if (some && (kTree ? key < it.prefix : key <= pa && (key > pb - p.window || key < p.sinks))) continue;
           if (ma_clean_row<T, D>(s.kv[r % kStages], row, some)) {
             const int at = atomicAdd(&s.n_bad[list][st][which], 1);
             if (at < kMaBad) s.bad[list][st][which][at] = key;
@@ -1278,11 +1288,11 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         T* at = dst;
         int head = 0;
 #pragma unroll 1
-        for (int n = 0; n < n_rows; n += 16) {
-          uint32_t o[16];
-          if (it.nt > 0) ma_tmem_ld_x16(o_tm + n, o);
+        for (int n = 0; n < n_rows; n += 4) {
+          uint32_t o[4];
+          if (it.nt > 0) ma_tmem_ld_x4(o_tm + n, o);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < 4; ++e) {
             const float inv = s.inv[st][n + e], y = inv == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
             if (n + e < n_rows && r < D) {
               if (p.split > 1)
@@ -1415,17 +1425,22 @@ int launch(const char* what, MaArgs p, cudaStream_t st) {
   }
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status(what);
-  // Clusters of the size with the least rounds of (tiles of a CTA + kMaFixed for a CTA's start and the join).
+  // The cluster size with the least time in tiles of 128 keys: the longest item, or all rounds of clusters, each with
+  // kMaFixed for the start of its CTAs and the join (a tile of two kv heads takes 1.7 us, a round without any 10 to
+  // 15: 16 drafts over 1024 keys of 32 heads in 25.1, 21.2, 17.2 and 29.6 us split 1, 2, 4 and 8 ways). Contexts may
+  // have any length up to the table's: three quarters of it are taken as usual. Windows are mostly full.
   long long keys = (long long)p.max_blocks * p.block_size;  // the most that an item's rows may see
   if (!kTree) keys = std::min(keys, (long long)p.window + p.sinks + 2 * p.tokens);
   const int sms = num_sms() > 0 ? num_sms() : 148;
   p.split_log = 0;
-  long long least = 0;
-  for (int lg = 0; (1 << lg) <= kMaMaxSplit && (lg == 0 || p.n_items << (lg - 1) < sms); ++lg) {
+  double least = 0.0;
+  for (int lg = 0; (1 << lg) <= kMaMaxSplit && (lg == 0 || p.n_items << (lg - 1) < 2 * sms); ++lg) {
     const int fit = lg == 0 ? sms : max_active_clusters(reinterpret_cast<const void*>(kernel), smem, 1 << lg, kMaThreads);
     if (fit <= 0) break;
-    const long long tiles = ((keys >> lg) + kMaTile - 1) / kMaTile;
-    const long long cost = (p.n_items + fit - 1) / fit * (tiles + kMaFixed);
+    const double most = (double)((keys >> lg) + kMaTile - 1) / kMaTile, usual = kTree ? 0.75 * most : most;
+    const int rounds = (p.n_items + fit - 1) / fit;  // without a split the CTAs stay
+    const double all = lg == 0 ? rounds * usual + kMaFixed : rounds * (usual + kMaFixed);
+    const double cost = std::max(most + kMaFixed, all);
     if (lg == 0 || cost < least) least = cost, p.split_log = lg;
   }
   p.split = 1 << p.split_log;

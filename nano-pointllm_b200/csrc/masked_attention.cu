@@ -55,6 +55,7 @@ constexpr int kMaBad = 12;             // keys with V elements that are not fini
 constexpr int kMaPieceLog = 5;         // 32 keys of a piece at most
 constexpr int kMaBoxLog = 7;           // 128 keys of a load at most
 constexpr int kMaMaxSplit = 8;          // CTAs of a cluster at most
+constexpr int kMaPoly = 4;              // of as many pairs of exponentials one by a polynomial
 constexpr float kMaShift = 6.f;        // p = 2^(x - m + 6)
 constexpr float kMaSlack = 8.f;        // m moves when a score is more than this above it
 
@@ -235,6 +236,10 @@ __device__ __forceinline__ void ma_tmem_wait_ld(uint32_t (&r)[32]) {
                  "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]));
   asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
+__device__ __forceinline__ void ma_tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  ma_tmem_st_x16(taddr, r);
+  ma_tmem_st_x16(taddr + 16, r + 16);
+}
 __device__ __forceinline__ void ma_tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float4 ma_ld_cluster(uint32_t addr) {
@@ -251,24 +256,86 @@ __device__ __forceinline__ float2 ma_ld_cluster2(uint32_t addr) {
   return v;
 }
 
-// Scores of columns that are not seen become minus infinity.
-__device__ __forceinline__ void ma_hide(uint32_t (&v)[32], uint32_t seen) {
+// Scores of columns that are not seen become minus infinity. False: every row of the warp sees all of them.
+__device__ __forceinline__ bool ma_hide(uint32_t (&v)[32], uint32_t seen) {
+  if (__all_sync(0xffffffffu, seen == 0xffffffffu)) return false;
 #pragma unroll
   for (int c = 0; c < 32; ++c)
     if (!(seen & (1u << c))) v[c] = 0xff800000u;
+  return true;
 }
 
-// p = 2^(score c2 + add) of 32 columns, packed; their sums go to ls.
-template <typename T>
-__device__ __forceinline__ void ma_exp_pack(const uint32_t (&v)[32], float c2, float add, float (&ls)[4],
+__device__ __forceinline__ void ma_max32(const uint32_t (&v)[32], float (&mx)[4]) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 2)
+    mx[c >> 1 & 3] = fmaxf(mx[c >> 1 & 3], fmaxf(__uint_as_float(v[c]), __uint_as_float(v[c + 1])));
+}
+
+// Two fp32 numbers in one operation.
+__device__ __forceinline__ uint64_t ma_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 ma_unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t ma_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t ma_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 2^x for two x <= 127 without the special function unit, which is what the
+// softmax of many rows waits for: x = n + f with the whole number n next to x (by
+// adding 1.5 * 2^23), 2^f by the polynomial of degree 5 with the least relative
+// error on [-1/2, 1/2] (Remez; 7.5e-8), n added to its exponent. x below -127
+// gives a denormal number or 0.
+__device__ __forceinline__ float2 ma_exp2_poly(uint64_t x2) {
+  const float2 u = ma_unpair(x2);
+  float x0, x1;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(u.x), "f"(-127.f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(u.y), "f"(-127.f));
+  const uint64_t x = ma_pair(x0, x1);
+  const uint64_t t = ma_add2(x, ma_pair(12582912.f, 12582912.f));
+  const uint64_t n = ma_add2(t, ma_pair(-12582912.f, -12582912.f));
+  const uint64_t f = ma_fma2(n, ma_pair(-1.f, -1.f), x);
+  uint64_t y = ma_pair(1.3276472454890609e-03f, 1.3276472454890609e-03f);
+  y = ma_fma2(y, f, ma_pair(9.675540961325169e-03f, 9.675540961325169e-03f));
+  y = ma_fma2(y, f, ma_pair(5.550713092088699e-02f, 5.550713092088699e-02f));
+  y = ma_fma2(y, f, ma_pair(2.4022120237350464e-01f, 2.4022120237350464e-01f));
+  y = ma_fma2(y, f, ma_pair(6.931469440460205e-01f, 6.931469440460205e-01f));
+  y = ma_fma2(y, f, ma_pair(1.0000001192092896f, 1.0000001192092896f));
+  const float2 r = ma_unpair(y), tt = ma_unpair(t);
+  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(tt.x) << 23)),
+                     __int_as_float(__float_as_int(r.y) + (__float_as_int(tt.y) << 23)));
+}
+
+// p = 2^(score c2 + add) of 32 columns, packed; their sums go to ls. One pair of
+// kPoly takes the polynomial (0: none).
+template <typename T, int kPoly>
+__device__ __forceinline__ void ma_exp_pack(const uint32_t (&v)[32], float c2, float add, uint64_t (&ls)[2],
                                             uint32_t (&pk)[16]) {
+  const uint64_t c22 = ma_pair(c2, c2), add2 = ma_pair(add, add);
 #pragma unroll
   for (int c = 0; c < 16; ++c) {
-    const float p0 = ma_exp2(fmaf(__uint_as_float(v[2 * c]), c2, add));
-    const float p1 = ma_exp2(fmaf(__uint_as_float(v[2 * c + 1]), c2, add));
-    ls[(2 * c) & 3] += p0;
-    ls[(2 * c + 1) & 3] += p1;
-    pk[c] = MaType<T>::pack(p0, p1);
+    const uint64_t x = ma_fma2(ma_pair(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), c22, add2);
+    float2 e;
+    if (kPoly && c % kPoly == kPoly - 1) {
+      e = ma_exp2_poly(x);
+    } else {
+      const float2 u = ma_unpair(x);
+      e = make_float2(ma_exp2(u.x), ma_exp2(u.y));
+    }
+    ls[c & 1] = ma_add2(ls[c & 1], ma_pair(e.x, e.y));
+    pk[c] = MaType<T>::pack(e.x, e.y);
   }
 }
 
@@ -282,6 +349,7 @@ struct MaItem {
   int b, kvh, tok0, n, ctx, start, prefix;
   int lo, hi;  // keys that some row of the item sees: lo <= key < hi, and the sinks
   int sink_x, hole_x, shift, x0, x1, nt;
+  int full0, full1;  // full0 <= x < full1: every row of the item sees the key
   bool skip, second;  // no such rows; the second stream has rows
 };
 
@@ -324,25 +392,26 @@ __device__ __forceinline__ MaItem ma_item(const MaArgs& p, int i, int rank) {
   it.x0 = t0 * kMaTile;
   it.x1 = min(end, it.x0 + it.nt * kMaTile);
   if (it.skip) it.nt = 0;
+  it.full0 = 0;
+  it.full1 = min(it.prefix, it.x1);
+  if (!kTree) {
+    // what the item's first row and its last row both see
+    const int from = max(0, it.prefix + last - p.window);
+    it.full0 = from <= p.sinks && !it.shift ? 0 : from - it.shift;
+    it.full1 = min(it.prefix + it.tok0 + 1 - it.shift, it.x1);
+  }
   return it;
 }
 
 // The n lowest bits of word w of a 128-bit mask of columns.
 __device__ __forceinline__ uint32_t ma_low(int n, int w) {
-  n -= w * 32;
-  return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+  uint32_t above;  // shl takes more than 31 places too
+  asm("shl.b32 %0, %1, %2;" : "=r"(above) : "r"(0xffffffffu), "r"(max(n - w * 32, 0)));
+  return ~above;
 }
 
 // Whether some row of a CTA's item does not see some of the tile's columns from xt on.
-template <bool kTree, bool kShared>
-__device__ __forceinline__ bool ma_part(const MaArgs& p, const MaItem& it, int xt) {
-  if (kTree) return xt + kMaTile > min(it.prefix, it.x1);
-  // the columns that the item's first row and its last row both see, every row sees
-  const int pa = it.prefix + it.tok0, pb = it.prefix + min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1)) - 1;
-  const int a = min(it.sink_x ? p.sinks : min(p.sinks, pa + 1), it.x1) - xt;
-  const int b = max(0, pb - p.window + 1) - it.shift - xt, e = min(pa + 1 - it.shift, it.x1) - xt;
-  return a < kMaTile && (e < kMaTile || b > max(0, a));
-}
+__device__ __forceinline__ bool ma_part(const MaItem& it, int xt) { return xt < it.full0 || xt + kMaTile > it.full1; }
 
 // Whether the row of a token sees a key (the same as the bits below, for one key).
 template <bool kTree>
@@ -498,7 +567,7 @@ __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, 
 #pragma unroll 1
     for (int t = 0; ok && t < it.nt; ++t) {
       const int xt = it.x0 + t * kMaTile;
-      if (!ma_part<kTree, kShared>(p, it, xt)) continue;
+      if (!ma_part(it, xt)) continue;
 #pragma unroll 1
       for (int st = 0; ok && st < streams; ++st) {
         // V's place in the order of the loads
@@ -602,7 +671,7 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
     const int streams = !kShared && it.second ? 2 : 1;
 #pragma unroll 1
     for (int t = -1; ok && t < it.nt; ++t) {
-      const bool part = t >= 0 && ma_part<kTree, kShared>(p, it, it.x0 + t * kMaTile);
+      const bool part = t >= 0 && ma_part(it, it.x0 + t * kMaTile);
       const int after = t + 2 < it.nt ? lookup(t + 2) : -1;  // ahead of the wait for a free stage
 #pragma unroll 1
       for (int n = t < 0 ? 1 : 0; ok && n < 2 * streams; ++n) {
@@ -862,11 +931,12 @@ __global__ void __launch_bounds__(kMaThreads, 1)
     uint32_t s_phase = 0, o_phase = 0;
     int item_no = 0;
     bool ok = true;
+    MaItem ahead = ma_item<kTree, kShared>(p, min(first, p.n_items - 1), rank);
     for (int i = first; ok && i < p.n_items; i += stride) {
-      const MaItem it = ma_item<kTree, kShared>(p, i, rank);
-      if (it.skip) continue;
-      if (st == 1 && !it.second) {
-        if (it.nt > 0) ++item_no;
+      const MaItem it = ahead;
+      if (it.skip || (st == 1 && !it.second)) {
+        if (!it.skip && it.nt > 0) ++item_no;
+        ahead = ma_item<kTree, kShared>(p, min(i + stride, p.n_items - 1), rank);
         continue;
       }
       const int kvh = it.kvh + (kShared ? 0 : st);
@@ -878,11 +948,14 @@ __global__ void __launch_bounds__(kMaThreads, 1)
       const int list = item_no % kMaLists;
       bool any_part = false;
       float m = -INFINITY, l = 0.f;  // m in units of log2
+      // this row sees x < row_a and row_b <= x < row_e (window)
+      const int row_a = row_ok ? min(it.sink_x ? p.sinks : min(p.sinks, pos + 1), it.x1) : 0;
+      const int row_b = max(0, pos - p.window + 1) - it.shift, row_e = row_ok ? min(pos + 1 - it.shift, it.x1) : 0;
       for (int t = 0; ok && t < it.nt; ++t) {
         const int xt = it.x0 + t * kMaTile;
         // which of the tile's columns this row sees
         uint32_t seen[4];
-        const bool part = ma_part<kTree, kShared>(p, it, xt);
+        const bool part = ma_part(it, xt);
         any_part |= part;
         if (kTree) {
 #pragma unroll
@@ -908,10 +981,9 @@ __global__ void __launch_bounds__(kMaThreads, 1)
 #pragma unroll
           for (int w = 0; w < 4; ++w) seen[w] = 0xffffffffu;
           if (part) {
-            const int a = min(it.sink_x ? p.sinks : min(p.sinks, pos + 1), it.x1) - xt;
-            const int b = max(0, pos - p.window + 1) - it.shift - xt, e = min(pos + 1 - it.shift, it.x1) - xt;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) seen[w] = row_ok ? ma_low(a, w) | (ma_low(e, w) & ~ma_low(b, w)) : 0u;
+            for (int w = 0; w < 4; ++w)
+              seen[w] = ma_low(row_a - xt, w) | (ma_low(row_e - xt, w) & ~ma_low(row_b - xt, w));
           }
         }
         if (!ma_wait_warp(&s.s_full[st], s_phase, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE)) {
@@ -921,70 +993,77 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         s_phase ^= 1;
         tc_fence_after();
         if (warp_on) {
-          // The row is read twice, 32 columns at a time and the next ones ahead: its maximum, then the exponentials.
-          // (Held in registers, its 128 scores spilled; and the loops stay rolled for the sake of short calls.)
           const bool masked = __any_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu);
-          uint32_t va[32], vb[32];
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          tmem_ld_x32(s_tm, va);
+          uint64_t ls[2] = {ma_pair(0.f, 0.f), ma_pair(0.f, 0.f)};
+          // m moves to the tile's maximum where that is far above it, and the sums with it
+          auto settle = [&]() -> float {
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c2;
+            const bool move = t == 0 || top > m + kMaSlack;
+            const float m_new = move ? top : m;
+            if (t > 0 && __any_sync(0xffffffffu, move)) {
+              const float alpha = !move ? 1.f : m == -INFINITY ? 0.f : ma_exp2(m - m_new);
+              l *= alpha;
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            ma_tmem_wait_ld(va);
-            tmem_ld_x32(s_tm + h * 64 + 32, vb);
-            if (masked) ma_hide(va, h ? seen[2] : seen[0]);
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld_x32(o_tm + c * 32, o);
+                ma_tmem_wait_ld(o);
 #pragma unroll
-            for (int c = 0; c < 32; c += 2)
-              mx[c >> 1 & 3] = fmaxf(mx[c >> 1 & 3], fmaxf(__uint_as_float(va[c]), __uint_as_float(va[c + 1])));
-            ma_tmem_wait_ld(vb);
-            tmem_ld_x32(s_tm + (h ? 0 : 64), va);  // at the end: the first columns again
-            if (masked) ma_hide(vb, h ? seen[3] : seen[1]);
-#pragma unroll
-            for (int c = 0; c < 32; c += 2)
-              mx[c >> 1 & 3] = fmaxf(mx[c >> 1 & 3], fmaxf(__uint_as_float(vb[c]), __uint_as_float(vb[c + 1])));
-          }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c2;
-          const bool move = t == 0 || top > m + kMaSlack;
-          const float m_new = move ? top : m;
-          if (t > 0 && __any_sync(0xffffffffu, move)) {
-            const float alpha = !move ? 1.f : m == -INFINITY ? 0.f : ma_exp2(m - m_new);
-            l *= alpha;
-            ma_tmem_wait_ld(va);
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld_x32(o_tm + c * 32, o);
-              ma_tmem_wait_ld(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              ma_tmem_st_x16(o_tm + c * 32, o);
-              ma_tmem_st_x16(o_tm + c * 32 + 16, o + 16);
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                ma_tmem_st_x16(o_tm + c * 32, o);
+                ma_tmem_st_x16(o_tm + c * 32 + 16, o + 16);
+              }
             }
-          }
-          m = m_new;
-          const float add = m == -INFINITY ? 0.f : kMaShift - m;
-          float ls[4] = {0.f, 0.f, 0.f, 0.f};
+            m = m_new;
+            const float add = m == -INFINITY ? 0.f : kMaShift - m;
+            return add;
+          };
+          // The row is read twice, 32 columns at a time and the next ones ahead: its maximum, then the exponentials.
+          // (Held in registers, its 128 scores spilled.) Masked scores are written back in between.
+          uint32_t v[2][32];
+          tmem_ld_x32(s_tm, v[0]);
+          if (!masked) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              ma_tmem_wait_ld(v[h & 1]);
+              tmem_ld_x32(s_tm + (h < 3 ? h + 1 : 0) * 32, v[(h + 1) & 1]);
+              ma_max32(v[h & 1], mx);
+            }
+          } else {
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            // P goes over columns of S that have been read
-            uint32_t pk[16];
-            ma_tmem_wait_ld(va);
-            tmem_ld_x32(s_tm + h * 64 + 32, vb);
-            if (masked) ma_hide(va, h ? seen[2] : seen[0]);
-            ma_exp_pack<T>(va, p.c2, add, ls, pk);
-            ma_tmem_st_x16(s_tm + h * 32, pk);
-            ma_tmem_wait_ld(vb);
-            if (h == 0) tmem_ld_x32(s_tm + 64, va);
-            if (masked) ma_hide(vb, h ? seen[3] : seen[1]);
-            ma_exp_pack<T>(vb, p.c2, add, ls, pk);
-            ma_tmem_st_x16(s_tm + h * 32 + 16, pk);
+            for (int h = 0; h < 4; h += 2) {
+              ma_tmem_wait_ld(v[0]);
+              tmem_ld_x32(s_tm + (h + 1) * 32, v[1]);
+              if (ma_hide(v[0], h ? seen[2] : seen[0])) ma_tmem_st_x32(s_tm + h * 32, v[0]);
+              ma_max32(v[0], mx);
+              ma_tmem_wait_ld(v[1]);
+              if (h == 0) tmem_ld_x32(s_tm + 64, v[0]);
+              if (ma_hide(v[1], h ? seen[3] : seen[1])) ma_tmem_st_x32(s_tm + h * 32 + 32, v[1]);
+              ma_max32(v[1], mx);
+            }
+            ma_tmem_wait_st();
+            tmem_ld_x32(s_tm, v[0]);
           }
-          l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+          ma_tmem_wait_ld(v[0]);
+          const float add = settle();
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            uint32_t pk[16];
+            if (h > 0) ma_tmem_wait_ld(v[h & 1]);
+            if (h < 3) tmem_ld_x32(s_tm + (h + 1) * 32, v[(h + 1) & 1]);
+            ma_exp_pack<T, kMaPoly>(v[h & 1], p.c2, add, ls, pk);
+            ma_tmem_st_x16(s_tm + h * 16, pk);  // over columns that have been read
+          }
+          const float2 l0 = ma_unpair(ls[0]), l1 = ma_unpair(ls[1]);
+          l += (l0.x + l0.y) + (l1.x + l1.y);
           ma_tmem_wait_st();
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.p_full[st]);
       }
+      ahead = ma_item<kTree, kShared>(p, min(i + stride, p.n_items - 1), rank);  // while the last products run
       // every MMA of the item has completed; before the partial sums go over the ring, those of the other stream too
       if (ok && it.nt > 0) {
         ok = ma_wait_warp(&s.o_full[st], o_phase, &s.abort, p.status, NPL_DEV_TIMEOUT_EPILOGUE);
@@ -1008,24 +1087,24 @@ __global__ void __launch_bounds__(kMaThreads, 1)
             tmem_ld_x32(o_tm + c * 32, o);
             ma_tmem_wait_ld(o);
           }
-          float acc[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) acc[e] = l == 0.f ? 0.f : __uint_as_float(o[e]);
           if (!row_ok) continue;
+          if (l == 0.f) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
           if (p.split > 1) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)  // 16-byte chunks exchanged within 8, so that 8 rows use all banks
-              *reinterpret_cast<float4*>(stage + (((c * 8 + e) ^ (r & 7)) << 2)) =
-                  make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+              *reinterpret_cast<uint4*>(stage + (((c * 8 + e) ^ (r & 7)) << 2)) =
+                  make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              uint4 w;
-              w.x = MaType<T>::pack(acc[8 * e] * inv, acc[8 * e + 1] * inv);
-              w.y = MaType<T>::pack(acc[8 * e + 2] * inv, acc[8 * e + 3] * inv);
-              w.z = MaType<T>::pack(acc[8 * e + 4] * inv, acc[8 * e + 5] * inv);
-              w.w = MaType<T>::pack(acc[8 * e + 6] * inv, acc[8 * e + 7] * inv);
-              reinterpret_cast<uint4*>(dst)[c * 4 + e] = w;
+              uint32_t w[4];
+#pragma unroll
+              for (int d = 0; d < 4; ++d)
+                w[d] = MaType<T>::pack(__uint_as_float(o[8 * e + 2 * d]) * inv, __uint_as_float(o[8 * e + 2 * d + 1]) * inv);
+              reinterpret_cast<uint4*>(dst)[c * 4 + e] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
         }
@@ -1132,7 +1211,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
       for (int t = 0; ok && t < it.nt; ++t) {
         const int xt = it.x0 + t * kMaTile, x = xt + r, key = x < it.sink_x ? x : x + it.shift;
         // which rows see this thread's key, and whether all rows see all of the tile's keys
-        const bool part = ma_part<kTree, false>(p, it, xt);
+        const bool part = ma_part(it, xt);
         any_part |= part;
         uint32_t seen[(kN + 31) / 32];
         const bool some = x < it.x1 && key < it.hi && (kTree || key >= it.lo || key < p.sinks);

@@ -59,6 +59,20 @@ constexpr int kMaPoly = 4;              // of as many pairs of exponentials one 
 constexpr float kMaShift = 6.f;        // p = 2^(x - m + 6)
 constexpr float kMaSlack = 8.f;        // m moves when a score is more than this above it
 
+// Division of 0 <= n < 2^31 by a number known at the launch: with s = ceil(log2 d) and mul = ceil(2^(31 + s) / d),
+// floor(n / d) = floor(n mul / 2^(31 + s)), since n (mul d - 2^(31 + s)) < 2^31 2^s. One number needs one of these
+// instead of 30 instructions, which a CTA that runs them once has to fetch.
+struct MaDiv {
+  uint32_t mul;
+  int shift;  // s - 1, -1 for d = 1
+  static MaDiv of(int d) {
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s - 1};
+  }
+  __device__ __forceinline__ int operator()(int n) const { return shift < 0 ? n : (int)(__umulhi(n, mul) >> shift); }
+};
+
 struct MaArgs {
   const void* q;
   void* out;
@@ -80,6 +94,7 @@ struct MaArgs {
   int box_log;           // pieces of a large load, a power of two
   int levels;   // items of a sequence and kv head (or pair of them)
   int n_items;  // levels * B * (kv heads, or pairs of them)
+  MaDiv by_levels, by_units, by_group, by_page;
   int split, split_log;  // CTAs of a cluster, which share an item's keys, a power of two
   float c2;     // scale * log2(e)
   int* status;
@@ -357,8 +372,8 @@ template <bool kTree, bool kShared>
 __device__ __forceinline__ MaItem ma_item(const MaArgs& p, int i, int rank) {
   MaItem it;
   const int units = kShared ? p.Hkv : (p.Hkv + 1) / 2;
-  const int level = i % p.levels, rem = i / p.levels;
-  it.b = rem / units;
+  const int rem = p.by_levels(i), level = i - rem * p.levels;
+  it.b = p.by_units(rem);
   it.kvh = (rem - it.b * units) * (kShared ? 1 : 2);
   it.tok0 = level * p.tokens * (kShared ? 2 : 1);
   it.n = p.q_lens ? p.q_lens[it.b] : 1;
@@ -466,10 +481,10 @@ __device__ __noinline__ float ma_bad_sum(const MaArgs* args, const int* counts, 
     const int x = it.x0 + j;
     const int key = all ? (x < it.sink_x ? x : x + it.shift) : j < counts[0] ? lists[0][j] : lists[1][j - counts[0]];
     if (key >= it.hi || !ma_sees<kTree>(p, it, token, key)) continue;
-    const int page = key / p.block_size;
+    const int page = p.by_page(key);
     const int blk = page < p.max_blocks ? p.bt[it.b * p.bt_stride + page] : -1;
     if (blk < 0 || blk >= p.num_blocks) continue;
-    const size_t at = (((size_t)blk * p.block_size + key % p.block_size) * p.Hkv + kvh) * D + col;
+    const size_t at = (((size_t)blk * p.block_size + (key - page * p.block_size)) * p.Hkv + kvh) * D + col;
     const float v = MaType<T>::get(p.v, at);
     if (!isfinite(v)) sum += v;
   }
@@ -633,7 +648,7 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
       const int x = it.x0 + t * kMaTile + (lane << p.piece_log);
       if (lane >= per_tile || x >= it.x1 || (x >= it.sink_x && x < it.hole_x)) return -1;
       const int key = x < it.sink_x ? x : x + it.shift;
-      const int page = key / p.block_size;
+      const int page = p.by_page(key);
       const int blk = page < p.max_blocks ? table[page] : -1;
       if (blk < 0 || blk >= p.num_blocks) {
         atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
@@ -887,8 +902,9 @@ __device__ __forceinline__ void ma_join(const MaArgs& p, const MaItem& it, int r
     }
     const float inv = l == 0.f ? 0.f : __frcp_rn(l);
     if (on) {
-      T* const dst = static_cast<T*>(p.out) + (it.start + it.tok0 + token_of(st) + r / p.G) * p.ld_out +
-                     (long long)((it.kvh + head_of(st)) * p.G + r % p.G) * D;
+      const int tok = p.by_group(r);
+      T* const dst = static_cast<T*>(p.out) + (it.start + it.tok0 + token_of(st) + tok) * p.ld_out +
+                     (long long)((it.kvh + head_of(st)) * p.G + r - tok * p.G) * D;
       reinterpret_cast<uint2*>(dst)[col] =
           make_uint2(MaType<T>::pack(acc.x * inv, acc.y * inv), MaType<T>::pack(acc.z * inv, acc.w * inv));
     }
@@ -924,7 +940,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
     // -------------------------------------------------------- softmax
     const int st = warp >> 2;            // stream
     const int r = threadIdx.x & 127;     // row of the tile = TMEM lane
-    const int row_tok = r / p.G, row_head = r - row_tok * p.G;
+    const int row_tok = p.by_group(r), row_head = r - row_tok * p.G;
     const uint32_t lane_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_tm = lane_tm + st * 128, o_tm = lane_tm + 256 + st * 128;
     const int owner = kShared ? 0 : st;  // the stream whose V tiles this one reads
@@ -1389,7 +1405,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
 #pragma unroll 1
           for (int n = 0; n < n_rows; ++n) {
             if (r >= D || s.ml[st][n].y == 0.f) continue;
-            const int of = n / p.G;
+            const int of = p.by_group(n);
             const float x = ma_bad_sum<T, D, kTree, false>(&p, n_bad, s.bad[list][st], i, rank, it.tok0 + of,
                                                                      kvh, r);
             if (x == 0.f) continue;
@@ -1485,6 +1501,10 @@ int launch(const char* what, MaArgs p, cudaStream_t st) {
   const long long items = (long long)p.levels * p.B * (kShared ? p.Hkv : (p.Hkv + 1) / 2);
   if (items >= (1ll << 27)) return fail(NPL_ERR_UNSUPPORTED, "%s: too many row tiles", what);
   p.n_items = (int)items;
+  p.by_levels = MaDiv::of(p.levels);
+  p.by_units = MaDiv::of(kShared ? p.Hkv : (p.Hkv + 1) / 2);
+  p.by_group = MaDiv::of(p.G);
+  p.by_page = MaDiv::of(p.block_size);
   CUtensorMap tq, tk, tv, tkb, tvb;
   const long long slots = (long long)p.num_blocks * p.block_size;
   const int box = p.piece << p.box_log;

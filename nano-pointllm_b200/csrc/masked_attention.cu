@@ -132,7 +132,7 @@ struct MaFewSmem : MaBarriers {
   static constexpr uint32_t kQHalf = kN * 128;
   static constexpr uint32_t kGroup = 8 * D * 2;
   static constexpr uint32_t kTileBytes = kMaTile * D * 2;
-  static constexpr int kStages = D == 64 ? 10 : kN == 64 ? 4 : 5;
+  static constexpr int kStages = D == 64 ? 10 : 5;
   static constexpr uint32_t kScoreCols = kN, kOutCols = kN, kTmemCols = 4 * kN;  // S of the streams, then O
   uint64_t full[kStages], empty[kStages], raw[kStages];
   alignas(16) float add[2][kN];  // of a row: 6 - m
@@ -140,15 +140,16 @@ struct MaFewSmem : MaBarriers {
   float top[2][4][kN];           // a warp's maxima, at the end its sums
   float2 ml[2][kN];              // m and the normaliser at the end
   float inv[2][kN];              // and what a row of sums is multiplied with
-  static constexpr int kQBufs = kN == 64 ? 1 : 2;  // Q of this item and of the next one
+  static constexpr int kQBufs = kN == 16 ? 2 : 1;  // Q of this item, and of the next one where there is room
   alignas(1024) uint8_t q[kQBufs][2][kN * D * 2];
   alignas(1024) uint8_t p[2][kMaTile * 128];  // P^T: a key's rows in one 128-byte line
   alignas(1024) uint8_t kv[kStages][kTileBytes];
 };
 
-static_assert(sizeof(MaSmem<128>) + 1024 <= 232448 && sizeof(MaSmem<64>) + 1024 <= 232448 &&
-                  sizeof(MaFewSmem<128, 64>) + 1024 <= 232448 && sizeof(MaFewSmem<64, 64>) + 1024 <= 232448,
-              "shared memory of an SM");
+constexpr size_t kMaMaxSmem = 232448 - 1024;  // of a CTA, without the room to align
+static_assert(sizeof(MaSmem<128>) <= kMaMaxSmem && sizeof(MaSmem<64>) <= kMaMaxSmem, "shared memory");
+static_assert(sizeof(MaFewSmem<128, 16>) <= kMaMaxSmem && sizeof(MaFewSmem<64, 16>) <= kMaMaxSmem, "shared memory");
+static_assert(sizeof(MaFewSmem<128, 32>) <= kMaMaxSmem && sizeof(MaFewSmem<64, 32>) <= kMaMaxSmem, "shared memory");
 
 template <typename T>
 struct MaType;
@@ -1553,7 +1554,6 @@ int run_type(const char* what, const MaArgs& p, cudaStream_t st) {
   const long long rows = (long long)p.max_q_len * p.G;
   if (rows <= 16) return launch<T, D, kTree, 16>(what, p, st);
   if (rows <= 32) return launch<T, D, kTree, 32>(what, p, st);
-  if (rows <= 64) return launch<T, D, kTree, 64>(what, p, st);
   if (p.max_q_len <= kMaTile / p.G) return launch<T, D, kTree, 128>(what, p, st);
   return launch<T, D, kTree, 0>(what, p, st);
 }

@@ -123,6 +123,10 @@ TREES = [
     ([(40, 3000)], 16, 1, 128, 48),
     ([(3, 127), (3, 128), (3, 129), (3, 131), (1, 0), (2, 9000)], 6, 2, 128, 8),
     ([(5, 260)] * 40, 4, 4, 64, 128),
+    ([(32, 500), (17, 900), (1, 40)], 4, 4, 128, 256),
+    ([(31, 1500), (24, 333)], 3, 3, 64, 16),
+    ([(6, 700), (5, 2000)], 10, 2, 128, 32),
+    ([(33, 600), (9, 64)], 4, 4, 128, 16),
 ]
 
 
@@ -185,6 +189,10 @@ WINDOWS = [
     ([(260, 1260)], 2, 2, 128, 64, 1, 1),
     ([(333, 1333), (20, 20)], 3, 1, 128, 40, 100, 200),
     ([(128, 600), (127, 600), (3, 600)], 2, 2, 128, 128, 5000, 10000),
+    ([(1, 900), (1, 5)], 32, 1, 128, 16, 200, 3),
+    ([(1, 900), (1, 5)], 34, 1, 64, 64, 200, 3),
+    ([(20, 300), (3, 3000)], 3, 3, 128, 256, 256, 4),
+    ([(1, 3000)], 80, 1, 128, 16, 1000, 0),
 ]
 
 

@@ -51,7 +51,7 @@ constexpr int kMaThreads = 384;
 constexpr int kMaTile = 128;
 constexpr int kMaFixed = 10;            // what a round of clusters costs beside its tiles, in tiles
 constexpr int kMaLists = 8;            // items whose lists of such keys are kept: more than the ring can be ahead
-constexpr int kMaBad = 12;             // keys with V elements that are not finite, remembered by a warp for an item
+constexpr int kMaBad = 12;             // keys with V elements that are not finite, remembered for an item
 constexpr int kMaPieceLog = 5;         // 32 keys of a piece at most
 constexpr int kMaBoxLog = 7;           // 128 keys of a load at most
 constexpr int kMaMaxSplit = 8;          // CTAs of a cluster at most
@@ -104,8 +104,8 @@ struct MaBarriers {
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], mma_done;
   uint32_t tmem_base;
   int abort;
-  // keys whose V rows held elements that are not finite: [item % kMaLists][stream whose V it is][warp 10 or 11]
-  int n_bad[kMaLists][2][2];
+  // keys whose V rows held elements that are not finite: [item % kMaLists][stream whose V it is]
+  int n_bad[kMaLists][2][2];  // the last: warp 10 or 11
   int bad[kMaLists][2][2][kMaBad];
 };
 
@@ -163,6 +163,11 @@ struct MaType<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   __device__ static float get(const void* p, size_t i) { return __half2float(static_cast<const __half*>(p)[i]); }
+  __device__ static uint32_t times0(uint32_t v, uint32_t sum) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v), __half2half2(__ushort_as_half(0)),
+                              *reinterpret_cast<const __half2*>(&sum));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
   __device__ static void put(__half* p, float x) { *p = __float2half_rn(x); }
   __device__ static void add(__half* p, float x) { *p = __float2half_rn(__half2float(*p) + x); }
 };
@@ -177,6 +182,11 @@ struct MaType<__nv_bfloat16> {
   }
   __device__ static float get(const void* p, size_t i) {
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  }
+  __device__ static uint32_t times0(uint32_t v, uint32_t sum) {
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(0.f),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&sum));
+    return *reinterpret_cast<const uint32_t*>(&r);
   }
   __device__ static void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
   __device__ static void add(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(__bfloat162float(*p) + x); }
@@ -441,7 +451,7 @@ __device__ __forceinline__ bool ma_sees(const MaArgs& p, const MaItem& it, int t
 // whether it held elements that are not finite, which are now 0.
 template <typename T, int D>
 __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) {
-  uint32_t any = 0;
+  uint32_t any[4] = {0, 0, 0, 0};  // sums of 0 * v: NaN where v is not finite
 #pragma unroll 1
   for (int hf = 0; hf < D / 64; ++hf) {
     uint4* line = reinterpret_cast<uint4*>(tile + (row >> 3) * (8 * D * 2) + hf * 1024 + (row & 7) * 128);
@@ -452,12 +462,12 @@ __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) 
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const uint4 x = line[c ^ (row & 7)];  // 8 rows use all banks
-        any |= ((x.x & MaType<T>::kExp) + MaType<T>::kOne) | ((x.y & MaType<T>::kExp) + MaType<T>::kOne) |
-               ((x.z & MaType<T>::kExp) + MaType<T>::kOne) | ((x.w & MaType<T>::kExp) + MaType<T>::kOne);
+        any[0] = MaType<T>::times0(x.x, any[0]), any[1] = MaType<T>::times0(x.y, any[1]);
+        any[2] = MaType<T>::times0(x.z, any[2]), any[3] = MaType<T>::times0(x.w, any[3]);
       }
     }
   }
-  if (!(any & 0x80008000u)) return false;
+  if (!((any[0] | any[1] | any[2] | any[3]) & 0x7fff7fffu)) return false;
 #pragma unroll 1
   for (int c = 0; c < D / 2; ++c) {
     uint32_t* w = reinterpret_cast<uint32_t*>(tile + (row >> 3) * (8 * D * 2) + (c >> 5) * 1024 + (row & 7) * 128) + (c & 31);
@@ -480,6 +490,7 @@ __device__ __noinline__ float ma_bad_sum(const MaArgs* args, const int* counts, 
 #pragma unroll 1
   for (int j = 0; j < n; ++j) {
     const int x = it.x0 + j;
+    if (all && x >= it.full0 && x < it.full1) continue;  // every row sees it: it went through the product
     const int key = all ? (x < it.sink_x ? x : x + it.shift) : j < counts[0] ? lists[0][j] : lists[1][j - counts[0]];
     if (key >= it.hi || !ma_sees<kTree>(p, it, token, key)) continue;
     const int page = p.by_page(key);
@@ -563,13 +574,15 @@ __device__ __forceinline__ void ma_load_rows(void* dst, const CUtensorMap* map, 
       : "memory");
 }
 
-// Warps 10 and 11: in tiles that some row sees in part, V rows are made safe to
-// multiply by 0 before the P.V product reads them. Such a tile's load arrives
-// at a barrier of its own, the tiles of the kind one after the other, and these
-// two warps arrive at the stage's in its place.
+// Warp 10, and warp 11 where row tiles share their keys: in tiles that some row
+// sees in part, V rows are made safe to multiply by 0 before the P.V product
+// reads them. Such a tile's load arrives at a barrier of its own, the tiles of
+// the kind one after the other, and these warps arrive at the stage's in its
+// place.
 template <typename S, typename T, int D, bool kTree, bool kShared>
 __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, int stride, int rank) {
   constexpr int kStages = S::kStages;
+  constexpr int kWarps = kShared ? 2 : 1;
   const int lane = threadIdx.x & 31, which = (threadIdx.x >> 5) - 10;
   int ring = 0, n_raw = 0, item_no = 0;
   bool ok = true;
@@ -579,6 +592,7 @@ __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, 
     const int streams = !kShared && it.second ? 2 : 1, list = item_no % kMaLists;
     const int pa = it.prefix + it.tok0, pb = it.prefix + min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1)) - 1;
     if (lane < 2) s.n_bad[list][lane][which] = 0;
+    if (kWarps == 1 && lane < 2) s.n_bad[list][lane][1] = 0;
     __syncwarp();
 #pragma unroll 1
     for (int t = 0; ok && t < it.nt; ++t) {
@@ -593,7 +607,7 @@ __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, 
         if (!ok) break;
         ++n_raw;
 #pragma unroll 1
-        for (int row = which * 64 + lane; row < which * 64 + 64; row += 32) {
+        for (int row = which * 32 + lane; row < kMaTile; row += 32 * kWarps) {
           const int x = xt + row, key = x < it.sink_x ? x : x + it.shift;
           const bool some = x < it.x1 && key < it.hi && (kTree || key >= it.lo || key < p.sinks);
           // a row that every row of the item sees is left as it is
@@ -613,19 +627,21 @@ __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, 
   }
 }
 
-// Warp 8: loads by TMA. Lane i looks up and loads piece i of a tile.
-template <typename S, int D, bool kTree, bool kShared>
+// Loads by TMA: warp 8 of Q and K and, where row tiles share their keys, of V;
+// else warp 11 of V: in pages of 16 slots a tile takes 8 loads, which one warp
+// does not issue as fast as memory delivers them (32 x 25 drafts over 500 to 8000
+// keys in such pages: 173 us with one warp, 137 with two). Lane i looks up and
+// loads piece i of a tile. Both warps count all tiles in their order.
+template <typename S, int D, bool kTree, bool kShared, bool kV>
 __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtensorMap& tmap_q, const CUtensorMap& tmap_k,
-                                             const CUtensorMap& tmap_v, const CUtensorMap& tmap_kb,
+                                             const CUtensorMap& tmap_kb, const CUtensorMap& tmap_v,
                                              const CUtensorMap& tmap_vb, int first, int stride, int rank) {
   constexpr int kStages = S::kStages;
   const int lane = threadIdx.x & 31;
   if (lane == 0) {
-    prefetch_tensormap(&tmap_q);
-    prefetch_tensormap(&tmap_k);
-    prefetch_tensormap(&tmap_v);
-    prefetch_tensormap(&tmap_kb);
-    prefetch_tensormap(&tmap_vb);
+    if (!kV) prefetch_tensormap(&tmap_q);
+    prefetch_tensormap(kV ? &tmap_v : &tmap_k);
+    prefetch_tensormap(kV ? &tmap_vb : &tmap_kb);
   }
   const uint64_t pol_q = policy_evict_first();
   const uint64_t pol_kv = policy_evict_normal();
@@ -636,7 +652,7 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
   for (int i = first; ok && i < p.n_items; i += stride) {
     const MaItem it = ma_item<kTree, kShared>(p, i, rank);
     if (it.skip) {
-      if (lane == 0 && it.tok0 < it.n) atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
+      if (!kV && lane == 0 && it.tok0 < it.n) atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
       continue;
     }
     if (lane == 0 && (it.ctx < 0 || (it.prefix < 0 && it.ctx != 0) ||
@@ -659,12 +675,16 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
     };
     auto load = [&](bool k, bool part, int t, int row, int kvh) -> bool {
       const int st = ring % kStages;
+      if (!kShared && k == kV) {  // the other warp's
+        ++ring;
+        return true;
+      }
       const uint32_t loaded = __ballot_sync(0xffffffffu, row >= 0);
       bool go = true;
       if (lane == 0) {
         go = ma_wait(&s.empty[st], ((ring / kStages) & 1) ^ 1, &s.abort, p.status, NPL_DEV_TIMEOUT_TMA);
         if (go) {
-          if (!part) mbar_arrive(&s.full[st]);  // the second of its two arrivals
+          if (kShared && !part) mbar_arrive(&s.full[st]);  // in the place of the second warp that cleans
           mbar_arrive_expect_tx(part ? &s.raw[n_raw % kStages] : &s.full[st], (__popc(loaded) << p.piece_log) * D * 2);
         }
       }
@@ -695,7 +715,7 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
         if (t < 0 && !k) continue;
         if (!k || t + 1 < it.nt) ok = load(k, !k && part, k ? t + 1 : t, k ? next : row, it.kvh + (n >> 1));
       }
-      if (t == (kShared ? 0 : -1) && ok) {  // three or two tiles ahead: less than the ring holds
+      if (!kV && t == (kShared ? 0 : -1) && ok) {  // three or two tiles ahead: less than the ring holds
         // Q after the first tiles: those need not wait until the Q before has been read
         if (lane == 0) {
           const int buf = nq % S::kQBufs;
@@ -829,12 +849,12 @@ __device__ __forceinline__ void ma_mma_role(S& s, const MaArgs& p, uint32_t tmem
 }
 
 // Barriers and tensor memory of a CTA.
-template <typename S>
+template <typename S, bool kShared>
 __device__ __forceinline__ void ma_start(S& s) {
   constexpr int kStages = S::kStages;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&s.full[i], 2);
+      mbar_init(&s.full[i], kShared ? 2 : 1);
       mbar_init(&s.empty[i], 1);
       mbar_init(&s.raw[i], 1);
     }
@@ -926,15 +946,17 @@ __global__ void __launch_bounds__(kMaThreads, 1)
   const int first = blockIdx.x >> p.split_log;
   const int stride = p.split > 1 ? p.n_items : gridDim.x;
 
-  ma_start(s);
+  ma_start<S, kShared>(s);
   const uint32_t tmem = s.tmem_base;
   pdl_wait();  // q, the pool and the metadata come from earlier work on the stream
   pdl_trigger();
 
   if (warp == 8) {
-    ma_load_role<S, D, kTree, kShared>(s, p, tmap_q, tmap_k, tmap_v, tmap_kb, tmap_vb, first, stride, rank);
+    ma_load_role<S, D, kTree, kShared, false>(s, p, tmap_q, tmap_k, tmap_kb, tmap_v, tmap_vb, first, stride, rank);
   } else if (warp == 9) {
     ma_mma_role<S, T, D, kTree, kShared>(s, p, tmem, first, stride, rank);
+  } else if (!kShared && warp == 11) {
+    ma_load_role<S, D, kTree, kShared, true>(s, p, tmap_q, tmap_k, tmap_kb, tmap_v, tmap_vb, first, stride, rank);
   } else if (warp >= 10) {
     ma_clean_role<S, T, D, kTree, kShared>(s, p, first, stride, rank);
   } else {
@@ -1187,16 +1209,18 @@ __global__ void __launch_bounds__(kMaThreads, 1)
   const int rank = blockIdx.x & (p.split - 1);
   const int first = blockIdx.x >> p.split_log;
   const int stride = p.split > 1 ? p.n_items : gridDim.x;
-  ma_start(s);
+  ma_start<S, false>(s);
   const uint32_t tmem = s.tmem_base;
   pdl_wait();  // q, the pool and the metadata come from earlier work on the stream
   pdl_trigger();
 
   if (warp == 8) {
-    ma_load_role<S, D, kTree, false>(s, p, tmap_q, tmap_k, tmap_v, tmap_kb, tmap_vb, first, stride, rank);
+    ma_load_role<S, D, kTree, false, false>(s, p, tmap_q, tmap_k, tmap_kb, tmap_v, tmap_vb, first, stride, rank);
   } else if (warp == 9) {
     ma_mma_role<S, T, D, kTree, false>(s, p, tmem, first, stride, rank);
-  } else if (warp >= 10) {
+  } else if (warp == 11) {
+    ma_load_role<S, D, kTree, false, true>(s, p, tmap_q, tmap_k, tmap_kb, tmap_v, tmap_vb, first, stride, rank);
+  } else if (warp == 10) {
     ma_clean_role<S, T, D, kTree, false>(s, p, first, stride, rank);
   } else {
     // -------------------------------------------------------- softmax

@@ -439,7 +439,7 @@ __device__ __forceinline__ uint32_t ma_low(int n, int w) {
 // Whether some row of a CTA's item does not see some of the tile's columns from xt on.
 __device__ __forceinline__ bool ma_part(const MaItem& it, int xt) { return xt < it.full0 || xt + kMaTile > it.full1; }
 
-// Whether the row of a token sees a key (the same as the bits below, for one key).
+// Whether the row of a token sees a key: the bits of a tile, for one key.
 template <bool kTree>
 __device__ __forceinline__ bool ma_sees(const MaArgs& p, const MaItem& it, int token, int key) {
   if (kTree) return key < it.prefix || p.mask[(it.start + token) * p.ld_mask + (key - it.prefix)] != 0;
@@ -477,30 +477,37 @@ __device__ __forceinline__ bool ma_clean_row(uint8_t* tile, int row, bool seen) 
   return true;
 }
 
-// Sum of the V elements of column col that are not finite, that ma_clean_row
-// took out, and whose keys the row of a token sees (a rare path).
-template <typename T, int D, bool kTree, bool kShared>
-__device__ __noinline__ float ma_bad_sum(const MaArgs* args, const int* counts, const int (*lists)[kMaBad], int item,
-                                         int rank, int token, int kvh, int col) {
+// Keys whose V rows ma_clean_row took elements out of, for a row that sees them
+// (a rare path). ma_bad_count says how many are to be looked at: those that were
+// remembered, or, where there were more, all in the CTA's tiles that are seen in
+// part. ma_bad_key gives one of them, -1 for none, and where its V row begins.
+template <bool kTree, bool kShared>
+__device__ __noinline__ int ma_bad_count(const MaArgs* args, const int* counts, int item, int rank) {
+  if (max(counts[0], counts[1]) <= kMaBad) return counts[0] + counts[1];
+  const MaItem it = ma_item<kTree, kShared>(*args, item, rank);
+  const int ahead = min(max(it.full0 - it.x0, 0), it.x1 - it.x0);
+  return ahead + max(it.x1 - max(it.full1, it.x0 + ahead), 0);
+}
+template <int D, bool kTree, bool kShared>
+__device__ __noinline__ int ma_bad_key(const MaArgs* args, const int* counts, const int (*lists)[kMaBad], int item,
+                                       int rank, int kvh, int j, size_t* at) {
   const MaArgs& p = *args;
   const MaItem it = ma_item<kTree, kShared>(p, item, rank);
-  const bool all = max(counts[0], counts[1]) > kMaBad;  // more than were remembered: look at every key of this CTA
-  const int n = all ? it.x1 - it.x0 : counts[0] + counts[1];
-  float sum = 0.f;
-#pragma unroll 1
-  for (int j = 0; j < n; ++j) {
-    const int x = it.x0 + j;
-    if (all && x >= it.full0 && x < it.full1) continue;  // every row sees it: it went through the product
-    const int key = all ? (x < it.sink_x ? x : x + it.shift) : j < counts[0] ? lists[0][j] : lists[1][j - counts[0]];
-    if (key >= it.hi || !ma_sees<kTree>(p, it, token, key)) continue;
-    const int page = p.by_page(key);
-    const int blk = page < p.max_blocks ? p.bt[it.b * p.bt_stride + page] : -1;
-    if (blk < 0 || blk >= p.num_blocks) continue;
-    const size_t at = (((size_t)blk * p.block_size + (key - page * p.block_size)) * p.Hkv + kvh) * D + col;
-    const float v = MaType<T>::get(p.v, at);
-    if (!isfinite(v)) sum += v;
+  int key;
+  if (max(counts[0], counts[1]) <= kMaBad) {
+    key = j < counts[0] ? lists[0][j] : lists[1][j - counts[0]];
+  } else {
+    const int ahead = min(max(it.full0 - it.x0, 0), it.x1 - it.x0);
+    const int x = j < ahead ? it.x0 + j : max(it.full1, it.x0 + ahead) + j - ahead;
+    if (x >= it.sink_x && x < it.hole_x) return -1;
+    key = x < it.sink_x ? x : x + it.shift;
   }
-  return sum;
+  if (key >= it.hi) return -1;
+  const int page = p.by_page(key);
+  const int blk = page < p.max_blocks ? p.bt[it.b * p.bt_stride + page] : -1;
+  if (blk < 0 || blk >= p.num_blocks) return -1;
+  *at = (((size_t)blk * p.block_size + (key - page * p.block_size)) * p.Hkv + kvh) * D;
+  return key;
 }
 
 // Barriers among the 128 threads of a stream.
@@ -1112,6 +1119,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         tc_fence_after();
       }
       if (!ok) break;
+      if (l < 1e-30f) l = 0.f;  // no key seen (the largest p of a row is 2^-2 or more): the polynomial leaves 2^-149 a key
       if (warp_on) {
         const int* const n_bad = s.n_bad[list][owner];
         const bool bad = any_part && n_bad[0] + n_bad[1] > 0;  // written before the P.V products of such tiles
@@ -1148,14 +1156,21 @@ __global__ void __launch_bounds__(kMaThreads, 1)
           }
         }
         if (bad && row_ok && l != 0.f) {
+          const int n = ma_bad_count<kTree, kShared>(&p, n_bad, i, rank);
 #pragma unroll 1
-          for (int d = 0; d < D; ++d) {
-            const float x = ma_bad_sum<T, D, kTree, kShared>(&p, n_bad, s.bad[list][owner], i, rank, token, kvh, d);
-            if (x == 0.f) continue;
-            if (p.split > 1)
-              stage[(((d >> 2) ^ (r & 7)) << 2) + (d & 3)] += x;
-            else
-              MaType<T>::add(dst + d, x);
+          for (int j = 0; j < n; ++j) {
+            size_t at;
+            const int key = ma_bad_key<D, kTree, kShared>(&p, n_bad, s.bad[list][owner], i, rank, kvh, j, &at);
+            if (key < 0 || !ma_sees<kTree>(p, it, token, key)) continue;
+#pragma unroll 1
+            for (int d = 0; d < D; ++d) {
+              const float x = MaType<T>::get(p.v, at + d);
+              if (isfinite(x)) continue;
+              if (p.split > 1)
+                stage[(((d >> 2) ^ (r & 7)) << 2) + (d & 3)] += x;
+              else
+                MaType<T>::add(dst + d, x);
+            }
           }
         }
         if (p.split > 1 && row_ok)
@@ -1427,17 +1442,23 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         const int* const n_bad = s.n_bad[list][st];
         if (any_part && n_bad[0] + n_bad[1] > 0) {  // written before the P.V products of such tiles
           ma_stream_sync(st);
+          const int n_keys = ma_bad_count<kTree, false>(&p, n_bad, i, rank);
 #pragma unroll 1
-          for (int n = 0; n < n_rows; ++n) {
-            if (r >= D || s.ml[st][n].y == 0.f) continue;
-            const int of = p.by_group(n);
-            const float x = ma_bad_sum<T, D, kTree, false>(&p, n_bad, s.bad[list][st], i, rank, it.tok0 + of,
-                                                                     kvh, r);
-            if (x == 0.f) continue;
-            if (p.split > 1)
-              stage[n * D] += x;
-            else
-              MaType<T>::add(dst + of * p.ld_out + (n - of * p.G) * D, x);
+          for (int j = 0; r < D && j < n_keys; ++j) {
+            size_t from;
+            const int key = ma_bad_key<D, kTree, false>(&p, n_bad, s.bad[list][st], i, rank, kvh, j, &from);
+            if (key < 0) continue;
+            const float x = MaType<T>::get(p.v, from + r);
+            if (isfinite(x)) continue;
+#pragma unroll 1
+            for (int n = 0; n < n_rows; ++n) {
+              const int of = p.by_group(n);
+              if (s.ml[st][n].y == 0.f || !ma_sees<kTree>(p, it, it.tok0 + of, key)) continue;
+              if (p.split > 1)
+                stage[n * D] += x;
+              else
+                MaType<T>::add(dst + of * p.ld_out + (n - of * p.G) * D, x);
+            }
           }
         }
       }

@@ -443,3 +443,30 @@ def test_mask_from_parents(PA):
     cpu = PA.tree_mask_from_parents(p, offs, 20)
     gpu = PA.tree_mask_from_parents(p.cuda(), offs.cuda(), 20)
     assert torch.equal(cpu, gpu.cpu())
+
+
+@pytest.mark.parametrize("new,heads", [(20, 2), (90, 2), (150, 2)])
+def test_scores_of_minus_infinity(PA, new, heads):
+    """Keys whose scores are all minus infinity count as unseen: rows of nothing else give zeros."""
+    c = Case([(new, new + 300)], heads, heads, 64, 16, BF16, seed=41)
+    c.q.abs_()
+    c.k[...] = -float("inf")
+    got = PA.paged_window_attention(*c.args(), 200, 4)
+    assert (got == 0).all()
+    blk, at = c.slot(0, new + 150)
+    c.k[blk, at] = 0.25  # seen by the rows from new + 150 on
+    got = PA.paged_window_attention(*c.args(), 200, 4)
+    first = max(0, 150 - 300 + new)
+    assert (got[:first] == 0).all() and first < new
+    assert (got[first:] == c.v[blk, at]).all()
+
+
+def test_many_bad_values_over_a_long_context(PA):
+    """The rare path is bounded: every key in tiles that are seen in part is bad, beside a long context."""
+    c = Case([(300, 12000), (3, 9000)], 2, 1, 128, 16, F16, seed=43)
+    m = tree(c)
+    for b, (n, ctx) in enumerate(c.seqs):
+        for i in range(ctx - n, ctx):
+            blk, at = c.slot(b, i)
+            c.v[blk, at, 0, i % 128] = float("nan")
+    check(PA.paged_tree_attention(*c.args(), m), c.tree_oracle(m))

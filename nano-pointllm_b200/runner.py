@@ -43,6 +43,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib as L
+from . import logprobs as LP
 from . import package as P
 from . import paged_attention as PA
 from . import w8a8 as W
@@ -59,6 +60,10 @@ class ForwardContext:
     context_lens: Optional[torch.Tensor]          # [B] int32
     position_ids: Optional[torch.Tensor] = None   # [1, T] int64
     seq_lens: list[int] = field(default_factory=list)
+    # a step that verifies drafts (the reference has none): what each draft sees of its sequence's drafts, as
+    # paged_attention.paged_tree_attention takes it; seq_lens holds the sequences' numbers of drafts, slot_mapping
+    # their slots in that order, context_lens counts them in, position_ids are those of their paths
+    tree_mask: Optional[torch.Tensor] = None      # [T, >= max(seq_lens)] bool
 
 
 _ctx = threading.local()
@@ -135,11 +140,22 @@ class W8A8LlamaRunner:
     ``state_dict``: HF-named float weights (each Linear is quantised per
     output channel on the GPU as its layer is built) or a weight source with
     linear()/dense(), e.g. a checksummed int8 package (see from_package).
+
+    ``window`` / ``sinks``: every layer attends to the last ``window`` tokens
+    and the first ``sinks`` ones only (paged_attention.paged_window_attention),
+    so that pages between them may be freed. A step whose context has a
+    ``tree_mask`` verifies a tree of drafted tokens of each sequence in one
+    forward (paged_attention.paged_tree_attention) and returns every draft's
+    logits.
     """
+
+    window: Optional[int] = None
+    sinks: int = 0
 
     def __init__(self, shape: LlamaShape, state_dict: dict[str, torch.Tensor], *, device: torch.device,
                  kv_pool: torch.Tensor | None = None, num_blocks: int = 0, block_size: int = 256,
-                 fuse_mlp_quant: bool = False, fuse_silu_quant: bool = False, forward_context=None):
+                 fuse_mlp_quant: bool = False, fuse_silu_quant: bool = False, forward_context=None,
+                 window: Optional[int] = None, sinks: int = 0):
         """``forward_context``: a callable returning the current step's
         context. Default: this module's get_forward_context. The reference
         engine passes its own nanopointllm.engine.forward_context.
@@ -149,6 +165,9 @@ class W8A8LlamaRunner:
         self.shape = shape
         self.device = torch.device(device)
         self.forward_context = forward_context or get_forward_context
+        if window is not None and (window < 1 or sinks < 0):
+            raise ValueError("window must be at least 1 and sinks at least 0")
+        self.window, self.sinks = window, sinks
         # fuse_mlp_quant, decode batches (<= 64 tokens): the gate/up epilogue
         # also records each token's absmax of SiLU(gate)*up, and down quantises
         # its fp16 input itself, so no separate quantisation kernel runs between
@@ -213,19 +232,46 @@ class W8A8LlamaRunner:
         quantisation is fused into the attention kernel."""
         s = self.shape
         t = q.shape[0]
-        if all(n == 1 for n in ctx.seq_lens):
+        masked = self._masked_attention(layer, q, ctx)
+        if masked is None and all(n == 1 for n in ctx.seq_lens):
             q8 = torch.empty((t, s.heads * s.head_dim), dtype=torch.int8, device=q.device)
             qs = torch.empty((t,), dtype=torch.float32, device=q.device)
             PA.paged_decode_attention(q, layer.k_cache, layer.v_cache, ctx.block_tables, ctx.context_lens,
                                       self.scale, s.heads // s.kv_heads, quant_out=(q8, qs))
             return q8, qs
-        q8, qs = W.dynamic_per_token_quant(self._attention(layer, q, ctx))
+        q8, qs = W.dynamic_per_token_quant(self._attention(layer, q, ctx) if masked is None else masked)
         return q8, qs.reshape(-1)
+
+    def _masked_attention(self, layer: W8A8Layer, q: torch.Tensor, ctx: ForwardContext) -> Optional[torch.Tensor]:
+        """[T, H*D] fp16 of a step with a tree of drafts or under a window; None for a causal one."""
+        mask = getattr(ctx, "tree_mask", None)
+        if mask is None and self.window is None:
+            return None
+        if mask is not None and self.window is not None:
+            raise ValueError("a tree of drafts is not verified under a window")
+        s, t, dev = self.shape, q.shape[0], q.device
+        cache = (q, layer.k_cache, layer.v_cache, ctx.block_tables, ctx.context_lens)
+        groups = s.heads // s.kv_heads
+        if mask is None and all(n == 1 for n in ctx.seq_lens):
+            return PA.paged_window_attention(*cache, None, None, self.scale, groups, self.window,
+                                             self.sinks).reshape(t, -1)
+        offs = [0]
+        for n in ctx.seq_lens:
+            offs.append(offs[-1] + n)
+        rows = (torch.tensor(ctx.seq_lens, dtype=torch.int32, device=dev),
+                torch.tensor(offs[:-1], dtype=torch.int32, device=dev), self.scale, groups)
+        most = max(ctx.seq_lens)
+        if mask is not None:
+            return PA.paged_tree_attention(*cache, *rows, mask, max_q_len=most).reshape(t, -1)
+        return PA.paged_window_attention(*cache, *rows, self.window, self.sinks, max_q_len=most).reshape(t, -1)
 
     def _attention(self, layer: W8A8Layer, q: torch.Tensor, ctx: ForwardContext) -> torch.Tensor:
         """q [T, H, D] (rotated) -> [T, H*D] fp16."""
         s = self.shape
         t = q.shape[0]
+        masked = self._masked_attention(layer, q, ctx)
+        if masked is not None:
+            return masked
         if all(n == 1 for n in ctx.seq_lens):
             out = PA.paged_decode_attention(q, layer.k_cache, layer.v_cache, ctx.block_tables, ctx.context_lens,
                                             self.scale, s.heads // s.kv_heads)
@@ -332,9 +378,11 @@ class W8A8LlamaRunner:
 class DecodeGraph:
     """Strict CUDA-graph decode step for a fixed batch and block-table width
     (engine/cuda_graph.py:30-77): static metadata buffers, one replay per step,
-    greedy argmax inside the graph."""
+    greedy argmax inside the graph. With ``logprobs`` (a number of top
+    alternatives, 0 or more) the graph also scores the tokens it chose:
+    ``scores`` is a logprobs.TokenLogprobs of the last replay."""
 
-    def __init__(self, runner: W8A8LlamaRunner, batch: int, max_blocks: int):
+    def __init__(self, runner: W8A8LlamaRunner, batch: int, max_blocks: int, logprobs: Optional[int] = None):
         dev = runner.device
         self.runner = runner
         self.ids = torch.zeros(batch, dtype=torch.int64, device=dev)
@@ -348,6 +396,8 @@ class DecodeGraph:
         self.graph: torch.cuda.CUDAGraph | None = None
         self.logits: torch.Tensor | None = None
         self.next_tokens: torch.Tensor | None = None
+        self.logprobs = logprobs
+        self.scores: Optional[LP.TokenLogprobs] = None
 
     def _run(self):
         set_forward_context(self.ctx)
@@ -355,7 +405,9 @@ class DecodeGraph:
             logits = self.runner.forward(self.ids, position_ids=self.positions)
         finally:
             clear_forward_context()
-        return logits, torch.argmax(logits[0], dim=-1)
+        tokens = torch.argmax(logits[0], dim=-1)
+        scores = None if self.logprobs is None else LP.token_logprobs(logits[0], tokens, self.logprobs)
+        return logits, tokens, scores
 
     def capture(self) -> None:
         s = torch.cuda.Stream(device=self.runner.device)
@@ -366,7 +418,7 @@ class DecodeGraph:
         torch.cuda.current_stream().wait_stream(s)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            self.logits, self.next_tokens = self._run()
+            self.logits, self.next_tokens, self.scores = self._run()
         self.graph = g
 
     def load(self, ids, positions, slots, context_lens, block_tables, non_blocking: bool = True) -> None:

@@ -30,7 +30,7 @@ import time
 from collections import deque
 from dataclasses import dataclass, field
 from enum import Enum, auto
-from typing import Callable, Optional, Sequence as Seq
+from typing import Callable, NamedTuple, Optional, Sequence as Seq
 
 import torch
 import torch.nn.functional as F
@@ -54,6 +54,14 @@ class Request:
     point_seed: int = 0
 
 
+class TokenScore(NamedTuple):
+    """How likely a generated token was (logprobs.token_logprobs)."""
+    logprob: float
+    entropy: float
+    top_ids: list[int]
+    top_logprobs: list[float]
+
+
 class Sequence:
     """A request being served (sequence.py:17-80). Positions 0..n_point_rows-1
     hold the point rows, then the text ids, then the generated ids."""
@@ -67,6 +75,7 @@ class Sequence:
         self.t_first_token: Optional[float] = None
         self.t_done: Optional[float] = None
         self.preemptions = 0
+        self.scores: list[TokenScore] = []  # of the generated tokens, where the engine scores them
 
     @property
     def num_tokens(self) -> int:
@@ -210,9 +219,16 @@ class ServingEngine:
 
     def __init__(self, runner, *, max_num_seqs: int = 64, max_num_batched_tokens: int = 16384,
                  max_blocks_per_seq: int, eos_token_id: Optional[int] = None, use_graphs: bool = True,
-                 point_rows_fn: Optional[Callable[[Request], torch.Tensor]] = None):
-        from . import runner as R
-        self.R = R
+                 point_rows_fn: Optional[Callable[[Request], torch.Tensor]] = None, logprobs: Optional[int] = None):
+        """``logprobs``: None, or the number of top alternatives (0 to 32) to
+        report with every generated token's log probability and the entropy
+        of its distribution (``run(...)["scores"]``)."""
+        from . import logprobs as LP, runner as R
+        self.R, self.LP = R, LP
+        if logprobs is not None and not 0 <= logprobs <= LP.MAX_TOP:
+            raise ValueError(f"logprobs must be 0 to {LP.MAX_TOP}")
+        self.logprobs = logprobs
+        self.last_scores: list[TokenScore] = []  # of the last step's tokens
         self.runner = runner
         self.bm = BlockManager(runner.num_blocks, runner.block_size)
         self.sched = Scheduler(max_num_seqs, max_num_batched_tokens, self.bm, eos_token_id)
@@ -291,7 +307,14 @@ class ServingEngine:
         finally:
             self.R.clear_forward_context()
         self.steps["mixed"] += 1
-        return logits[0].argmax(-1).tolist()
+        tokens = logits[0].argmax(-1)
+        if self.logprobs is not None:
+            self._keep_scores(self.LP.token_logprobs(logits[0], tokens, self.logprobs), len(seqs))
+        return tokens.tolist()
+
+    def _keep_scores(self, r, n: int) -> None:
+        self.last_scores = [TokenScore(*x) for x in zip(r.logprobs[:n].tolist(), r.entropy[:n].tolist(),
+                                                        r.top_ids[:n].tolist(), r.top_logprobs[:n].tolist())]
 
     def _run_decode(self, decode: list[Sequence]) -> list[int]:
         n = len(decode)
@@ -300,14 +323,18 @@ class ServingEngine:
             return self._run_mixed([], decode)
         dg = self.graphs.get(bucket)
         if dg is None:
-            dg = self.graphs[bucket] = self.R.DecodeGraph(self.runner, bucket, self.max_blocks)
+            dg = self.graphs[bucket] = self.R.DecodeGraph(self.runner, bucket, self.max_blocks,
+                                                                logprobs=self.logprobs)
         ids, pos, slots, ctx, bt = self._decode_metadata(decode, bucket)
         if dg.graph is None:
             dg.load(ids, pos, slots, ctx, bt, non_blocking=False)
             dg.capture()  # runs the step twice eagerly: the KV writes are the same values
         dg.load(ids, pos, slots, ctx, bt, non_blocking=False)
         self.steps["decode"] += 1
-        return dg.replay()[:n].tolist()
+        tokens = dg.replay()
+        if self.logprobs is not None:
+            self._keep_scores(dg.scores, n)
+        return tokens[:n].tolist()
 
     def step(self) -> list[Sequence]:
         prefill, decode = self.sched.schedule()
@@ -319,6 +346,9 @@ class ServingEngine:
         tokens = self._run_mixed(prefill, decode) if prefill else self._run_decode(decode)
         now = time.perf_counter()
         self.step_s["mixed" if prefill else "decode"] += now - t0
+        if self.logprobs is not None:
+            for seq, score in zip(prefill + decode, self.last_scores):
+                seq.scores.append(score)
         return self.sched.postprocess(prefill + decode, tokens, now)
 
     def run(self, requests: Seq[Request]) -> dict:
@@ -343,6 +373,7 @@ class ServingEngine:
             "preemptions": sum(s.preemptions for s in seqs),
             "steps": dict(self.steps),
             "step_s": {k: round(v, 4) for k, v in self.step_s.items()},
+            **({} if self.logprobs is None else {"scores": {s.req.rid: s.scores for s in seqs}}),
         }
 
 

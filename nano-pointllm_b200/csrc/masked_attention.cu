@@ -368,9 +368,8 @@ __device__ __forceinline__ void ma_exp_pack(const uint32_t (&v)[32], float c2, f
 // One item: 128 rows (or twice 128, shared) of one sequence and kv head (or
 // the same rows of two). Every role decodes the same items from the same
 // read-only metadata. Tiles are numbered through x: key(x) = x below sink_x
-// (the sinks' pieces), x + shift from hole_x on (the window's; shift is a
-// multiple of 128, so that a tile's keys lie in its pages as in its rows), and
-// nothing is loaded between. This CTA takes the tiles x0 <= x < x1.
+// (the sinks' pieces), x + shift from hole_x on (the window's), and nothing is
+// loaded between. This CTA takes the tiles x0 <= x < x1.
 struct MaItem {
   int b, kvh, tok0, n, ctx, start, prefix;
   int lo, hi;  // keys that some row of the item sees: lo <= key < hi, and the sinks
@@ -405,8 +404,10 @@ __device__ __forceinline__ MaItem ma_item(const MaArgs& p, int i, int rank) {
       const int sp = (min(p.sinks, it.lo) + p.piece - 1) >> p.piece_log << p.piece_log;
       const int lp = it.lo >> p.piece_log << p.piece_log;
       if (sp < lp) {
+        // the first x from sp on with lp's place in a tile, so that tiles lie in pages; sp itself if that saves a tile
+        const int hole = (lp - sp) & (kMaTile - 1), used = (sp + end - lp - 1) & (kMaTile - 1);
         it.sink_x = sp;
-        it.hole_x = sp + ((lp - sp) & (kMaTile - 1));  // the first x from sp on with lp's place in a tile
+        it.hole_x = used + hole >= kMaTile ? sp : sp + hole;
         it.shift = lp - it.hole_x;
         end -= it.shift;
       }
@@ -700,7 +701,8 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
       // pieces that lie together in the pool by one load, the ragged ends of a context or a window one by one
       const int lead = lane >> p.box_log << p.box_log, lead_x = it.x0 + t * kMaTile + (lead << p.piece_log);
       const uint32_t group = (1u << (1 << p.box_log)) - 1;  // at most 16 pieces of 8 keys
-      const bool big = ((loaded >> lead) & group) == group &&
+      const int row0 = __shfl_sync(0xffffffffu, row, lead), row1 = __shfl_sync(0xffffffffu, row, lead + (1 << p.box_log) - 1);
+      const bool big = ((loaded >> lead) & group) == group && row1 - row0 == (p.piece << p.box_log) - p.piece &&
                        (lead_x >= it.hole_x || lead_x + (p.piece << p.box_log) <= it.sink_x);
       if (row >= 0 && (!big || lane == lead))
         ma_load_rows(s.kv[st] + (lane << p.piece_log) * D * 2, k ? (big ? &tmap_kb : &tmap_k) : (big ? &tmap_vb : &tmap_v),

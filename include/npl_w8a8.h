@@ -479,9 +479,11 @@ int npl_fp8_linear(const uint8_t* qa, int64_t lda, const float* sa, int64_t ld_s
  * holds, infinities and NaN included, never reaches a row that does not see it.
  * Rows of no sequence are not written; context_lens[b] == 0 gives zeros.
  * max_q_len >= every q_lens[b] sizes the launch. D is 64 or 128, block_size a
- * multiple of 8, H / Hkv at most 128. Bad table entries (read as zeros),
- * offsets and lengths (skipped) set NPL_DEV code 5 (npl_device_status). No
- * workspace; graph-capturable.
+ * multiple of 8, H / Hkv at most 128. Bad table entries (read as zeros), and
+ * offsets, lengths and contexts that do not fit q, max_q_len and the table (the
+ * sequence is skipped) or a context shorter than its drafts (zeros) set NPL_DEV
+ * code 5 (npl_device_status). A row whose scores are all minus infinity gives
+ * zeros too. No workspace; graph-capturable.
  */
 int npl_paged_tree_attention(const void* q, int dtype, int64_t ld_q, int total_q, int H, int Hkv, int D,
                              const void* k_cache, const void* v_cache, int num_blocks, int block_size,

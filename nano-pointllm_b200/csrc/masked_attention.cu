@@ -89,7 +89,8 @@ struct MaArgs {
   int mask_cols;
   int window, sinks;
   int B, H, Hkv, G, num_blocks, block_size, max_blocks, total_q, max_q_len;
-  int tokens;   // of a row tile: 128 / G
+  int tokens;    // of a row tile: 128 / G
+  int capacity;  // keys that a row of the table has room for
   int piece, piece_log;  // keys of a piece, a power of two
   int box_log;           // pieces of a large load, a power of two
   int levels;   // items of a sequence and kv head (or pair of them)
@@ -390,7 +391,8 @@ __device__ __forceinline__ MaItem ma_item(const MaArgs& p, int i, int rank) {
   it.start = p.q_offsets ? p.q_offsets[it.b] : it.b;
   it.ctx = p.ctx_lens[it.b];
   it.prefix = it.ctx - it.n;
-  it.skip = it.tok0 >= it.n || it.n > p.max_q_len || it.start < 0 || it.start > p.total_q - it.n;
+  it.skip = it.tok0 >= it.n || it.n > p.max_q_len || it.start < 0 || it.start > p.total_q - it.n || it.ctx < 0 ||
+            it.ctx > p.capacity;
   it.second = kShared ? it.tok0 + p.tokens < it.n : it.kvh + 1 < p.Hkv;
   const int last = min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1));  // one past the item's last token
   int end = 0;
@@ -663,8 +665,7 @@ __device__ __forceinline__ void ma_load_role(S& s, const MaArgs& p, const CUtens
       if (!kV && lane == 0 && it.tok0 < it.n) atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
       continue;
     }
-    if (lane == 0 && (it.ctx < 0 || (it.prefix < 0 && it.ctx != 0) ||
-                      (long long)it.ctx > (long long)p.max_blocks * p.block_size))
+    if (!kV && lane == 0 && it.prefix < 0 && it.ctx != 0)
       atomicCAS(p.status, 0, NPL_DEV_BAD_INDEX);
     if (it.nt == 0) continue;
     const int32_t* table = p.bt + it.b * p.bt_stride;
@@ -1608,6 +1609,7 @@ int run_type(const char* what, const MaArgs& p, cudaStream_t st) {
 template <bool kTree>
 int run(const char* what, MaArgs p, int dtype, int D, float scale, cudaStream_t st) {
   p.c2 = scale * 1.4426950408889634f;
+  p.capacity = p.max_blocks * p.block_size;
   p.piece_log = kMaPieceLog;
   while (p.block_size & ((1 << p.piece_log) - 1)) --p.piece_log;
   p.piece = 1 << p.piece_log;

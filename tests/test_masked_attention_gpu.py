@@ -317,7 +317,9 @@ def test_bad_tables_and_offsets(PA):
     c.v = torch.cat([c.v, torch.zeros_like(c.v[:1])])
     check(got, c.tree_oracle(m))
     c.k, c.v, c.bt[0, 2] = saved_k, saved_v, 0
-    for field, value in (("offs", -1), ("offs", c.total - 5), ("new", 7), ("ctx", 3)):
+    room = c.bt.shape[1] * 16
+    for field, value in (("offs", -1), ("offs", c.total - 5), ("new", 7), ("ctx", 3), ("ctx", -1), ("ctx", -2 ** 31),
+                         ("ctx", room + 1), ("ctx", 2 ** 31 - 1), ("new", 2 ** 31 - 1), ("offs", 2 ** 31 - 1)):
         t = getattr(c, field)
         keep = int(t[1])
         t[1] = value
@@ -327,7 +329,7 @@ def test_bad_tables_and_offsets(PA):
         with pytest.raises(_lib.NplTimeout):
             _lib.device_status()
         t[1] = keep
-        assert (out[5:] == (0.0 if field == "ctx" else 3.0)).all(), field
+        assert (out[5:] == (0.0 if value == 3 else 3.0)).all(), field
         out, tol = out, c.tree_oracle(m)
         tol[1][5:] = np.nan
         check(out, tol, field)

@@ -11,12 +11,14 @@
 //
 // Top k: of the threads' maxima, the k-th largest is no larger than the k-th
 // largest logit, so only threads whose own maximum reaches it (k of them, and
-// those that tie) read their logits once more, from L2, for the logits that
+// those that tie) have their words read once more, from L2, for the logits that
 // reach it. Those few are ranked by counting: larger first, of equal ones the
 // lowest index.
 //
-// Bound by the read of the logits. One CTA takes a row; few rows are split over
-// a cluster of CTAs each, whose sums and best logits its first CTA joins.
+// One CTA of 128 threads takes a row, each with 8 words in flight and two sums an
+// instruction (16000 x 32003 fp16, top 5: 180 us,
+// 5.7 TB/s); few rows are split over a cluster of CTAs each, whose sums and best
+// logits its first CTA joins (64 x 32003 fp32, top 20: 11.5 us).
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -31,7 +33,7 @@ constexpr int kLpThreads = 128;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpUnroll = 8;      // 16-byte words that a thread has in flight
 constexpr int kLpCandidates = 512;  // at least kLpMaxTop * (kLpMaxSplit + 1)
-constexpr int kLpRounds = 6;
+constexpr int kLpRounds = 6;        // top tokens from which on every thread ranks its maximum
 constexpr int kLpStep = 2048;     // logits that a CTA looks through at a time for equal ones
 constexpr int kLpMaxSplit = 8;    // CTAs of a cluster at most
 constexpr float kLpFar = -200.f;  // e^-200 is 0 in fp32: distances are cut here, so that 0 * infinity cannot arise

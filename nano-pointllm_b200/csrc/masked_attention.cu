@@ -13,29 +13,37 @@
 // largest. p is rounded to the type of the caches because it is an operand of
 // the P.V product; the normaliser sums the unrounded p.
 //
-// On the tensor cores (tcgen05 kind::f16, fp32 sums in TMEM): the rows of a
-// tile are (token, query head of one kv head), so grouped heads share the keys
-// they read. A CTA works on two streams, each with its own 128 rows, its own
-// warpgroup (one thread a row) and its own TMEM, so that one stream's softmax
-// runs while the tensor core works for the other:
-//   shared (more rows than one tile): two neighbouring row tiles of one kv head
-//     read the same K and V tiles;
-//   not shared (decode, small trees): the same rows of two kv heads.
-// 384 threads: warps 0-3 and 4-7 softmax of the streams, warp 8 TMA, warp 9 MMA
-// (one thread). S_j = Q K_j^T goes to TMEM, a thread reads its row of 128
-// scores, writes p over them in TMEM, and O += P V_j reads it there. The order
-// S0, S1, then O0 S0 O1 S1 ... makes every S of a stream arrive after the O
-// before it, so no further barrier guards a rescale.
+// On the tensor cores (tcgen05 kind::f16, fp32 sums in TMEM). A CTA works on two
+// streams, each with its own rows, its own warpgroup and its own TMEM, so that
+// one stream's softmax runs while the tensor core works for the other:
+//   shared (more rows than one tile of 128): two neighbouring row tiles of one
+//     kv head read the same K and V tiles;
+//   not shared (single tokens, trees): the same rows of two kv heads.
+// Rows are (token, query head of one kv head): grouped heads share their keys.
+// Two kernels: masked_attn_kernel has rows as M and one thread a row; P goes over
+// S in TMEM, where the P.V product reads it. few_rows_kernel (at most 32 rows) has
+// them as N. 384 threads: warps 0-3 and 4-7 softmax of the streams, warp 8 loads,
+// warp 9 products, warps 10 and 11 clean V or load it. The order S0, S1, then
+// O0 S0 O1 S1 ... makes every S of a stream arrive after the O before it, so no
+// further barrier guards a rescale.
 //
 // Keys come in pieces of gcd(block_size, 32): the visible ones of a CTA's rows
-// only (the sinks' pieces, then the window's), four or more pieces to a tile.
-// A long axis with few rows is split over a cluster of CTAs, whose partial sums
-// are joined through distributed shared memory.
+// only (the sinks' pieces, then the window's). Whole pieces that lie together in
+// the pool, up to 128 rows, come in one load with both halves of the head; loads
+// of 32 rows and one half made the load warp the bottleneck (32 x 25 drafts in
+// pages of 16: 270 us, now 140). A long axis with few rows is split over a cluster of
+// CTAs, whose partial sums are joined through distributed shared memory.
 //
 // What a masked slot holds must not reach a row that does not see it, and
 // 0 * infinity would: in tiles that some row sees in part, the V rows that no
 // row sees are zeroed, and V elements that are not finite are replaced by 0 and
 // added at the end to the rows that do see them.
+//
+// Bound by memory where there are few rows (64 tokens, 32 heads, 1028 keys each:
+// 165 us, 6.0 TB/s); for prompts by a stream's chain of product, scores out of
+// TMEM (twice: held in registers they spill), exponentials (a quarter of them by
+// a polynomial: 375 us for 16000 tokens of 32/8 heads under a window of 1024, none
+// 409, half 415; 325 with tiles packed) and P back.
 #include <algorithm>
 #include <initializer_list>
 
@@ -50,7 +58,7 @@ namespace {
 constexpr int kMaThreads = 384;
 constexpr int kMaTile = 128;
 constexpr int kMaFixed = 10;            // what a round of clusters costs beside its tiles, in tiles
-constexpr int kMaLists = 8;            // items whose lists of such keys are kept: more than the ring can be ahead
+constexpr int kMaLists = 8;            // items whose lists of bad keys are kept: more than the ring can be ahead
 constexpr int kMaBad = 12;             // keys with V elements that are not finite, remembered for an item
 constexpr int kMaPieceLog = 5;         // 32 keys of a piece at most
 constexpr int kMaBoxLog = 7;           // 128 keys of a load at most
@@ -1208,7 +1216,9 @@ __global__ void __launch_bounds__(kMaThreads, 1)
   }
 }
 
-// Few rows (at most kN of a kv head: single tokens, small trees) as the N side:
+// Few rows (at most kN of a kv head: single tokens, small trees) as the N side
+// (8 x 16 drafts over 560 to 2000 keys of 32 heads 40.1 us, as rows of a tile 45.3;
+// 8 x 32 44.4 and 47.7; from 33 rows on the other kernel is as fast):
 // S^T = K Q^T has a key a TMEM lane and a row a column, so that a thread takes
 // kN exponentials a tile and none is spent on rows that do not exist. O^T =
 // V^T P^T has a column of the head a lane. The rows' references m are kept in

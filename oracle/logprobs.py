@@ -16,9 +16,9 @@ def token_logprobs(logits, ids, top_k):
 
     With d = max - x >= 0 (exact in fp32 up to half a step), an fp32 kernel has
     e^-d to a factor of 1 + (d + 4) 2^-23 (the argument's two roundings and 2
-    ulp for the exponential), and each of the two sums, in whatever order, to
-    V' 2^-24 of its terms, where V' <= V / 256 + 64 is the depth of a sum by
-    256 threads or more and their tree. Weighted with p the exponentials' factor
+    ulp for the exponential), and each of the two sums to V' 2^-24 of its
+    terms, where V' <= V / 256 + 64 bounds the additions that a term passes
+    through: sums of a thread's words, of threads, of CTAs. Weighted with p the exponentials' factor
     is at most (E[d] + 4) 2^-23. ln S is off by the sum's relative error and an
     ulp of itself; ln p by that and half an ulp of d and of the result; the
     entropy ln S + E[d] by ln S's error and E[d] times the errors of both sums

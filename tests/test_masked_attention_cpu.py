@@ -274,3 +274,31 @@ def test_division_by_multiplication():
                                       (np.arange(1, 4) * d)[np.arange(1, 4) * d < 2 ** 31] - 1]).astype(np.int64))
         for m in n.tolist():
             assert (m if s == 0 else (m * mul) >> (31 + s)) == m // d
+
+
+def test_polynomial_exponential():
+    """2^x as the kernels form it for a part of the exponentials, in fp32 step by step with the source's own
+    coefficients: within 2^-22 relative down to 2^-126, and no more than 2^-126 below."""
+    import re
+    from conftest import REPO
+    text = (REPO / "nano-pointllm_b200" / "csrc" / "masked_attention.cu").read_text()
+    body = text[text.index("ma_exp2_poly(uint64_t x2) {"):]
+    body = body[:body.index("return make_float2")]
+    coeff = [np.float32(m) for m in re.findall(r"ma_pair\((\d\.\d+e[+-]\d+)f, ", body)]
+    coeff += [np.float32(m) for m in re.findall(r"ma_pair\((1\.00\d+)f, ", body)]
+    assert len(coeff) == 6
+    rng = np.random.default_rng(0)
+    x = np.concatenate([rng.uniform(-140, 16, 400000), np.arange(-140, 16), np.arange(-140, 16) + 0.5,
+                        [-np.inf, -1e30, -127, -126.5]]).astype(np.float32)
+    c = np.maximum(x, np.float32(-127))
+    magic = np.float32(12582912)
+    t = c + magic
+    f = (c - (t - magic)).astype(np.float32)  # exact
+    y = np.full_like(f, coeff[0])
+    for a in coeff[1:]:
+        y = (y.astype(np.float64) * f + a).astype(np.float32)  # a fused step
+    r = (y.view(np.int32) + (t.view(np.int32) << 23)).view(np.float32).astype(np.float64)
+    want = np.exp2(x.astype(np.float64))
+    far = x < -126
+    assert (np.abs(r - want) <= want * 2.0 ** -22)[~far].all()
+    assert (r[far] >= 0).all() and (r[far] <= 2.0 ** -125).all()

@@ -609,9 +609,7 @@ __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, 
     if (it.nt == 0) continue;
     const int streams = !kShared && it.second ? 2 : 1, list = item_no % kMaLists;
     const int pa = it.prefix + it.tok0, pb = it.prefix + min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1)) - 1;
-    if (lane < 2) s.n_bad[list][lane][which] = 0;
-    if (kWarps == 1 && lane < 2) s.n_bad[list][lane][1] = 0;
-    __syncwarp();
+    bool fresh = true;
 #pragma unroll 1
     for (int t = 0; ok && t < it.nt; ++t) {
       const int xt = it.x0 + t * kMaTile;
@@ -624,6 +622,12 @@ __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, 
                           NPL_DEV_TIMEOUT_EPILOGUE);
         if (!ok) break;
         ++n_raw;
+        if (fresh) {  // not before a tile of the item has come: till then this warp may be any number of items ahead
+          if (lane < 2) s.n_bad[list][lane][which] = 0;
+          if (kWarps == 1 && lane < 2) s.n_bad[list][lane][1] = 0;
+          __syncwarp();
+          fresh = false;
+        }
 #pragma unroll 1
         for (int row = which * 32 + lane; row < kMaTile; row += 32 * kWarps) {
           const int x = xt + row, key = x < it.sink_x ? x : x + it.shift;

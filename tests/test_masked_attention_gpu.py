@@ -127,6 +127,10 @@ TREES = [
     ([(31, 1500), (24, 333)], 3, 3, 64, 16),
     ([(6, 700), (5, 2000)], 10, 2, 128, 32),
     ([(33, 600), (9, 64)], 4, 4, 128, 16),
+    ([(50, 400), (1, 700)], 3, 3, 128, 16),
+    ([(3, 200), (2, 900)], 100, 1, 64, 16),
+    ([(2, 300)], 128, 1, 128, 32),
+    ([((7 * i) % 300, (7 * i) % 300 + 40 * (i % 5)) for i in range(60)], 4, 4, 64, 16),
 ]
 
 
@@ -193,6 +197,9 @@ WINDOWS = [
     ([(1, 900), (1, 5)], 34, 1, 64, 64, 200, 3),
     ([(20, 300), (3, 3000)], 3, 3, 128, 256, 256, 4),
     ([(1, 3000)], 80, 1, 128, 16, 1000, 0),
+    ([(1, (i * 37) % 900) for i in range(600)], 3, 3, 64, 16, 200, 4),
+    ([((11 * i) % 260, (11 * i) % 260 + 70 * (i % 4)) for i in range(70)], 4, 2, 128, 8, 64, 9),
+    ([(3, 200), (5, 40)], 128, 1, 64, 8, 30, 2),
 ]
 
 
@@ -472,3 +479,42 @@ def test_many_bad_values_over_a_long_context(PA):
             blk, at = c.slot(b, i)
             c.v[blk, at, 0, i % 128] = float("nan")
     check(PA.paged_tree_attention(*c.args(), m), c.tree_oracle(m))
+
+
+def test_first_call_in_a_capture(cuda_device):
+    """A process whose first call of each operator is captured into a graph."""
+    import subprocess
+    import sys
+    from conftest import REPO
+    code = """
+import sys; sys.path.insert(0, 'tests')
+import conftest, torch
+from nanopointllm_b200 import logprobs, paged_attention as PA
+from test_masked_attention_gpu import Case, check, tree
+c = Case([(9, 900), (20, 300)], 4, 2, 128, 16, torch.float16)
+a, m = c.args(), tree(c)
+x, ids = torch.randn(3, 5000, device='cuda'), torch.zeros(3, dtype=torch.int64, device='cuda')
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    t = PA.paged_tree_attention(*a, m, max_q_len=20)
+    w = PA.paged_window_attention(*a, 100, 4, max_q_len=20)
+    r = logprobs.token_logprobs(x, ids, 4)
+g.replay()
+torch.cuda.synchronize()
+check(t, c.tree_oracle(m))
+check(w, c.window_oracle(100, 4))
+assert torch.equal(r.top_ids, x.topk(4).indices)
+"""
+    subprocess.run([sys.executable, "-c", code], cwd=REPO, check=True, timeout=300)
+
+
+def test_bad_values_ahead_of_full_tiles(PA):
+    """Sequences whose tiles need no cleaning behind ones with a bad value that one of two tokens sees: the warp that
+    cleans may run ahead through all of them."""
+    first = 148
+    c = Case([(2, 130)] * first + [(1, 128)] * (9 * first), 1, 1, 64, 128, F16, seed=47)
+    for b in range(first):
+        blk, at = c.slot(b, 129)
+        c.v[blk, at, 0, b % 64] = float("inf")
+    check(PA.paged_window_attention(*c.args(), 1000, 0), c.window_oracle(1000, 0))

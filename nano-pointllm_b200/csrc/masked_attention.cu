@@ -97,6 +97,7 @@ struct MaArgs {
   int mask_cols;
   int window, sinks;
   int B, H, Hkv, G, num_blocks, block_size, max_blocks, total_q, max_q_len;
+  bool out32;    // rows of out start on 32-byte boundaries
   int tokens;    // of a row tile: 128 / G
   int capacity;  // keys that a row of the table has room for
   int piece, piece_log;  // keys of a piece, a power of two
@@ -289,6 +290,12 @@ __device__ __forceinline__ float2 ma_ld_cluster2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
+}
+
+__device__ __forceinline__ void ma_st_32b(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 // Scores of columns that are not seen become minus infinity. False: every row of the warp sees all of them.
@@ -1160,13 +1167,17 @@ __global__ void __launch_bounds__(kMaThreads, 1)
               *reinterpret_cast<uint4*>(stage + (((c * 8 + e) ^ (r & 7)) << 2)) =
                   make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           } else {
+            uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t w[4];
+            for (int e = 0; e < 16; ++e)
+              w[e] = MaType<T>::pack(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            if (p.out32) {
 #pragma unroll
-              for (int d = 0; d < 4; ++d)
-                w[d] = MaType<T>::pack(__uint_as_float(o[8 * e + 2 * d]) * inv, __uint_as_float(o[8 * e + 2 * d + 1]) * inv);
-              reinterpret_cast<uint4*>(dst)[c * 4 + e] = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int e = 0; e < 2; ++e) ma_st_32b(dst + c * 32 + e * 16, w + e * 8);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                reinterpret_cast<uint4*>(dst)[c * 4 + e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
             }
           }
         }
@@ -1624,6 +1635,7 @@ template <bool kTree>
 int run(const char* what, MaArgs p, int dtype, int D, float scale, cudaStream_t st) {
   p.c2 = scale * 1.4426950408889634f;
   p.capacity = p.max_blocks * p.block_size;
+  p.out32 = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.ld_out * 2)) & 31u) == 0;
   p.piece_log = kMaPieceLog;
   while (p.block_size & ((1 << p.piece_log) - 1)) --p.piece_log;
   p.piece = 1 << p.piece_log;

@@ -1699,6 +1699,7 @@ extern "C" int npl_paged_tree_attention(const void* q, int dtype, int64_t ld_q, 
                 (long long)ld_mask, max_q_len);
   if (int rc = check_device()) return rc;
   if (B == 0 || total_q == 0 || max_q_len == 0) return NPL_OK;
+  p.max_q_len = std::min(max_q_len, total_q);  // a loose bound costs nothing, and no count of tiles overflows
   p.status = device_status_ptr();
   return run<true>(what, p, dtype, D, scale, static_cast<cudaStream_t>(stream));
 }
@@ -1721,6 +1722,7 @@ extern "C" int npl_paged_window_attention(const void* q, int dtype, int64_t ld_q
     return fail(NPL_ERR_ARG, "%s: window %d (at least 1), sinks %d (at least 0)", what, window, sinks);
   if (int rc = check_device()) return rc;
   if (B == 0 || total_q == 0 || p.max_q_len == 0) return NPL_OK;
+  p.max_q_len = std::min(p.max_q_len, total_q);
   p.status = device_status_ptr();
   return run<false>(what, p, dtype, D, scale, static_cast<cudaStream_t>(stream));
 }

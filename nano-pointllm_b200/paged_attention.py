@@ -212,6 +212,8 @@ def _masked_arguments(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         q_lens, q_offsets = q_lens.contiguous(), q_offsets.contiguous()
         if max_q_len is None:
             max_q_len = int(q_lens.max().item()) if b else 0
+        if not 0 <= max_q_len < 2 ** 31:
+            raise ValueError("max_q_len must be at least 0, below 2^31")
         lens, offsets = q_lens.data_ptr(), q_offsets.data_ptr()
     if not q.is_contiguous():
         ld, step, one = q.stride()
@@ -223,6 +225,7 @@ def _masked_arguments(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         ld, one = block_tables.stride()
         if one != 1 or ld < width:
             block_tables = block_tables.contiguous()
+    ld_table = block_tables.stride(0) if b > 1 else width  # one row's stride may be anything
     context_lens = context_lens.contiguous()
     if out is None:
         ld_out = h * d
@@ -231,12 +234,14 @@ def _masked_arguments(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         if out.shape != (total_q, h, d) or out.dtype is not dt:
             raise ValueError("out must have the shape and type of q")
         ld_out, step, one = out.stride()
+        if total_q == 1:
+            ld_out = h * d
         if out.numel() and (one != 1 or step != d or ld_out % 8 or ld_out < h * d or out.data_ptr() % 16):
             raise ValueError("out needs contiguous heads and tokens on 16-byte boundaries that do not overlap")
         if _overlap(out, q, k_cache, v_cache):
             raise ValueError("out may not overlap q or the caches")
-    args = (q.data_ptr(), code, q.stride(0), total_q, h, hkv, d, k_cache.data_ptr(), v_cache.data_ptr(), nb, bs,
-            block_tables.data_ptr(), block_tables.stride(0), width, context_lens.data_ptr(), lens, offsets, b,
+    args = (q.data_ptr(), code, q.stride(0) if total_q > 1 else h * d, total_q, h, hkv, d, k_cache.data_ptr(), v_cache.data_ptr(), nb, bs,
+            block_tables.data_ptr(), ld_table, width, context_lens.data_ptr(), lens, offsets, b,
             max_q_len)
     return args, out, ld_out, (q, block_tables, context_lens, q_lens, q_offsets)
 
@@ -267,10 +272,11 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if tree_mask.dim() != 2 or tree_mask.shape[0] != total_q or tree_mask.shape[1] < most:
         raise ValueError("tree_mask must be [total_q, at least max_q_len]")
     cols = tree_mask.shape[1]
-    if tree_mask.stride(1) != 1 or tree_mask.stride(0) < cols:
-        tree_mask = tree_mask.contiguous()
+    if tree_mask.stride(1) != 1 or (tree_mask.stride(0) < cols and total_q > 1):
+        tree_mask = tree_mask.clone(memory_format=torch.contiguous_format)
+    ld_mask = tree_mask.stride(0) if total_q > 1 else cols
     if total_q and most and args[-2]:
-        _call(_tree_attention, out.device, *args, tree_mask.data_ptr(), tree_mask.stride(0), cols, scale,
+        _call(_tree_attention, out.device, *args, tree_mask.data_ptr(), ld_mask, cols, scale,
               out.data_ptr(), ld_out)
     return out
 
@@ -279,12 +285,14 @@ def tree_mask_from_parents(parents: torch.Tensor, q_offsets: torch.Tensor, max_q
     """bool [total_q, max_q_len] for ``paged_tree_attention``: each draft sees
     itself and the drafts that it follows. ``parents`` [total_q] holds the
     place of each draft's parent within its sequence (0 to max_q_len - 1), -1
-    where it follows the last token of the cache; parents come before their
-    children. Rows of no sequence come out as if they belonged to the one
+    where it follows the last token of the cache; one outside that range ends
+    the path as -1 does. Parents come before their children. Rows of no sequence come out as if they belonged to the one
     before. Elementary torch operations, on any device: built once per tree."""
     total = parents.shape[0]
     if parents.dim() != 1 or parents.is_floating_point() or q_offsets.dim() != 1 or max_q_len < 1:
         raise ValueError("parents must be whole numbers [total_q], q_offsets [B], max_q_len at least 1")
+    if total and not q_offsets.numel():
+        raise ValueError("q_offsets must hold each sequence's first row")
     row = torch.arange(total, device=parents.device)
     order = torch.sort(q_offsets.long()).values
     first = order[(torch.searchsorted(order, row, right=True) - 1).clamp_min(0)]  # each draft's first row
@@ -292,9 +300,10 @@ def tree_mask_from_parents(parents: torch.Tensor, q_offsets: torch.Tensor, max_q
     mask = torch.zeros((total, max_q_len + 1), dtype=torch.bool, device=parents.device)
     at = place
     for _ in range(max_q_len):
-        # a finished path stays at -1, in the spare last column
-        mask[row, torch.where(at < 0, torch.full_like(at, max_q_len), at)] = True
-        at = torch.where(at < 0, at, parents.long()[(first + at).clamp(0, total - 1)])
+        # a finished path stays where it is, in the spare last column
+        done = (at < 0) | (at >= max_q_len)
+        mask[row, torch.where(done, torch.full_like(at, max_q_len), at)] = True
+        at = torch.where(done, at, parents.long()[(first + at).clamp(0, total - 1)])
     return mask[:, :max_q_len]
 
 

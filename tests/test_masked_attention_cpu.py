@@ -205,6 +205,32 @@ def test_tree_mask_from_parents():
         pa.tree_mask_from_parents(torch.zeros(3), torch.tensor([0]), 3)
 
 
+def test_strides_of_a_single_row(PA):
+    """A tensor with one row may have any stride there: it is never used."""
+    pa, calls = PA
+    c = _case(T=1, B=1)
+    c["q"] = torch.zeros(256, dtype=F16).as_strided((1, 4, 64), (259, 64, 1))
+    c["block_tables"] = torch.zeros(3, dtype=I32).as_strided((1, 3), (0, 1))
+    out = torch.zeros(256, dtype=F16).as_strided((1, 4, 64), (261, 64, 1))
+    mask = torch.ones(5, dtype=torch.bool).as_strided((1, 5), (0, 1))
+    assert pa.paged_tree_attention(**c, tree_mask=mask, max_q_len=1, out=out) is out
+    _, a = calls.pop()
+    assert (a[0], a[2], a[12], a[20], a[-2:]) == (c["q"].data_ptr(), 256, 3, 5, (out.data_ptr(), 256))
+    for most in (-1, 1 << 31):
+        with pytest.raises(ValueError, match="max_q_len"):
+            pa.paged_window_attention(**c, window=5, max_q_len=most)
+    assert not calls
+
+
+def test_tree_mask_from_odd_parents():
+    from nanopointllm_b200 import paged_attention as pa
+    got = pa.tree_mask_from_parents(torch.tensor([-5, 0, 9, 4]), torch.tensor([0]), 4)
+    assert torch.equal(got, torch.tensor([[1, 0, 0, 0], [1, 1, 0, 0], [0, 0, 1, 0], [0, 0, 0, 1]]).bool())
+    assert pa.tree_mask_from_parents(torch.zeros(0, dtype=I32), torch.zeros(0, dtype=I32), 4).shape == (0, 4)
+    with pytest.raises(ValueError, match="q_offsets"):
+        pa.tree_mask_from_parents(torch.zeros(2, dtype=I32), torch.zeros(0, dtype=I32), 4)
+
+
 def test_refusals_and_layouts_of_log_probabilities(LP, L):
     lp, calls = LP
     x, ids = torch.zeros(4, 50), torch.zeros(4, dtype=torch.int64)

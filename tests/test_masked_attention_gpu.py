@@ -216,6 +216,35 @@ def test_window(PA, seqs, H, Hkv, D, bs, window, sinks, dtype):
         check(PA.paged_window_attention(*a, window, sinks), want, "one token each")
 
 
+@pytest.mark.parametrize("at", [0, 8, 16], ids=["32-byte", "16-byte", "32-byte, within a row"])
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 64)])
+def test_window_outputs_inside_wider_rows(PA, at, D, bs):
+    """Rows that one CTA finishes are stored 32 bytes at a time, or 16 where they start between such boundaries;
+    what lies beside them stays."""
+    c = Case([(700, 900), (150, 150)] * 12, 8, 4, D, bs, F16, seed=at)
+    store = torch.full((c.total, 8 * D + 32), 7.0, dtype=F16, device="cuda")
+    out = store[:, at:at + 8 * D].view(c.total, 8, D)
+    PA.paged_window_attention(*c.args(), 100, 4, max_q_len=700, out=out)
+    check(out, c.window_oracle(100, 4))
+    assert (store[:, :at] == 7).all() and (store[:, at + 8 * D:] == 7).all()
+
+
+def test_loose_bounds_and_a_single_row(PA):
+    """A bound far above the lengths gives what the exact one gives; one row may have any stride."""
+    c = Case([(150, 400), (3, 90)], 4, 2, 128, 16, F16, seed=41)
+    want = PA.paged_window_attention(*c.args(), 70, 4, max_q_len=c.total)
+    for most in (c.total + 1, 5000, 2 ** 31 - 1):
+        assert torch.equal(PA.paged_window_attention(*c.args(), 70, 4, max_q_len=most), want)
+    c = Case([(1, 333)], 4, 2, 64, 8, BF16, seed=43)
+    a = list(c.args())
+    a[0] = c.q.as_strided((1, 4, 64), (259, 64, 1))
+    a[3] = a[3].as_strided(a[3].shape, (0, 1))
+    out = torch.zeros(256, dtype=BF16, device="cuda").as_strided((1, 4, 64), (261, 64, 1))
+    check(PA.paged_window_attention(*a, 100, 3, max_q_len=1, out=out), c.window_oracle(100, 3))
+    mask = torch.ones(3, dtype=torch.bool, device="cuda").as_strided((1, 3), (0, 1))
+    check(PA.paged_tree_attention(*a, mask, max_q_len=1), c.tree_oracle(mask))
+
+
 def test_window_of_everything_is_causal(PA):
     """A window longer than the context: the causal kernel's results, within both kernels' roundings."""
     c = Case([(300, 300), (129, 700)], 8, 2, 128, 16, F16, seed=2)

@@ -43,7 +43,7 @@
 // 165 us, 6.0 TB/s); for prompts by a stream's chain of product, scores out of
 // TMEM (twice: held in registers they spill), exponentials (a quarter of them by
 // a polynomial: 375 us for 16000 tokens of 32/8 heads under a window of 1024, none
-// 409, half 415; 325 with tiles packed) and P back.
+// 409, half 415; 325 with tiles packed, 310 with 32-byte stores) and P back.
 #include <algorithm>
 #include <initializer_list>
 

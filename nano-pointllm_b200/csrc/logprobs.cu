@@ -309,12 +309,12 @@ __device__ void lp_top(LpSmem& s, const LpRow<T>& r, float own_max, bool any, in
     // Many equal logits (the zeros of a padding row, say), or many large ones with one thread. A pass finds the best
     // logit after the last one taken; then those equal to it are taken in the order of their places, a few at a time.
     const int from = r.first ? 0 : r.head + r.w0 * LpWord<T>::kN;
-    unsigned long long last = ~0ull;
+    unsigned long long most = ~0ull;  // not taken yet: this (a NaN in the first place) and less
     for (int j = 0; j < k;) {
       unsigned long long c = 0;
       lp_each(r, [&](float x, int i) {
         const unsigned long long y = lp_pack(lp_key(x), i);
-        if (y < last && y > c) c = y;
+        if (y <= most && y > c) c = y;
       });
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) c = max(c, __shfl_xor_sync(0xffffffffu, c, o));
@@ -348,7 +348,7 @@ __device__ void lp_top(LpSmem& s, const LpRow<T>& r, float own_max, bool any, in
           ++j;
         }
       }
-      last = (unsigned long long)key << 32;  // where places are left, all that are equal have been taken
+      most = ((unsigned long long)key << 32) - 1;  // where places are left, all that are equal have been taken; key > 0
       __syncthreads();
     }
     __syncthreads();

@@ -207,3 +207,25 @@ def test_large_logits_that_share_their_places(P, n, kind):
     x = x.to(TYPES[kind]).cuda()
     ids = torch.arange(n).cuda()
     check(P.token_logprobs(x, ids, 32), x, ids, 32)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [7, 310])
+@pytest.mark.parametrize("v", [600, 5001, 70001])
+def test_nan_before_all_others(P, n, v, kind):
+    """A NaN in the first place, with more equal logits than any list of candidates holds, beside it or behind it."""
+    x, ids = rows(n, v, TYPES[kind], seed=v)
+    nan = float("nan")
+    x[0] = nan
+    x[1] = 0.0
+    x[1, 0] = nan
+    x[2, 0] = nan
+    x[3] = 1.0
+    x[3, 0] = x[3, 7] = x[3, v - 1] = nan
+    x[4] = -x[0]  # with the sign set
+    x[5] = nan
+    x[5, 0] = float("inf")
+    x[6] = -float("inf")
+    x[6, 0] = nan
+    for k in (1, 5, 20):
+        check(P.token_logprobs(x, ids, k), x, ids, k)

@@ -335,11 +335,18 @@ __device__ __forceinline__ uint64_t ma_fma2(uint64_t a, uint64_t b, uint64_t c) 
   return r;
 }
 
+__device__ __forceinline__ uint64_t ma_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // 2^x for two x <= 127 without the special function unit, which is what the
 // softmax of many rows waits for: x = n + f with the whole number n next to x (by
 // adding 1.5 * 2^23), 2^f by the polynomial of degree 5 with the least relative
-// error on [-1/2, 1/2] (Remez; 7.5e-8), n added to its exponent. x below -127
-// gives a denormal number or 0.
+// error on [-1/2, 1/2] (Remez; 7.5e-8), times 2^n, whose bits come from those of
+// n. x below -126.5 (n = -127) gives 0. NaN gives NaN: 2^f is NaN, and a product
+// keeps it (n added to its exponent would make a number of it).
 __device__ __forceinline__ float2 ma_exp2_poly(uint64_t x2) {
   const float2 u = ma_unpair(x2);
   float x0, x1;
@@ -355,9 +362,11 @@ __device__ __forceinline__ float2 ma_exp2_poly(uint64_t x2) {
   y = ma_fma2(y, f, ma_pair(2.4022120237350464e-01f, 2.4022120237350464e-01f));
   y = ma_fma2(y, f, ma_pair(6.931469440460205e-01f, 6.931469440460205e-01f));
   y = ma_fma2(y, f, ma_pair(1.0000001192092896f, 1.0000001192092896f));
-  const float2 r = ma_unpair(y), tt = ma_unpair(t);
-  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(tt.x) << 23)),
-                     __int_as_float(__float_as_int(r.y) + (__float_as_int(tt.y) << 23)));
+  const float2 tt = ma_unpair(t);
+  const uint64_t power = ma_pair(__int_as_float((__float_as_int(tt.x) << 23) + 0x3f800000),
+                                 __int_as_float((__float_as_int(tt.y) << 23) + 0x3f800000));
+  const float2 r = ma_unpair(ma_mul2(y, power));
+  return make_float2(r.x, r.y);
 }
 
 // p = 2^(score c2 + add) of 32 columns, packed; their sums go to ls. One pair of
@@ -1141,7 +1150,6 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         tc_fence_after();
       }
       if (!ok) break;
-      if (l < 1e-30f) l = 0.f;  // no key seen (the largest p of a row is 2^-2 or more): the polynomial leaves 2^-149 a key
       if (warp_on) {
         const int* const n_bad = s.n_bad[list][owner];
         const bool bad = any_part && n_bad[0] + n_bad[1] > 0;  // written before the P.V products of such tiles

@@ -328,3 +328,34 @@ def test_polynomial_exponential():
     far = x < -126
     assert (np.abs(r - want) <= want * 2.0 ** -22)[~far].all()
     assert (r[far] >= 0).all() and (r[far] <= 2.0 ** -125).all()
+
+
+def test_polynomial_exponential_by_a_product():
+    """2^x as the kernels form it for a part of the exponentials, with 2^n from the bits of n as a factor: within
+    2^-22 relative, 0 from x = -127 down (n = -127), and NaN where x is NaN."""
+    import re
+    from conftest import REPO
+    text = (REPO / "nano-pointllm_b200" / "csrc" / "masked_attention.cu").read_text()
+    body = text[text.index("ma_exp2_poly(uint64_t x2) {"):]
+    body = body[:body.index("\n}")]
+    assert "<< 23) + 0x3f800000" in body and "ma_mul2(y, power)" in body
+    coeff = [np.float32(m) for m in re.findall(r"ma_pair\((\d\.\d+(?:e[+-]\d+)?)f, ", body) if m != "12582912."]
+    coeff = [c for c in coeff if c < 2]
+    assert len(coeff) == 6
+    rng = np.random.default_rng(1)
+    x = np.concatenate([rng.uniform(-140, 16, 400000), np.arange(-140, 128), np.arange(-140, 127) + 0.5,
+                        [-np.inf, -1e30, -127, -126.5, -126.49, np.nan]]).astype(np.float32)
+    with np.errstate(invalid="ignore", over="ignore"):
+        c = np.where(np.isnan(x), x, np.maximum(x, np.float32(-127)))
+        t = c + np.float32(12582912)
+        f = (c - (t - np.float32(12582912))).astype(np.float32)  # exact
+        y = np.full_like(f, coeff[0])
+        for a in coeff[1:]:
+            y = (y.astype(np.float64) * f + a).astype(np.float32)  # a fused step
+        power = ((t.view(np.int32).astype(np.int64) << 23) + 0x3f800000).astype(np.uint32).view(np.float32)
+        r = (y * power).astype(np.float64)
+    want = np.exp2(x.astype(np.float64))
+    assert (np.isnan(r) == np.isnan(x)).all()
+    near = x >= -126.0
+    assert (np.abs(r - want) <= want * 2.0 ** -22)[near].all()
+    assert (r[x <= -127] == 0).all() and (r[x < -126.0] >= 0).all() and (r[x < -126.0] <= 2.0 ** -125).all()

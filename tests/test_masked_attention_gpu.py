@@ -547,3 +547,24 @@ def test_bad_values_ahead_of_full_tiles(PA):
         blk, at = c.slot(b, 129)
         c.v[blk, at, 0, b % 64] = float("inf")
     check(PA.paged_window_attention(*c.args(), 1000, 0), c.window_oracle(1000, 0))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("new,before", [(12, 400), (20, 400), (40, 400), (150, 400), (300, 300), (40, 6000)])
+def test_scores_that_are_no_numbers(PA, new, before, dtype):
+    """A key that is NaN or infinite makes the rows that see it with a score of NaN or plus infinity NaN as a whole,
+    wherever it stands in its tile; a score of minus infinity has no weight."""
+    for i, bad in enumerate([float("nan"), float("inf"), -float("inf")]):
+        c = Case([(new, new + before)], 4, 2, 128, 16, dtype, seed=51 + i)
+        for place in range(8):
+            blk, at = c.slot(0, before + place)  # some rows of a window of 60 see it, others do not
+            keep = c.k[blk, at].clone()
+            c.k[blk, at, place % 2, 3] = bad
+            for what, got, want in (
+                    ("window", PA.paged_window_attention(*c.args(), 60, 4), c.window_oracle(60, 4)),
+                    ("all", PA.paged_window_attention(*c.args(), 1 << 20, 0), c.window_oracle(1 << 20, 0))):
+                none = np.isnan(want[0])
+                assert none.any() and not none.all()
+                assert np.isnan(got.float().cpu().numpy()[none]).all(), (what, bad, place)
+                check(got, want, f"{what}, {bad} at {place}")
+            c.k[blk, at] = keep

@@ -58,7 +58,6 @@ namespace {
 constexpr int kMaThreads = 384;
 constexpr int kMaTile = 128;
 constexpr int kMaFixed = 10;            // what a round of clusters costs beside its tiles, in tiles
-constexpr int kMaLists = 8;            // items whose lists of bad keys are kept: more than the ring can be ahead
 constexpr int kMaBad = 12;             // keys with V elements that are not finite, remembered for an item
 constexpr int kMaPieceLog = 5;         // 32 keys of a piece at most
 constexpr int kMaBoxLog = 7;           // 128 keys of a load at most
@@ -110,17 +109,27 @@ struct MaArgs {
   int* status;
 };
 
+// Lists of keys whose V rows held elements that are not finite, of the last kLists items of one stream and of the last
+// kLists of two. A list is written again when the first V tile of an item of its kind has come. That tile's stage, one
+// of kStages, has been free, and an item takes two stages or more, so every product of the item kStages / 2 + 1 before
+// it has been issued, for which every stream that has rows in it has left the items before. The two kinds are counted
+// apart because the second stream takes no part in items of one: it may still read its last list while the first goes
+// through any number of those.
+template <int kLists>
 struct MaBarriers {
+  static_assert((kLists & (kLists - 1)) == 0, "a power of two");
+  static constexpr int kListMask = (kLists - 1) * 0x10001;  // the count of items of one stream, and of two above it
+  __device__ static int list(int count, bool second) { return second ? kLists + (count >> 16) : count & 0xffff; }
+  __device__ static int next(int count, bool second) { return (count + (second ? 0x10000 : 1)) & kListMask; }
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], mma_done;
   uint32_t tmem_base;
   int abort;
-  // keys whose V rows held elements that are not finite: [item % kMaLists][stream whose V it is]
-  int n_bad[kMaLists][2][2];  // the last: warp 10 or 11
-  int bad[kMaLists][2][2][kMaBad];
+  int n_bad[2 * kLists][2][2];  // [list][stream whose V it is][warp 10 or 11]
+  int bad[2 * kLists][2][2][kMaBad];
 };
 
 template <int D>
-struct MaSmem : MaBarriers {
+struct MaSmem : MaBarriers<D == 128 ? 4 : 8> {
   static constexpr bool kFew = false;
   static constexpr int kRows = kMaTile;
   static constexpr uint32_t kQHalf = kMaTile * 128;  // Q: 128 rows x 64 elements (one swizzle span), twice for D = 128
@@ -136,7 +145,7 @@ struct MaSmem : MaBarriers {
 
 // Few rows, as the N side of the products.
 template <int D, int kN>
-struct MaFewSmem : MaBarriers {
+struct MaFewSmem : MaBarriers<D == 128 ? 4 : 8> {
   static constexpr bool kFew = true;
   static constexpr int kRows = kN;
   static constexpr uint32_t kQHalf = kN * 128;
@@ -159,6 +168,8 @@ struct MaFewSmem : MaBarriers {
 constexpr size_t kMaMaxSmem = 232448 - 1024;  // of a CTA, without the room to align
 static_assert(sizeof(MaSmem<128>) <= kMaMaxSmem && sizeof(MaSmem<64>) <= kMaMaxSmem, "shared memory");
 static_assert(sizeof(MaFewSmem<128, 16>) <= kMaMaxSmem && sizeof(MaFewSmem<64, 16>) <= kMaMaxSmem, "shared memory");
+static_assert(std::max(MaSmem<128>::kStages, MaFewSmem<128, 16>::kStages) / 2 + 2 <= 4, "lists");
+static_assert(std::max(MaSmem<64>::kStages, MaFewSmem<64, 16>::kStages) / 2 + 2 <= 8, "lists");
 static_assert(sizeof(MaFewSmem<128, 32>) <= kMaMaxSmem && sizeof(MaFewSmem<64, 32>) <= kMaMaxSmem, "shared memory");
 
 template <typename T>
@@ -623,7 +634,7 @@ __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, 
   for (int i = first; ok && i < p.n_items; i += stride) {
     const MaItem it = ma_item<kTree, kShared>(p, i, rank);
     if (it.nt == 0) continue;
-    const int streams = !kShared && it.second ? 2 : 1, list = item_no % kMaLists;
+    const int streams = !kShared && it.second ? 2 : 1, list = S::list(item_no, it.second);
     const int pa = it.prefix + it.tok0, pb = it.prefix + min(it.n, it.tok0 + p.tokens * (kShared ? 2 : 1)) - 1;
     bool fresh = true;
 #pragma unroll 1
@@ -661,7 +672,7 @@ __device__ __forceinline__ void ma_clean_role(S& s, const MaArgs& p, int first, 
       }
     }
     ring += 2 * it.nt * streams;
-    ++item_no;
+    item_no = S::next(item_no, it.second);
   }
 }
 
@@ -1012,7 +1023,6 @@ __global__ void __launch_bounds__(kMaThreads, 1)
     for (int i = first; ok && i < p.n_items; i += stride) {
       const MaItem it = ahead;
       if (it.skip || (st == 1 && !it.second)) {
-        if (!it.skip && it.nt > 0) ++item_no;
         ahead = ma_item<kTree, kShared>(p, min(i + stride, p.n_items - 1), rank);
         continue;
       }
@@ -1022,7 +1032,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
       const bool row_ok = r < n_rows;
       const bool warp_on = (warp & 3) * 32 < n_rows;
       const int token = tok0 + row_tok, pos = it.prefix + token;
-      const int list = item_no % kMaLists;
+      const int list = S::list(item_no, it.second);
       bool any_part = false;
       float m = -INFINITY, l = 0.f;  // m in units of log2
       // this row sees x < row_a and row_b <= x < row_e (window)
@@ -1211,7 +1221,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
           reinterpret_cast<float2*>(reinterpret_cast<float*>(s.kv) + 2 * kMaTile * D)[st * kMaTile + r] =
               make_float2(m, l);
       }
-      if (it.nt > 0) ++item_no;
+      if (it.nt > 0) item_no = S::next(item_no, it.second);
     }
   }
 
@@ -1285,13 +1295,10 @@ __global__ void __launch_bounds__(kMaThreads, 1)
     for (int i = first; ok && i < p.n_items; i += stride) {
       const MaItem it = ma_item<kTree, false>(p, i, rank);
       if (it.skip) continue;
-      if (st == 1 && !it.second) {
-        if (it.nt > 0) ++item_no;
-        continue;
-      }
+      if (st == 1 && !it.second) continue;
       const int kvh = it.kvh + st;
       const int n_rows = min(p.tokens, it.n - it.tok0) * p.G;
-      const int list = item_no % kMaLists;
+      const int list = S::list(item_no, it.second);
       bool any_part = false;
       float m = -INFINITY;  // of row r, units of log2 (threads r < kN)
       if (r < kN) s.add[st][r] = r < n_rows ? kNone : -INFINITY;  // p = 0 in rows that do not exist
@@ -1498,7 +1505,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
           }
         }
       }
-      if (it.nt > 0) ++item_no;
+      if (it.nt > 0) item_no = S::next(item_no, it.second);
       tc_fence_before();  // O has been read before this thread's next arrival, which the next O waits for
       ma_stream_sync(st);  // and the normalisers, before the next item's
     }

@@ -359,3 +359,31 @@ def test_polynomial_exponential_by_a_product():
     near = x >= -126.0
     assert (np.abs(r - want) <= want * 2.0 ** -22)[near].all()
     assert (r[x <= -127] == 0).all() and (r[x < -126.0] >= 0).all() and (r[x < -126.0] <= 2.0 ** -125).all()
+
+
+@pytest.mark.parametrize("stages,lists", [(5, 4), (8, 8), (10, 8)])
+def test_lists_of_bad_values_are_free_when_taken_again(stages, lists):
+    """The order of a CTA's roles at its worst: a stream still reads its lists of item j, so that the products of the
+    next item in which it has rows wait for it, and with them the stages of the tiles behind (two an item at the
+    least). No item whose V tile may come meanwhile has the lists of item j: items of one stream and of two count
+    apart. (Counted together, eight lists are not enough.)"""
+    from conftest import REPO
+    text = (REPO / "nano-pointllm_b200" / "csrc" / "masked_attention.cu").read_text()
+    assert text.count(": MaBarriers<D == 128 ? 4 : 8> {") == 2
+    assert "kStages = D == 128 ? 5 : 8;" in text and "kStages = D == 64 ? 10 : 5;" in text
+    rng = np.random.default_rng(stages)
+    together = 0
+    for _ in range(200):
+        two = rng.random(60) < rng.choice([0.1, 0.5, 0.9])
+        count, lists_of = [0, 0], []
+        for t in two.tolist():
+            lists_of.append((t, count[t] % lists))
+            count[t] += 1
+        for j in range(60):
+            for stream in ((0, 1) if two[j] else (0,)):
+                next_item = next((i for i in range(j + 1, 60) if stream == 0 or two[i]), 1000)
+                free = 2 * next_item  # K and V of item i are tiles 2 i and 2 i + 1 of the ring; K of the next is read
+                meanwhile = [i for i in range(j + 1, 60) if 2 * i + 1 - stages <= free]
+                assert all(lists_of[i] != lists_of[j] for i in meanwhile)
+                together += any(i % 8 == j % 8 for i in meanwhile)
+    assert together > 0

@@ -568,3 +568,19 @@ def test_scores_that_are_no_numbers(PA, new, before, dtype):
                 assert np.isnan(got.float().cpu().numpy()[none]).all(), (what, bad, place)
                 check(got, want, f"{what}, {bad} at {place}")
             c.k[blk, at] = keep
+
+
+@pytest.mark.parametrize("bad", [12, 72])
+@pytest.mark.parametrize("Hkv,D", [(1, 64), (5, 128)])
+def test_bad_values_of_a_stream_that_falls_behind(PA, Hkv, D, bad):
+    """Sequences of two row tiles, whose bad values only the second tile's rows see, ahead of many sequences of one:
+    the first tile's stream goes on to those while the second still adds its bad values. Few, and more than a list
+    holds."""
+    first, later = 148, 12 * 148
+    c = Case([(200, 200)] * first + [(3, 100)] * (later if Hkv == 1 else later // 3), Hkv, Hkv, D, 16, F16, seed=53)
+    for b in range(len(c.seqs)):
+        for i in (range(128, 128 + bad) if b < first else [98, 99]):
+            blk, at = c.slot(b, i)
+            c.v[blk, at, :, (b + 5 * i) % D] = float("inf") if i % 2 else -float("inf")
+    check(PA.paged_window_attention(*c.args(), 1000, 0, max_q_len=200), c.window_oracle(1000, 0))
+    check(PA.paged_tree_attention(*c.args(), m := tree(c), max_q_len=200), c.tree_oracle(m))

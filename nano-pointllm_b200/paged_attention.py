@@ -281,18 +281,25 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     return out
 
 
-def tree_mask_from_parents(parents: torch.Tensor, q_offsets: torch.Tensor, max_q_len: int) -> torch.Tensor:
+def tree_mask_from_parents(parents: torch.Tensor, q_offsets: torch.Tensor, max_q_len: int,
+                           q_lens: torch.Tensor | None = None) -> torch.Tensor:
     """bool [total_q, max_q_len] for ``paged_tree_attention``: each draft sees
     itself and the drafts that it follows. ``parents`` [total_q] holds the
     place of each draft's parent within its sequence (0 to max_q_len - 1), -1
     where it follows the last token of the cache; one outside that range ends
     the path as -1 does. Parents come before their children. Rows of no sequence come out as if they belonged to the one
-    before. Elementary torch operations, on any device: built once per tree."""
+    before. ``q_lens`` [B] says which sequences have no drafts: their offsets, which may be any, are left out; without
+    it every offset begins a sequence's rows. Elementary torch operations, on any device, none of which waits for it:
+    built once per tree."""
     total = parents.shape[0]
     if parents.dim() != 1 or parents.is_floating_point() or q_offsets.dim() != 1 or max_q_len < 1:
         raise ValueError("parents must be whole numbers [total_q], q_offsets [B], max_q_len at least 1")
     if total and not q_offsets.numel():
         raise ValueError("q_offsets must hold each sequence's first row")
+    if q_lens is not None:
+        if q_lens.is_floating_point() or q_lens.shape != q_offsets.shape:
+            raise ValueError("q_lens must be whole numbers [B], as q_offsets")
+        q_offsets = torch.where(q_lens > 0, q_offsets.long(), total)  # behind all rows
     row = torch.arange(total, device=parents.device)
     order = torch.sort(q_offsets.long()).values
     first = order[(torch.searchsorted(order, row, right=True) - 1).clamp_min(0)]  # each draft's first row
@@ -302,7 +309,7 @@ def tree_mask_from_parents(parents: torch.Tensor, q_offsets: torch.Tensor, max_q
     for _ in range(max_q_len):
         # a finished path stays where it is, in the spare last column
         done = (at < 0) | (at >= max_q_len)
-        mask[row, torch.where(done, torch.full_like(at, max_q_len), at)] = True
+        mask.scatter_(1, torch.where(done, max_q_len, at)[:, None], True)
         at = torch.where(done, at, parents.long()[(first + at).clamp(0, total - 1)])
     return mask[:, :max_q_len]
 

@@ -387,3 +387,18 @@ def test_lists_of_bad_values_are_free_when_taken_again(stages, lists):
                 assert all(lists_of[i] != lists_of[j] for i in meanwhile)
                 together += any(i % 8 == j % 8 for i in meanwhile)
     assert together > 0
+
+
+def test_tree_mask_leaves_out_sequences_without_drafts():
+    """Their offsets may be any, inside other sequences' rows too."""
+    from nanopointllm_b200 import paged_attention as pa
+    parents = torch.tensor([-1, 0, 1, 0, -1, 0, 0])
+    want = pa.tree_mask_from_parents(parents, torch.tensor([0, 4]), 4)
+    for offs, lens in (([0, 2, 4], [4, 0, 3]), ([2, 0, 4, 5], [0, 4, 3, 0]), ([0, 100, 4], [4, 0, 3]),
+                       ([4, -3, 0, 3, 6, 7], [3, 0, 4, 0, 0, 0])):
+        o, n = torch.tensor(offs, dtype=I32), torch.tensor(lens, dtype=I32)
+        assert torch.equal(pa.tree_mask_from_parents(parents, o, 4, n), want), (offs, lens)
+    assert torch.equal(pa.tree_mask_from_parents(parents, torch.tensor([4, 0]), 4, torch.tensor([3, 4])), want)
+    for wrong in (torch.tensor([4]), torch.tensor([4.0, 3.0])):
+        with pytest.raises(ValueError, match="q_lens"):
+            pa.tree_mask_from_parents(parents, torch.tensor([0, 4]), 4, wrong)

@@ -584,3 +584,19 @@ def test_bad_values_of_a_stream_that_falls_behind(PA, Hkv, D, bad):
             c.v[blk, at, :, (b + 5 * i) % D] = float("inf") if i % 2 else -float("inf")
     check(PA.paged_window_attention(*c.args(), 1000, 0, max_q_len=200), c.window_oracle(1000, 0))
     check(PA.paged_tree_attention(*c.args(), m := tree(c), max_q_len=200), c.tree_oracle(m))
+
+
+def test_mask_of_sequences_without_drafts(PA):
+    """A sequence without drafts whose offset lies inside another's rows, through the mask and the attention."""
+    c = Case([(6, 200), (0, 70), (4, 90)], 4, 2, 128, 16, F16, seed=61)
+    c.offs[1] = 3
+    parents = torch.tensor([-1, 0, 0, 1, 2, 4, -1, 0, 1, -1])
+    offs, lens = c.offs.cuda(), c.new.cuda()
+    g = torch.cuda.CUDAGraph()
+    p = parents.cuda()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        m = PA.tree_mask_from_parents(p, offs, 6, lens)
+    g.replay()
+    assert torch.equal(m.cpu(), PA.tree_mask_from_parents(parents, torch.tensor([0, 6]), 6))
+    check(PA.paged_tree_attention(*c.args(), m, max_q_len=6), c.tree_oracle(m))

@@ -1714,7 +1714,9 @@ extern "C" int npl_paged_tree_attention(const void* q, int dtype, int64_t ld_q, 
                 (long long)ld_mask, max_q_len);
   if (int rc = check_device()) return rc;
   if (B == 0 || total_q == 0 || max_q_len == 0) return NPL_OK;
-  p.max_q_len = std::min(max_q_len, total_q);  // a loose bound costs nothing, and no count of tiles overflows
+  // No count of tiles overflows. A bound far above the lengths still costs: row tiles that do not exist are looked at
+  // and passed over, and the kernel and the cluster size, and with them a row's last bits, go by the bound.
+  p.max_q_len = std::min(max_q_len, total_q);
   p.status = device_status_ptr();
   return run<true>(what, p, dtype, D, scale, static_cast<cudaStream_t>(stream));
 }

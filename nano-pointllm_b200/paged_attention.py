@@ -261,7 +261,9 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     (``tree_mask_from_parents``). A draft that sees nothing gets zeros. What a
     masked slot holds, infinities and NaN included, never reaches a row that
     does not see it. Probabilities are rounded to the type of the caches.
-    ``max_q_len`` (>= every q_lens) avoids reading q_lens back to the host."""
+    ``max_q_len`` (>= every q_lens) avoids reading q_lens back to the host; the
+    nearer it is, the less work is looked at in vain, and a row's last bits may
+    change with it."""
     if tree_mask.dtype not in (torch.bool, torch.uint8):
         raise ValueError("tree_mask must be bool or uint8")
     if q_lens is None or q_offsets is None:
@@ -329,7 +331,8 @@ def paged_window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     not read, so those pages may have been freed. What a masked slot holds,
     infinities and NaN included, never reaches a row that does not see it.
     Probabilities are rounded to the type of the caches. ``max_q_len`` (>= every
-    q_lens) avoids reading q_lens back to the host."""
+    q_lens) avoids reading q_lens back to the host, as in
+    ``paged_tree_attention``."""
     if not 1 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31:
         raise ValueError("window must be at least 1 and sinks at least 0, below 2^31")
     args, out, ld_out, _held = _masked_arguments(q, k_cache, v_cache, block_tables, context_lens, q_lens, q_offsets,

@@ -600,3 +600,15 @@ def test_mask_of_sequences_without_drafts(PA):
     g.replay()
     assert torch.equal(m.cpu(), PA.tree_mask_from_parents(parents, torch.tensor([0, 6]), 6))
     check(PA.paged_tree_attention(*c.args(), m, max_q_len=6), c.tree_oracle(m))
+
+
+@pytest.mark.parametrize("most", [150, 153, 2 ** 31 - 1])
+def test_bounds_on_the_lengths(PA, most):
+    """The longest length itself and bounds above it, which may select another kernel and split: each within the
+    oracle's bounds. Single tokens under a loose bound too."""
+    c = Case([(150, 400), (3, 90)], 4, 2, 128, 16, F16, seed=41)
+    check(PA.paged_window_attention(*c.args(), 70, 4, max_q_len=most), c.window_oracle(70, 4))
+    check(PA.paged_tree_attention(*c.args(), m := tree(c, cols=160 if most < 160 else c.total), max_q_len=min(most, c.total)),
+          c.tree_oracle(m))
+    c = Case([(1, 40 * i) for i in range(1, 65)], 4, 4, 64, 16, BF16, seed=42)
+    check(PA.paged_window_attention(*c.args(), 300, 4, max_q_len=1 if most == 150 else most), c.window_oracle(300, 4))

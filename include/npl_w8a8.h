@@ -475,7 +475,8 @@ int npl_fp8_linear(const uint8_t* qa, int64_t lda, const float* sa, int64_t ld_s
  * (tree_mask uint8 [total_q, mask_cols], row stride ld_mask); a row that sees
  * nothing gives zeros. Scores are fp32 dot products times `scale`, the softmax
  * runs in fp32, probabilities are rounded to the type of the caches for the
- * P.V product (fp32 accumulation), and out is rounded once. What a masked slot
+ * P.V product (fp32 accumulation; to twice its bits where max_q_len * H / Hkv is
+ * at most 32), and out is rounded once. What a masked slot
  * holds, infinities and NaN included, never reaches a row that does not see it.
  * Rows of no sequence are not written; context_lens[b] == 0 gives zeros.
  * max_q_len >= every q_lens[b] sizes the launch. D is 64 or 128, block_size a

@@ -10,8 +10,11 @@
 // maximum: it moves only when a tile's maximum is more than 2^8 above it (in
 // the exponentials), so that the sums in tensor memory are rarely rescaled.
 // p = 2^(s log2(e) + 6 - m): at most 2^14, and an fp16 p keeps 2^-30 of the
-// largest. p is rounded to the type of the caches because it is an operand of
-// the P.V product; the normaliser sums the unrounded p.
+// largest. The normaliser sums the unrounded p. For P.V, whose operands have
+// the type of the caches, up to 32 rows of a kv head have p as two numbers of it,
+// p rounded and the rest (below 2^-22 of p in fp16, 2^-16 in bf16: single
+// tokens keep what a product in fp32 keeps); more rows have p rounded once, as
+// in causal prompts: the rest has no room beside S and O in tensor memory.
 //
 // On the tensor cores (tcgen05 kind::f16, fp32 sums in TMEM). A CTA works on two
 // streams, each with its own rows, its own warpgroup and its own TMEM, so that
@@ -152,7 +155,7 @@ struct MaFewSmem : MaBarriers<D == 128 ? 4 : 8> {
   static constexpr uint32_t kGroup = 8 * D * 2;
   static constexpr uint32_t kTileBytes = kMaTile * D * 2;
   static constexpr int kStages = D == 64 ? 10 : 5;
-  static constexpr uint32_t kScoreCols = kN, kOutCols = kN, kTmemCols = 4 * kN;  // S of the streams, then O
+  static constexpr uint32_t kScoreCols = kN, kOutCols = 2 * kN, kTmemCols = 8 * kN;  // S of the streams, then O
   uint64_t full[kStages], empty[kStages], raw[kStages];
   alignas(16) float add[2][kN];  // of a row: 6 - m
   float alpha[2][kN];            // what its sums are scaled with
@@ -161,7 +164,7 @@ struct MaFewSmem : MaBarriers<D == 128 ? 4 : 8> {
   float inv[2][kN];              // and what a row of sums is multiplied with
   static constexpr int kQBufs = kN == 16 ? 2 : 1;  // Q of this item, and of the next one where there is room
   alignas(1024) uint8_t q[kQBufs][2][kN * D * 2];
-  alignas(1024) uint8_t p[2][kMaTile * 128];  // P^T: a key's rows in one 128-byte line
+  alignas(1024) uint8_t p[2][kMaTile * 128];  // P^T: a key's rows, then what their roundings left, in one 128-byte line
   alignas(1024) uint8_t kv[kStages][kTileBytes];
 };
 
@@ -179,6 +182,7 @@ struct MaType<__half> {
   static constexpr uint32_t kIdesc = 0;  // a_format, b_format: F16
   static constexpr uint32_t kExp = 0x7c007c00u, kOne = 0x04000400u;
   static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  __device__ static float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
   __device__ static uint32_t pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -197,6 +201,9 @@ struct MaType<__nv_bfloat16> {
   static constexpr uint32_t kIdesc = (1u << 7) | (1u << 10);
   static constexpr uint32_t kExp = 0x7f807f80u, kOne = 0x00800080u;
   static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  __device__ static float2 unpack(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
   __device__ static uint32_t pack(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -581,12 +588,13 @@ __device__ __forceinline__ void ma_warp_reduce(float (&v)[16], int lane, Op&& op
   v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
 }
 
-// 4 or 16 columns of this lane from TMEM.
-__device__ __forceinline__ void ma_tmem_ld_x4(uint32_t taddr, uint32_t (&r)[4]) {
+// Twice 4, or 16 columns of this lane from TMEM.
+__device__ __forceinline__ void ma_tmem_ld_2x4(uint32_t at0, uint32_t at1, uint32_t (&r)[4], uint32_t (&q)[4]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];\n\ttcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-      : "r"(taddr)
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%8];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%4, %5, %6, %7}, [%9];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]), "=&r"(q[0]), "=&r"(q[1]), "=&r"(q[2]), "=&r"(q[3])
+      : "r"(at0), "r"(at1)
       : "memory");
 }
 __device__ __forceinline__ void ma_tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -807,7 +815,7 @@ __device__ __forceinline__ void ma_mma_role(S& s, const MaArgs& p, uint32_t tmem
   // D = 64 the rows of O^T come twice, the second time to lanes that nobody reads)
   constexpr uint32_t kIdQK = idesc_f16(kMaTile, S::kFew ? S::kRows : kMaTile, false) | MaType<T>::kIdesc;
   constexpr uint32_t kIdPV =
-      idesc_f16(kMaTile, S::kFew ? S::kRows : D, true) | (S::kFew ? 1u << 15 : 0u) | MaType<T>::kIdesc;
+      idesc_f16(kMaTile, S::kFew ? 2 * S::kRows : D, true) | (S::kFew ? 1u << 15 : 0u) | MaType<T>::kIdesc;
   const bool issuer = elect_one();
   const uint64_t q_desc = sdesc_k_sw128(smem_u32(s.q)), k_desc = ma_desc_k(smem_u32(s.kv), S::kGroup);
   const uint64_t v_desc = ma_desc_mn(smem_u32(s.kv), S::kFew && D == 64 ? 0 : 1024, S::kGroup);
@@ -1254,7 +1262,9 @@ __global__ void __launch_bounds__(kMaThreads, 1)
 // 8 x 32 44.4 and 47.7; from 33 rows on the other kernel is as fast):
 // S^T = K Q^T has a key a TMEM lane and a row a column, so that a thread takes
 // kN exponentials a tile and none is spent on rows that do not exist. O^T =
-// V^T P^T has a column of the head a lane. The rows' references m are kept in
+// V^T P^T has a column of the head a lane. P^T has twice kN columns, p rounded and
+// what the rounding left, in one product whose two halves are added at the end
+// (1 token 14.1 -> 14.2 us, 64 tokens 165.1 -> 166.2). The rows' references m are kept in
 // shared memory and moved, by all threads of the stream together, in the rare
 // tile that exceeds one by more than 2^8. Columns are taken 16 at a time.
 template <typename T, int D, bool kTree, int kN>
@@ -1288,7 +1298,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
     const int st = warp >> 2;         // stream
     const int r = threadIdx.x & 127;  // key of the tile, and column of the output: TMEM lane
     const uint32_t lane_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t s_tm = lane_tm + st * kN, o_tm = lane_tm + 2 * kN + st * kN;
+    const uint32_t s_tm = lane_tm + st * kN, o_tm = lane_tm + 2 * kN + st * 2 * kN;
     uint32_t s_phase = 0, o_phase = 0;
     int item_no = 0;
     bool ok = true;  // the same for all threads of the stream at the top of a loop
@@ -1393,12 +1403,12 @@ __global__ void __launch_bounds__(kMaThreads, 1)
           for (int n = 0; n < kN; ++n) l[n] *= s.alpha[st][n];
           if (t > 0) {
 #pragma unroll 1
-            for (int n = 0; n < kN; n += 16) {
+            for (int n = 0; n < 2 * kN; n += 16) {
               uint32_t o[16];
               ma_tmem_ld_x16(o_tm + n, o);
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                o[e] = __float_as_uint(__uint_as_float(o[e]) * s.alpha[st][n + e]);
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * s.alpha[st][(n & (kN - 1)) + e]);
               ma_tmem_st_x16(o_tm + n, o);
             }
             ma_tmem_wait_st();
@@ -1412,7 +1422,7 @@ __global__ void __launch_bounds__(kMaThreads, 1)
             ma_tmem_ld_x16(s_tm + n, v);
             if (part) hide(v, n);
           }
-          uint32_t w[8];
+          uint32_t w[8], rest[8];  // p, and p less what w holds of it
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
             const float4 add = *reinterpret_cast<const float4*>(&s.add[st][n + e]);
@@ -1426,9 +1436,14 @@ __global__ void __launch_bounds__(kMaThreads, 1)
             l[n + e + 3] += p3;
             w[e / 2] = MaType<T>::pack(p0, p1);
             w[e / 2 + 1] = MaType<T>::pack(p2, p3);
+            const float2 a = MaType<T>::unpack(w[e / 2]), b = MaType<T>::unpack(w[e / 2 + 1]);
+            rest[e / 2] = MaType<T>::pack(p0 - a.x, p1 - a.y);
+            rest[e / 2 + 1] = MaType<T>::pack(p2 - b.x, p3 - b.y);
           }
           *reinterpret_cast<uint4*>(line + (((n >> 3) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           *reinterpret_cast<uint4*>(line + (((n >> 3) + 1 ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+          *reinterpret_cast<uint4*>(line + (((kN + n) >> 3 ^ (r & 7)) << 4)) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+          *reinterpret_cast<uint4*>(line + (((kN + n) >> 3) + 1 ^ (r & 7)) * 16) = make_uint4(rest[4], rest[5], rest[6], rest[7]);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -1467,11 +1482,12 @@ __global__ void __launch_bounds__(kMaThreads, 1)
         int head = 0;
 #pragma unroll 1
         for (int n = 0; n < n_rows; n += 4) {
-          uint32_t o[4];
-          if (it.nt > 0) ma_tmem_ld_x4(o_tm + n, o);
+          uint32_t o[4], rest[4];
+          if (it.nt > 0) ma_tmem_ld_2x4(o_tm + n, o_tm + kN + n, o, rest);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float inv = s.inv[st][n + e], y = inv == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
+            const float inv = s.inv[st][n + e];
+            const float y = inv == 0.f ? 0.f : (__uint_as_float(o[e]) + __uint_as_float(rest[e])) * inv;
             if (n + e < n_rows && r < D) {
               if (p.split > 1)
                 stage[(n + e) * D] = y;

@@ -260,8 +260,9 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     (bool or uint8) says so: itself and those that it follows
     (``tree_mask_from_parents``). A draft that sees nothing gets zeros. What a
     masked slot holds, infinities and NaN included, never reaches a row that
-    does not see it. Probabilities are rounded to the type of the caches.
-    ``max_q_len`` (>= every q_lens) avoids reading q_lens back to the host; the
+    does not see it. Probabilities are rounded to the type of the caches where
+    max_q_len times num_kv_groups is above 32; up to there twice its bits are
+    kept. ``max_q_len`` (>= every q_lens) avoids reading q_lens back to the host; the
     nearer it is, the less work is looked at in vain, and a row's last bits may
     change with it."""
     if tree_mask.dtype not in (torch.bool, torch.uint8):
@@ -330,8 +331,9 @@ def paged_window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     in ``paged_decode_attention``. Table entries of pages that no query sees are
     not read, so those pages may have been freed. What a masked slot holds,
     infinities and NaN included, never reaches a row that does not see it.
-    Probabilities are rounded to the type of the caches. ``max_q_len`` (>= every
-    q_lens) avoids reading q_lens back to the host, as in
+    Probabilities are rounded as in ``paged_tree_attention`` (single tokens of
+    up to 32 query heads for each kv head: not, but to twice the bits of the type).
+    ``max_q_len`` (>= every q_lens) avoids reading q_lens back to the host, as in
     ``paged_tree_attention``."""
     if not 1 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31:
         raise ValueError("window must be at least 1 and sinks at least 0, below 2^31")

@@ -612,3 +612,37 @@ def test_bounds_on_the_lengths(PA, most):
           c.tree_oracle(m))
     c = Case([(1, 40 * i) for i in range(1, 65)], 4, 4, 64, 16, BF16, seed=42)
     check(PA.paged_window_attention(*c.args(), 300, 4, max_q_len=1 if most == 150 else most), c.window_oracle(300, 4))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("new,heads,kv_heads,D,ctx", [(1, 2, 2, 64, 300), (1, 8, 1, 128, 5000), (12, 4, 2, 128, 700),
+                                                      (5, 3, 3, 64, 90)])
+def test_probabilities_of_few_rows(PA, new, heads, kv_heads, D, ctx, dtype):
+    """Single tokens and small trees (at most 32 rows of a kv head) keep the probabilities to twice the bits of their
+    type. Key 0 scores 0, all others x, a single product; V is 0 and 1: every product p v of a row is off by the same
+    factor, so that a p rounded once shows whole in the result. With u half a step of the type, a right one is off by
+    u for the output, u^2 for p, 2 e_s + 2^-21 for scores of two fp32 steps and exp2, 2 n 2^-24 for the sums, and in
+    fp16 by 2^-31 a key where the second part of p is subnormal."""
+    c = Case([(new, ctx + i) for i in range(40)], heads, kv_heads, D, 16, dtype, seed=67)
+    c.scale = 1.0
+    g = torch.Generator().manual_seed(5)
+    c.q.zero_()
+    c.q[:, :, 0] = (-torch.rand(c.total, heads, generator=g) * 3 - float(np.log(ctx)) + 2).to(dtype).cuda()
+    c.k.zero_()
+    c.k[..., 0] = 1.0
+    c.v.fill_(1.0)
+    for b in range(len(c.seqs)):
+        blk, at = c.slot(b, 0)
+        c.k[blk, at] = 0.0
+        c.v[blk, at] = 0.0
+    u = O.HALF_STEP[NAME[dtype]]
+    x = c.q[:, :, :1].double().abs().cpu().numpy()
+    m = tree(c, density=0.5)
+    for got, (out, _) in ((PA.paged_tree_attention(*c.args(), m), c.tree_oracle(m)),
+                          (PA.paged_window_attention(*c.args(), 1 << 20, 0), c.window_oracle(1 << 20, 0))):
+        n = ctx + 40
+        tol = out * (u + u * u + 4 * 2.0 ** -23 * x + 2.0 ** -21 + 2 * n * 2.0 ** -24)
+        if dtype == F16:
+            tol = tol + n * 2.0 ** -31 + 2.0 ** -25
+        err = np.abs(got.double().cpu().numpy() - out)
+        assert (err <= tol).all(), f"{(err / tol).max()} times its bound"

@@ -15,7 +15,10 @@ Public surface, mirroring the reference ``nanopointllm`` API for this path:
   int8 ones (quantize_token_blocks, quantize_weight_blocks,
   rmsnorm_quant_blocks, silu_mul_quant_blocks, linear_blocks, Fp8BlockLinear)
 * ``nanopointllm_b200.paged_attention`` - store_kvcache, paged_decode_attention,
-  rope_store_kvcache
+  paged_varlen_attention, rope_store_kvcache; beside them paged_tree_attention,
+  tree_mask_from_parents and paged_window_attention
+* ``nanopointllm_b200.logprobs``        - log probabilities of tokens, entropy
+  and the most likely tokens (token_logprobs)
 * ``nanopointllm_b200.runner``          - W8A8 Llama decode runner
   (inject/quantize a model, prefill + decode steps, CUDA-graph decode)
 * ``nanopointllm_b200.tp``              - the same runner split over GPUs
@@ -33,4 +36,4 @@ from ``csrc/``; there is no CPU or library fallback.
 """
 from __future__ import annotations
 
-__all__ = ["w8a8", "fp8", "paged_attention", "runner", "synthetic", "tp", "package", "serving"]
+__all__ = ["w8a8", "fp8", "paged_attention", "logprobs", "runner", "synthetic", "tp", "package", "serving"]

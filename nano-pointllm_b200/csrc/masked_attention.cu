@@ -43,10 +43,14 @@
 // added at the end to the rows that do see them.
 //
 // Bound by memory where there are few rows (64 tokens, 32 heads, 1028 keys each:
-// 165 us, 6.0 TB/s); for prompts by a stream's chain of product, scores out of
+// 166 us, 6.0 TB/s); for long prompts by a stream's chain of product, scores out of
 // TMEM (twice: held in registers they spill), exponentials (a quarter of them by
 // a polynomial: 375 us for 16000 tokens of 32/8 heads under a window of 1024, none
-// 409, half 415; 325 with tiles packed, 310 with 32-byte stores) and P back.
+// 409, half 415; 325 with tiles packed, 310 with 32-byte stores, 314 with NaN kept)
+// and P back. For many prompts of few row tiles by uneven shares: the row tile is
+// the fastest index of the items and a CTA takes every 148th, so that with 4 row
+// tiles (20 x 800 tokens) a CTA meets one of them only, of 2, 4, 5 or 3 key tiles,
+// and has 34 to 90 key tiles to do, 61 in the mean (312 us).
 #include <algorithm>
 #include <initializer_list>
 
@@ -1630,9 +1634,13 @@ int launch(const char* what, MaArgs p, cudaStream_t st) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status(what);
   // The cluster size with the least time in tiles of 128 keys: the longest item, or all rounds of clusters, each with
-  // kMaFixed for the start of its CTAs and the join (a tile of two kv heads takes 1.7 us, a round without any 10 to
-  // 15: 16 drafts over 1024 keys of 32 heads in 25.1, 21.2, 17.2 and 29.6 us split 1, 2, 4 and 8 ways). Contexts may
-  // have any length up to the table's: three quarters of it are taken as usual. Windows are mostly full.
+  // kMaFixed for the start of its CTAs and the join. Contexts may have any length up to the table's: three quarters of
+  // it are taken as usual. Windows are mostly full. Split 1, 2, 4 and 8 ways, us (* is taken): 16 drafts over 1040 keys
+  // of 32 heads 22.0, 19.9, 16.7*, 29.8; 8 x 64 drafts over 2000 keys 56.2*, 79.5, 110, 191; 61 drafts over 4000 keys of
+  // 28/4 heads of 64 62.9, 42.1, 28.0, 21.3*; windows of 4096 of 16 tokens, 32/8 heads 71.3, 49.2*, 57.8, 89.4. Of 54
+  // such (1 to 64 sequences, 1 to 2000 rows, heads of 64 and 128, even and uneven contexts, all kernels) the least time
+  // is taken in 53, and one 6% above it, by any kMaFixed from 8 to 14; 6 loses up to 23%, and so does taking half the
+  // table as usual. A table four times as wide as the contexts need costs up to 41%.
   long long keys = (long long)p.max_blocks * p.block_size;  // the most that an item's rows may see
   if (!kTree) keys = std::min(keys, (long long)p.window + p.sinks + 2 * p.tokens);
   const int sms = num_sms() > 0 ? num_sms() : 148;

@@ -264,7 +264,9 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     max_q_len times num_kv_groups is above 32; up to there twice its bits are
     kept. ``max_q_len`` (>= every q_lens) avoids reading q_lens back to the host; the
     nearer it is, the less work is looked at in vain, and a row's last bits may
-    change with it."""
+    change with it. How keys are split over CTAs goes by the width of
+    ``block_tables``: pass its first columns, as many as the longest context
+    needs (any stride will do)."""
     if tree_mask.dtype not in (torch.bool, torch.uint8):
         raise ValueError("tree_mask must be bool or uint8")
     if q_lens is None or q_offsets is None:
